@@ -364,6 +364,73 @@ int32_t mb_sample_tokens(const void* logits, int32_t logits_f32, int32_t N, int3
  * counterpart: keeps a captured step replayable). */
 int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
 
+/* ---- Drafted decoding (no reference counterpart: the reference verifies one token per
+ * step, batch_generator.py:255-300, and its cache grows until it overflows, :79-107) ----
+ * A trace's drafted tokens form a tree of m <= 64 nodes in topological order (node 0 the
+ * last chosen token, whose keys are not cached yet). All element types are 16-bit: fp16,
+ * or bf16 where is_bf16 = 1. `strides` are HOST arrays of element strides; the head dim is
+ * contiguous. Device lengths are clamped to [0, Lmax].
+ *
+ * mb_tree_attn: exact softmax attention of every node over the lens[t] committed rows of
+ * its trace and the nodes in its mask (bit j of masks[t][i]: node i sees node j; a mask of
+ * 0 is padding and gives a zero output):
+ *   x_l = scale q_i . k_l, p = softmax(x) (fp32), out_i = sum_l p_l v_l.
+ * q / out [T, m, H, d], caches [T, Hkv, Lmax, d], drafts [T, m, Hkv, d]; query head h reads
+ * KV head h / (H / Hkv); d <= 256. strides[18]: (t, i, h) of q, (t, h, l) of k_cache and of
+ * v_cache, (t, i, h) of k_draft, v_draft and out. masks [T, m], or [m] if shared_masks.
+ * scores_out (optional, [T, Hkv, Lmax] fp32): row l < lens[t] gets scores[l] (0 if scores
+ * is NULL; scores may be scores_out) plus its weight summed over the nodes and heads;
+ * draft_scores [T, Hkv, m] the draft rows' sums. No atomics: results repeat bit for bit.
+ * The workspace needs no initial contents. */
+size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d);
+int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
+                     const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* masks, int32_t shared_masks,
+                     uint16_t* out, const int64_t* strides, int32_t is_bf16, int32_t T, int32_t m, int32_t H,
+                     int32_t Hkv, int32_t Lmax, int32_t d, float scale, const float* scores, float* scores_out,
+                     float* draft_scores, void* workspace, size_t workspace_bytes, void* stream);
+
+/* mb_tree_accept: the accepted path of every trace (from the root, the lowest child whose
+ * token equals target[parent]; parents [T, m], or [m] if shared_parents; a negative token
+ * is never accepted, a negative root token means an idle trace: count 0, next id -1), and
+ * the append of its rows to the caches of all layers: row lens[t] + j gets the j-th
+ * accepted node's draft row, scores (optional) its draft score, positions (optional)
+ * next_pos[t] + j. caches [layers, T, Hkv, Lmax, d], drafts [layers, T, m, Hkv, d], scores
+ * / positions [layers, T, Hkv, Lmax], draft_scores [layers, T, Hkv, m]. strides[16]:
+ * (layer, t, h, l) of k_cache and v_cache, (layer, t, i, h) of k_draft and v_draft. Writes
+ * path [T, m] (-1 after the last), counts, next_ids (target at the last accepted node),
+ * lens_out and pos_out [T] (not the inputs' buffers). A trace without room keeps its state
+ * (count 0) and sets MB_DEVERR_INDEX in the optional dev_err. */
+int32_t mb_tree_accept(const int32_t* tokens, const int32_t* parents, int32_t shared_parents, const int32_t* target,
+                       const int32_t* lens, const int32_t* next_pos, uint16_t* k_cache, uint16_t* v_cache,
+                       const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* strides, int32_t layers,
+                       int32_t T, int32_t m, int32_t Hkv, int32_t Lmax, int32_t d, float* scores,
+                       const float* draft_scores, int32_t* positions, int32_t* path, int32_t* counts,
+                       int32_t* next_ids, int32_t* lens_out, int32_t* pos_out, uint32_t* dev_err, void* stream);
+
+/* mb_tree_rope: mb_rope_append's rotation for a tree, into draft buffers: qkv [T, m,
+ * (H + 2 Hkv) * dh] (q | k | v), node i at position next_pos[t] + depths[t][i] (depths
+ * [T, m], or [m] if shared_depths) -> q_out [T, m, H, dh], k_out [T, m, Hkv, dh]; cs as
+ * in mb_rope_append for `positions` positions. A position outside skips the node and sets
+ * MB_DEVERR_INDEX. */
+int32_t mb_tree_rope(const uint16_t* qkv, int32_t is_bf16, int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t dh,
+                     const int32_t* next_pos, const int32_t* depths, int32_t shared_depths, const float* cs,
+                     int32_t positions, uint16_t* q_out, uint16_t* k_out, uint32_t* dev_err, void* stream);
+
+/* mb_cache_evict: every (layer, trace, KV head) keeps min(lens[t], budget) rows: first the
+ * guarded ones (position >= next_pos[t] - recent, or < sinks; recent + sinks <= budget; all
+ * alike), then larger scores, ties to the lowest row, a NaN below everything. Kept rows below the
+ * budget stay in place; the j-th kept row at or beyond it moves into the j-th row below it
+ * that leaves (K, V, score and position). caches [layers, T, Hkv, Lmax, d], strides[8]:
+ * (layer, t, h, l) of k_cache and v_cache; scores / positions [layers, T, Hkv, Lmax], their
+ * _out either the same buffers (both) or others, whose rows beyond the kept ones are not
+ * written. lens_out [T] (not lens). The workspace needs no initial contents. */
+size_t mb_cache_evict_workspace_size(int32_t layers, int32_t T, int32_t Hkv, int32_t Lmax, int32_t budget);
+int32_t mb_cache_evict(uint16_t* k_cache, uint16_t* v_cache, const int64_t* strides, const float* scores,
+                       const int32_t* positions, float* scores_out, int32_t* positions_out, const int32_t* lens,
+                       const int32_t* next_pos, int32_t* lens_out, int32_t layers, int32_t T, int32_t Hkv,
+                       int32_t Lmax, int32_t d, int32_t budget, int32_t recent, int32_t sinks, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,411 @@
+// Drafted decoding over a KV cache on B200 (sm_100a): attention of a tree of drafted
+// tokens, and acceptance of the verified tree with the append of its accepted rows.
+//
+// One trace t holds lens[t] committed rows in its cache and m drafted tokens (nodes of a
+// tree in topological order, node 0 its root) whose keys and values lie in draft buffers.
+// Node i sees every committed row and the nodes in its 64-bit mask (its ancestors and
+// itself):
+//   x_l = scale * q_i . k_l,   p = softmax of x over the visible l,   out_i = sum_l p_l v_l.
+// Query heads h = kvh * G + g share the keys of KV head kvh (G = H / Hkv).
+// Optionally every row's attention weight, summed over the nodes and the G heads of its
+// KV head, is added to the row's running score.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "tree.cuh"
+
+namespace mb {
+
+// ---------------------------------------------------------------------------
+// Any shape, stride and alignment: one CTA per (trace, node, head), fp32 online softmax.
+// ---------------------------------------------------------------------------
+constexpr int kAnyBlock = 128;
+constexpr int kMaxHeadDim = 256;
+
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t x) {
+  if (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);
+  return __half2float(__ushort_as_half(x));
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint16_t from_f32(float x) {
+  if (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  return __half_as_ushort(__float2half_rn(x));
+}
+
+// Key row l of (t, kvh): committed rows first, then the draft's nodes.
+__device__ __forceinline__ const uint16_t* tree_row(const uint16_t* cache, const int64_t* cs, const uint16_t* draft,
+                                                    const int64_t* ds, int t, int kvh, int len, int l) {
+  if (l < len) return cache + t * cs[0] + kvh * cs[1] + l * cs[2];
+  return draft + t * ds[0] + (l - len) * ds[1] + kvh * ds[2];
+}
+
+// lse[t, h, i] (log2 units, +inf for a node that sees nothing) is written for the weight pass.
+template <bool BF16>
+__global__ void __launch_bounds__(kAnyBlock) k_tree_attn_any(TreeAttnArgs a, float* __restrict__ lse) {
+  __shared__ float qs[kMaxHeadDim];
+  __shared__ float p[kAnyBlock];
+  __shared__ float red[kAnyBlock / 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x;
+  const int h = blockIdx.x % a.H, i = (blockIdx.x / a.H) % a.m, t = blockIdx.x / (a.H * a.m);
+  const int kvh = h / (a.H / a.Hkv);
+  const uint64_t mask = a.masks[t * a.mask_stride + i];
+  const int len = max(0, min(a.lens[t], a.Lmax));
+  const uint16_t* q = a.q + t * a.qs[0] + i * a.qs[1] + h * a.qs[2];
+  for (int c = tid; c < a.d; c += kAnyBlock) qs[c] = to_f32<BF16>(q[c]) * a.scale_log2;
+  float acc[kMaxHeadDim / kAnyBlock] = {};
+  float top = -INFINITY, sum = 0.0f;
+  const int total = mask ? len + a.m : 0;
+  for (int l0 = 0; l0 < total; l0 += kAnyBlock) {
+    const int l = l0 + tid;
+    float x = -INFINITY;
+    __syncthreads();  // qs written; the previous chunk's p read
+    if (l < total && (l < len || (mask >> (l - len)) & 1)) {
+      const uint16_t* k = tree_row(a.k, a.ks, a.kd, a.kds, t, kvh, len, l);
+      x = 0.0f;
+      for (int c = 0; c < a.d; ++c) x = fmaf(qs[c], to_f32<BF16>(k[c]), x);
+    }
+    float mx = x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((tid & 31) == 0) red[tid >> 5] = mx;
+    __syncthreads();
+    mx = top;
+#pragma unroll
+    for (int w = 0; w < kAnyBlock / 32; ++w) mx = fmaxf(mx, red[w]);
+    const float base = mx == -INFINITY ? 0.0f : mx;  // nothing seen yet: every weight is 0
+    p[tid] = exp2f(x - base);
+    const float fade = exp2f(top - base);
+    top = mx;
+    __syncthreads();
+    sum *= fade;
+    const int n = min(kAnyBlock, total - l0);
+    for (int j = 0; j < n; ++j) sum += p[j];
+#pragma unroll
+    for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) {
+      const int c = tid + u * kAnyBlock;
+      if (c < a.d) {
+        float s = acc[u] * fade;
+        for (int j = 0; j < n; ++j) {
+          const float w = p[j];
+          if (w != 0.0f) s = fmaf(w, to_f32<BF16>(tree_row(a.v, a.vs, a.vd, a.vds, t, kvh, len, l0 + j)[c]), s);
+        }
+        acc[u] = s;
+      }
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t* o = a.out + t * a.os[0] + i * a.os[1] + h * a.os[2];
+#pragma unroll
+  for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) {
+    const int c = tid + u * kAnyBlock;
+    if (c < a.d) o[c] = from_f32<BF16>(acc[u] * inv);
+  }
+  if (lse && tid == 0) lse[(static_cast<int64_t>(t) * a.H + h) * a.m + i] = sum == 0.0f ? INFINITY : top + log2f(sum);
+}
+
+// Weight of one row: a thread recomputes its row's score against every query of the KV
+// head, in a fixed order (no atomics: the sums repeat bit for bit).
+template <bool BF16>
+__global__ void __launch_bounds__(kAnyBlock) k_tree_weights_any(TreeAttnArgs a, const float* __restrict__ lse) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int kvh = blockIdx.y % a.Hkv, t = blockIdx.y / a.Hkv;
+  const int len = max(0, min(a.lens[t], a.Lmax));
+  const int l = blockIdx.x * kAnyBlock + threadIdx.x;
+  if (l >= len + a.m) return;
+  const int G = a.H / a.Hkv;
+  const uint16_t* k = tree_row(a.k, a.ks, a.kd, a.kds, t, kvh, len, l);
+  float w = 0.0f;
+  for (int i = 0; i < a.m; ++i) {
+    const uint64_t mask = a.masks[t * a.mask_stride + i];
+    if (mask == 0 || (l >= len && !((mask >> (l - len)) & 1))) continue;
+    for (int g = 0; g < G; ++g) {
+      const int h = kvh * G + g;
+      const uint16_t* q = a.q + t * a.qs[0] + i * a.qs[1] + h * a.qs[2];
+      float x = 0.0f;
+      for (int c = 0; c < a.d; ++c) x = fmaf(to_f32<BF16>(q[c]) * a.scale_log2, to_f32<BF16>(k[c]), x);
+      w += exp2f(x - lse[(static_cast<int64_t>(t) * a.H + h) * a.m + i]);
+    }
+  }
+  const int64_t unit = static_cast<int64_t>(t) * a.Hkv + kvh;
+  if (l < len)
+    a.scores_out[unit * a.Lmax + l] = (a.scores ? a.scores[unit * a.Lmax + l] : 0.0f) + w;
+  else
+    a.draft_scores[unit * a.m + (l - len)] = w;
+}
+
+// ---------------------------------------------------------------------------
+// Acceptance
+// ---------------------------------------------------------------------------
+struct AcceptArgs {
+  const int32_t *tokens, *parents, *target, *lens, *next_pos;
+  uint16_t *k, *v;
+  const uint16_t *kd, *vd;
+  int64_t ks[4], vs[4], kds[4], vds[4];  // element strides: caches (layer, t, h, l), drafts (layer, t, i, h)
+  float* scores;
+  const float* draft_scores;
+  int32_t* positions;
+  int32_t *path, *counts, *next_ids, *lens_out, *pos_out;
+  uint32_t* err;
+  int64_t parent_stride;
+  int layers, T, m, Hkv, Lmax, d, vec;
+};
+
+constexpr int kAcceptBlock = 128;
+
+// The accepted path of trace t, found by one warp: from the root, the first child whose
+// drafted token is what the model chose at its parent. Returns the number of nodes.
+__device__ __forceinline__ int walk_tree(const AcceptArgs& a, int t, int lane, int* path, int* next_id) {
+  const int32_t* tok = a.tokens + static_cast<int64_t>(t) * a.m;
+  const int32_t* par = a.parents + t * a.parent_stride;
+  const int32_t* tgt = a.target + static_cast<int64_t>(t) * a.m;
+  int token[2], parent[2], target[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = lane + 32 * u;
+    token[u] = i < a.m ? tok[i] : -1;
+    parent[u] = i < a.m ? par[i] : -1;
+    target[u] = i < a.m ? tgt[i] : -1;
+  }
+  if (__shfl_sync(0xffffffffu, token[0], 0) < 0) return 0;  // an idle trace
+  int cur = 0, n = 0;
+  for (;;) {
+    if (lane == 0) path[n] = cur;
+    ++n;
+    const int want = __shfl_sync(0xffffffffu, cur < 32 ? target[0] : target[1], cur & 31);
+    *next_id = want;
+    const uint32_t lo = __ballot_sync(0xffffffffu, token[0] >= 0 && lane > cur && parent[0] == cur && token[0] == want);
+    const uint32_t hi =
+        __ballot_sync(0xffffffffu, token[1] >= 0 && lane + 32 > cur && parent[1] == cur && token[1] == want);
+    if (!(lo | hi)) return n;
+    cur = lo ? __ffs(lo) - 1 : __ffs(hi) + 31;  // larger than the last one: at most m steps
+  }
+}
+
+// One CTA per (KV head, trace, layer).
+__global__ void __launch_bounds__(kAcceptBlock) k_tree_accept(AcceptArgs a) {
+  __shared__ int path[64];
+  __shared__ int count_s;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x;
+  const int h = blockIdx.x, t = blockIdx.y, layer = blockIdx.z;
+  const int len = a.lens[t];
+  if (tid < 32) {
+    int next_id = -1;
+    int n = walk_tree(a, t, tid, path, &next_id);
+    if (len < 0 || n > a.Lmax - len) {  // no room: the trace stays as it is
+      n = 0;
+      next_id = -1;
+      if (tid == 0 && a.err) atomicOr(a.err, MB_DEVERR_INDEX);
+    }
+    if (tid == 0) count_s = n;
+    __syncwarp();
+    if (h == 0 && layer == 0) {
+      for (int j = tid; j < a.m; j += 32) a.path[static_cast<int64_t>(t) * a.m + j] = j < n ? path[j] : -1;
+      if (tid == 0) {
+        a.counts[t] = n;
+        a.next_ids[t] = next_id;
+        a.lens_out[t] = len + n;
+        a.pos_out[t] = a.next_pos[t] + n;
+      }
+    }
+  }
+  __syncthreads();
+  const int n = count_s;
+  const uint16_t* kd = a.kd + layer * a.kds[0] + t * a.kds[1] + h * a.kds[3];
+  const uint16_t* vd = a.vd + layer * a.vds[0] + t * a.vds[1] + h * a.vds[3];
+  uint16_t* k = a.k + layer * a.ks[0] + t * a.ks[1] + h * a.ks[2] + len * a.ks[3];
+  uint16_t* v = a.v + layer * a.vs[0] + t * a.vs[1] + h * a.vs[2] + len * a.vs[3];
+  if (a.vec) {
+    const int per = a.d / 8;
+    for (int e = tid; e < n * per; e += kAcceptBlock) {
+      const int j = e / per, c = (e - j * per) * 8;
+      const uint4 x = *reinterpret_cast<const uint4*>(kd + path[j] * a.kds[2] + c);
+      const uint4 y = *reinterpret_cast<const uint4*>(vd + path[j] * a.vds[2] + c);
+      *reinterpret_cast<uint4*>(k + j * a.ks[3] + c) = x;
+      *reinterpret_cast<uint4*>(v + j * a.vs[3] + c) = y;
+    }
+  } else {
+    for (int e = tid; e < n * a.d; e += kAcceptBlock) {
+      const int j = e / a.d, c = e - j * a.d;
+      k[j * a.ks[3] + c] = kd[path[j] * a.kds[2] + c];
+      v[j * a.vs[3] + c] = vd[path[j] * a.vds[2] + c];
+    }
+  }
+  const int64_t unit = (static_cast<int64_t>(layer) * a.T + t) * a.Hkv + h;
+  for (int j = tid; j < n; j += kAcceptBlock) {
+    if (a.scores) a.scores[unit * a.Lmax + len + j] = a.draft_scores[unit * a.m + path[j]];
+    if (a.positions) a.positions[unit * a.Lmax + len + j] = a.next_pos[t] + j;
+  }
+}
+
+// RoPE of a drafted tree's queries and keys at next_pos[t] + depth[i]: adjacent pairs, as
+// mb_rope_append. One CTA per (head of q and k, node, trace).
+template <bool BF16>
+__global__ void __launch_bounds__(64) k_tree_rope(const uint16_t* __restrict__ qkv, int m, int H, int Hkv, int dh,
+                                                  const int32_t* __restrict__ next_pos,
+                                                  const int32_t* __restrict__ depth, int64_t depth_stride,
+                                                  const float2* __restrict__ cs, int positions,
+                                                  uint16_t* __restrict__ q_out, uint16_t* __restrict__ k_out,
+                                                  uint32_t* err) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int h = blockIdx.x, i = blockIdx.y, t = blockIdx.z;
+  const int64_t row = static_cast<int64_t>(t) * m + i;
+  const int p = next_pos[t] + depth[t * depth_stride + i];
+  const uint16_t* src = qkv + row * (H + 2 * Hkv) * dh + h * dh;
+  uint16_t* dst = h < H ? q_out + (row * H + h) * dh : k_out + (row * Hkv + (h - H)) * dh;
+  if (p < 0 || p >= positions) {
+    if (threadIdx.x == 0 && err) atomicOr(err, MB_DEVERR_INDEX);
+    return;
+  }
+  for (int c = threadIdx.x; c < dh / 2; c += 64) {
+    const float2 r = cs[static_cast<int64_t>(p) * (dh / 2) + c];
+    const float x = to_f32<BF16>(src[2 * c]), y = to_f32<BF16>(src[2 * c + 1]);
+    dst[2 * c] = from_f32<BF16>(x * r.x - y * r.y);
+    dst[2 * c + 1] = from_f32<BF16>(x * r.y + y * r.x);
+  }
+}
+
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" {
+
+size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d) {
+  if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim) return 0;
+  return (static_cast<size_t>(T) * H * m * 4 + 255) / 256 * 256;  // lse
+}
+
+int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
+                     const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* masks, int32_t shared_masks,
+                     uint16_t* out, const int64_t* strides, int32_t is_bf16, int32_t T, int32_t m, int32_t H,
+                     int32_t Hkv, int32_t Lmax, int32_t d, float scale, const float* scores, float* scores_out,
+                     float* draft_scores, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !lens || !k_draft || !v_draft || !masks || !out || !strides) return MB_ERR_NULL;
+  if (Lmax > 0 && (!k_cache || !v_cache)) return MB_ERR_NULL;
+  if ((scores_out != nullptr) != (draft_scores != nullptr) || (scores && !scores_out)) return MB_ERR_NULL;
+  if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim)
+    return MB_ERR_ARGS;
+  if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFFFF00)
+    return MB_ERR_UNSUPPORTED;
+  if (!(scale - scale == 0.0f) || is_bf16 < 0 || is_bf16 > 1) return MB_ERR_ARGS;
+  if (!aligned(q, 2) || !aligned(k_cache, 2) || !aligned(v_cache, 2) || !aligned(k_draft, 2) ||
+      !aligned(v_draft, 2) || !aligned(out, 2) || !aligned(lens, 4) || !aligned(masks, 8) || !aligned(scores, 4) ||
+      !aligned(scores_out, 4) || !aligned(draft_scores, 4))
+    return MB_ERR_ALIGN;
+  if (!workspace || workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d)) return MB_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
+  TreeAttnArgs a;
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.kd = k_draft;
+  a.vd = v_draft;
+  a.out = out;
+  a.lens = lens;
+  a.masks = reinterpret_cast<const uint64_t*>(masks);
+  a.mask_stride = shared_masks ? 0 : m;
+  for (int u = 0; u < 3; ++u) {
+    a.qs[u] = strides[u];
+    a.ks[u] = strides[3 + u];
+    a.vs[u] = strides[6 + u];
+    a.kds[u] = strides[9 + u];
+    a.vds[u] = strides[12 + u];
+    a.os[u] = strides[15 + u];
+  }
+  a.T = T;
+  a.m = m;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.Lmax = Lmax;
+  a.d = d;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scores = scores;
+  a.scores_out = scores_out;
+  a.draft_scores = draft_scores;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* lse = scores_out ? static_cast<float*>(workspace) : nullptr;
+  int rc = launch_with_pdl(is_bf16 ? k_tree_attn_any<true> : k_tree_attn_any<false>, dim3(T * m * H), dim3(kAnyBlock),
+                           0, st, a, lse);
+  if (rc != MB_OK || !scores_out) return rc;
+  return launch_with_pdl(is_bf16 ? k_tree_weights_any<true> : k_tree_weights_any<false>,
+                         dim3((Lmax + m + kAnyBlock - 1) / kAnyBlock, T * Hkv), dim3(kAnyBlock), 0, st, a,
+                         static_cast<const float*>(lse));
+}
+
+int32_t mb_tree_accept(const int32_t* tokens, const int32_t* parents, int32_t shared_parents, const int32_t* target,
+                       const int32_t* lens, const int32_t* next_pos, uint16_t* k_cache, uint16_t* v_cache,
+                       const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* strides, int32_t layers,
+                       int32_t T, int32_t m, int32_t Hkv, int32_t Lmax, int32_t d, float* scores,
+                       const float* draft_scores, int32_t* positions, int32_t* path, int32_t* counts,
+                       int32_t* next_ids, int32_t* lens_out, int32_t* pos_out, uint32_t* dev_err, void* stream) {
+  if (!tokens || !parents || !target || !lens || !next_pos || !k_cache || !v_cache || !k_draft || !v_draft ||
+      !strides || !path || !counts || !next_ids || !lens_out || !pos_out)
+    return MB_ERR_NULL;
+  if ((scores != nullptr) != (draft_scores != nullptr)) return MB_ERR_NULL;
+  if (layers < 1 || T < 1 || m < 1 || m > 64 || Hkv < 1 || Lmax < 1 || d < 1) return MB_ERR_ARGS;
+  if (lens_out == lens || pos_out == next_pos) return MB_ERR_ARGS;  // every CTA reads the old lengths
+  if (T > 65535 || layers > 65535) return MB_ERR_UNSUPPORTED;
+  AcceptArgs a;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.parent_stride = shared_parents ? 0 : m;
+  a.target = target;
+  a.lens = lens;
+  a.next_pos = next_pos;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.kd = k_draft;
+  a.vd = v_draft;
+  bool vec = d % 8 == 0 && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_draft, 16) && aligned(v_draft, 16);
+  for (int u = 0; u < 4; ++u) {
+    a.ks[u] = strides[u];
+    a.vs[u] = strides[4 + u];
+    a.kds[u] = strides[8 + u];
+    a.vds[u] = strides[12 + u];
+  }
+  for (int u = 0; u < 16; ++u) vec = vec && strides[u] % 8 == 0;
+  a.vec = vec;
+  a.scores = scores;
+  a.draft_scores = draft_scores;
+  a.positions = positions;
+  a.path = path;
+  a.counts = counts;
+  a.next_ids = next_ids;
+  a.lens_out = lens_out;
+  a.pos_out = pos_out;
+  a.err = dev_err;
+  a.layers = layers;
+  a.T = T;
+  a.m = m;
+  a.Hkv = Hkv;
+  a.Lmax = Lmax;
+  a.d = d;
+  return launch_with_pdl(k_tree_accept, dim3(Hkv, T, layers), dim3(kAcceptBlock), 0, static_cast<cudaStream_t>(stream),
+                         a);
+}
+
+int32_t mb_tree_rope(const uint16_t* qkv, int32_t is_bf16, int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t dh,
+                     const int32_t* next_pos, const int32_t* depths, int32_t shared_depths, const float* cs,
+                     int32_t positions, uint16_t* q_out, uint16_t* k_out, uint32_t* dev_err, void* stream) {
+  if (!qkv || !next_pos || !depths || !cs || !q_out || !k_out) return MB_ERR_NULL;
+  if (T < 1 || m < 1 || m > 64 || H < 1 || Hkv < 1 || dh < 2 || dh % 2 != 0 || positions < 1) return MB_ERR_ARGS;
+  if (is_bf16 < 0 || is_bf16 > 1) return MB_ERR_ARGS;
+  if (T > 65535) return MB_ERR_UNSUPPORTED;
+  if (!aligned(cs, 8)) return MB_ERR_ALIGN;
+  return launch_with_pdl(is_bf16 ? k_tree_rope<true> : k_tree_rope<false>, dim3(H + Hkv, m, T), dim3(64), 0,
+                         static_cast<cudaStream_t>(stream), qkv, m, H, Hkv, dh, next_pos, depths,
+                         static_cast<int64_t>(shared_depths ? 0 : m), reinterpret_cast<const float2*>(cs), positions,
+                         q_out, k_out, dev_err);
+}
+
+}  // extern "C"

@@ -1,0 +1,130 @@
+"""Host logic of drafted decoding: tree masks and depths, workspace sizes, and the
+argument checks of the C entry points (they fail before any CUDA call)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from moat_b200 import _lib
+from moat_b200.tree import tree_depths, tree_masks
+
+
+def test_masks_and_depths_of_a_small_tree():
+    #      0
+    #    1   2
+    #    4   3     node 5: its parent is padding, node 6: parent after itself
+    par = [-1, 0, 0, 2, 1, 7, 6, -1]
+    np.testing.assert_array_equal(tree_masks(par), [0b1, 0b11, 0b101, 0b1101, 0b10011, 0, 0, 0])
+    np.testing.assert_array_equal(tree_depths(par), [0, 1, 1, 2, 2, 0, 0, 0])
+
+
+def test_descendants_of_padding_are_padding():
+    np.testing.assert_array_equal(tree_masks([-1, -1, 1, 0]), [1, 0, 0, 0b1001])
+
+
+def test_full_width_chain_uses_all_64_bits():
+    par = np.arange(64) - 1
+    masks = tree_masks(np.stack([par, par])).view(np.uint64)
+    assert masks.shape == (2, 64)
+    for i in range(64):
+        assert int(masks[1, i]) == (1 << (i + 1)) - 1
+    np.testing.assert_array_equal(tree_depths(par), np.arange(64))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_masks_match_a_walk_to_the_root(seed):
+    rng = np.random.default_rng(seed)
+    par = np.array([[-1] + [int(rng.integers(-1, i)) for i in range(1, 40)] for _ in range(3)])
+    masks, depths = tree_masks(par).view(np.uint64), tree_depths(par)
+    for t in range(3):
+        for i in range(40):
+            seen, j = [i], i
+            while j > 0 and par[t, j] >= 0:
+                j = par[t, j]
+                seen.append(j)
+            want = sum(1 << s for s in seen) if j == 0 else 0
+            assert int(masks[t, i]) == want
+            assert depths[t, i] == (len(seen) - 1 if j == 0 else 0)
+
+
+@pytest.mark.parametrize("m", [0, 65])
+def test_tree_sizes_are_refused(m):
+    with pytest.raises(ValueError):
+        tree_masks([-1] * m)
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+def test_workspace_sizes(L):
+    assert L.mb_tree_attn_workspace_size(2, 8, 16, 4, 1024, 128) > 0
+    for bad in [(0, 8, 16, 4, 1024, 128), (2, 65, 16, 4, 1024, 128), (2, 8, 15, 4, 1024, 128),
+                (2, 8, 16, 4, 1024, 257), (2, 8, 16, 4, -1, 128)]:
+        assert L.mb_tree_attn_workspace_size(*bad) == 0
+    assert L.mb_cache_evict_workspace_size(1, 1, 4, 320, 256) >= 4 * 2 * 64 * 4
+    assert L.mb_cache_evict_workspace_size(1, 1, 4, 320, 0) == 0
+
+
+def test_attention_entry_checks_its_arguments(L):
+    fake = ctypes.c_void_p(0x10000)  # never dereferenced: validation fails first
+    st = (ctypes.c_int64 * 18)(*([128] * 18))
+
+    def attn(q=fake, k=fake, masks=fake, strides=st, bf16=0, T=1, m=4, H=8, Hkv=2, Lmax=64, d=128, scale=0.1,
+             scores=None, scores_out=None, draft=None, ws=fake, nbytes=1 << 30):
+        return L.mb_tree_attn(q, k, fake, fake, fake, fake, masks, 0, fake, strides, bf16, T, m, H, Hkv, Lmax, d,
+                              scale, scores, scores_out, draft, ws, nbytes, None)
+    assert attn(q=None) == -1
+    assert attn(k=None) == -1
+    assert attn(masks=None) == -1
+    assert attn(strides=None) == -1
+    assert attn(scores_out=fake) == -1  # draft_scores missing
+    assert attn(scores=fake) == -1  # nowhere to put the sums
+    assert attn(m=0) == -2 and attn(m=65) == -2
+    assert attn(H=7) == -2 and attn(Hkv=0) == -2
+    assert attn(d=257) == -2 and attn(T=0) == -2 and attn(Lmax=-1) == -2
+    assert attn(scale=float("inf")) == -2 and attn(scale=float("nan")) == -2
+    assert attn(bf16=2) == -2
+    assert attn(ws=None) == -3 and attn(nbytes=16) == -3
+    assert attn(q=ctypes.c_void_p(0x10001)) == -5
+    assert attn(masks=ctypes.c_void_p(0x10004)) == -5
+
+
+def test_accept_entry_checks_its_arguments(L):
+    fake, other = ctypes.c_void_p(0x10000), ctypes.c_void_p(0x20000)
+    st = (ctypes.c_int64 * 16)(*([128] * 16))
+
+    def accept(tokens=fake, lens=fake, layers=1, T=1, m=4, Hkv=2, Lmax=64, d=128, scores=None, draft=None,
+               lens_out=other, pos_out=other):
+        return L.mb_tree_accept(tokens, fake, 0, fake, lens, fake, fake, fake, fake, fake, st, layers, T, m, Hkv, Lmax,
+                                d, scores, draft, None, fake, fake, fake, lens_out, pos_out, None, None)
+    assert accept(tokens=None) == -1
+    assert accept(scores=fake) == -1  # draft_scores missing
+    assert accept(m=65) == -2 and accept(T=0) == -2 and accept(layers=0) == -2 and accept(Lmax=0) == -2
+    assert accept(lens_out=fake) == -2  # in place: another CTA may still read the old length
+    assert accept(pos_out=fake) == -2
+    assert accept(T=70000) == -6
+
+
+def test_rope_and_evict_entries_check_their_arguments(L):
+    fake, other = ctypes.c_void_p(0x10000), ctypes.c_void_p(0x20000)
+    assert L.mb_tree_rope(None, 0, 1, 4, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, None, None) == -1
+    assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 127, fake, fake, 0, fake, 64, fake, fake, None, None) == -2
+    assert L.mb_tree_rope(fake, 0, 1, 65, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, None, None) == -2
+    assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 128, fake, fake, 0, ctypes.c_void_p(0x10004), 64, fake, fake, None,
+                          None) == -5
+    st = (ctypes.c_int64 * 8)(*([128] * 8))
+
+    def evict(k=fake, so=other, po=other, lens_out=other, budget=32, recent=8, sinks=4, ws=fake, nbytes=1 << 30,
+              Lmax=64):
+        return L.mb_cache_evict(k, fake, st, fake, fake, so, po, fake, fake, lens_out, 1, 1, 2, Lmax, 128, budget,
+                                recent, sinks, ws, nbytes, None)
+    assert evict(k=None) == -1
+    assert evict(budget=0) == -2 and evict(recent=-1) == -2 and evict(sinks=-1) == -2
+    assert evict(budget=11) == -2  # cannot hold the recent rows and the sinks
+    assert evict(lens_out=fake) == -2
+    assert evict(so=fake) == -2  # scores in place, positions not
+    assert evict(Lmax=0) == -2
+    assert evict(ws=None) == -3 and evict(nbytes=16) == -3
