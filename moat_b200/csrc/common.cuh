@@ -31,6 +31,12 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 bool encode_tmap_3d_u8(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides[2],
                        const uint32_t box[3]);
 
+// Encode a 4-D tiled tensor map of 16-bit elements with 128-byte swizzle (dims inner ->
+// outer, strides of dims 1 to 3 in bytes, box[0] = 64); what lies outside reads as zero.
+// Returns false if the driver rejects the parameters.
+bool encode_tmap_4d_u16(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
+                        const uint32_t box[4]);
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

@@ -68,6 +68,20 @@ bool encode_tmap_3d_u8(CUtensorMap* map, const void* base, const uint64_t dims[3
   return r == CUDA_SUCCESS;
 }
 
+bool encode_tmap_4d_u16(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
+                        const uint32_t box[4]) {
+  auto fn = get_encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  cuuint64_t st[3] = {strides[0], strides[1], strides[2]};
+  cuuint32_t b[4] = {box[0], box[1], box[2], box[3]};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), d, st, b, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 static inline int grid_for(int64_t work, int per_block) {
   int64_t b = (work + per_block - 1) / per_block;
   const int64_t cap = static_cast<int64_t>(sm_count()) * 32;

@@ -19,7 +19,9 @@
 namespace mb {
 
 // ---------------------------------------------------------------------------
-// Any shape, stride and alignment: one CTA per (trace, node, head), fp32 online softmax.
+// What the tensor-core path (tree_mma.cu) does not take: head dims above 128 or no multiple of
+// 8, strides or addresses off 16 bytes, broadcast axes, groups of more than 128 heads. One CTA
+// per (trace, node, head), fp32 online softmax.
 // ---------------------------------------------------------------------------
 constexpr int kAnyBlock = 128;
 constexpr int kMaxHeadDim = 256;
@@ -282,14 +284,15 @@ extern "C" {
 
 size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d) {
   if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim) return 0;
-  return (static_cast<size_t>(T) * H * m * 4 + 255) / 256 * 256;  // lse
+  return std::max((static_cast<size_t>(T) * H * m * 4 + 255) / 256 * 256,  // lse of the general path
+                  tree_mma_workspace(T, m, H, Hkv, Lmax, d));
 }
 
 int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
                      const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* masks, int32_t shared_masks,
                      uint16_t* out, const int64_t* strides, int32_t is_bf16, int32_t T, int32_t m, int32_t H,
                      int32_t Hkv, int32_t Lmax, int32_t d, float scale, const float* scores, float* scores_out,
-                     float* draft_scores, void* workspace, size_t workspace_bytes, void* stream) {
+                     float* draft_scores, void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
   if (!q || !lens || !k_draft || !v_draft || !masks || !out || !strides) return MB_ERR_NULL;
   if (Lmax > 0 && (!k_cache || !v_cache)) return MB_ERR_NULL;
   if ((scores_out != nullptr) != (draft_scores != nullptr) || (scores && !scores_out)) return MB_ERR_NULL;
@@ -332,6 +335,9 @@ int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t*
   a.scores = scores;
   a.scores_out = scores_out;
   a.draft_scores = draft_scores;
+  a.err = dev_err;
+  if (tree_mma_workspace(T, m, H, Hkv, Lmax, d) && tree_mma_takes(a))
+    return tree_mma_launch(a, is_bf16 != 0, workspace, stream);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* lse = scores_out ? static_cast<float*>(workspace) : nullptr;
   int rc = launch_with_pdl(is_bf16 ? k_tree_attn_any<true> : k_tree_attn_any<false>, dim3(T * m * H), dim3(kAnyBlock),

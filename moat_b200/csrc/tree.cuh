@@ -1,6 +1,7 @@
-// Arguments of the tree attention kernels (tree.cu).
+// Arguments and host entry points of the tree attention kernels (tree.cu, tree_mma.cu).
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
 
 namespace mb {
@@ -18,6 +19,13 @@ struct TreeAttnArgs {
   const float* scores;  // [T, Hkv, Lmax] or null
   float* scores_out;    // [T, Hkv, Lmax] or null
   float* draft_scores;  // [T, Hkv, m] or null
+  uint32_t* err;        // optional device error word
 };
+
+// Tensor-core path. 0 bytes: the sizes are not among those it takes.
+size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d);
+// Whether pointers and strides suit its tensor maps.
+bool tree_mma_takes(const TreeAttnArgs& a);
+int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream);
 
 }  // namespace mb

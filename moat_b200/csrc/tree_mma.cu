@@ -1,0 +1,1090 @@
+// Tree attention on the fifth-generation tensor cores (sm_100a).
+//
+// Rows and keys. The queries that read one KV head, nodes x heads of its group, form R <= 128
+// rows (more are cut into row blocks). Keys come in tiles of 128 rows. The score product is
+// taken transposed,
+//   S^T[128 keys, R] = K_tile[128, d] Q^T[d, R],     O^T[d, R] += V_tile^T[d, 128] P^T[128, R],
+// so the 128 TMEM lanes are keys and d, never the few queries: a tile costs tensor time in
+// proportion to R (N of the instruction, in steps of 16), each thread holds one key, and the
+// exponentials of a tile are spread over all threads whatever R is. V needs no transposition:
+// its rows, as TMA brings them, are the M-major operand; P^T is written as the N-major one.
+//
+// Softmax. A running maximum per row would need a reduction across the key lanes for every
+// tile. Instead a row keeps a reference m_ref and p = 2^(x - m_ref) may grow to 2^8 (harmless
+// for the rounding of p: the precision is relative); only when some x exceeds m_ref + 8 (one
+// vote per tile) are the maxima taken, m_ref raised and O^T and the sums rescaled. Sums are
+// fp32 per thread (key lane), joined once per segment.
+//
+// Work. The tiles of all (trace, KV head, row block) units, from the device lengths, form one
+// sequence that is cut evenly among the CTAs (one per SM): unequal lengths, one long trace and
+// many short ones all fill the GPU. A unit inside one CTA is written directly; the pieces of a
+// unit cut between CTAs leave (m_ref, sum, O) in the workspace and k_tree_join adds them in
+// order. No atomics: results repeat bit for bit.
+//
+// Each CTA: 4 or 8 softmax warps, a TMA warp that streams K and V tiles through a ring, an MMA
+// warp one score product ahead of the softmax. Every wait is bounded; a wait that gives up
+// sets MB_DEVERR_TIMEOUT and the CTA runs through without waiting.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "tree.cuh"
+
+namespace mb {
+
+constexpr int kTile = 128;      // keys per tile
+constexpr int kBox = 64;        // rows per TMA box: a last tile loads no more boxes than it needs
+constexpr int kMaxRows = 128;   // rows of a block
+constexpr int kMaxTraces = 255;  // per launch (the prefix of tile counts lies in shared memory)
+constexpr int kPanel = kTile * 128;  // bytes of a 64-column panel of a tile (128-byte swizzled rows)
+constexpr float kNoRef = -1e30f;     // m_ref before any visible key
+constexpr float kSlack = 8.0f;       // p may reach 2^kSlack
+
+struct TreeMmaParams {
+  TreeAttnArgs a;
+  CUtensorMap mq, mk, mv, mkd, mvd;
+  float* part;  // [2 * grid][rows][DP] unnormalised O of a unit's pieces
+  float* ml;    // [2 * grid][2][kMaxRows] their m_ref and sum
+  float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
+  int t0, T;    // traces of this launch
+  int RB, mb, G, n16, grid, nst, nq;
+};
+
+// --- tcgen05 / TMEM -----------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 16 consecutive TMEM columns of this warp's lanes
+__device__ __forceinline__ void tc_ld16(uint32_t addr, float* r) {
+  uint32_t u[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __uint_as_float(u[i]);
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const float* r) {
+  uint32_t u[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(r[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
+
+// Shared-memory operand with 128-byte swizzle. K-major: rows of 64 elements, 8-row groups
+// 1024 bytes apart (lbo unused). MN-major: 64 elements of M or N per 128-byte line, lines
+// along K, 8-line groups 1024 bytes apart, the next 64 elements of M or N lbo bytes on.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
+  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16, fp32 accumulator, M = 128; a_mn / b_mn: operand is M- / N-major
+__device__ __forceinline__ uint32_t instr_desc(bool bf16, int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Largest value over the warp (NaN ignored, as fmaxf does).
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// CTA-wide "any" over the softmax warps.
+__device__ __forceinline__ bool vote_any(bool v, int threads) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(v ? 1u : 0u), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
+// A wait that can give up: the thread notes it and stops waiting for anything.
+__device__ __forceinline__ void guarded_wait(uint64_t* bar, uint32_t parity, bool& dead, uint32_t* err) {
+  if (dead) return;
+  if (!mbar_wait(bar, parity)) {
+    dead = true;
+    if (err) atomicOr(err, MB_DEVERR_TIMEOUT);
+  }
+}
+
+// Column sums over the 32 lanes: v[0..31] of every lane in, the sum of column `lane` out.
+__device__ __forceinline__ float column_sums32(float* v, int lane) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float give = up ? v[i] : v[i + o];
+      const float keep = up ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  return v[0];
+}
+
+// --- the sequence of tiles ------------------------------------------------------
+// Tiles of trace t per unit: its committed rows, then one tile of drafted rows.
+__device__ __forceinline__ int trace_len(const TreeAttnArgs& a, int t) { return max(0, min(a.lens[t], a.Lmax)); }
+__device__ __forceinline__ int trace_tiles(int len) { return (len + kTile - 1) / kTile + 1; }
+
+// First tile of CTA c of g when w tiles are cut evenly.
+__device__ __forceinline__ int cut(int64_t w, int c, int g) { return static_cast<int>(w * c / g); }
+
+struct Segment {  // a run of tiles of one unit
+  int t, kvh, rb, len, nt, j0, n;
+};
+
+// The segment that begins at flat tile f (at most up to `end`); cum[t] = tiles before trace t,
+// RB row blocks per (trace, KV head).
+__device__ __forceinline__ Segment segment_at(const TreeMmaParams& p, const int* cum, int f, int end, int RB) {
+  int lo = 0, hi = p.T - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cum[mid] <= f)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  Segment s;
+  s.t = p.t0 + lo;
+  const int units = p.a.Hkv * RB;
+  s.nt = (cum[lo + 1] - cum[lo]) / units;
+  const int rem = f - cum[lo], u = rem / s.nt;
+  s.j0 = rem - u * s.nt;
+  s.kvh = u / RB;
+  s.rb = u - s.kvh * RB;
+  s.n = min(s.nt - s.j0, end - f);
+  s.len = 0;
+  return s;
+}
+
+// Valid rows of tile j of a unit (its last tile holds the drafted rows).
+__device__ __forceinline__ int tile_rows(int len, int nt, int m, int j) {
+  return j == nt - 1 ? m : min(kTile, len - j * kTile);
+}
+
+// Fills cum[0..T] (warp 0) for `units` units per trace.
+__device__ __forceinline__ void prefix_tiles(const TreeMmaParams& p, int* cum, int lane, int units) {
+  int base = 0;
+  for (int c = 0; c < p.T; c += 32) {
+    const int t = c + lane;
+    int v = t < p.T ? trace_tiles(trace_len(p.a, p.t0 + t)) * units : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (t < p.T) cum[t + 1] = base + v;
+    base += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) cum[0] = 0;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t round16(float x) {
+  return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+}
+
+// Shared memory: ring | Q slots | P | barriers and small tables.
+struct TreeSmem {
+  uint32_t ring, q, p, stage, qslot;  // byte offsets, bytes per stage / slot
+  uint32_t misc, total;
+};
+constexpr int kMaxStages = 8;
+constexpr uint32_t kMiscBars = 256;                          // barriers, TMEM base
+constexpr uint32_t kMiscRef = kMiscBars;                     // m_ref [128]
+constexpr uint32_t kMiscMask = kMiscRef + kMaxRows * 4;      // draft masks by row [128]
+constexpr uint32_t kMiscCum = kMiscMask + kMaxRows * 8;      // [kMaxTraces + 1]
+constexpr uint32_t kMiscBytes = kMiscCum + (kMaxTraces + 1) * 4;
+
+__host__ __device__ inline TreeSmem tree_smem(int panels, int n16, int nst, int nq) {
+  TreeSmem s;
+  s.stage = panels * kPanel;
+  s.qslot = panels * n16 * 128;
+  s.ring = 0;
+  s.q = s.ring + nst * s.stage;
+  s.p = s.q + nq * s.qslot;
+  s.misc = s.p + (n16 > 64 ? 2 : 1) * kPanel;
+  s.total = s.misc + kMiscBytes;
+  return s;
+}
+
+// PANELS: 64-column panels of the head dim (1: d <= 64, 2: d <= 128). CW: rows per softmax
+// warpgroup, WG warpgroups.
+template <int PANELS, int CW, int WG, bool BF16>
+__global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_constant__ TreeMmaParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int DP = PANELS * 64;
+  constexpr int kSoft = 128 * WG;
+  const TreeSmem lay = tree_smem(PANELS, p.n16, p.nst, p.nq);
+  uint8_t* misc = smem + lay.misc;
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(misc);  // [kMaxStages]
+  uint64_t* kv_empty = kv_full + kMaxStages;              // [kMaxStages]
+  uint64_t* s_full = kv_empty + kMaxStages;               // [2]
+  uint64_t* s_empty = s_full + 2;                         // [2]
+  uint64_t* q_full = s_empty + 2;                         // [2]
+  uint64_t* q_empty = q_full + 2;                         // [2]
+  uint64_t* o_empty = q_empty + 2;                        // [2]
+  uint64_t* p_full = o_empty + 2;
+  uint64_t* pv_done = p_full + 1;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 1);
+  float* ref = reinterpret_cast<float*>(misc + kMiscRef);
+  uint64_t* rowmask = reinterpret_cast<uint64_t*>(misc + kMiscMask);
+  int* cum = reinterpret_cast<int*>(misc + kMiscCum);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const TreeAttnArgs& a = p.a;
+  const int R = p.mb * p.G;
+  bool dead = false;
+
+  if (warp == 4 * WG) {  // TMA warp
+    if (lane == 0) {
+      for (int i = 0; i < kMaxStages; ++i) {
+        mbar_init(kv_full + i, 1);
+        mbar_init(kv_empty + i, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full + i, 1);
+        mbar_init(s_empty + i, kSoft);
+        mbar_init(q_full + i, 1);
+        mbar_init(q_empty + i, 1);
+        mbar_init(o_empty + i, kSoft);
+      }
+      mbar_init(p_full, kSoft);
+      mbar_init(pv_done, 1);
+      fence_mbar_init();
+    }
+  } else if (warp == 4 * WG + 1) {
+    tmem_alloc(smem_u32(tmem_base), 512);
+  } else {
+    // rows beyond R of the Q slots stay zero (the boxes never write them)
+    uint4* qz = reinterpret_cast<uint4*>(smem + lay.q);
+    for (uint32_t i = tid; i < p.nq * lay.qslot / 16; i += kSoft) qz[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+    for (int i = tid; i < kMaxRows; i += kSoft) ref[i] = kNoRef;
+  }
+  pdl_wait();  // the lengths, masks, queries and drafts may come from the kernel before
+  pdl_launch_dependents();
+  if (warp == 0) prefix_tiles(p, cum, lane, a.Hkv * p.RB);
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  const uint32_t tmem = *tmem_base;
+  const int total = cum[p.T];
+  const int g = min(p.grid, total);  // CTAs with work
+  const int c = blockIdx.x;
+  const int beg = c < g ? cut(total, c, g) : 0, end = c < g ? cut(total, c + 1, g) : 0;
+  const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q), pbase = smem_u32(smem + lay.p);
+
+  if (warp == 4 * WG) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0) {
+      // a cache that is read once streams past what L2 should keep; several row blocks or the
+      // weight pass read it again
+      uint64_t policy;
+      if (p.RB == 1 && !p.lse)
+        policy = policy_evict_first();
+      else
+        asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+      const uint64_t keep = policy_evict_last();
+      int item = 0, seg = 0;  // K and V tiles of the ring, segments
+      for (int f = beg; f < end; ++seg) {
+        const Segment s = segment_at(p, cum, f, end, p.RB);
+        const int len = trace_len(a, s.t);
+        const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+        if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
+        mbar_expect_tx(q_full + qs, PANELS * R * 128);
+        for (int pn = 0; pn < PANELS; ++pn)
+          tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G,
+                      s.rb * p.mb, s.t, keep);
+        for (int j = s.j0; j < s.j0 + s.n; ++j) {
+          const bool draft = j == s.nt - 1;
+          const int boxes = draft ? 0 : (tile_rows(len, s.nt, a.m, j) + kBox - 1) / kBox;
+          for (int kv = 0; kv < 2; ++kv, ++item) {
+            const int st = item % p.nst, use = item / p.nst;
+            if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
+            const uint32_t dst = ring + st * lay.stage;
+            mbar_expect_tx(kv_full + st, PANELS * 128 * (draft ? a.m : boxes * kBox));
+            for (int pn = 0; pn < PANELS; ++pn) {
+              if (draft)
+                tma_load_4d(dst + pn * kPanel, kv ? &p.mvd : &p.mkd, kv_full + st, pn * 64, s.kvh, 0, s.t, keep);
+              else
+                for (int b = 0; b < boxes; ++b)
+                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, kv ? &p.mv : &p.mk, kv_full + st, pn * 64,
+                              j * kTile + b * kBox, s.kvh, s.t, policy);
+            }
+          }
+        }
+        f += s.n;
+      }
+      if (dead)  // copies still in flight must land before this CTA's shared memory goes
+        for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 4 * WG + 1) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0) {
+      const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
+      const uint32_t id_pv = instr_desc(BF16, p.n16, true, true);
+      const int n = end - beg;
+      // two cursors over the same tiles: scores run one tile ahead of the value product
+      Segment sq = {}, sv = {};
+      int jq = 0, jv = 0, nq = 0, nv = 0, seg_q = -1, seg_v = -1, len_v = 0;
+      for (int k = 0; k <= n; ++k) {
+        if (k < n) {
+          if (jq == nq) {
+            sq = segment_at(p, cum, beg + k, end, p.RB);
+            jq = 0;
+            nq = sq.n;
+            ++seg_q;
+          }
+          const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
+          if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
+          const int st = (2 * k) % p.nst, use = (2 * k) / p.nst;
+          guarded_wait(kv_full + st, use & 1, dead, a.err);
+          if (k >= 2) guarded_wait(s_empty + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
+          tc_after_sync();
+          const uint32_t ka = ring + st * lay.stage, qb = qbase + qs * lay.qslot;
+#pragma unroll
+          for (int kk = 0; kk < PANELS * 4; ++kk)
+            tc_mma(tmem + (k & 1) * kMaxRows, smem_desc(ka + (kk >> 2) * kPanel + (kk & 3) * 32, 16),
+                   smem_desc(qb + (kk >> 2) * p.n16 * 128 + (kk & 3) * 32, 16), id_qk, kk > 0);
+          tc_commit(s_full + (k & 1));
+          tc_commit(kv_empty + st);
+          if (++jq == nq) tc_commit(q_empty + qs);
+        }
+        if (k > 0) {
+          const int e = k - 1;
+          if (jv == nv) {
+            sv = segment_at(p, cum, beg + e, end, p.RB);
+            jv = 0;
+            nv = sv.n;
+            len_v = trace_len(a, sv.t);
+            ++seg_v;
+          }
+          const int st = (2 * e + 1) % p.nst, use = (2 * e + 1) / p.nst;
+          guarded_wait(kv_full + st, use & 1, dead, a.err);
+          guarded_wait(p_full, e & 1, dead, a.err);
+          if (jv == 0 && seg_v >= 2) guarded_wait(o_empty + (seg_v & 1), ((seg_v >> 1) - 1) & 1, dead, a.err);
+          tc_after_sync();
+          const uint32_t va = ring + st * lay.stage;
+          const int steps = (tile_rows(len_v, sv.nt, a.m, sv.j0 + jv) + 15) / 16;
+          for (int kk = 0; kk < steps; ++kk)
+            tc_mma(tmem + (2 + (seg_v & 1)) * kMaxRows, smem_desc(va + kk * 2048, kPanel),
+                   smem_desc(pbase + kk * 2048, kPanel), id_pv, jv > 0 || kk > 0);
+          tc_commit(kv_empty + st);
+          tc_commit(pv_done);
+          ++jv;
+        }
+      }
+      if (dead && n > 0) {  // products still in flight must end before TMEM is freed
+        tc_commit(pv_done);
+        const long long t0 = clock64();
+        while (clock64() - t0 < 1000000) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int grp = warp >> 2, wq = warp & 3;
+    const int key = wq * 32 + lane;  // this thread's key of a tile, and its d of O^T
+    const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+    const int col0 = grp * CW;
+    const float sc = a.scale_log2;
+    float l[CW];
+#pragma unroll
+    for (int i = 0; i < CW; ++i) l[i] = 0.0f;
+    float* scratch = reinterpret_cast<float*>(smem + lay.p);  // P's space, while no product reads it
+    int seg = 0, k = 0;
+    for (int f = beg; f < end; ++seg) {
+      const Segment s = segment_at(p, cum, f, end, p.RB);
+      const int len = trace_len(a, s.t);
+      for (int jj = 0; jj < s.n; ++jj, ++k) {
+        const int j = s.j0 + jj;
+        const bool draft = j == s.nt - 1;
+        const int rows = tile_rows(len, s.nt, a.m, j);
+        const uint32_t sbuf = tmem + lanes + (k & 1) * kMaxRows + col0;
+        const int vst = (2 * k + 1) % p.nst, vuse = (2 * k + 1) / p.nst;
+        uint64_t used = ~0ull;  // drafted rows that some node sees
+        if (draft) {
+          const uint64_t* mk = a.masks + s.t * a.mask_stride;
+          uint64_t u = 0;
+          for (int i = lane; i < a.m; i += 32) u |= mk[i];
+#pragma unroll
+          for (int o = 16; o; o >>= 1) u |= __shfl_xor_sync(0xffffffffu, u, o);
+          used = u;
+          for (int r = tid; r < kMaxRows; r += kSoft) {
+            const int i = s.rb * p.mb + r / p.G;
+            rowmask[r] = r < R && i < a.m ? mk[i] : 0;
+          }
+          named_bar_sync(1, kSoft);
+        }
+        guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
+        tc_after_sync();
+        float x[CW];
+#pragma unroll
+        for (int i = 0; i < CW; i += 16) {
+          if (col0 + i < p.n16) {
+            tc_ld16(sbuf + i, x + i);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) x[i + u] = 0.0f;
+          }
+        }
+        tc_wait_ld();
+        tc_before_sync();
+        mbar_arrive(s_empty + (k & 1));
+        if (draft) {
+#pragma unroll
+          for (int i = 0; i < CW; ++i) {
+            const bool see = key < rows && (rowmask[col0 + i] >> (key & 63)) & 1;
+            x[i] = see ? x[i] * sc : -INFINITY;
+          }
+        } else if (key < rows) {
+#pragma unroll
+          for (int i = 0; i < CW; ++i) x[i] *= sc;
+        } else {
+#pragma unroll
+          for (int i = 0; i < CW; ++i) x[i] = -INFINITY;
+        }
+        bool over = false;
+#pragma unroll
+        for (int i = 0; i < CW; ++i) over |= x[i] > ref[col0 + i] + kSlack;
+        over = vote_any(over, kSoft);
+        // P and, for a new maximum, O are free once the previous value product has finished
+        if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
+        if (over) {
+          float mine[(CW + 31) / 32];
+#pragma unroll
+          for (int i = 0; i < CW; ++i) {
+            const float mx = warp_max(x[i]);
+            if ((i & 31) == lane) mine[i / 32] = mx;
+          }
+#pragma unroll
+          for (int u = 0; u < (CW + 31) / 32; ++u)
+            if (u * 32 + lane < CW) scratch[wq * kMaxRows + col0 + u * 32 + lane] = mine[u];
+          named_bar_sync(1, kSoft);
+          if (tid < CW * WG) {
+            const float old = ref[tid];
+            float mx = old;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, scratch[w * kMaxRows + tid]);
+            ref[tid] = mx;
+            scratch[4 * kMaxRows + tid] = ex2(old - mx);
+          }
+          named_bar_sync(1, kSoft);
+          const float* fade = scratch + 4 * kMaxRows + col0;
+#pragma unroll
+          for (int i = 0; i < CW; ++i) l[i] *= fade[i];
+          if (jj > 0) {
+            tc_after_sync();
+            const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
+#pragma unroll
+            for (int i = 0; i < CW; i += 16) {
+              float o[16];
+              tc_ld16(ob + i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int u = 0; u < 16; ++u) o[u] *= fade[i + u];
+              tc_st16(ob + i, o);
+            }
+            tc_wait_st();
+          }
+          named_bar_sync(1, kSoft);  // scratch read: its space becomes P again
+        }
+        // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
+#pragma unroll
+        for (int i = 0; i < CW; i += 8) {
+          float e[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            e[u] = ex2(x[i + u] - ref[col0 + i + u]);
+            l[i + u] += e[u];
+          }
+          uint4 w;
+          w.x = pack2<BF16>(e[0], e[1]);
+          w.y = pack2<BF16>(e[2], e[3]);
+          w.z = pack2<BF16>(e[4], e[5]);
+          w.w = pack2<BF16>(e[6], e[7]);
+          const int n = col0 + i;
+          if (n < p.n16)
+            *reinterpret_cast<uint4*>(smem + lay.p + (n >> 6) * kPanel + key * 128 +
+                                      ((((n & 63) >> 3) ^ (key & 7)) << 4)) = w;
+        }
+        // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
+        // product's last 16-row step reads beyond the valid rows, and unused drafted rows
+        if (grp == 0 && (rows & 15 || draft)) {
+          const bool clear = key >= rows ? key < ((rows + 15) & ~15) : draft && !((used >> (key & 63)) & 1);
+          if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
+          if (clear) {
+            for (int pn = 0; pn < PANELS; ++pn)
+              for (int u = 0; u < 8; ++u)
+                *reinterpret_cast<uint4*>(smem + lay.ring + vst * lay.stage + pn * kPanel + key * 128 + u * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_before_sync();
+        mbar_arrive(p_full);
+      }
+      // ------------------------------------------------ end of the segment: sums, output
+      guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
+      tc_after_sync();
+#pragma unroll
+      for (int i = 0; i < CW; i += 32) {
+        float v[32];
+#pragma unroll
+        for (int u = 0; u < 32; ++u) v[u] = i + u < CW ? l[i + u < CW ? i + u : 0] : 0.0f;
+        const float sum = column_sums32(v, lane);
+        if (i + lane < CW) scratch[wq * kMaxRows + col0 + i + lane] = sum;
+      }
+      named_bar_sync(1, kSoft);
+      const bool whole = s.n == s.nt;
+      const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
+      if (tid < CW * WG) {
+        const float sum = scratch[tid] + scratch[kMaxRows + tid] + scratch[2 * kMaxRows + tid] +
+                          scratch[3 * kMaxRows + tid];
+        const int i = s.rb * p.mb + tid / p.G;
+        const bool real = tid < R && i < a.m && a.masks[s.t * a.mask_stride + i] != 0;
+        float* ml = p.ml + static_cast<int64_t>(slot) * 2 * kMaxRows;
+        if (!whole) {
+          ml[tid] = ref[tid];
+          ml[kMaxRows + tid] = real ? sum : 0.0f;
+        } else if (p.lse && tid < kMaxRows) {
+          const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
+          p.lse[unit * kMaxRows + tid] = real && sum != 0.0f ? ref[tid] + log2f(sum) : INFINITY;
+        }
+        scratch[4 * kMaxRows + tid] = real && sum != 0.0f ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
+        ref[tid] = kNoRef;
+      }
+      named_bar_sync(1, kSoft);
+      const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
+      const int i0 = s.rb * p.mb;
+#pragma unroll
+      for (int i = 0; i < CW; i += 16) {
+        if (col0 + i >= p.n16) break;
+        float o[16];
+        tc_ld16(ob + i, o);
+        tc_wait_ld();
+        if (whole) {
+          if (key < a.d) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+              const int n = col0 + i + u, node = i0 + n / p.G;
+              const float inv = scratch[4 * kMaxRows + n];
+              if (n < R && node < a.m)
+                a.out[s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + n % p.G) * a.os[2] + key] =
+                    round16<BF16>(inv == 0.0f ? 0.0f : o[u] * inv);
+            }
+          }
+        } else if (key < DP) {
+          float* dst = p.part + (static_cast<int64_t>(slot) * R + col0 + i) * DP + key;
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+            if (col0 + i + u < R) dst[u * DP] = o[u];
+        }
+      }
+      tc_before_sync();
+      mbar_arrive(o_empty + (seg & 1));
+#pragma unroll
+      for (int i = 0; i < CW; ++i) l[i] = 0.0f;
+      named_bar_sync(1, kSoft);  // scratch read, m_ref reset
+      f += s.n;
+    }
+  }
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 4 * WG + 1) tmem_dealloc(tmem, 512);
+}
+
+// Joins the pieces of the units that were cut between CTAs, in order. One CTA per unit and
+// group of 8 rows; a unit that one CTA held is done already.
+constexpr int kJoinBlock = 256;
+constexpr int kJoinRows = 8;
+
+template <int PANELS, bool BF16>
+__global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant__ TreeMmaParams p) {
+  constexpr int DP = PANELS * 64;
+  __shared__ int red[2][kJoinBlock / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const TreeAttnArgs& a = p.a;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int units = a.Hkv * p.RB;
+  const int t = blockIdx.x / units, u = blockIdx.x - t * units;  // trace of this launch
+  int before = 0, total = 0;
+  for (int i = tid; i < p.T; i += kJoinBlock) {
+    const int n = trace_tiles(trace_len(a, p.t0 + i)) * units;
+    total += n;
+    before += i < t ? n : 0;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) {
+    red[0][warp] = total;
+    red[1][warp] = before;
+  }
+  __syncthreads();
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinBlock / 32; ++w) {
+    total += red[0][w];
+    before += red[1][w];
+  }
+  const int nt = trace_tiles(trace_len(a, p.t0 + t));
+  const int f0 = before + u * nt, f1 = f0 + nt - 1;
+  const int g = min(p.grid, total);
+  // the CTA that holds tile f: the largest c with cut(c) <= f
+  const int c0 = static_cast<int>(((static_cast<int64_t>(f0) + 1) * g - 1) / total);
+  const int c1 = static_cast<int>(((static_cast<int64_t>(f1) + 1) * g - 1) / total);
+  if (c0 == c1) return;
+  const int R = p.mb * p.G;
+  const int kvh = u / p.RB, rb = u - kvh * p.RB;
+  constexpr int kLanes = DP / 4;  // threads of a row, four values each
+  for (int rr = tid / kLanes; rr < kJoinRows; rr += kJoinBlock / kLanes) {
+    const int n = blockIdx.y * kJoinRows + rr, v = (tid % kLanes) * 4;
+    const int node = rb * p.mb + n / p.G;
+    if (n >= R || node >= a.m) continue;
+    float top = kNoRef;
+    for (int c = c0; c <= c1; ++c)
+      top = fmaxf(top, p.ml[static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * 2 * kMaxRows + n]);
+    float sum = 0.0f, o[4] = {};
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
+      const float w = ex2(p.ml[slot * 2 * kMaxRows + n] - top);
+      const float4 x = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
+      sum = fmaf(w, p.ml[(slot * 2 + 1) * kMaxRows + n], sum);
+      o[0] = fmaf(w, x.x, o[0]);
+      o[1] = fmaf(w, x.y, o[1]);
+      o[2] = fmaf(w, x.z, o[2]);
+      o[3] = fmaf(w, x.w, o[3]);
+    }
+    const int tr = p.t0 + t;
+    const bool real = a.masks[tr * a.mask_stride + node] != 0 && sum != 0.0f;
+    const float inv = real ? 1.0f / sum : 0.0f;
+    uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (v + i < a.d) out[v + i] = round16<BF16>(real ? o[i] * inv : 0.0f);
+    if (p.lse && v == 0)
+      p.lse[((static_cast<int64_t>(tr) * a.Hkv + kvh) * p.RB + rb) * kMaxRows + n] =
+          real ? top + log2f(sum) : INFINITY;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention weight of every row, summed over the nodes and heads that read it:
+//   w_l = sum_rows 2^(x_l - lse_row),  x = scale log2(e) q . k.
+// The row maxima are known only when all keys have been seen, so the scores are formed again
+// (K once more through the same ring and product; V is not needed) and a thread, which holds
+// one key, adds over the rows of its lane: no exchange between threads. Row blocks follow one
+// another within a CTA, and a row's sum is always kept by the same thread.
+// ---------------------------------------------------------------------------
+constexpr int kWeightThreads = 256 + 64;
+
+template <int PANELS, bool BF16>
+__global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid_constant__ TreeMmaParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int kSoft = 256;  // two warpgroups take alternate tiles
+  const TreeSmem lay = tree_smem(PANELS, p.n16, p.nst, p.nq);
+  uint8_t* misc = smem + lay.misc;
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(misc);
+  uint64_t* kv_empty = kv_full + kMaxStages;
+  uint64_t* s_full = kv_empty + kMaxStages;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* q_full = s_empty + 2;
+  uint64_t* q_empty = q_full + 2;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(q_empty + 2);
+  int* cum = reinterpret_cast<int*>(misc + kMiscCum);
+  // the space of P: per warpgroup the rows' lse and draft masks
+  float* lse_s = reinterpret_cast<float*>(smem + lay.p);
+  uint64_t* mask_s = reinterpret_cast<uint64_t*>(smem + lay.p + 2 * kMaxRows * 4);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const TreeAttnArgs& a = p.a;
+  const int R = p.mb * p.G;
+  bool dead = false;
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int i = 0; i < kMaxStages; ++i) {
+        mbar_init(kv_full + i, 1);
+        mbar_init(kv_empty + i, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full + i, 1);
+        mbar_init(s_empty + i, 128);
+        mbar_init(q_full + i, 1);
+        mbar_init(q_empty + i, 1);
+      }
+      fence_mbar_init();
+    }
+  } else if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_base), 256);
+  } else {
+    uint4* qz = reinterpret_cast<uint4*>(smem + lay.q);
+    for (uint32_t i = tid; i < p.nq * lay.qslot / 16; i += kSoft) qz[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  // units are (trace, KV head) here: the sequence has no row blocks
+  if (warp == 0) prefix_tiles(p, cum, lane, a.Hkv);
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  const uint32_t tmem = *tmem_base;
+  const int total = cum[p.T];
+  const int g = min(p.grid, total);
+  const int c = blockIdx.x;
+  const int beg = c < g ? cut(total, c, g) : 0, end = c < g ? cut(total, c + 1, g) : 0;
+  const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q);
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const uint64_t policy = policy_evict_first(), keep = policy_evict_last();
+      int item = 0, seg = 0;
+      for (int f = beg; f < end;) {
+        const Segment s = segment_at(p, cum, f, end, 1);
+        const int len = trace_len(a, s.t);
+        for (int rb = 0; rb < p.RB; ++rb, ++seg) {
+          const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+          if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
+          mbar_expect_tx(q_full + qs, PANELS * R * 128);
+          for (int pn = 0; pn < PANELS; ++pn)
+            tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G, rb * p.mb,
+                        s.t, keep);
+          for (int j = s.j0; j < s.j0 + s.n; ++j, ++item) {
+            const bool draft = j == s.nt - 1;
+            const int boxes = draft ? 0 : (tile_rows(len, s.nt, a.m, j) + kBox - 1) / kBox;
+            const int st = item % p.nst, use = item / p.nst;
+            if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
+            const uint32_t dst = ring + st * lay.stage;
+            mbar_expect_tx(kv_full + st, PANELS * 128 * (draft ? a.m : boxes * kBox));
+            for (int pn = 0; pn < PANELS; ++pn) {
+              if (draft)
+                tma_load_4d(dst + pn * kPanel, &p.mkd, kv_full + st, pn * 64, s.kvh, 0, s.t, keep);
+              else
+                for (int b = 0; b < boxes; ++b)
+                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, &p.mk, kv_full + st, pn * 64, j * kTile + b * kBox,
+                              s.kvh, s.t, rb + 1 < p.RB ? keep : policy);
+            }
+          }
+        }
+        f += s.n;
+      }
+      if (dead)
+        for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
+      int k = 0, seg = 0;
+      for (int f = beg; f < end;) {
+        const Segment s = segment_at(p, cum, f, end, 1);
+        for (int rb = 0; rb < p.RB; ++rb, ++seg) {
+          const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+          guarded_wait(q_full + qs, quse & 1, dead, a.err);
+          for (int jj = 0; jj < s.n; ++jj, ++k) {
+            const int st = k % p.nst, use = k / p.nst;
+            guarded_wait(kv_full + st, use & 1, dead, a.err);
+            if (k >= 2) guarded_wait(s_empty + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
+            tc_after_sync();
+            const uint32_t ka = ring + st * lay.stage, qb = qbase + qs * lay.qslot;
+#pragma unroll
+            for (int kk = 0; kk < PANELS * 4; ++kk)
+              tc_mma(tmem + (k & 1) * kMaxRows, smem_desc(ka + (kk >> 2) * kPanel + (kk & 3) * 32, 16),
+                     smem_desc(qb + (kk >> 2) * p.n16 * 128 + (kk & 3) * 32, 16), id_qk, kk > 0);
+            tc_commit(s_full + (k & 1));
+            tc_commit(kv_empty + st);
+          }
+          tc_commit(q_empty + qs);
+        }
+        f += s.n;
+      }
+      if (dead) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 1000000) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int grp = warp >> 2, wq = warp & 3;
+    const int key = wq * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+    const float sc = a.scale_log2;
+    float* lse = lse_s + grp * kMaxRows;
+    uint64_t* rowmask = mask_s + grp * kMaxRows;
+    int k = 0;
+    for (int f = beg; f < end;) {
+      const Segment s = segment_at(p, cum, f, end, 1);
+      const int len = trace_len(a, s.t);
+      const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
+      for (int rb = 0; rb < p.RB; ++rb) {
+        named_bar_sync(1 + grp, 128);  // the last block's tables read
+        const int i = rb * p.mb + key / p.G;
+        const bool node = key < R && i < a.m;  // the last block may hold fewer nodes
+        lse[key] = node ? p.lse[(unit * p.RB + rb) * kMaxRows + key] : INFINITY;
+        rowmask[key] = node ? a.masks[s.t * a.mask_stride + i] : 0;
+        named_bar_sync(1 + grp, 128);
+        for (int jj = 0; jj < s.n; ++jj, ++k) {
+          if ((jj & 1) != grp) continue;
+          const int j = s.j0 + jj;
+          const bool draft = j == s.nt - 1;
+          const int rows = tile_rows(len, s.nt, a.m, j);
+          guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
+          tc_after_sync();
+          const uint32_t sbuf = tmem + lanes + (k & 1) * kMaxRows;
+          float w = 0.0f;
+          for (int n = 0; n < p.n16; n += 16) {
+            float x[16];
+            tc_ld16(sbuf + n, x);
+            tc_wait_ld();
+            float part = 0.0f;
+            if (draft) {
+#pragma unroll
+              for (int u = 0; u < 16; ++u)
+                part += (rowmask[n + u] >> (key & 63)) & 1 ? ex2(fmaf(x[u], sc, -lse[n + u])) : 0.0f;
+            } else {
+#pragma unroll
+              for (int u = 0; u < 16; ++u) part += ex2(fmaf(x[u], sc, -lse[n + u]));
+            }
+            w += part;
+          }
+          tc_before_sync();
+          mbar_arrive(s_empty + (k & 1));
+          if (key < rows) {
+            float* dst = draft ? a.draft_scores + unit * a.m + key : a.scores_out + unit * a.Lmax + j * kTile + key;
+            const float base = rb > 0 ? *dst : draft || !a.scores ? 0.0f : a.scores[unit * a.Lmax + j * kTile + key];
+            *dst = base + w;
+          }
+        }
+      }
+      f += s.n;
+    }
+  }
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 9) tmem_dealloc(tmem, 256);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+struct TreePlan {
+  int G, RB, mb, n16, panels, nst, nq, grid;
+  uint32_t smem;
+};
+
+static bool tree_plan(int T, int m, int H, int Hkv, int Lmax, int d, TreePlan* pl) {
+  pl->G = H / Hkv;
+  if (pl->G > kMaxRows || d > 128 || d % 8 != 0) return false;
+  const int fit = kMaxRows / pl->G;  // nodes of a full block
+  pl->RB = (m + fit - 1) / fit;
+  pl->mb = (m + pl->RB - 1) / pl->RB;  // even blocks
+  pl->RB = (m + pl->mb - 1) / pl->mb;
+  pl->n16 = (pl->mb * pl->G + 15) / 16 * 16;
+  pl->panels = d > 64 ? 2 : 1;
+  pl->grid = sm_count();
+  // flat tile numbers are 32-bit
+  if (static_cast<int64_t>(std::min(T, kMaxTraces)) * Hkv * pl->RB * (Lmax / kTile + 2) > 0x7FFFFFFFll) return false;
+  // two Q slots (the next unit's queries load early) where they leave a ring of six stages
+  const uint32_t cap = 227 * 1024;
+  for (pl->nq = 2;; --pl->nq) {
+    const uint32_t fixed = tree_smem(pl->panels, pl->n16, 0, pl->nq).total;
+    pl->nst = std::min<int>(kMaxStages, (cap - fixed) / (pl->panels * kPanel));
+    if (pl->nst >= 5 || pl->nq == 1) break;
+  }
+  pl->smem = tree_smem(pl->panels, pl->n16, pl->nst, pl->nq).total;
+  return pl->nst >= 4;
+}
+
+size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d) {
+  TreePlan pl;
+  if (!tree_plan(T, m, H, Hkv, Lmax, d, &pl)) return 0;
+  const size_t part = static_cast<size_t>(2) * pl.grid * pl.mb * pl.G * pl.panels * 64 * 4;
+  const size_t ml = static_cast<size_t>(2) * pl.grid * 2 * kMaxRows * 4;
+  const size_t lse = static_cast<size_t>(T) * Hkv * pl.RB * kMaxRows * 4;
+  return part + ml + lse + 256;
+}
+
+bool tree_mma_takes(const TreeAttnArgs& a) {
+  // tensor maps: 16-byte bases, positive strides in multiples of 16 bytes below 2^40
+  const struct {
+    const void* p;
+    const int64_t* s;
+    int n[3];
+  } t[] = {{a.q, a.qs, {a.T, a.m, a.H}},         {a.k, a.ks, {a.T, a.Hkv, a.Lmax}}, {a.v, a.vs, {a.T, a.Hkv, a.Lmax}},
+           {a.kd, a.kds, {a.T, a.m, a.Hkv}}, {a.vd, a.vds, {a.T, a.m, a.Hkv}}};
+  for (const auto& x : t) {
+    if (!aligned(x.p, 16)) return false;
+    for (int u = 0; u < 3; ++u)
+      if (x.n[u] > 1 && (x.s[u] <= 0 || x.s[u] % 8 != 0 || x.s[u] >= (1ll << 38))) return false;
+  }
+  return true;
+}
+
+// Tensor map of 16-bit elements [n2][n1][n0][d], strides in elements, 64-column boxes.
+static bool tree_map(CUtensorMap* map, const void* base, int d, int n0, int64_t s0, int n1, int64_t s1, int n2,
+                     int64_t s2, int b0, int b1) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(n0), static_cast<uint64_t>(n1),
+                            static_cast<uint64_t>(n2)};
+  // the stride of an axis of length 1 is never used, but it is checked
+  const uint64_t strides[3] = {n0 > 1 ? s0 * 2ull : 256, n1 > 1 ? s1 * 2ull : 256, n2 > 1 ? s2 * 2ull : 256};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(b0), static_cast<uint32_t>(b1), 1};
+  return encode_tmap_4d_u16(map, base, dims, strides, box);
+}
+
+// Lets a kernel take all of an SM's shared memory (a host-side attribute of the function).
+template <typename Kern>
+static int allow_smem(Kern kern) {
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return MB_ERR_LAUNCH;
+  }
+  return MB_OK;
+}
+
+template <int PANELS, int CW, int WG, bool BF16>
+static int launch_attn(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
+  auto kern = k_tree_attn<PANELS, CW, WG, BF16>;
+  const int rc = allow_smem(kern);
+  return rc != MB_OK ? rc : launch_with_pdl(kern, dim3(p.grid), dim3(128 * WG + 64), smem, st, p);
+}
+
+template <int PANELS, bool BF16>
+static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
+  int rc;
+  if (p.n16 <= 16)
+    rc = launch_attn<PANELS, 16, 1, BF16>(p, smem, st);
+  else if (p.n16 <= 32)
+    rc = launch_attn<PANELS, 16, 2, BF16>(p, smem, st);
+  else if (p.n16 <= 64)
+    rc = launch_attn<PANELS, 32, 2, BF16>(p, smem, st);
+  else
+    rc = launch_attn<PANELS, 64, 2, BF16>(p, smem, st);
+  if (rc != MB_OK) return rc;
+  const int R = p.mb * p.G;
+  return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.T * p.a.Hkv * p.RB, (R + kJoinRows - 1) / kJoinRows),
+                         dim3(kJoinBlock), 0, st, p);
+}
+
+template <int PANELS, bool BF16>
+static int launch_weights(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
+  auto kern = k_tree_weights<PANELS, BF16>;
+  const int rc = allow_smem(kern);
+  return rc != MB_OK ? rc : launch_with_pdl(kern, dim3(p.grid), dim3(kWeightThreads), smem, st, p);
+}
+
+template <int PANELS, bool BF16>
+static int launch_all(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
+  const int rc = launch_rows<PANELS, BF16>(p, smem, st);
+  return rc != MB_OK || !p.lse ? rc : launch_weights<PANELS, BF16>(p, smem, st);
+}
+
+int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
+  TreePlan pl;
+  if (!tree_plan(a.T, a.m, a.H, a.Hkv, a.Lmax, a.d, &pl)) return MB_ERR_UNSUPPORTED;
+  TreeMmaParams p;
+  p.a = a;
+  const bool cache = a.Lmax > 0;  // without a cache its maps are never used
+  if (!tree_map(&p.mq, a.q, a.d, a.H, a.qs[2], a.m, a.qs[1], a.T, a.qs[0], pl.G, pl.mb) ||
+      !tree_map(&p.mkd, a.kd, a.d, a.Hkv, a.kds[2], a.m, a.kds[1], a.T, a.kds[0], 1, a.m) ||
+      !tree_map(&p.mvd, a.vd, a.d, a.Hkv, a.vds[2], a.m, a.vds[1], a.T, a.vds[0], 1, a.m) ||
+      !tree_map(&p.mk, cache ? a.k : a.kd, a.d, cache ? a.Lmax : 1, a.ks[2], a.Hkv, cache ? a.ks[1] : 128, a.T,
+                cache ? a.ks[0] : 128, kBox, 1) ||
+      !tree_map(&p.mv, cache ? a.v : a.vd, a.d, cache ? a.Lmax : 1, a.vs[2], a.Hkv, cache ? a.vs[1] : 128, a.T,
+                cache ? a.vs[0] : 128, kBox, 1))
+    return MB_ERR_LAUNCH;
+  p.G = pl.G;
+  p.RB = pl.RB;
+  p.mb = pl.mb;
+  p.n16 = pl.n16;
+  p.grid = pl.grid;
+  p.nst = pl.nst;
+  p.nq = pl.nq;
+  char* w = static_cast<char*>(ws);
+  p.part = reinterpret_cast<float*>(w);
+  w += static_cast<size_t>(2) * pl.grid * pl.mb * pl.G * pl.panels * 64 * 4;
+  p.ml = reinterpret_cast<float*>(w);
+  w += static_cast<size_t>(2) * pl.grid * 2 * kMaxRows * 4;
+  p.lse = a.scores_out ? reinterpret_cast<float*>(w) : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int t0 = 0; t0 < a.T; t0 += kMaxTraces) {
+    p.t0 = t0;
+    p.T = std::min(kMaxTraces, a.T - t0);
+    int rc;
+    if (pl.panels == 2)
+      rc = bf16 ? launch_all<2, true>(p, pl.smem, st) : launch_all<2, false>(p, pl.smem, st);
+    else
+      rc = bf16 ? launch_all<1, true>(p, pl.smem, st) : launch_all<1, false>(p, pl.smem, st);
+    if (rc != MB_OK) return rc;
+  }
+  return MB_OK;
+}
+
+}  // namespace mb

@@ -86,7 +86,7 @@ _Strides16 = ctypes.c_int64 * 16
 
 
 def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=None, out=None, scores=None,
-                   scores_out=None, draft_scores=None):
+                   scores_out=None, draft_scores=None, dev_err=None):
     """Attention of every node of every trace's tree.
 
     * ``q [T, m, H, d]``, ``k_cache`` / ``v_cache [T, Hkv, Lmax, d]`` (the first ``lens[t]``
@@ -100,6 +100,9 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
       weight summed over the nodes and the heads of its group. ``scores_out`` (default: in
       place) gets ``scores`` plus that sum in the first ``lens[t]`` rows and keeps the
       others; ``draft_scores`` float32 ``[T, Hkv, m]`` gets the sums of the draft's rows.
+
+    * ``dev_err``: optional int32 CUDA tensor whose first word receives device error bits
+      (bounded waits).
 
     fp32 scores, softmax and sums; one rounding at the output (and one of each unnormalised
     probability to the inputs' type before its product with V). Repeated calls give the same
@@ -156,6 +159,8 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
         ps, pso, pds = scores.data_ptr(), scores_out.data_ptr(), draft_scores.data_ptr()
     else:
         _need(scores_out is None and draft_scores is None, "scores_out and draft_scores need scores")
+    if dev_err is not None:
+        _on_device(t, dev, dev_err=dev_err)
     L = lib()
     with t.cuda.device(dev):
         st = stream_of(dev)
@@ -163,7 +168,7 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
         rc = L.mb_tree_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(), k_draft.data_ptr(),
                             v_draft.data_ptr(), masks.data_ptr(), 1 if shared else 0, out.data_ptr(),
                             _Strides18(*strides), 1 if dt is t.bfloat16 else 0, T, m, H, Hkv, Lmax, d, sc, ps, pso,
-                            pds, ws.data_ptr(), ws.numel(), st)
+                            pds, ws.data_ptr(), ws.numel(), None if dev_err is None else dev_err.data_ptr(), st)
     if rc != 0:
         check(rc, "mb_tree_attn")
     return out if scores is None else (out, scores_out, draft_scores)

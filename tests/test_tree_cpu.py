@@ -75,7 +75,7 @@ def test_attention_entry_checks_its_arguments(L):
     def attn(q=fake, k=fake, masks=fake, strides=st, bf16=0, T=1, m=4, H=8, Hkv=2, Lmax=64, d=128, scale=0.1,
              scores=None, scores_out=None, draft=None, ws=fake, nbytes=1 << 30):
         return L.mb_tree_attn(q, k, fake, fake, fake, fake, masks, 0, fake, strides, bf16, T, m, H, Hkv, Lmax, d,
-                              scale, scores, scores_out, draft, ws, nbytes, None)
+                              scale, scores, scores_out, draft, ws, nbytes, None, None)
     assert attn(q=None) == -1
     assert attn(k=None) == -1
     assert attn(masks=None) == -1
