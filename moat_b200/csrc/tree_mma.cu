@@ -841,7 +841,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   } else if (warp == 9) {
     if (lane == 0) {
       const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
-      int k = 0, seg = 0;
+      int k = 0, seg = 0, fills[2] = {0, 0};
       for (int f = beg; f < end;) {
         const Segment s = segment_at(p, cum, f, end, 1);
         for (int rb = 0; rb < p.RB; ++rb, ++seg) {
@@ -850,14 +850,16 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
           for (int jj = 0; jj < s.n; ++jj, ++k) {
             const int st = k % p.nst, use = k / p.nst;
             guarded_wait(kv_full + st, use & 1, dead, a.err);
-            if (k >= 2) guarded_wait(s_empty + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
+            // buffer b belongs to warpgroup b, which waits for every one of its fills
+            const int b = jj & 1, fill = b ? fills[1]++ : fills[0]++;
+            if (fill > 0) guarded_wait(s_empty + b, (fill - 1) & 1, dead, a.err);
             tc_after_sync();
             const uint32_t ka = ring + st * lay.stage, qb = qbase + qs * lay.qslot;
 #pragma unroll
             for (int kk = 0; kk < PANELS * 4; ++kk)
-              tc_mma(tmem + (k & 1) * kMaxRows, smem_desc(ka + (kk >> 2) * kPanel + (kk & 3) * 32, 16),
+              tc_mma(tmem + b * kMaxRows, smem_desc(ka + (kk >> 2) * kPanel + (kk & 3) * 32, 16),
                      smem_desc(qb + (kk >> 2) * p.n16 * 128 + (kk & 3) * 32, 16), id_qk, kk > 0);
-            tc_commit(s_full + (k & 1));
+            tc_commit(s_full + b);
             tc_commit(kv_empty + st);
           }
           tc_commit(q_empty + qs);
@@ -878,7 +880,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     const float sc = a.scale_log2;
     float* lse = lse_s + grp * kMaxRows;
     uint64_t* rowmask = mask_s + grp * kMaxRows;
-    int k = 0;
+    const uint32_t sbuf = tmem + lanes + grp * kMaxRows;
+    int fill = 0;
     for (int f = beg; f < end;) {
       const Segment s = segment_at(p, cum, f, end, 1);
       const int len = trace_len(a, s.t);
@@ -890,14 +893,12 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
         lse[key] = node ? p.lse[(unit * p.RB + rb) * kMaxRows + key] : INFINITY;
         rowmask[key] = node ? a.masks[s.t * a.mask_stride + i] : 0;
         named_bar_sync(1 + grp, 128);
-        for (int jj = 0; jj < s.n; ++jj, ++k) {
-          if ((jj & 1) != grp) continue;
+        for (int jj = grp; jj < s.n; jj += 2, ++fill) {
           const int j = s.j0 + jj;
           const bool draft = j == s.nt - 1;
           const int rows = tile_rows(len, s.nt, a.m, j);
-          guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
+          guarded_wait(s_full + grp, fill & 1, dead, a.err);
           tc_after_sync();
-          const uint32_t sbuf = tmem + lanes + (k & 1) * kMaxRows;
           float w = 0.0f;
           for (int n = 0; n < p.n16; n += 16) {
             float x[16];
@@ -915,7 +916,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
             w += part;
           }
           tc_before_sync();
-          mbar_arrive(s_empty + (k & 1));
+          mbar_arrive(s_empty + grp);
           if (key < rows) {
             float* dst = draft ? a.draft_scores + unit * a.m + key : a.scores_out + unit * a.Lmax + j * kTile + key;
             const float base = rb > 0 ? *dst : draft || !a.scores ? 0.0f : a.scores[unit * a.Lmax + j * kTile + key];

@@ -97,6 +97,8 @@ def check(x, weights=False, scale=None, **kw):
     import torch
     from moat_b200.tree import tree_attention
     ref, tol, wc, wd, rel = reference(x, scale)
+    dev_err = torch.zeros(1, dtype=torch.int32, device=ref.device)
+    kw["dev_err"] = dev_err
     if not weights:
         got = tree_attention(**x, scale=scale, **kw)
     else:
@@ -111,6 +113,7 @@ def check(x, weights=False, scale=None, **kw):
         want = torch.where(valid, old.double() + wc, old.double())
         assert bool(((so.double() - want).abs() <= rel * wc + 2.0 ** -23 * want.abs()).all())
         assert bool(((ds.double() - wd).abs() <= rel * wd + 1e-30).all())
+    assert int(dev_err) == 0  # no bounded wait gave up
     err = (got.double() - ref).abs()
     assert bool((err <= tol).all()), f"largest error over tolerance {(err / tol.clamp(min=1e-30)).max().item():.3g}"
     assert bool((got[tol.sum(-1) == 0] == 0).all())  # padding
@@ -135,6 +138,8 @@ SHAPES = [
     (1, 3, 2, 1, 33, [90], 100),
     (1, 1, 8, 1, 128, [5000], 5001),
     (5, 16, 32, 8, 128, [1, 1025, 64, 0, 2000], 2048),
+    (16, 1, 16, 16, 128, [1100 - 67 * t for t in range(16)], 1100),  # several odd-length pieces per CTA
+    (6, 40, 16, 2, 64, [130, 1300, 700, 0, 901, 2500], 2500),  # row blocks and such pieces
 ]
 
 
