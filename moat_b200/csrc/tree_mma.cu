@@ -34,16 +34,16 @@
 namespace mb {
 
 constexpr int kTile = 128;      // keys per tile
-constexpr int kBox = 64;        // rows per TMA box: a last tile loads no more boxes than it needs
+constexpr int kBox = 32;        // rows per TMA box of a unit's last cached tile: no more boxes than it needs
 constexpr int kMaxRows = 128;   // rows of a block
-constexpr int kMaxTraces = 255;  // per launch (the prefix of tile counts lies in shared memory)
+constexpr int kMaxTraces = 127;  // per launch (their lengths and tile counts lie in shared memory)
 constexpr int kPanel = kTile * 128;  // bytes of a 64-column panel of a tile (128-byte swizzled rows)
 constexpr float kNoRef = -1e30f;     // m_ref before any visible key
 constexpr float kSlack = 8.0f;       // p may reach 2^kSlack
 
 struct TreeMmaParams {
   TreeAttnArgs a;
-  CUtensorMap mq, mk, mv, mkd, mvd;
+  CUtensorMap mq, mk, mv, mk_end, mv_end, mkd, mvd;
   float* part;  // [2 * grid][rows][DP] unnormalised O of a unit's pieces
   float* ml;    // [2 * grid][2][kMaxRows] their m_ref and sum
   float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
@@ -64,11 +64,14 @@ __device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// a, b: low words of the operands' descriptors (smem_desc); their high words are alike.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "n"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -99,12 +102,11 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const float* r) {
       : "memory");
 }
 
-// Shared-memory operand with 128-byte swizzle. K-major: rows of 64 elements, 8-row groups
-// 1024 bytes apart (lbo unused). MN-major: 64 elements of M or N per 128-byte line, lines
+// Low word of a shared-memory operand with 128-byte swizzle. K-major: rows of 64 elements, 8-row
+// groups 1024 bytes apart (lbo unused). MN-major: 64 elements of M or N per 128-byte line, lines
 // along K, 8-line groups 1024 bytes apart, the next 64 elements of M or N lbo bytes on.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
-  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint32_t smem_desc(uint32_t addr, uint32_t lbo) {
+  return ((addr & 0x3FFFF) >> 4) | ((lbo >> 4) << 16);
 }
 // kind::f16, fp32 accumulator, M = 128; a_mn / b_mn: operand is M- / N-major
 __device__ __forceinline__ uint32_t instr_desc(bool bf16, int n, bool a_mn, bool b_mn) {
@@ -119,6 +121,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
       : "memory");
+}
+
+// One lane of a converged warp. Branches on it stay uniform for the compiler, so that
+// descriptors and addresses live in uniform registers (a test of the lane number made each
+// MMA and each TMA instruction cost 100 to 350 cycles to issue).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -154,16 +165,23 @@ __device__ __forceinline__ void guarded_wait(uint64_t* bar, uint32_t parity, boo
   }
 }
 
-// Column sums over the 32 lanes: v[0..31] of every lane in, the sum of column `lane` out.
-__device__ __forceinline__ float column_sums32(float* v, int lane) {
+// Sums over the 32 lanes of N (16 or 32) columns: v[0..N) of every lane in, the sum of column
+// lane % N out.
+template <int N>
+__device__ __forceinline__ float column_sums(float* v, int lane) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const bool up = lane & o;
+    if (2 * o > N) {
 #pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float give = up ? v[i] : v[i + o];
-      const float keep = up ? v[i + o] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    } else {
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const float give = up ? v[i] : v[i + o];
+        const float keep = up ? v[i + o] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
     }
   }
   return v[0];
@@ -181,27 +199,32 @@ struct Segment {  // a run of tiles of one unit
   int t, kvh, rb, len, nt, j0, n;
 };
 
-// The segment that begins at flat tile f (at most up to `end`); cum[t] = tiles before trace t,
-// RB row blocks per (trace, KV head).
-__device__ __forceinline__ Segment segment_at(const TreeMmaParams& p, const int* cum, int f, int end, int RB) {
+// Lengths of the launch's traces and the tiles before each, in shared memory.
+struct TraceTable {
+  int cum[kMaxTraces + 1];
+  int len[kMaxTraces + 1];
+};
+
+// The segment that begins at flat tile f (at most up to `end`), RB row blocks per (trace, KV
+// head).
+__device__ __forceinline__ Segment segment_at(const TreeMmaParams& p, const TraceTable& tab, int f, int end, int RB) {
   int lo = 0, hi = p.T - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cum[mid] <= f)
+    if (tab.cum[mid] <= f)
       lo = mid;
     else
       hi = mid - 1;
   }
   Segment s;
   s.t = p.t0 + lo;
-  const int units = p.a.Hkv * RB;
-  s.nt = (cum[lo + 1] - cum[lo]) / units;
-  const int rem = f - cum[lo], u = rem / s.nt;
+  s.len = tab.len[lo];
+  s.nt = trace_tiles(s.len);
+  const int rem = f - tab.cum[lo], u = rem / s.nt;
   s.j0 = rem - u * s.nt;
   s.kvh = u / RB;
   s.rb = u - s.kvh * RB;
   s.n = min(s.nt - s.j0, end - f);
-  s.len = 0;
   return s;
 }
 
@@ -210,21 +233,25 @@ __device__ __forceinline__ int tile_rows(int len, int nt, int m, int j) {
   return j == nt - 1 ? m : min(kTile, len - j * kTile);
 }
 
-// Fills cum[0..T] (warp 0) for `units` units per trace.
-__device__ __forceinline__ void prefix_tiles(const TreeMmaParams& p, int* cum, int lane, int units) {
+// Fills the table (warp 0) for `units` units per trace.
+__device__ __forceinline__ void prefix_tiles(const TreeMmaParams& p, TraceTable& tab, int lane, int units) {
   int base = 0;
   for (int c = 0; c < p.T; c += 32) {
     const int t = c + lane;
-    int v = t < p.T ? trace_tiles(trace_len(p.a, p.t0 + t)) * units : 0;
+    const int len = t < p.T ? trace_len(p.a, p.t0 + t) : 0;
+    int v = t < p.T ? trace_tiles(len) * units : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
-    if (t < p.T) cum[t + 1] = base + v;
+    if (t < p.T) {
+      tab.cum[t + 1] = base + v;
+      tab.len[t] = len;
+    }
     base += __shfl_sync(0xffffffffu, v, 31);
   }
-  if (lane == 0) cum[0] = 0;
+  if (lane == 0) tab.cum[0] = 0;
 }
 
 template <bool BF16>
@@ -250,8 +277,8 @@ constexpr int kMaxStages = 8;
 constexpr uint32_t kMiscBars = 256;                          // barriers, TMEM base
 constexpr uint32_t kMiscRef = kMiscBars;                     // m_ref [128]
 constexpr uint32_t kMiscMask = kMiscRef + kMaxRows * 4;      // draft masks by row [128]
-constexpr uint32_t kMiscCum = kMiscMask + kMaxRows * 8;      // [kMaxTraces + 1]
-constexpr uint32_t kMiscBytes = kMiscCum + (kMaxTraces + 1) * 4;
+constexpr uint32_t kMiscTab = kMiscMask + kMaxRows * 8;      // TraceTable
+constexpr uint32_t kMiscBytes = kMiscTab + sizeof(TraceTable);
 
 __host__ __device__ inline TreeSmem tree_smem(int panels, int n16, int nst, int nq) {
   TreeSmem s;
@@ -286,7 +313,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 1);
   float* ref = reinterpret_cast<float*>(misc + kMiscRef);
   uint64_t* rowmask = reinterpret_cast<uint64_t*>(misc + kMiscMask);
-  int* cum = reinterpret_cast<int*>(misc + kMiscCum);
+  TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TreeAttnArgs& a = p.a;
@@ -312,7 +339,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
     }
   } else if (warp == 4 * WG + 1) {
     tmem_alloc(smem_u32(tmem_base), 512);
-  } else {
+  } else if (warp < 4 * WG) {
     // rows beyond R of the Q slots stay zero (the boxes never write them)
     uint4* qz = reinterpret_cast<uint4*>(smem + lay.q);
     for (uint32_t i = tid; i < p.nq * lay.qslot / 16; i += kSoft) qz[i] = make_uint4(0, 0, 0, 0);
@@ -321,12 +348,12 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   }
   pdl_wait();  // the lengths, masks, queries and drafts may come from the kernel before
   pdl_launch_dependents();
-  if (warp == 0) prefix_tiles(p, cum, lane, a.Hkv * p.RB);
+  if (warp == 0) prefix_tiles(p, tab, lane, a.Hkv * p.RB);
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
   const uint32_t tmem = *tmem_base;
-  const int total = cum[p.T];
+  const int total = tab.cum[p.T];
   const int g = min(p.grid, total);  // CTAs with work
   const int c = blockIdx.x;
   const int beg = c < g ? cut(total, c, g) : 0, end = c < g ? cut(total, c + 1, g) : 0;
@@ -334,194 +361,223 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 
   if (warp == 4 * WG) {
     // ---------------------------------------------------------------- TMA
-    if (lane == 0) {
-      // a cache that is read once streams past what L2 should keep; several row blocks or the
-      // weight pass read it again
-      uint64_t policy;
-      if (p.RB == 1 && !p.lse)
-        policy = policy_evict_first();
-      else
-        asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
-      const uint64_t keep = policy_evict_last();
-      int item = 0, seg = 0;  // K and V tiles of the ring, segments
-      for (int f = beg; f < end; ++seg) {
-        const Segment s = segment_at(p, cum, f, end, p.RB);
-        const int len = trace_len(a, s.t);
-        const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
-        if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
-        mbar_expect_tx(q_full + qs, PANELS * R * 128);
-        for (int pn = 0; pn < PANELS; ++pn)
-          tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G,
-                      s.rb * p.mb, s.t, keep);
-        for (int j = s.j0; j < s.j0 + s.n; ++j) {
-          const bool draft = j == s.nt - 1;
-          const int boxes = draft ? 0 : (tile_rows(len, s.nt, a.m, j) + kBox - 1) / kBox;
-          for (int kv = 0; kv < 2; ++kv, ++item) {
-            const int st = item % p.nst, use = item / p.nst;
-            if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
-            const uint32_t dst = ring + st * lay.stage;
-            mbar_expect_tx(kv_full + st, PANELS * 128 * (draft ? a.m : boxes * kBox));
-            for (int pn = 0; pn < PANELS; ++pn) {
-              if (draft)
+    // a cache that is read once streams past what L2 should keep; several row blocks or the
+    // weight pass read it again
+    uint64_t policy;
+    if (p.RB == 1 && !p.lse)
+      policy = policy_evict_first();
+    else
+      asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    const uint64_t keep = policy_evict_last();
+    int item = 0, seg = 0, st = 0, use = 0;  // K and V tiles of the ring (stage, times used), segments
+    for (int f = beg; f < end; ++seg) {
+      const Segment s = segment_at(p, tab, f, end, p.RB);
+      const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+      for (int j = s.j0; j < s.j0 + s.n; ++j) {
+        const bool draft = j == s.nt - 1;
+        const int rows = tile_rows(s.len, s.nt, a.m, j);
+        for (int kv = 0; kv < 2; ++kv, ++item) {
+          if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
+          const uint32_t dst = ring + st * lay.stage;
+          if (elect_one()) {
+            if (draft) {
+              mbar_expect_tx(kv_full + st, PANELS * 128 * a.m);
+              for (int pn = 0; pn < PANELS; ++pn)
                 tma_load_4d(dst + pn * kPanel, kv ? &p.mvd : &p.mkd, kv_full + st, pn * 64, s.kvh, 0, s.t, keep);
-              else
+            } else if (rows == kTile) {
+              mbar_expect_tx(kv_full + st, PANELS * kPanel);
+              for (int pn = 0; pn < PANELS; ++pn)
+                tma_load_4d(dst + pn * kPanel, kv ? &p.mv : &p.mk, kv_full + st, pn * 64, j * kTile, s.kvh, s.t,
+                            policy);
+            } else {
+              const int boxes = (rows + kBox - 1) / kBox;
+              mbar_expect_tx(kv_full + st, PANELS * 128 * boxes * kBox);
+              for (int pn = 0; pn < PANELS; ++pn)
                 for (int b = 0; b < boxes; ++b)
-                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, kv ? &p.mv : &p.mk, kv_full + st, pn * 64,
+                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, kv ? &p.mv_end : &p.mk_end, kv_full + st, pn * 64,
                               j * kTile + b * kBox, s.kvh, s.t, policy);
             }
           }
+          __syncwarp();
+          if (++st == p.nst) {
+            st = 0;
+            ++use;
+          }
         }
-        f += s.n;
+        if (j == s.j0) {  // the queries after the first keys: their slot may still be in use
+          if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
+          if (elect_one()) {
+            mbar_expect_tx(q_full + qs, PANELS * R * 128);
+            for (int pn = 0; pn < PANELS; ++pn)
+              tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G,
+                          s.rb * p.mb, s.t, keep);
+          }
+          __syncwarp();
+        }
       }
-      if (dead)  // copies still in flight must land before this CTA's shared memory goes
-        for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
+      f += s.n;
     }
-    __syncwarp();
+    if (dead)  // copies still in flight must land before this CTA's shared memory goes
+      for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
   } else if (warp == 4 * WG + 1) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
-      const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
-      const uint32_t id_pv = instr_desc(BF16, p.n16, true, true);
-      const int n = end - beg;
-      // two cursors over the same tiles: scores run one tile ahead of the value product
-      Segment sq = {}, sv = {};
-      int jq = 0, jv = 0, nq = 0, nv = 0, seg_q = -1, seg_v = -1, len_v = 0;
-      for (int k = 0; k <= n; ++k) {
-        if (k < n) {
-          if (jq == nq) {
-            sq = segment_at(p, cum, beg + k, end, p.RB);
-            jq = 0;
-            nq = sq.n;
-            ++seg_q;
-          }
-          const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
-          if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
-          const int st = (2 * k) % p.nst, use = (2 * k) / p.nst;
-          guarded_wait(kv_full + st, use & 1, dead, a.err);
-          if (k >= 2) guarded_wait(s_empty + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
-          tc_after_sync();
-          const uint32_t ka = ring + st * lay.stage, qb = qbase + qs * lay.qslot;
+    const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
+    const uint32_t id_pv = instr_desc(BF16, p.n16, true, true);
+    const uint32_t ring_k = smem_desc(ring, 16), ring_v = smem_desc(ring, kPanel);
+    const uint32_t q_desc = smem_desc(qbase, 16), p_desc = smem_desc(pbase, kPanel);
+    const int n = end - beg;
+    // two cursors over the same tiles: scores run one tile ahead of the value product
+    Segment sq = {}, sv = {};
+    int jq = 0, jv = 0, nq = 0, nv = 0, seg_q = -1, seg_v = -1;
+    int st_k = 0, use_k = 0, st_v = 1, use_v = 0;  // their ring stages: tile k's K and V are items 2k, 2k + 1
+    for (int k = 0; k <= n; ++k) {
+      if (k < n) {
+        if (jq == nq) {
+          sq = segment_at(p, tab, beg + k, end, p.RB);
+          jq = 0;
+          nq = sq.n;
+          ++seg_q;
+        }
+        const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
+        if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
+        guarded_wait(kv_full + st_k, use_k & 1, dead, a.err);
+        if (k >= 2) guarded_wait(s_empty + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
+        tc_after_sync();
+        ++jq;
+        if (elect_one()) {
+          const uint32_t ka = ring_k + (st_k * lay.stage >> 4), qb = q_desc + (qs * lay.qslot >> 4);
+          const uint32_t qpanel = p.n16 * 128 >> 4;
 #pragma unroll
           for (int kk = 0; kk < PANELS * 4; ++kk)
-            tc_mma(tmem + (k & 1) * kMaxRows, smem_desc(ka + (kk >> 2) * kPanel + (kk & 3) * 32, 16),
-                   smem_desc(qb + (kk >> 2) * p.n16 * 128 + (kk & 3) * 32, 16), id_qk, kk > 0);
+            tc_mma(tmem + (k & 1) * kMaxRows, ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2,
+                   qb + (kk >> 2) * qpanel + (kk & 3) * 2, id_qk, kk > 0);
           tc_commit(s_full + (k & 1));
-          tc_commit(kv_empty + st);
-          if (++jq == nq) tc_commit(q_empty + qs);
+          tc_commit(kv_empty + st_k);
+          if (jq == nq) tc_commit(q_empty + qs);
         }
-        if (k > 0) {
-          const int e = k - 1;
-          if (jv == nv) {
-            sv = segment_at(p, cum, beg + e, end, p.RB);
-            jv = 0;
-            nv = sv.n;
-            len_v = trace_len(a, sv.t);
-            ++seg_v;
-          }
-          const int st = (2 * e + 1) % p.nst, use = (2 * e + 1) / p.nst;
-          guarded_wait(kv_full + st, use & 1, dead, a.err);
-          guarded_wait(p_full, e & 1, dead, a.err);
-          if (jv == 0 && seg_v >= 2) guarded_wait(o_empty + (seg_v & 1), ((seg_v >> 1) - 1) & 1, dead, a.err);
-          tc_after_sync();
-          const uint32_t va = ring + st * lay.stage;
-          const int steps = (tile_rows(len_v, sv.nt, a.m, sv.j0 + jv) + 15) / 16;
-          for (int kk = 0; kk < steps; ++kk)
-            tc_mma(tmem + (2 + (seg_v & 1)) * kMaxRows, smem_desc(va + kk * 2048, kPanel),
-                   smem_desc(pbase + kk * 2048, kPanel), id_pv, jv > 0 || kk > 0);
-          tc_commit(kv_empty + st);
-          tc_commit(pv_done);
-          ++jv;
+        __syncwarp();
+        st_k += 2;
+        if (st_k >= p.nst) {
+          st_k -= p.nst;
+          ++use_k;
         }
       }
-      if (dead && n > 0) {  // products still in flight must end before TMEM is freed
-        tc_commit(pv_done);
-        const long long t0 = clock64();
-        while (clock64() - t0 < 1000000) {
+      if (k > 0) {
+        const int e = k - 1;
+        if (jv == nv) {
+          sv = segment_at(p, tab, beg + e, end, p.RB);
+          jv = 0;
+          nv = sv.n;
+          ++seg_v;
+        }
+        guarded_wait(kv_full + st_v, use_v & 1, dead, a.err);
+        if (jv == 0 && seg_v >= 2) guarded_wait(o_empty + (seg_v & 1), ((seg_v >> 1) - 1) & 1, dead, a.err);
+        guarded_wait(p_full, e & 1, dead, a.err);
+        tc_after_sync();
+        const int steps = (tile_rows(sv.len, sv.nt, a.m, sv.j0 + jv) + 15) / 16;
+        if (elect_one()) {
+          const uint32_t va = ring_v + (st_v * lay.stage >> 4);
+          const uint32_t o = tmem + (2 + (seg_v & 1)) * kMaxRows;
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            if (kk < steps) tc_mma(o, va + kk * (2048 >> 4), p_desc + kk * (2048 >> 4), id_pv, jv > 0 || kk > 0);
+          tc_commit(kv_empty + st_v);
+          tc_commit(pv_done);
+        }
+        __syncwarp();
+        ++jv;
+        st_v += 2;
+        if (st_v >= p.nst) {
+          st_v -= p.nst;
+          ++use_v;
         }
       }
     }
-    __syncwarp();
-  } else {
+    if (dead) {  // products still in flight must end before TMEM is freed
+      const long long t0 = clock64();
+      while (clock64() - t0 < 1000000) {
+      }
+    }
+  } else if (warp < 4 * WG) {
     // ---------------------------------------------------------------- softmax
     const int grp = warp >> 2, wq = warp & 3;
     const int key = wq * 32 + lane;  // this thread's key of a tile, and its d of O^T
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int col0 = grp * CW;
     const float sc = a.scale_log2;
+    const float* refs = ref + col0;
+    const int my_node = tid / p.G;  // node of row tid within a block
     float l[CW];
 #pragma unroll
     for (int i = 0; i < CW; ++i) l[i] = 0.0f;
     float* scratch = reinterpret_cast<float*>(smem + lay.p);  // P's space, while no product reads it
-    int seg = 0, k = 0;
+    int seg = 0, k = 0, vst = 1, vuse = 0;
     for (int f = beg; f < end; ++seg) {
-      const Segment s = segment_at(p, cum, f, end, p.RB);
-      const int len = trace_len(a, s.t);
+      const Segment s = segment_at(p, tab, f, end, p.RB);
+      // this row's mask, and the rows of the draft that any node sees (loads in flight over the
+      // first tile)
+      const uint64_t* mk = a.masks + s.t * a.mask_stride;
+      const int node = s.rb * p.mb + my_node;
+      const uint64_t my_mask = tid < R && node < a.m ? mk[node] : 0;
+      const uint64_t mk0 = lane < a.m ? mk[lane] : 0, mk1 = lane + 32 < a.m ? mk[lane + 32] : 0;
       for (int jj = 0; jj < s.n; ++jj, ++k) {
         const int j = s.j0 + jj;
         const bool draft = j == s.nt - 1;
-        const int rows = tile_rows(len, s.nt, a.m, j);
+        const int rows = tile_rows(s.len, s.nt, a.m, j);
         const uint32_t sbuf = tmem + lanes + (k & 1) * kMaxRows + col0;
-        const int vst = (2 * k + 1) % p.nst, vuse = (2 * k + 1) / p.nst;
-        uint64_t used = ~0ull;  // drafted rows that some node sees
         if (draft) {
-          const uint64_t* mk = a.masks + s.t * a.mask_stride;
-          uint64_t u = 0;
-          for (int i = lane; i < a.m; i += 32) u |= mk[i];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) u |= __shfl_xor_sync(0xffffffffu, u, o);
-          used = u;
-          for (int r = tid; r < kMaxRows; r += kSoft) {
-            const int i = s.rb * p.mb + r / p.G;
-            rowmask[r] = r < R && i < a.m ? mk[i] : 0;
-          }
+          if (tid < kMaxRows) rowmask[tid] = my_mask;
           named_bar_sync(1, kSoft);
         }
+        // Scores of rows i .. i + 15 less sub (log2 units), -inf for what a row does not see.
+        // Sixteen at a time, read from TMEM again for the exponentials: with all of a thread's
+        // scores in registers it spills, and with L1 given to shared memory a spill goes to L2
+        // (5,600 cycles for a tile's exponentials of 64 rows).
+        float x[16];
+        auto form = [&](int i, auto sub) {
+          tc_ld16(sbuf + i, x);
+          tc_wait_ld();
+#pragma unroll
+          for (int u = 0; u < 16; ++u) x[u] = fmaf(x[u], sc, sub(i + u));
+          if (draft) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+              if (key >= rows || !((rowmask[col0 + i + u] >> (key & 63)) & 1)) x[u] = -INFINITY;
+          } else if (key >= rows) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) x[u] = -INFINITY;
+          }
+        };
+        auto less_ref = [&](int i) { return -refs[i]; };
         guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
-        float x[CW];
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < CW; i += 16) {
+        for (int i = 0; i < CW; i += 16)
           if (col0 + i < p.n16) {
-            tc_ld16(sbuf + i, x + i);
-          } else {
+            form(i, less_ref);
 #pragma unroll
-            for (int u = 0; u < 16; ++u) x[i + u] = 0.0f;
+            for (int u = 0; u < 16; ++u) top = fmaxf(top, x[u]);
           }
-        }
-        tc_wait_ld();
-        tc_before_sync();
-        mbar_arrive(s_empty + (k & 1));
-        if (draft) {
+        const bool raise = vote_any(top > kSlack, kSoft);
+        if (raise) {
+          // P's space and O are free once the previous value product has finished
+          if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
+          tc_after_sync();
 #pragma unroll
-          for (int i = 0; i < CW; ++i) {
-            const bool see = key < rows && (rowmask[col0 + i] >> (key & 63)) & 1;
-            x[i] = see ? x[i] * sc : -INFINITY;
-          }
-        } else if (key < rows) {
+          for (int i = 0; i < CW; i += 16)
+            if (col0 + i < p.n16) {
+              form(i, [](int) { return 0.0f; });
+              float mine = 0.0f;
 #pragma unroll
-          for (int i = 0; i < CW; ++i) x[i] *= sc;
-        } else {
-#pragma unroll
-          for (int i = 0; i < CW; ++i) x[i] = -INFINITY;
-        }
-        bool over = false;
-#pragma unroll
-        for (int i = 0; i < CW; ++i) over |= x[i] > ref[col0 + i] + kSlack;
-        over = vote_any(over, kSoft);
-        // P and, for a new maximum, O are free once the previous value product has finished
-        if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
-        if (over) {
-          float mine[(CW + 31) / 32];
-#pragma unroll
-          for (int i = 0; i < CW; ++i) {
-            const float mx = warp_max(x[i]);
-            if ((i & 31) == lane) mine[i / 32] = mx;
-          }
-#pragma unroll
-          for (int u = 0; u < (CW + 31) / 32; ++u)
-            if (u * 32 + lane < CW) scratch[wq * kMaxRows + col0 + u * 32 + lane] = mine[u];
+              for (int u = 0; u < 16; ++u) {
+                const float mx = warp_max(x[u]);
+                if (u == lane) mine = mx;
+              }
+              if (lane < 16) scratch[wq * kMaxRows + col0 + i + lane] = mine;
+            }
           named_bar_sync(1, kSoft);
-          if (tid < CW * WG) {
+          if (tid < p.n16) {
             const float old = ref[tid];
             float mx = old;
 #pragma unroll
@@ -531,46 +587,51 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
           }
           named_bar_sync(1, kSoft);
           const float* fade = scratch + 4 * kMaxRows + col0;
+          const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
 #pragma unroll
-          for (int i = 0; i < CW; ++i) l[i] *= fade[i];
-          if (jj > 0) {
-            tc_after_sync();
-            const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
+          for (int i = 0; i < CW; i += 16)
+            if (col0 + i < p.n16) {
 #pragma unroll
-            for (int i = 0; i < CW; i += 16) {
-              float o[16];
-              tc_ld16(ob + i, o);
-              tc_wait_ld();
+              for (int u = 0; u < 16; ++u) l[i + u] *= fade[i + u];
+              if (jj > 0) {
+                tc_ld16(ob + i, x);
+                tc_wait_ld();
 #pragma unroll
-              for (int u = 0; u < 16; ++u) o[u] *= fade[i + u];
-              tc_st16(ob + i, o);
+                for (int u = 0; u < 16; ++u) x[u] *= fade[i + u];
+                tc_st16(ob + i, x);
+              }
             }
-            tc_wait_st();
-          }
+          tc_wait_st();
           named_bar_sync(1, kSoft);  // scratch read: its space becomes P again
         }
         // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
+        uint8_t* prow = smem + lay.p + key * 128;
 #pragma unroll
-        for (int i = 0; i < CW; i += 8) {
-          float e[8];
+        for (int i = 0; i < CW; i += 16)
+          if (col0 + i < p.n16) {
+            if (CW > 16 || raise) form(i, less_ref);
+            uint32_t pk[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            e[u] = ex2(x[i + u] - ref[col0 + i + u]);
-            l[i + u] += e[u];
+            for (int u = 0; u < 16; u += 2) {
+              const float e0 = ex2(x[u]), e1 = ex2(x[u + 1]);
+              l[i + u] += e0;
+              l[i + u + 1] += e1;
+              pk[u / 2] = pack2<BF16>(e0, e1);
+            }
+            if (i == 0 && k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);  // P's space is free
+            const int n = col0 + i, chunk = (n & 63) >> 3;
+            uint8_t* dst = prow + (n >> 6) * kPanel;
+            *reinterpret_cast<uint4*>(dst + ((chunk ^ (key & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(dst + (((chunk + 1) ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
           }
-          uint4 w;
-          w.x = pack2<BF16>(e[0], e[1]);
-          w.y = pack2<BF16>(e[2], e[3]);
-          w.z = pack2<BF16>(e[4], e[5]);
-          w.w = pack2<BF16>(e[6], e[7]);
-          const int n = col0 + i;
-          if (n < p.n16)
-            *reinterpret_cast<uint4*>(smem + lay.p + (n >> 6) * kPanel + key * 128 +
-                                      ((((n & 63) >> 3) ^ (key & 7)) << 4)) = w;
-        }
+        tc_before_sync();
+        mbar_arrive(s_empty + (k & 1));
         // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
         // product's last 16-row step reads beyond the valid rows, and unused drafted rows
         if (grp == 0 && (rows & 15 || draft)) {
+          uint64_t used = mk0 | mk1;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
           const bool clear = key >= rows ? key < ((rows + 15) & ~15) : draft && !((used >> (key & 63)) & 1);
           if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
           if (clear) {
@@ -583,62 +644,68 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
         fence_proxy_async_smem();
         tc_before_sync();
         mbar_arrive(p_full);
+        vst += 2;
+        if (vst >= p.nst) {
+          vst -= p.nst;
+          ++vuse;
+        }
       }
       // ------------------------------------------------ end of the segment: sums, output
+      constexpr int kSum = CW < 32 ? CW : 32;
+      float sums[CW / kSum];
+#pragma unroll
+      for (int i = 0; i < CW; i += kSum) sums[i / kSum] = column_sums<kSum>(l + i, lane);
       guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
       tc_after_sync();
 #pragma unroll
-      for (int i = 0; i < CW; i += 32) {
-        float v[32];
-#pragma unroll
-        for (int u = 0; u < 32; ++u) v[u] = i + u < CW ? l[i + u < CW ? i + u : 0] : 0.0f;
-        const float sum = column_sums32(v, lane);
-        if (i + lane < CW) scratch[wq * kMaxRows + col0 + i + lane] = sum;
-      }
+      for (int i = 0; i < CW; i += kSum)
+        if (lane < kSum) scratch[wq * kMaxRows + col0 + i + lane] = sums[i / kSum];
       named_bar_sync(1, kSoft);
       const bool whole = s.n == s.nt;
       const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
       if (tid < CW * WG) {
         const float sum = scratch[tid] + scratch[kMaxRows + tid] + scratch[2 * kMaxRows + tid] +
                           scratch[3 * kMaxRows + tid];
-        const int i = s.rb * p.mb + tid / p.G;
-        const bool real = tid < R && i < a.m && a.masks[s.t * a.mask_stride + i] != 0;
-        float* ml = p.ml + static_cast<int64_t>(slot) * 2 * kMaxRows;
-        if (!whole) {
-          ml[tid] = ref[tid];
-          ml[kMaxRows + tid] = real ? sum : 0.0f;
-        } else if (p.lse && tid < kMaxRows) {
-          const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
-          p.lse[unit * kMaxRows + tid] = real && sum != 0.0f ? ref[tid] + log2f(sum) : INFINITY;
-        }
-        scratch[4 * kMaxRows + tid] = real && sum != 0.0f ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
+        const bool real = my_mask != 0 && sum != 0.0f;
+        const float top = ref[tid];
+        scratch[4 * kMaxRows + tid] = real ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
         ref[tid] = kNoRef;
+        if (!whole) {
+          float* ml = p.ml + static_cast<int64_t>(slot) * 2 * kMaxRows;
+          ml[tid] = top;
+          ml[kMaxRows + tid] = real ? sum : 0.0f;
+        } else if (p.lse) {
+          const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
+          p.lse[unit * kMaxRows + tid] = real ? top + log2f(sum) : INFINITY;
+        }
       }
       named_bar_sync(1, kSoft);
       const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
-      const int i0 = s.rb * p.mb;
-#pragma unroll
+      int row = col0, nd = s.rb * p.mb + col0 / p.G, gh = col0 % p.G;  // row, its node, its head of the group
+      uint16_t* out = a.out + s.t * a.os[0] + nd * a.os[1] + (s.kvh * p.G + gh) * a.os[2] + key;
+      float* part = p.part + (static_cast<int64_t>(slot) * R + col0) * DP + key;
       for (int i = 0; i < CW; i += 16) {
-        if (col0 + i >= p.n16) break;
+        if (row >= R) break;
         float o[16];
         tc_ld16(ob + i, o);
         tc_wait_ld();
         if (whole) {
-          if (key < a.d) {
 #pragma unroll
-            for (int u = 0; u < 16; ++u) {
-              const int n = col0 + i + u, node = i0 + n / p.G;
-              const float inv = scratch[4 * kMaxRows + n];
-              if (n < R && node < a.m)
-                a.out[s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + n % p.G) * a.os[2] + key] =
-                    round16<BF16>(inv == 0.0f ? 0.0f : o[u] * inv);
+          for (int u = 0; u < 16; ++u, ++row) {
+            if (u % 4 == 0) asm volatile("" ::: "memory");
+            const float inv = scratch[4 * kMaxRows + row];
+            if (row < R && nd < a.m && key < a.d) *out = round16<BF16>(inv == 0.0f ? 0.0f : o[u] * inv);
+            out += a.os[2];
+            if (++gh == p.G) {
+              gh = 0;
+              ++nd;
+              out += a.os[1] - p.G * a.os[2];
             }
           }
-        } else if (key < DP) {
-          float* dst = p.part + (static_cast<int64_t>(slot) * R + col0 + i) * DP + key;
+        } else {
 #pragma unroll
-          for (int u = 0; u < 16; ++u)
-            if (col0 + i + u < R) dst[u * DP] = o[u];
+          for (int u = 0; u < 16; ++u, ++row, part += DP)
+            if (row < R && key < DP) *part = o[u];
         }
       }
       tc_before_sync();
@@ -757,7 +824,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   uint64_t* q_full = s_empty + 2;
   uint64_t* q_empty = q_full + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(q_empty + 2);
-  int* cum = reinterpret_cast<int*>(misc + kMiscCum);
+  TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
   // the space of P: per warpgroup the rows' lse and draft masks
   float* lse_s = reinterpret_cast<float*>(smem + lay.p);
   uint64_t* mask_s = reinterpret_cast<uint64_t*>(smem + lay.p + 2 * kMaxRows * 4);
@@ -790,89 +857,108 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   pdl_wait();
   pdl_launch_dependents();
   // units are (trace, KV head) here: the sequence has no row blocks
-  if (warp == 0) prefix_tiles(p, cum, lane, a.Hkv);
+  if (warp == 0) prefix_tiles(p, tab, lane, a.Hkv);
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
   const uint32_t tmem = *tmem_base;
-  const int total = cum[p.T];
+  const int total = tab.cum[p.T];
   const int g = min(p.grid, total);
   const int c = blockIdx.x;
   const int beg = c < g ? cut(total, c, g) : 0, end = c < g ? cut(total, c + 1, g) : 0;
   const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q);
 
   if (warp == 8) {
-    if (lane == 0) {
-      const uint64_t policy = policy_evict_first(), keep = policy_evict_last();
-      int item = 0, seg = 0;
-      for (int f = beg; f < end;) {
-        const Segment s = segment_at(p, cum, f, end, 1);
-        const int len = trace_len(a, s.t);
-        for (int rb = 0; rb < p.RB; ++rb, ++seg) {
-          const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
-          if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
-          mbar_expect_tx(q_full + qs, PANELS * R * 128);
-          for (int pn = 0; pn < PANELS; ++pn)
-            tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G, rb * p.mb,
-                        s.t, keep);
-          for (int j = s.j0; j < s.j0 + s.n; ++j, ++item) {
-            const bool draft = j == s.nt - 1;
-            const int boxes = draft ? 0 : (tile_rows(len, s.nt, a.m, j) + kBox - 1) / kBox;
-            const int st = item % p.nst, use = item / p.nst;
-            if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
-            const uint32_t dst = ring + st * lay.stage;
-            mbar_expect_tx(kv_full + st, PANELS * 128 * (draft ? a.m : boxes * kBox));
-            for (int pn = 0; pn < PANELS; ++pn) {
-              if (draft)
+    const uint64_t policy = policy_evict_first(), keep = policy_evict_last();
+    int item = 0, seg = 0, st = 0, use = 0;
+    for (int f = beg; f < end;) {
+      const Segment s = segment_at(p, tab, f, end, 1);
+      for (int rb = 0; rb < p.RB; ++rb, ++seg) {
+        const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+        const uint64_t pol = rb + 1 < p.RB ? keep : policy;
+        for (int j = s.j0; j < s.j0 + s.n; ++j, ++item) {
+          const int rows = tile_rows(s.len, s.nt, a.m, j);
+          if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
+          const uint32_t dst = ring + st * lay.stage;
+          if (elect_one()) {
+            if (j == s.nt - 1) {
+              mbar_expect_tx(kv_full + st, PANELS * 128 * a.m);
+              for (int pn = 0; pn < PANELS; ++pn)
                 tma_load_4d(dst + pn * kPanel, &p.mkd, kv_full + st, pn * 64, s.kvh, 0, s.t, keep);
-              else
+            } else if (rows == kTile) {
+              mbar_expect_tx(kv_full + st, PANELS * kPanel);
+              for (int pn = 0; pn < PANELS; ++pn)
+                tma_load_4d(dst + pn * kPanel, &p.mk, kv_full + st, pn * 64, j * kTile, s.kvh, s.t, pol);
+            } else {
+              const int boxes = (rows + kBox - 1) / kBox;
+              mbar_expect_tx(kv_full + st, PANELS * 128 * boxes * kBox);
+              for (int pn = 0; pn < PANELS; ++pn)
                 for (int b = 0; b < boxes; ++b)
-                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, &p.mk, kv_full + st, pn * 64, j * kTile + b * kBox,
-                              s.kvh, s.t, rb + 1 < p.RB ? keep : policy);
+                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, &p.mk_end, kv_full + st, pn * 64,
+                              j * kTile + b * kBox, s.kvh, s.t, pol);
             }
           }
+          __syncwarp();
+          if (++st == p.nst) {
+            st = 0;
+            ++use;
+          }
+          if (j == s.j0) {
+            if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
+            if (elect_one()) {
+              mbar_expect_tx(q_full + qs, PANELS * R * 128);
+              for (int pn = 0; pn < PANELS; ++pn)
+                tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G,
+                            rb * p.mb, s.t, keep);
+            }
+            __syncwarp();
+          }
         }
-        f += s.n;
       }
-      if (dead)
-        for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
+      f += s.n;
     }
-    __syncwarp();
+    if (dead)
+      for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
   } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
-      int k = 0, seg = 0, fills[2] = {0, 0};
-      for (int f = beg; f < end;) {
-        const Segment s = segment_at(p, cum, f, end, 1);
-        for (int rb = 0; rb < p.RB; ++rb, ++seg) {
-          const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
-          guarded_wait(q_full + qs, quse & 1, dead, a.err);
-          for (int jj = 0; jj < s.n; ++jj, ++k) {
-            const int st = k % p.nst, use = k / p.nst;
-            guarded_wait(kv_full + st, use & 1, dead, a.err);
-            // buffer b belongs to warpgroup b, which waits for every one of its fills
-            const int b = jj & 1, fill = b ? fills[1]++ : fills[0]++;
-            if (fill > 0) guarded_wait(s_empty + b, (fill - 1) & 1, dead, a.err);
-            tc_after_sync();
-            const uint32_t ka = ring + st * lay.stage, qb = qbase + qs * lay.qslot;
+    const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
+    const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
+    const uint32_t qpanel = p.n16 * 128 >> 4;
+    int seg = 0, st = 0, use = 0, fills0 = 0, fills1 = 0;
+    for (int f = beg; f < end;) {
+      const Segment s = segment_at(p, tab, f, end, 1);
+      for (int rb = 0; rb < p.RB; ++rb, ++seg) {
+        const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+        guarded_wait(q_full + qs, quse & 1, dead, a.err);
+        for (int jj = 0; jj < s.n; ++jj) {
+          guarded_wait(kv_full + st, use & 1, dead, a.err);
+          // buffer b belongs to warpgroup b, which waits for every one of its fills
+          const int b = jj & 1, fill = b ? fills1++ : fills0++;
+          if (fill > 0) guarded_wait(s_empty + b, (fill - 1) & 1, dead, a.err);
+          tc_after_sync();
+          if (elect_one()) {
+            const uint32_t ka = ring_k + (st * lay.stage >> 4), qb = q_desc + (qs * lay.qslot >> 4);
 #pragma unroll
             for (int kk = 0; kk < PANELS * 4; ++kk)
-              tc_mma(tmem + b * kMaxRows, smem_desc(ka + (kk >> 2) * kPanel + (kk & 3) * 32, 16),
-                     smem_desc(qb + (kk >> 2) * p.n16 * 128 + (kk & 3) * 32, 16), id_qk, kk > 0);
+              tc_mma(tmem + b * kMaxRows, ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2,
+                     qb + (kk >> 2) * qpanel + (kk & 3) * 2, id_qk, kk > 0);
             tc_commit(s_full + b);
             tc_commit(kv_empty + st);
+            if (jj + 1 == s.n) tc_commit(q_empty + qs);
           }
-          tc_commit(q_empty + qs);
+          __syncwarp();
+          if (++st == p.nst) {
+            st = 0;
+            ++use;
+          }
         }
-        f += s.n;
       }
-      if (dead) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 1000000) {
-        }
+      f += s.n;
+    }
+    if (dead) {
+      const long long t0 = clock64();
+      while (clock64() - t0 < 1000000) {
       }
     }
-    __syncwarp();
   } else {
     const int grp = warp >> 2, wq = warp & 3;
     const int key = wq * 32 + lane;
@@ -883,8 +969,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     const uint32_t sbuf = tmem + lanes + grp * kMaxRows;
     int fill = 0;
     for (int f = beg; f < end;) {
-      const Segment s = segment_at(p, cum, f, end, 1);
-      const int len = trace_len(a, s.t);
+      const Segment s = segment_at(p, tab, f, end, 1);
       const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
       for (int rb = 0; rb < p.RB; ++rb) {
         named_bar_sync(1 + grp, 128);  // the last block's tables read
@@ -896,7 +981,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
         for (int jj = grp; jj < s.n; jj += 2, ++fill) {
           const int j = s.j0 + jj;
           const bool draft = j == s.nt - 1;
-          const int rows = tile_rows(len, s.nt, a.m, j);
+          const int rows = tile_rows(s.len, s.nt, a.m, j);
           guarded_wait(s_full + grp, fill & 1, dead, a.err);
           tc_after_sync();
           float w = 0.0f;
@@ -1025,9 +1110,9 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
   else if (p.n16 <= 32)
     rc = launch_attn<PANELS, 16, 2, BF16>(p, smem, st);
   else if (p.n16 <= 64)
-    rc = launch_attn<PANELS, 32, 2, BF16>(p, smem, st);
+    rc = launch_attn<PANELS, 16, 4, BF16>(p, smem, st);
   else
-    rc = launch_attn<PANELS, 64, 2, BF16>(p, smem, st);
+    rc = launch_attn<PANELS, 32, 4, BF16>(p, smem, st);
   if (rc != MB_OK) return rc;
   const int R = p.mb * p.G;
   return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.T * p.a.Hkv * p.RB, (R + kJoinRows - 1) / kJoinRows),
@@ -1057,8 +1142,12 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
       !tree_map(&p.mkd, a.kd, a.d, a.Hkv, a.kds[2], a.m, a.kds[1], a.T, a.kds[0], 1, a.m) ||
       !tree_map(&p.mvd, a.vd, a.d, a.Hkv, a.vds[2], a.m, a.vds[1], a.T, a.vds[0], 1, a.m) ||
       !tree_map(&p.mk, cache ? a.k : a.kd, a.d, cache ? a.Lmax : 1, a.ks[2], a.Hkv, cache ? a.ks[1] : 128, a.T,
-                cache ? a.ks[0] : 128, kBox, 1) ||
+                cache ? a.ks[0] : 128, kTile, 1) ||
       !tree_map(&p.mv, cache ? a.v : a.vd, a.d, cache ? a.Lmax : 1, a.vs[2], a.Hkv, cache ? a.vs[1] : 128, a.T,
+                cache ? a.vs[0] : 128, kTile, 1) ||
+      !tree_map(&p.mk_end, cache ? a.k : a.kd, a.d, cache ? a.Lmax : 1, a.ks[2], a.Hkv, cache ? a.ks[1] : 128, a.T,
+                cache ? a.ks[0] : 128, kBox, 1) ||
+      !tree_map(&p.mv_end, cache ? a.v : a.vd, a.d, cache ? a.Lmax : 1, a.vs[2], a.Hkv, cache ? a.vs[1] : 128, a.T,
                 cache ? a.vs[0] : 128, kBox, 1))
     return MB_ERR_LAUNCH;
   p.G = pl.G;
