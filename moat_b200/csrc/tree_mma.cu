@@ -43,7 +43,7 @@ constexpr float kSlack = 8.0f;       // p may reach 2^kSlack
 
 struct TreeMmaParams {
   TreeAttnArgs a;
-  CUtensorMap mq, mk, mv, mk_end, mv_end, mkd, mvd;
+  CUtensorMap mq, mk, mv, mk_end, mv_end, mkd, mvd;  // (seven in a row: prefetched by index)
   float* part;  // [2 * grid][rows][DP] unnormalised O of a unit's pieces
   float* ml;    // [2 * grid][2][kMaxRows] their m_ref and sum
   float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
@@ -114,6 +114,9 @@ __device__ __forceinline__ uint32_t instr_desc(bool bf16, int n, bool a_mn, bool
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
                                             int w, uint64_t policy) {
   asm volatile(
@@ -121,6 +124,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
       : "memory");
+}
+
+// 16 floats that lie 64-byte aligned in shared memory.
+__device__ __forceinline__ void load16(const float* p, float* r) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p + i);
+    r[i] = v.x;
+    r[i + 1] = v.y;
+    r[i + 2] = v.z;
+    r[i + 3] = v.w;
+  }
 }
 
 // One lane of a converged warp. Branches on it stay uniform for the compiler, so that
@@ -321,6 +336,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   bool dead = false;
 
   if (warp == 4 * WG) {  // TMA warp
+    if (lane < 7) prefetch_map(&p.mq + lane);
     if (lane == 0) {
       for (int i = 0; i < kMaxStages; ++i) {
         mbar_init(kv_full + i, 1);
@@ -525,37 +541,42 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
         const bool draft = j == s.nt - 1;
         const int rows = tile_rows(s.len, s.nt, a.m, j);
         const uint32_t sbuf = tmem + lanes + (k & 1) * kMaxRows + col0;
+        // which of this thread's rows see its key, a bit each
+        uint32_t see = key < rows ? ~0u : 0u;
         if (draft) {
           if (tid < kMaxRows) rowmask[tid] = my_mask;
           named_bar_sync(1, kSoft);
+          if (key < rows) {
+            see = 0;
+#pragma unroll 4
+            for (int i = 0; i < CW; ++i) see |= static_cast<uint32_t>((rowmask[col0 + i] >> key) & 1) << i;
+          }
         }
+        const bool full = !draft && rows == kTile;
         // Scores of rows i .. i + 15 less sub (log2 units), -inf for what a row does not see.
         // Sixteen at a time, read from TMEM again for the exponentials: with all of a thread's
         // scores in registers it spills, and with L1 given to shared memory a spill goes to L2
         // (5,600 cycles for a tile's exponentials of 64 rows).
         float x[16];
-        auto form = [&](int i, auto sub) {
+        auto form = [&](int i, bool less_ref) {
+          float r[16];
+          if (less_ref) load16(refs + i, r);
           tc_ld16(sbuf + i, x);
           tc_wait_ld();
 #pragma unroll
-          for (int u = 0; u < 16; ++u) x[u] = fmaf(x[u], sc, sub(i + u));
-          if (draft) {
+          for (int u = 0; u < 16; ++u) x[u] = less_ref ? fmaf(x[u], sc, -r[u]) : x[u] * sc;
+          if (!full) {
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
-              if (key >= rows || !((rowmask[col0 + i + u] >> (key & 63)) & 1)) x[u] = -INFINITY;
-          } else if (key >= rows) {
-#pragma unroll
-            for (int u = 0; u < 16; ++u) x[u] = -INFINITY;
+            for (int u = 0; u < 16; ++u) x[u] = (see >> (i + u)) & 1 ? x[u] : -INFINITY;
           }
         };
-        auto less_ref = [&](int i) { return -refs[i]; };
         guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < CW; i += 16)
           if (col0 + i < p.n16) {
-            form(i, less_ref);
+            form(i, true);
 #pragma unroll
             for (int u = 0; u < 16; ++u) top = fmaxf(top, x[u]);
           }
@@ -567,7 +588,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 #pragma unroll
           for (int i = 0; i < CW; i += 16)
             if (col0 + i < p.n16) {
-              form(i, [](int) { return 0.0f; });
+              form(i, false);
               float mine = 0.0f;
 #pragma unroll
               for (int u = 0; u < 16; ++u) {
@@ -591,13 +612,15 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 #pragma unroll
           for (int i = 0; i < CW; i += 16)
             if (col0 + i < p.n16) {
+              float r[16];
+              load16(fade + i, r);
 #pragma unroll
-              for (int u = 0; u < 16; ++u) l[i + u] *= fade[i + u];
+              for (int u = 0; u < 16; ++u) l[i + u] *= r[u];
               if (jj > 0) {
                 tc_ld16(ob + i, x);
                 tc_wait_ld();
 #pragma unroll
-                for (int u = 0; u < 16; ++u) x[u] *= fade[i + u];
+                for (int u = 0; u < 16; ++u) x[u] *= r[u];
                 tc_st16(ob + i, x);
               }
             }
@@ -609,7 +632,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 #pragma unroll
         for (int i = 0; i < CW; i += 16)
           if (col0 + i < p.n16) {
-            if (CW > 16 || raise) form(i, less_ref);
+            if (CW > 16 || raise) form(i, true);
             uint32_t pk[8];
 #pragma unroll
             for (int u = 0; u < 16; u += 2) {
@@ -688,13 +711,14 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
         if (row >= R) break;
         float o[16];
         tc_ld16(ob + i, o);
-        tc_wait_ld();
         if (whole) {
+          float inv[16];
+          load16(scratch + 4 * kMaxRows + row, inv);
+          tc_wait_ld();
 #pragma unroll
           for (int u = 0; u < 16; ++u, ++row) {
             if (u % 4 == 0) asm volatile("" ::: "memory");
-            const float inv = scratch[4 * kMaxRows + row];
-            if (row < R && nd < a.m && key < a.d) *out = round16<BF16>(inv == 0.0f ? 0.0f : o[u] * inv);
+            if (row < R && nd < a.m && key < a.d) *out = round16<BF16>(inv[u] == 0.0f ? 0.0f : o[u] * inv[u]);
             out += a.os[2];
             if (++gh == p.G) {
               gh = 0;
@@ -703,6 +727,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
             }
           }
         } else {
+          tc_wait_ld();
 #pragma unroll
           for (int u = 0; u < 16; ++u, ++row, part += DP)
             if (row < R && key < DP) *part = o[u];
@@ -986,17 +1011,18 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
           tc_after_sync();
           float w = 0.0f;
           for (int n = 0; n < p.n16; n += 16) {
-            float x[16];
+            float x[16], ls[16];
+            load16(lse + n, ls);
             tc_ld16(sbuf + n, x);
             tc_wait_ld();
             float part = 0.0f;
             if (draft) {
 #pragma unroll
               for (int u = 0; u < 16; ++u)
-                part += (rowmask[n + u] >> (key & 63)) & 1 ? ex2(fmaf(x[u], sc, -lse[n + u])) : 0.0f;
+                part += (rowmask[n + u] >> (key & 63)) & 1 ? ex2(fmaf(x[u], sc, -ls[u])) : 0.0f;
             } else {
 #pragma unroll
-              for (int u = 0; u < 16; ++u) part += ex2(fmaf(x[u], sc, -lse[n + u]));
+              for (int u = 0; u < 16; ++u) part += ex2(fmaf(x[u], sc, -ls[u]));
             }
             w += part;
           }
