@@ -36,7 +36,7 @@ namespace mb {
 constexpr int kTile = 128;      // keys per tile
 constexpr int kBox = 32;        // rows per TMA box of a unit's last cached tile: no more boxes than it needs
 constexpr int kMaxRows = 128;   // rows of a block
-constexpr int kMaxTraces = 127;  // per launch (their lengths and tile counts lie in shared memory)
+constexpr int kMaxTraces = 127;  // per launch (the table of their lengths lies in shared memory)
 constexpr int kPanel = kTile * 128;  // bytes of a 64-column panel of a tile (128-byte swizzled rows)
 constexpr float kNoRef = -1e30f;     // m_ref before any visible key
 constexpr float kSlack = 8.0f;       // p may reach 2^kSlack
@@ -49,6 +49,7 @@ struct TreeMmaParams {
   float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
   int t0, T;    // traces of this launch
   int RB, mb, G, n16, grid, nst, nq;
+  int whole;  // every unit in one CTA: nothing to join
 };
 
 // --- tcgen05 / TMEM -----------------------------------------------------------
@@ -89,6 +90,15 @@ __device__ __forceinline__ void tc_ld16(uint32_t addr, float* r) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) r[i] = __uint_as_float(u[i]);
+}
+__device__ __forceinline__ void tc_ld4(uint32_t addr, float* r) {
+  uint32_t u[4];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+               : "r"(addr)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __uint_as_float(u[i]);
 }
 __device__ __forceinline__ void tc_st16(uint32_t addr, const float* r) {
   uint32_t u[16];
@@ -207,40 +217,51 @@ __device__ __forceinline__ float column_sums(float* v, int lane) {
 __device__ __forceinline__ int trace_len(const TreeAttnArgs& a, int t) { return max(0, min(a.lens[t], a.Lmax)); }
 __device__ __forceinline__ int trace_tiles(int len) { return (len + kTile - 1) / kTile + 1; }
 
-// First tile of CTA c of g when w tiles are cut evenly.
+// First position of CTA c of g when a sequence of w is cut evenly.
 __device__ __forceinline__ int cut(int64_t w, int c, int g) { return static_cast<int>(w * c / g); }
 
 struct Segment {  // a run of tiles of one unit
   int t, kvh, rb, len, nt, j0, n;
 };
 
-// Lengths of the launch's traces and the tiles before each, in shared memory.
+// Lengths of the launch's traces and where each begins in the sequence, in shared memory.
 struct TraceTable {
   int cum[kMaxTraces + 1];
   int len[kMaxTraces + 1];
 };
 
-// The segment that begins at flat tile f (at most up to `end`), RB row blocks per (trace, KV
-// head).
-__device__ __forceinline__ Segment segment_at(const TreeMmaParams& p, const TraceTable& tab, int f, int end, int RB) {
-  int lo = 0, hi = p.T - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (tab.cum[mid] <= f)
-      lo = mid;
-    else
-      hi = mid - 1;
+// Starting and ending a piece costs about as much as a tile; it counts as one in the sequence,
+// before the unit's first tile (without it a CTA with many short units finished last by 3x).
+constexpr int kUnitCost = 1;
+
+__device__ __forceinline__ int unit_span(int nt) { return nt + kUnitCost; }
+
+// The next segment at or after position f of the sequence (RB row blocks per trace and KV head);
+// moves f past it. False at the end of this CTA's share.
+__device__ __forceinline__ bool next_segment(const TreeMmaParams& p, const TraceTable& tab, int& f, int end, int RB,
+                                             Segment& s) {
+  while (f < end) {
+    int lo = 0, hi = p.T - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tab.cum[mid] <= f)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    s.t = p.t0 + lo;
+    s.len = tab.len[lo];
+    s.nt = trace_tiles(s.len);
+    const int span = unit_span(s.nt), rem = f - tab.cum[lo], u = rem / span;
+    const int tile0 = tab.cum[lo] + u * span + kUnitCost;  // position of the unit's first tile
+    s.kvh = u / RB;
+    s.rb = u - s.kvh * RB;
+    s.j0 = max(0, f - tile0);
+    s.n = min(s.nt, end - tile0) - s.j0;
+    f = s.n > 0 ? tile0 + s.j0 + s.n : end;
+    if (s.n > 0) return true;
   }
-  Segment s;
-  s.t = p.t0 + lo;
-  s.len = tab.len[lo];
-  s.nt = trace_tiles(s.len);
-  const int rem = f - tab.cum[lo], u = rem / s.nt;
-  s.j0 = rem - u * s.nt;
-  s.kvh = u / RB;
-  s.rb = u - s.kvh * RB;
-  s.n = min(s.nt - s.j0, end - f);
-  return s;
+  return false;
 }
 
 // Valid rows of tile j of a unit (its last tile holds the drafted rows).
@@ -254,7 +275,7 @@ __device__ __forceinline__ void prefix_tiles(const TreeMmaParams& p, TraceTable&
   for (int c = 0; c < p.T; c += 32) {
     const int t = c + lane;
     const int len = t < p.T ? trace_len(p.a, p.t0 + t) : 0;
-    int v = t < p.T ? trace_tiles(len) * units : 0;
+    int v = t < p.T ? unit_span(trace_tiles(len)) * units : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -307,6 +328,16 @@ __host__ __device__ inline TreeSmem tree_smem(int panels, int n16, int nst, int 
   return s;
 }
 
+// Rows R .. n16 - 1 of every panel of the Q slots: the boxes never write them, they stay zero.
+__device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16, int R, int tid, int threads) {
+  const int per = (n16 - R) * 8;  // 16-byte pieces per panel
+  for (int i = tid; i < panels * per; i += threads) {
+    const int pn = i / per;
+    *reinterpret_cast<uint4*>(q + (pn * n16 + R) * 128 + (i - pn * per) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+
 // PANELS: 64-column panels of the head dim (1: d <= 64, 2: d <= 128). CW: rows per softmax
 // warpgroup, WG warpgroups.
 template <int PANELS, int CW, int WG, bool BF16>
@@ -356,23 +387,34 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   } else if (warp == 4 * WG + 1) {
     tmem_alloc(smem_u32(tmem_base), 512);
   } else if (warp < 4 * WG) {
-    // rows beyond R of the Q slots stay zero (the boxes never write them)
-    uint4* qz = reinterpret_cast<uint4*>(smem + lay.q);
-    for (uint32_t i = tid; i < p.nq * lay.qslot / 16; i += kSoft) qz[i] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
+    zero_query_tail(smem + lay.q, PANELS * p.nq, p.n16, R, tid, kSoft);
     for (int i = tid; i < kMaxRows; i += kSoft) ref[i] = kNoRef;
   }
   pdl_wait();  // the lengths, masks, queries and drafts may come from the kernel before
   pdl_launch_dependents();
-  if (warp == 0) prefix_tiles(p, tab, lane, a.Hkv * p.RB);
   tc_before_sync();
-  __syncthreads();
+  if (warp == 4 * WG) {  // builds the table and goes straight on to its loads
+    prefix_tiles(p, tab, lane, a.Hkv * p.RB);
+    __syncwarp();
+    asm volatile("bar.arrive 2, %0;" ::"n"(128 * WG + 64) : "memory");
+  } else {
+    named_bar_sync(2, 128 * WG + 64);
+  }
   tc_after_sync();
-  const uint32_t tmem = *tmem_base;
-  const int total = tab.cum[p.T];
-  const int g = min(p.grid, total);  // CTAs with work
   const int c = blockIdx.x;
-  const int beg = c < g ? cut(total, c, g) : 0, end = c < g ? cut(total, c + 1, g) : 0;
+  int beg = 0, end = 0;
+  if (p.whole) {  // one unit per CTA
+    const int units = a.Hkv * p.RB, t = c / units;
+    const int span = unit_span(trace_tiles(tab.len[t]));
+    beg = tab.cum[t] + (c - t * units) * span;
+    end = beg + span;
+  } else {
+    const int total = tab.cum[p.T], g = min(p.grid, total);  // CTAs with work
+    if (c < g) {
+      beg = cut(total, c, g);
+      end = cut(total, c + 1, g);
+    }
+  }
   const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q), pbase = smem_u32(smem + lay.p);
 
   if (warp == 4 * WG) {
@@ -386,8 +428,8 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
       asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
     const uint64_t keep = policy_evict_last();
     int item = 0, seg = 0, st = 0, use = 0;  // K and V tiles of the ring (stage, times used), segments
-    for (int f = beg; f < end; ++seg) {
-      const Segment s = segment_at(p, tab, f, end, p.RB);
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
       const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
       for (int j = s.j0; j < s.j0 + s.n; ++j) {
         const bool draft = j == s.nt - 1;
@@ -431,7 +473,6 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
           __syncwarp();
         }
       }
-      f += s.n;
     }
     if (dead)  // copies still in flight must land before this CTA's shared memory goes
       for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
@@ -441,19 +482,19 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
     const uint32_t id_pv = instr_desc(BF16, p.n16, true, true);
     const uint32_t ring_k = smem_desc(ring, 16), ring_v = smem_desc(ring, kPanel);
     const uint32_t q_desc = smem_desc(qbase, 16), p_desc = smem_desc(pbase, kPanel);
-    const int n = end - beg;
+    const uint32_t tmem = *tmem_base;
     // two cursors over the same tiles: scores run one tile ahead of the value product
     Segment sq = {}, sv = {};
-    int jq = 0, jv = 0, nq = 0, nv = 0, seg_q = -1, seg_v = -1;
+    int jq = 0, jv = 0, seg_q = -1, seg_v = -1, fq = beg, fv = beg;
+    bool more = true;
     int st_k = 0, use_k = 0, st_v = 1, use_v = 0;  // their ring stages: tile k's K and V are items 2k, 2k + 1
-    for (int k = 0; k <= n; ++k) {
-      if (k < n) {
-        if (jq == nq) {
-          sq = segment_at(p, tab, beg + k, end, p.RB);
-          jq = 0;
-          nq = sq.n;
-          ++seg_q;
-        }
+    for (int k = 0; more; ++k) {
+      if (jq == sq.n) {
+        more = next_segment(p, tab, fq, end, p.RB, sq);
+        jq = 0;
+        ++seg_q;
+      }
+      if (more) {
         const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
         if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
         guarded_wait(kv_full + st_k, use_k & 1, dead, a.err);
@@ -469,7 +510,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
                    qb + (kk >> 2) * qpanel + (kk & 3) * 2, id_qk, kk > 0);
           tc_commit(s_full + (k & 1));
           tc_commit(kv_empty + st_k);
-          if (jq == nq) tc_commit(q_empty + qs);
+          if (jq == sq.n) tc_commit(q_empty + qs);
         }
         __syncwarp();
         st_k += 2;
@@ -480,10 +521,9 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
       }
       if (k > 0) {
         const int e = k - 1;
-        if (jv == nv) {
-          sv = segment_at(p, tab, beg + e, end, p.RB);
+        if (jv == sv.n) {
+          next_segment(p, tab, fv, end, p.RB, sv);
           jv = 0;
-          nv = sv.n;
           ++seg_v;
         }
         guarded_wait(kv_full + st_v, use_v & 1, dead, a.err);
@@ -527,9 +567,10 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 #pragma unroll
     for (int i = 0; i < CW; ++i) l[i] = 0.0f;
     float* scratch = reinterpret_cast<float*>(smem + lay.p);  // P's space, while no product reads it
+    const uint32_t tmem = *tmem_base;
     int seg = 0, k = 0, vst = 1, vuse = 0;
-    for (int f = beg; f < end; ++seg) {
-      const Segment s = segment_at(p, tab, f, end, p.RB);
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
       // this row's mask, and the rows of the draft that any node sees (loads in flight over the
       // first tile)
       const uint64_t* mk = a.masks + s.t * a.mask_stride;
@@ -585,7 +626,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
           // P's space and O are free once the previous value product has finished
           if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
           tc_after_sync();
-#pragma unroll
+#pragma unroll 1  // rarely run: short code rather than fast code (cold instructions cost most)
           for (int i = 0; i < CW; i += 16)
             if (col0 + i < p.n16) {
               form(i, false);
@@ -608,23 +649,23 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
           }
           named_bar_sync(1, kSoft);
           const float* fade = scratch + 4 * kMaxRows + col0;
-          const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
+          if (jj > 0) {
+            const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
 #pragma unroll
-          for (int i = 0; i < CW; i += 16)
-            if (col0 + i < p.n16) {
-              float r[16];
-              load16(fade + i, r);
-#pragma unroll
-              for (int u = 0; u < 16; ++u) l[i + u] *= r[u];
-              if (jj > 0) {
+            for (int i = 0; i < CW; ++i) l[i] *= fade[i];
+#pragma unroll 1
+            for (int i = 0; i < CW; i += 16)
+              if (col0 + i < p.n16) {
+                float r[16];
+                load16(fade + i, r);
                 tc_ld16(ob + i, x);
                 tc_wait_ld();
 #pragma unroll
                 for (int u = 0; u < 16; ++u) x[u] *= r[u];
                 tc_st16(ob + i, x);
               }
-            }
-          tc_wait_st();
+            tc_wait_st();
+          }
           named_bar_sync(1, kSoft);  // scratch read: its space becomes P again
         }
         // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
@@ -707,30 +748,29 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
       int row = col0, nd = s.rb * p.mb + col0 / p.G, gh = col0 % p.G;  // row, its node, its head of the group
       uint16_t* out = a.out + s.t * a.os[0] + nd * a.os[1] + (s.kvh * p.G + gh) * a.os[2] + key;
       float* part = p.part + (static_cast<int64_t>(slot) * R + col0) * DP + key;
-      for (int i = 0; i < CW; i += 16) {
-        if (row >= R) break;
-        float o[16];
-        tc_ld16(ob + i, o);
-        if (whole) {
-          float inv[16];
-          load16(scratch + 4 * kMaxRows + row, inv);
-          tc_wait_ld();
+#pragma unroll 1
+      for (int i = 0; i < CW && row < R; i += 4) {
+        float o[4];
+        tc_ld4(ob + i, o);
+        const float4 inv = *reinterpret_cast<const float4*>(scratch + 4 * kMaxRows + row);
+        tc_wait_ld();
 #pragma unroll
-          for (int u = 0; u < 16; ++u, ++row) {
-            if (u % 4 == 0) asm volatile("" ::: "memory");
-            if (row < R && nd < a.m && key < a.d) *out = round16<BF16>(inv[u] == 0.0f ? 0.0f : o[u] * inv[u]);
-            out += a.os[2];
-            if (++gh == p.G) {
-              gh = 0;
-              ++nd;
-              out += a.os[1] - p.G * a.os[2];
+        for (int u = 0; u < 4; ++u, ++row) {
+          const float scale = u == 0 ? inv.x : u == 1 ? inv.y : u == 2 ? inv.z : inv.w;
+          if (row < R) {
+            if (!whole) {
+              if (key < DP) *part = o[u];
+              part += DP;
+            } else {
+              if (nd < a.m && key < a.d) *out = round16<BF16>(scale == 0.0f ? 0.0f : o[u] * scale);
+              out += a.os[2];
+              if (++gh == p.G) {
+                gh = 0;
+                ++nd;
+                out += a.os[1] - p.G * a.os[2];
+              }
             }
           }
-        } else {
-          tc_wait_ld();
-#pragma unroll
-          for (int u = 0; u < 16; ++u, ++row, part += DP)
-            if (row < R && key < DP) *part = o[u];
         }
       }
       tc_before_sync();
@@ -738,13 +778,12 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 #pragma unroll
       for (int i = 0; i < CW; ++i) l[i] = 0.0f;
       named_bar_sync(1, kSoft);  // scratch read, m_ref reset
-      f += s.n;
     }
   }
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  if (warp == 4 * WG + 1) tmem_dealloc(tmem, 512);
+  if (warp == 4 * WG + 1) tmem_dealloc(*tmem_base, 512);
 }
 
 // Joins the pieces of the units that were cut between CTAs, in order. One CTA per unit and
@@ -764,7 +803,7 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   const int t = blockIdx.x / units, u = blockIdx.x - t * units;  // trace of this launch
   int before = 0, total = 0;
   for (int i = tid; i < p.T; i += kJoinBlock) {
-    const int n = trace_tiles(trace_len(a, p.t0 + i)) * units;
+    const int n = unit_span(trace_tiles(trace_len(a, p.t0 + i))) * units;
     total += n;
     before += i < t ? n : 0;
   }
@@ -785,9 +824,9 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
     before += red[1][w];
   }
   const int nt = trace_tiles(trace_len(a, p.t0 + t));
-  const int f0 = before + u * nt, f1 = f0 + nt - 1;
+  const int f0 = before + u * unit_span(nt) + kUnitCost, f1 = f0 + nt - 1;  // its first and last tile
   const int g = min(p.grid, total);
-  // the CTA that holds tile f: the largest c with cut(c) <= f
+  // the CTA that holds position f: the largest c with cut(c) <= f
   const int c0 = static_cast<int>(((static_cast<int64_t>(f0) + 1) * g - 1) / total);
   const int c1 = static_cast<int>(((static_cast<int64_t>(f1) + 1) * g - 1) / total);
   if (c0 == c1) return;
@@ -875,9 +914,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   } else if (warp == 9) {
     tmem_alloc(smem_u32(tmem_base), 256);
   } else {
-    uint4* qz = reinterpret_cast<uint4*>(smem + lay.q);
-    for (uint32_t i = tid; i < p.nq * lay.qslot / 16; i += kSoft) qz[i] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
+    zero_query_tail(smem + lay.q, PANELS * p.nq, p.n16, R, tid, kSoft);
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -896,8 +933,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   if (warp == 8) {
     const uint64_t policy = policy_evict_first(), keep = policy_evict_last();
     int item = 0, seg = 0, st = 0, use = 0;
-    for (int f = beg; f < end;) {
-      const Segment s = segment_at(p, tab, f, end, 1);
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, 1, s);) {
       for (int rb = 0; rb < p.RB; ++rb, ++seg) {
         const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
         const uint64_t pol = rb + 1 < p.RB ? keep : policy;
@@ -940,7 +977,6 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
           }
         }
       }
-      f += s.n;
     }
     if (dead)
       for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
@@ -949,8 +985,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
     const uint32_t qpanel = p.n16 * 128 >> 4;
     int seg = 0, st = 0, use = 0, fills0 = 0, fills1 = 0;
-    for (int f = beg; f < end;) {
-      const Segment s = segment_at(p, tab, f, end, 1);
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, 1, s);) {
       for (int rb = 0; rb < p.RB; ++rb, ++seg) {
         const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
         guarded_wait(q_full + qs, quse & 1, dead, a.err);
@@ -977,7 +1013,6 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
           }
         }
       }
-      f += s.n;
     }
     if (dead) {
       const long long t0 = clock64();
@@ -993,8 +1028,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     uint64_t* rowmask = mask_s + grp * kMaxRows;
     const uint32_t sbuf = tmem + lanes + grp * kMaxRows;
     int fill = 0;
-    for (int f = beg; f < end;) {
-      const Segment s = segment_at(p, tab, f, end, 1);
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, 1, s);) {
       const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
       for (int rb = 0; rb < p.RB; ++rb) {
         named_bar_sync(1 + grp, 128);  // the last block's tables read
@@ -1035,7 +1070,6 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
           }
         }
       }
-      f += s.n;
     }
   }
   tc_before_sync();
@@ -1047,6 +1081,9 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+// Caches this short are not cut: a CTA does its whole unit and no join follows.
+constexpr int kWholeRows = 512;
+
 struct TreePlan {
   int G, RB, mb, n16, panels, nst, nq, grid;
   uint32_t smem;
@@ -1125,7 +1162,8 @@ template <int PANELS, int CW, int WG, bool BF16>
 static int launch_attn(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
   auto kern = k_tree_attn<PANELS, CW, WG, BF16>;
   const int rc = allow_smem(kern);
-  return rc != MB_OK ? rc : launch_with_pdl(kern, dim3(p.grid), dim3(128 * WG + 64), smem, st, p);
+  return rc != MB_OK ? rc : launch_with_pdl(kern, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid), dim3(128 * WG + 64), smem,
+                                                st, p);
 }
 
 template <int PANELS, bool BF16>
@@ -1139,7 +1177,7 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
     rc = launch_attn<PANELS, 16, 4, BF16>(p, smem, st);
   else
     rc = launch_attn<PANELS, 32, 4, BF16>(p, smem, st);
-  if (rc != MB_OK) return rc;
+  if (rc != MB_OK || p.whole) return rc;
   const int R = p.mb * p.G;
   return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.T * p.a.Hkv * p.RB, (R + kJoinRows - 1) / kJoinRows),
                          dim3(kJoinBlock), 0, st, p);
@@ -1193,6 +1231,7 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   for (int t0 = 0; t0 < a.T; t0 += kMaxTraces) {
     p.t0 = t0;
     p.T = std::min(kMaxTraces, a.T - t0);
+    p.whole = a.Lmax <= kWholeRows && p.T * a.Hkv * pl.RB <= pl.grid;
     int rc;
     if (pl.panels == 2)
       rc = bf16 ? launch_all<2, true>(p, pl.smem, st) : launch_all<2, false>(p, pl.smem, st);
