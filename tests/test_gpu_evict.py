@@ -71,6 +71,9 @@ def run(cuda, layers, T, Hkv, Lmax, d, lens, budget, recent, sinks, scores=None,
     (1, 1, 1, 5000, 33, [4999], 3333, 10, 1),
     (3, 2, 2, 130, 80, [130, 129], 129, 0, 0),
     (1, 1, 2, 70000, 64, [69999], 20000, 300, 4),
+    (40, 1, 8, 1500, 64, [1400], 700, 64, 4),  # the units alone fill the GPU
+    (1, 2, 40, 9000, 64, [8999, 7000], 4000, 100, 4),
+    (1, 1, 1, 400003, 8, [400001], 150000, 300, 4),
 ])
 def test_evict(cuda, layers, T, Hkv, Lmax, d, lens, budget, recent, sinks, in_place):
     run(cuda, layers, T, Hkv, Lmax, d, lens, budget, recent, sinks, in_place=in_place, seed=Lmax)
