@@ -381,9 +381,10 @@ int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
  * scores_out (optional, [T, Hkv, Lmax] fp32): row l < lens[t] gets scores[l] (0 if scores
  * is NULL; scores may be scores_out) plus its weight summed over the nodes and heads;
  * draft_scores [T, Hkv, m] the draft rows' sums. No atomics: results repeat bit for bit.
- * The workspace needs no initial contents. dev_err (optional) receives MB_DEVERR_TIMEOUT if a
+ * The workspace (with_scores = 1 if scores_out is given) needs no initial contents. dev_err (optional) receives MB_DEVERR_TIMEOUT if a
  * bounded wait inside a kernel gives up (the output is then undefined). */
-size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d);
+size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d,
+                                   int32_t with_scores);
 int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
                      const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* masks, int32_t shared_masks,
                      uint16_t* out, const int64_t* strides, int32_t is_bf16, int32_t T, int32_t m, int32_t H,

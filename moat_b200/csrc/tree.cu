@@ -282,10 +282,11 @@ using namespace mb;
 
 extern "C" {
 
-size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d) {
+size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d,
+                                   int32_t with_scores) {
   if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim) return 0;
   return std::max((static_cast<size_t>(T) * H * m * 4 + 255) / 256 * 256,  // lse of the general path
-                  tree_mma_workspace(T, m, H, Hkv, Lmax, d));
+                  tree_mma_workspace(T, m, H, Hkv, Lmax, d, with_scores != 0));
 }
 
 int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
@@ -305,7 +306,8 @@ int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t*
       !aligned(v_draft, 2) || !aligned(out, 2) || !aligned(lens, 4) || !aligned(masks, 8) || !aligned(scores, 4) ||
       !aligned(scores_out, 4) || !aligned(draft_scores, 4))
     return MB_ERR_ALIGN;
-  if (!workspace || workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d)) return MB_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, scores_out != nullptr))
+    return MB_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
   TreeAttnArgs a;
   a.q = q;
@@ -336,7 +338,7 @@ int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t*
   a.scores_out = scores_out;
   a.draft_scores = draft_scores;
   a.err = dev_err;
-  if (tree_mma_workspace(T, m, H, Hkv, Lmax, d) && tree_mma_takes(a))
+  if (tree_mma_workspace(T, m, H, Hkv, Lmax, d, false) && tree_mma_takes(a))
     return tree_mma_launch(a, is_bf16 != 0, workspace, stream);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* lse = scores_out ? static_cast<float*>(workspace) : nullptr;

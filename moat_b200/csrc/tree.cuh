@@ -23,7 +23,7 @@ struct TreeAttnArgs {
 };
 
 // Tensor-core path. 0 bytes: the sizes are not among those it takes.
-size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d);
+size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d, bool with_scores);
 // Whether pointers and strides suit its tensor maps.
 bool tree_mma_takes(const TreeAttnArgs& a);
 int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream);

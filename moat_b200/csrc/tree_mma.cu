@@ -47,6 +47,9 @@ struct TreeMmaParams {
   float* part;  // [2 * grid][rows][DP] unnormalised O of a unit's pieces
   float* ml;    // [2 * grid][2][kMaxRows] their m_ref and sum
   float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
+  float* kept;  // [units][R][kept_len] scores of the cached rows, kept for the weight pass, or null
+  float* kept_draft;  // [units][R][64] of the drafted rows
+  int kept_len;
   int t0, T;    // traces of this launch
   int RB, mb, G, n16, grid, nst, nq;
   int whole;  // every unit in one CTA: nothing to join
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
     // a cache that is read once streams past what L2 should keep; several row blocks or the
     // weight pass read it again
     uint64_t policy;
-    if (p.RB == 1 && !p.lse)
+    if (p.RB == 1 && (!p.lse || p.kept))
       policy = policy_evict_first();
     else
       asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
@@ -668,12 +671,30 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
           }
           named_bar_sync(1, kSoft);  // scratch read: its space becomes P again
         }
+        float* keep = nullptr;  // where this key's scores go
+        int64_t keep_step = 0;
+        if (CW == 16 && WG == 1 && p.kept && key < rows) {
+          const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
+          keep_step = draft ? 64 : p.kept_len;
+          keep = draft ? p.kept_draft + unit * R * 64 + key : p.kept + unit * R * p.kept_len + j * kTile + key;
+        }
         // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
         uint8_t* prow = smem + lay.p + key * 128;
 #pragma unroll
         for (int i = 0; i < CW; i += 16)
           if (col0 + i < p.n16) {
-            if (CW > 16 || raise) form(i, true);
+            if (CW == 16 && WG == 1 && p.kept) {
+              form(i, false);
+              float r[16];
+              load16(refs, r);
+#pragma unroll
+              for (int u = 0; u < 16; ++u) {
+                if (keep && u < R) keep[u * keep_step] = x[u];
+                x[u] -= r[u];
+              }
+            } else if (CW > 16 || raise) {
+              form(i, true);
+            }
             uint32_t pk[8];
 #pragma unroll
             for (int u = 0; u < 16; u += 2) {
@@ -1078,6 +1099,42 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   if (warp == 9) tmem_dealloc(tmem, 256);
 }
 
+// The same sums where the attention kept its scores (few rows): a thread per four cached rows.
+// R reads of four bytes per row instead of 2 d bytes of its key.
+constexpr int kKeptBlock = 128;
+
+__global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_constant__ TreeMmaParams p) {
+  __shared__ float lse[16];
+  pdl_wait();
+  pdl_launch_dependents();
+  const TreeAttnArgs& a = p.a;
+  const int R = p.mb * p.G, tid = threadIdx.x;
+  const int t = p.t0 + blockIdx.y / a.Hkv;
+  const int64_t unit = static_cast<int64_t>(p.t0) * a.Hkv + blockIdx.y;
+  const int len = trace_len(a, t), l0 = (blockIdx.x * kKeptBlock + tid) * 4;
+  if (blockIdx.x * kKeptBlock * 4 >= len && blockIdx.x > 0) return;
+  if (tid < R) lse[tid] = p.lse[unit * kMaxRows + tid];
+  __syncthreads();
+  if (l0 < len) {
+    float w[4] = {};
+    const float* x = p.kept + unit * R * p.kept_len + l0;
+    for (int r = 0; r < R; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(r) * p.kept_len);
+      w[0] += ex2(v.x - lse[r]);
+      w[1] += ex2(v.y - lse[r]);
+      w[2] += ex2(v.z - lse[r]);
+      w[3] += ex2(v.w - lse[r]);
+    }
+    const int64_t at = unit * a.Lmax + l0;
+    for (int i = 0; i < 4 && l0 + i < len; ++i) a.scores_out[at + i] = (a.scores ? a.scores[at + i] : 0.0f) + w[i];
+  }
+  if (blockIdx.x == 0 && tid < a.m) {
+    float w = 0.0f;
+    for (int r = 0; r < R; ++r) w += ex2(p.kept_draft[(unit * R + r) * 64 + tid] - lse[r]);
+    a.draft_scores[unit * a.m + tid] = w;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -1112,13 +1169,19 @@ static bool tree_plan(int T, int m, int H, int Hkv, int Lmax, int d, TreePlan* p
   return pl->nst >= 4;
 }
 
-size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d) {
+// Rows whose scores are kept for the weight pass rather than formed again from K.
+constexpr int kKeptRows = 16;
+
+size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d, bool with_scores) {
   TreePlan pl;
   if (!tree_plan(T, m, H, Hkv, Lmax, d, &pl)) return 0;
   const size_t part = static_cast<size_t>(2) * pl.grid * pl.mb * pl.G * pl.panels * 64 * 4;
   const size_t ml = static_cast<size_t>(2) * pl.grid * 2 * kMaxRows * 4;
+  if (!with_scores) return part + ml + 256;
   const size_t lse = static_cast<size_t>(T) * Hkv * pl.RB * kMaxRows * 4;
-  return part + ml + lse + 256;
+  const int R = pl.mb * pl.G;
+  const size_t kept = R <= kKeptRows ? static_cast<size_t>(T) * Hkv * R * ((Lmax + 3) / 4 * 4 + 64) * 4 : 0;
+  return part + ml + lse + kept + 256;
 }
 
 bool tree_mma_takes(const TreeAttnArgs& a) {
@@ -1148,22 +1211,27 @@ static bool tree_map(CUtensorMap* map, const void* base, int d, int n0, int64_t 
   return encode_tmap_4d_u16(map, base, dims, strides, box);
 }
 
-// Lets a kernel take all of an SM's shared memory (a host-side attribute of the function).
-template <typename Kern>
-static int allow_smem(Kern kern) {
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) {
+// Lets a kernel take all of an SM's shared memory, once per device.
+template <void (*KERN)(TreeMmaParams)>
+static int allow_smem() {
+  static bool done[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_ERR_LAUNCH;
+  if (done[dev]) return MB_OK;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) {
     (void)cudaGetLastError();
     return MB_ERR_LAUNCH;
   }
+  done[dev] = true;
   return MB_OK;
 }
 
 template <int PANELS, int CW, int WG, bool BF16>
 static int launch_attn(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  auto kern = k_tree_attn<PANELS, CW, WG, BF16>;
-  const int rc = allow_smem(kern);
-  return rc != MB_OK ? rc : launch_with_pdl(kern, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid), dim3(128 * WG + 64), smem,
-                                                st, p);
+  const int rc = allow_smem<k_tree_attn<PANELS, CW, WG, BF16>>();
+  if (rc != MB_OK) return rc;
+  return launch_with_pdl(k_tree_attn<PANELS, CW, WG, BF16>, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid),
+                         dim3(128 * WG + 64), smem, st, p);
 }
 
 template <int PANELS, bool BF16>
@@ -1185,15 +1253,20 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
 
 template <int PANELS, bool BF16>
 static int launch_weights(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  auto kern = k_tree_weights<PANELS, BF16>;
-  const int rc = allow_smem(kern);
-  return rc != MB_OK ? rc : launch_with_pdl(kern, dim3(p.grid), dim3(kWeightThreads), smem, st, p);
+  const int rc = allow_smem<k_tree_weights<PANELS, BF16>>();
+  if (rc != MB_OK) return rc;
+  return launch_with_pdl(k_tree_weights<PANELS, BF16>, dim3(p.grid), dim3(kWeightThreads), smem, st, p);
 }
 
 template <int PANELS, bool BF16>
 static int launch_all(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
   const int rc = launch_rows<PANELS, BF16>(p, smem, st);
-  return rc != MB_OK || !p.lse ? rc : launch_weights<PANELS, BF16>(p, smem, st);
+  if (rc != MB_OK || !p.lse) return rc;
+  if (p.kept)
+    return launch_with_pdl(k_tree_weights_kept,
+                           dim3(std::max(1, (p.a.Lmax + 4 * kKeptBlock - 1) / (4 * kKeptBlock)), p.T * p.a.Hkv),
+                           dim3(kKeptBlock), 0, st, p);
+  return launch_weights<PANELS, BF16>(p, smem, st);
 }
 
 int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
@@ -1226,7 +1299,16 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   w += static_cast<size_t>(2) * pl.grid * pl.mb * pl.G * pl.panels * 64 * 4;
   p.ml = reinterpret_cast<float*>(w);
   w += static_cast<size_t>(2) * pl.grid * 2 * kMaxRows * 4;
-  p.lse = a.scores_out ? reinterpret_cast<float*>(w) : nullptr;
+  p.lse = p.kept = p.kept_draft = nullptr;
+  p.kept_len = (a.Lmax + 3) / 4 * 4;
+  if (a.scores_out) {
+    p.lse = reinterpret_cast<float*>(w);
+    w += static_cast<size_t>(a.T) * a.Hkv * pl.RB * kMaxRows * 4;
+    if (pl.mb * pl.G <= kKeptRows) {  // RB = 1: units are (trace, KV head)
+      p.kept_draft = reinterpret_cast<float*>(w);
+      p.kept = p.kept_draft + static_cast<size_t>(a.T) * a.Hkv * pl.mb * pl.G * 64;
+    }
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int t0 = 0; t0 < a.T; t0 += kMaxTraces) {
     p.t0 = t0;

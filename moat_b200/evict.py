@@ -14,10 +14,12 @@ from __future__ import annotations
 import ctypes
 
 from . import _lib
-from ._lib import check, lib, stream_of
-from .tree import _five, _need, _on_device, _plain
+from ._lib import check, lib
+from .tree import _device_index, _five, _on, _on_device, _plain, _strides, _Workspaces
 
-_pool = _lib.WorkspacePool()
+_ws = _Workspaces()
+_sizes = {}  # workspace bytes by geometry
+_NAMES = ("v_cache", "scores", "positions", "lens", "next_pos", "scores_out", "positions_out")
 _Strides8 = ctypes.c_int64 * 8
 
 
@@ -40,44 +42,48 @@ def evict_cache(k_cache, v_cache, scores, positions, lens, next_pos, budget: int
 
     Returns ``(scores_out, positions_out, new_lens)``.
     """
-    t = _lib.require_cuda()
-    if not isinstance(k_cache, t.Tensor):
-        raise TypeError("k_cache must be a torch CUDA tensor")
-    dev = k_cache.device
+    t = _lib.torch()
+    idx = _device_index(k_cache, "k_cache")
     scores_out = scores if scores_out is None else scores_out
     positions_out = positions if positions_out is None else positions_out
-    _on_device(t, dev, k_cache=k_cache, v_cache=v_cache, scores=scores, positions=positions, lens=lens,
-               next_pos=next_pos, scores_out=scores_out, positions_out=positions_out)
+    _on_device(idx, _NAMES, (v_cache, scores, positions, lens, next_pos, scores_out, positions_out))
     kc, vc = _five(k_cache, "k_cache"), _five(v_cache, "v_cache")
     layers, T, Hkv, Lmax, d = kc.shape
-    _need(min(layers, T, Hkv, Lmax, d) >= 1, "the caches must not be empty")
-    _need(vc.shape == kc.shape, "k_cache and v_cache must have one shape")
-    strides = []
-    for x in (kc, vc):
-        st = x.stride()
-        if x.dtype is not kc.dtype or x.element_size() != 2 or (st[4] != 1 and d > 1):
-            raise ValueError("the caches must share one 16-bit dtype and be contiguous along the head dim")
-        strides += st[:4]
-    full = tuple(k_cache.shape[:-1])
-    for x, dtype, n in ((scores, t.float32, "scores"), (scores_out, t.float32, "scores_out"),
-                        (positions, t.int32, "positions"), (positions_out, t.int32, "positions_out")):
-        _plain(x, full, dtype, n)
+    if min(layers, T, Hkv, Lmax, d) < 1:
+        raise ValueError("the caches must not be empty")
+    if vc.shape != kc.shape:
+        raise ValueError("k_cache and v_cache must have one shape")
+    what = "the caches must share one 16-bit dtype and be contiguous along the head dim"
+    if kc.element_size() != 2:
+        raise ValueError(what)
+    strides = _strides((kc, vc), 4, kc.dtype, what)
+    full = k_cache.shape[:-1]
+    _plain(scores, full, t.float32, "scores")
+    _plain(scores_out, full, t.float32, "scores_out")
+    _plain(positions, full, t.int32, "positions")
+    _plain(positions_out, full, t.int32, "positions_out")
     _plain(lens, (T,), t.int32, "lens")
     _plain(next_pos, (T,), t.int32, "next_pos")
     budget, recent, sinks = int(budget), int(recent), int(sinks)
-    _need(budget >= 1 and recent >= 0 and sinks >= 0 and recent + sinks <= budget,
-          "budget must be positive and hold the recent rows and the sinks")
-    _need((scores_out.data_ptr() == scores.data_ptr()) == (positions_out.data_ptr() == positions.data_ptr()),
-          "scores and positions are both updated in place, or neither")
+    if not (budget >= 1 and recent >= 0 and sinks >= 0 and recent + sinks <= budget):
+        raise ValueError("budget must be positive and hold the recent rows and the sinks")
+    ps, pp, pso, ppo = (x.data_ptr() for x in (scores, positions, scores_out, positions_out))
+    if (pso == ps) != (ppo == pp):
+        raise ValueError("scores and positions are both updated in place, or neither")
     new_lens = t.empty_like(lens)
     L = lib()
-    with t.cuda.device(dev):
-        st = stream_of(dev)
-        ws = _pool.get(dev, st, int(L.mb_cache_evict_workspace_size(layers, T, Hkv, Lmax, budget)))
-        rc = L.mb_cache_evict(kc.data_ptr(), vc.data_ptr(), _Strides8(*strides), scores.data_ptr(),
-                              positions.data_ptr(), scores_out.data_ptr(), positions_out.data_ptr(), lens.data_ptr(),
-                              next_pos.data_ptr(), new_lens.data_ptr(), layers, T, Hkv, Lmax, d, budget, recent, sinks,
-                              ws.data_ptr(), ws.numel(), st)
+    geometry = (layers, T, Hkv, Lmax, budget)
+    nbytes = _sizes.get(geometry)
+    if nbytes is None:
+        nbytes = _sizes[geometry] = int(L.mb_cache_evict_workspace_size(*geometry))
+
+    def call(st):
+        ws = _ws.get(t, idx, st, nbytes)
+        return L.mb_cache_evict(kc.data_ptr(), vc.data_ptr(), _Strides8(*strides), ps, pp, pso, ppo, lens.data_ptr(),
+                                next_pos.data_ptr(), new_lens.data_ptr(), layers, T, Hkv, Lmax, d, budget, recent,
+                                sinks, ws.data_ptr(), ws.numel(), st)
+
+    rc = _on(t, idx, call)
     if rc != 0:
         check(rc, "mb_cache_evict")
     return scores_out, positions_out, new_lens

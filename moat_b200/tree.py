@@ -28,9 +28,6 @@ from ._lib import check, lib, stream_of
 
 MAX_NODES = 64  # one bit per node in a mask
 
-_pool = _lib.WorkspacePool()
-
-
 def tree_masks(parents) -> np.ndarray:
     """Ancestors-or-self of every node as the bits of an int64: ``parents [..., m]`` (any
     sequence; a parent that is not an earlier node marks padding) -> int64 ``[..., m]``, 0
@@ -62,27 +59,72 @@ def tree_depths(parents) -> np.ndarray:
     return out.reshape(par.shape)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _device_index(x, name: str) -> int:
+    """Index of the CUDA device a tensor lies on."""
+    try:
+        idx = x.get_device()
+    except AttributeError:
+        raise TypeError(f"{name} must be a torch CUDA tensor") from None
+    if idx < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return idx
 
 
-def _on_device(t, dev, **tensors) -> None:
-    for name, x in tensors.items():
-        if not isinstance(x, t.Tensor):
-            raise TypeError(f"{name} must be a torch CUDA tensor")
-        if not x.is_cuda or x.device != dev:
-            raise ValueError(f"{name} must be on {dev}")
+def _on_device(idx: int, names, tensors) -> None:
+    for name, x in zip(names, tensors):
+        if _device_index(x, name) != idx:
+            raise ValueError(f"{name} must be on cuda:{idx}")
 
 
 def _plain(x, shape, dtype, name) -> None:
     """A contiguous tensor of one shape and dtype."""
-    if tuple(x.shape) != shape or x.dtype != dtype or not x.is_contiguous():
+    if x.dtype is not dtype or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)}")
+
+
+def _strides(tensors, axes: int, dtype, what: str):
+    """The leading strides of tensors of one dtype that are contiguous along their last axis."""
+    out = ()
+    for x in tensors:
+        st = x.stride()
+        if x.dtype is not dtype or (st[axes] != 1 and x.shape[axes] > 1):
+            raise ValueError(what)
+        out += st[:axes]
+    return out
+
+
+class _Workspaces:
+    """Scratch per (device, stream), grown as needed; the kernels expect no initial contents,
+    and calls that share a buffer are ordered by their stream. A buffer that was outgrown is
+    kept: a captured graph may still use it."""
+
+    def __init__(self):
+        self._bufs, self._outgrown = {}, []
+
+    def get(self, t, idx: int, stream: int, nbytes: int):
+        buf = self._bufs.get((idx, stream))
+        if buf is None or buf.numel() < nbytes:
+            if buf is not None:
+                self._outgrown.append(buf)
+                nbytes = max(nbytes, 2 * buf.numel())
+            buf = t.empty(max(nbytes, 1 << 20), dtype=t.uint8, device=t.device("cuda", idx))
+            self._bufs[(idx, stream)] = buf
+        return buf
+
+
+def _on(t, idx: int, call):
+    """``call(stream)`` with device ``idx`` current."""
+    if idx == t.cuda.current_device():
+        return call(stream_of(idx))
+    with t.cuda.device(idx):
+        return call(stream_of(idx))
 
 
 _Strides18 = ctypes.c_int64 * 18
 _Strides16 = ctypes.c_int64 * 16
+_ws = _Workspaces()
+_sizes = {}  # workspace bytes by geometry
+_ATTN_NAMES = ("q", "k_cache", "v_cache", "lens", "k_draft", "v_draft", "masks")
 
 
 def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=None, out=None, scores=None,
@@ -104,29 +146,32 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     * ``dev_err``: optional int32 CUDA tensor whose first word receives device error bits
       (bounded waits).
 
+    Scratch belongs to the stream; a captured graph keeps that of the stream it was captured
+    on, so its replays and other calls of that stream must not overlap.
+
     fp32 scores, softmax and sums; one rounding at the output (and one of each unnormalised
     probability to the inputs' type before its product with V). Repeated calls give the same
     bits. Returns ``out``, or ``(out, scores_out, draft_scores)`` with ``scores``.
     """
-    t = _lib.require_cuda()
-    if not isinstance(q, t.Tensor):
-        raise TypeError("q must be a torch CUDA tensor")
-    dev = q.device
-    _on_device(t, dev, q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, k_draft=k_draft, v_draft=v_draft, masks=masks)
+    t = _lib.torch()
+    idx = _device_index(q, "q")
+    _on_device(idx, _ATTN_NAMES, (q, k_cache, v_cache, lens, k_draft, v_draft, masks))
     if q.dim() != 4 or k_cache.dim() != 4:
         raise ValueError("q must be [T, m, H, d] and the caches [T, Hkv, Lmax, d]")
     T, m, H, d = q.shape
-    Hkv, Lmax = k_cache.shape[1], k_cache.shape[2]
+    cache = k_cache.shape
+    Hkv, Lmax = cache[1], cache[2]
     if not 1 <= m <= MAX_NODES:
         raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {m}")
     if T < 1 or Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError(f"{H} query heads do not divide among {Hkv} KV heads")
     if not 1 <= d <= 256:
         raise ValueError(f"head dim must be 1 to 256, got {d}")
-    if k_cache.shape != (T, Hkv, Lmax, d) or v_cache.shape != (T, Hkv, Lmax, d):
+    if cache != (T, Hkv, Lmax, d) or v_cache.shape != cache:
         raise ValueError(f"k_cache / v_cache must be [{T}, {Hkv}, Lmax, {d}]")
-    if k_draft.shape != (T, m, Hkv, d) or v_draft.shape != (T, m, Hkv, d):
-        raise ValueError(f"k_draft / v_draft must be [{T}, {m}, {Hkv}, {d}]")
+    drafts = (T, m, Hkv, d)
+    if k_draft.shape != drafts or v_draft.shape != drafts:
+        raise ValueError(f"k_draft / v_draft must be {list(drafts)}")
     dt = q.dtype
     if dt is not t.float16 and dt is not t.bfloat16:
         raise ValueError("q must be fp16 or bf16")
@@ -134,44 +179,46 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     shared = masks.dim() == 1
     _plain(masks, (m,) if shared else (T, m), t.int64, "masks")
     if out is None:
-        out = t.empty((T, m, H, d), dtype=dt, device=dev)
-    else:
-        _on_device(t, dev, out=out)
-        _need(out.shape == q.shape, f"out must be [{T}, {m}, {H}, {d}]")
-    six = (q, k_cache, v_cache, k_draft, v_draft, out)
-    strides = []
-    for x in six:
-        st = x.stride()
-        if x.dtype is not dt or (st[3] != 1 and d > 1):
-            raise ValueError("q, out, caches and drafts must share one dtype and be contiguous along the head dim")
-        strides += st[:3]
+        out = t.empty((T, m, H, d), dtype=dt, device=q.device)
+    elif _device_index(out, "out") != idx or out.shape != q.shape:
+        raise ValueError(f"out must be [{T}, {m}, {H}, {d}] on cuda:{idx}")
+    strides = _strides((q, k_cache, v_cache, k_draft, v_draft, out), 3, dt,
+                       "q, out, caches and drafts must share one dtype and be contiguous along the head dim")
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    _need(math.isfinite(sc), "scale must be finite")
+    if not math.isfinite(sc):
+        raise ValueError("scale must be finite")
     ps = pso = pds = None
     if scores is not None:
         scores_out = scores if scores_out is None else scores_out
         if draft_scores is None:
-            draft_scores = t.empty((T, Hkv, m), dtype=t.float32, device=dev)
-        _on_device(t, dev, scores=scores, scores_out=scores_out, draft_scores=draft_scores)
-        _plain(scores, (T, Hkv, Lmax), t.float32, "scores")
-        _plain(scores_out, (T, Hkv, Lmax), t.float32, "scores_out")
-        _plain(draft_scores, (T, Hkv, m), t.float32, "draft_scores")
+            draft_scores = t.empty((T, Hkv, m), dtype=t.float32, device=q.device)
+        _on_device(idx, ("scores", "scores_out", "draft_scores"), (scores, scores_out, draft_scores))
+        f32, rows = t.float32, (T, Hkv, Lmax)
+        _plain(scores, rows, f32, "scores")
+        _plain(scores_out, rows, f32, "scores_out")
+        _plain(draft_scores, (T, Hkv, m), f32, "draft_scores")
         ps, pso, pds = scores.data_ptr(), scores_out.data_ptr(), draft_scores.data_ptr()
-    else:
-        _need(scores_out is None and draft_scores is None, "scores_out and draft_scores need scores")
+    elif scores_out is not None or draft_scores is not None:
+        raise ValueError("scores_out and draft_scores need scores")
     if dev_err is not None:
-        _on_device(t, dev, dev_err=dev_err)
+        _on_device(idx, ("dev_err",), (dev_err,))
     L = lib()
-    with t.cuda.device(dev):
-        st = stream_of(dev)
-        ws = _pool.get(dev, st, int(L.mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d)))
-        rc = L.mb_tree_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(), k_draft.data_ptr(),
-                            v_draft.data_ptr(), masks.data_ptr(), 1 if shared else 0, out.data_ptr(),
-                            _Strides18(*strides), 1 if dt is t.bfloat16 else 0, T, m, H, Hkv, Lmax, d, sc, ps, pso,
-                            pds, ws.data_ptr(), ws.numel(), None if dev_err is None else dev_err.data_ptr(), st)
+    geometry = (T, m, H, Hkv, Lmax, d, ps is not None)
+    nbytes = _sizes.get(geometry)
+    if nbytes is None:
+        nbytes = _sizes[geometry] = int(L.mb_tree_attn_workspace_size(*geometry))
+
+    def call(st):
+        ws = _ws.get(t, idx, st, nbytes)
+        return L.mb_tree_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(),
+                              k_draft.data_ptr(), v_draft.data_ptr(), masks.data_ptr(), shared, out.data_ptr(),
+                              _Strides18(*strides), dt is t.bfloat16, T, m, H, Hkv, Lmax, d, sc, ps, pso, pds,
+                              ws.data_ptr(), ws.numel(), None if dev_err is None else dev_err.data_ptr(), st)
+
+    rc = _on(t, idx, call)
     if rc != 0:
         check(rc, "mb_tree_attn")
-    return out if scores is None else (out, scores_out, draft_scores)
+    return out if ps is None else (out, scores_out, draft_scores)
 
 
 class Accepted(NamedTuple):
@@ -193,6 +240,9 @@ def _five(x, name):
     return x
 
 
+_ACCEPT_NAMES = ("tokens", "parents", "target", "lens", "next_pos", "v_cache", "k_draft", "v_draft")
+
+
 def accept_tree(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, *, scores=None,
                 draft_scores=None, positions=None, dev_err=None) -> Accepted:
     """Greedy acceptance of a verified tree, and the append of its accepted rows.
@@ -210,57 +260,60 @@ def accept_tree(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_dra
     ``next_pos[t] + j``. A trace without room for its accepted rows keeps its state (count
     0) and sets bit 2 of ``dev_err`` (int32 CUDA tensor, optional). 16-bit element types.
     """
-    t = _lib.require_cuda()
-    if not isinstance(k_cache, t.Tensor):
-        raise TypeError("k_cache must be a torch CUDA tensor")
-    dev = k_cache.device
-    _on_device(t, dev, tokens=tokens, parents=parents, target=target, lens=lens, next_pos=next_pos, k_cache=k_cache,
-               v_cache=v_cache, k_draft=k_draft, v_draft=v_draft)
+    t = _lib.torch()
+    idx = _device_index(k_cache, "k_cache")
+    _on_device(idx, _ACCEPT_NAMES, (tokens, parents, target, lens, next_pos, v_cache, k_draft, v_draft))
     kc, vc, kd, vd = (_five(x, n) for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (k_draft, "k_draft"),
                                                (v_draft, "v_draft")))
     layers, T, Hkv, Lmax, d = kc.shape
-    m = kd.shape[2]
+    drafts = kd.shape
+    m = drafts[2]
     if not 1 <= m <= MAX_NODES:
         raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {m}")
-    _need(min(layers, T, Hkv, Lmax, d) >= 1, "the caches must not be empty")
-    _need(vc.shape == kc.shape, "k_cache and v_cache must have one shape")
-    _need(kd.shape == (layers, T, m, Hkv, d) and vd.shape == kd.shape,
-          f"drafts must be [{layers}, {T}, m, {Hkv}, {d}]")
-    strides = []
-    for x in (kc, vc, kd, vd):
-        st = x.stride()
-        if x.dtype is not kc.dtype or x.element_size() != 2 or (st[4] != 1 and d > 1):
-            raise ValueError("caches and drafts must share one 16-bit dtype and be contiguous along the head dim")
-        strides += st[:4]
+    if min(layers, T, Hkv, Lmax, d) < 1:
+        raise ValueError("the caches must not be empty")
+    if vc.shape != kc.shape:
+        raise ValueError("k_cache and v_cache must have one shape")
+    if drafts != (layers, T, m, Hkv, d) or vd.shape != drafts:
+        raise ValueError(f"drafts must be [{layers}, {T}, m, {Hkv}, {d}]")
+    what = "caches and drafts must share one 16-bit dtype and be contiguous along the head dim"
+    if kc.element_size() != 2:
+        raise ValueError(what)
+    strides = _strides((kc, vc, kd, vd), 4, kc.dtype, what)
     i32 = t.int32
-    for x, shape, n in ((tokens, (T, m), "tokens"), (target, (T, m), "target"), (lens, (T,), "lens"),
-                        (next_pos, (T,), "next_pos")):
-        _plain(x, shape, i32, n)
+    _plain(tokens, (T, m), i32, "tokens")
+    _plain(target, (T, m), i32, "target")
+    _plain(lens, (T,), i32, "lens")
+    _plain(next_pos, (T,), i32, "next_pos")
     shared = parents.dim() == 1
     _plain(parents, (m,) if shared else (T, m), i32, "parents")
-    lead = tuple(kc.shape[:3]) if k_cache.dim() == 5 else (T, Hkv)
-    _need((scores is None) == (draft_scores is None), "scores and draft_scores go together")
-    for x, last, dtype, n in ((scores, Lmax, t.float32, "scores"), (draft_scores, m, t.float32, "draft_scores"),
-                              (positions, Lmax, i32, "positions")):
-        if x is not None:
-            _on_device(t, dev, **{n: x})
-            _plain(x, lead + (last,), dtype, n)
+    if (scores is None) != (draft_scores is None):
+        raise ValueError("scores and draft_scores go together")
+    lead = (layers, T, Hkv) if k_cache.dim() == 5 else (T, Hkv)
+    ps = pd = pp = None
+    if scores is not None:
+        _on_device(idx, ("scores", "draft_scores"), (scores, draft_scores))
+        _plain(scores, lead + (Lmax,), t.float32, "scores")
+        _plain(draft_scores, lead + (m,), t.float32, "draft_scores")
+        ps, pd = scores.data_ptr(), draft_scores.data_ptr()
+    if positions is not None:
+        _on_device(idx, ("positions",), (positions,))
+        _plain(positions, lead + (Lmax,), i32, "positions")
+        pp = positions.data_ptr()
     if dev_err is not None:
-        _on_device(t, dev, dev_err=dev_err)
-    ints = t.empty((m + 4) * T, dtype=i32, device=dev)  # one allocation for the five results
-    r = Accepted(ints[4 * T:].view(T, m), ints[:T], ints[T:2 * T], ints[2 * T:3 * T], ints[3 * T:4 * T])
-    with t.cuda.device(dev):
-        rc = lib().mb_tree_accept(tokens.data_ptr(), parents.data_ptr(), 1 if shared else 0, target.data_ptr(),
-                                  lens.data_ptr(), next_pos.data_ptr(), kc.data_ptr(), vc.data_ptr(), kd.data_ptr(),
-                                  vd.data_ptr(), _Strides16(*strides), layers, T, m, Hkv, Lmax, d,
-                                  None if scores is None else scores.data_ptr(),
-                                  None if scores is None else draft_scores.data_ptr(),
-                                  None if positions is None else positions.data_ptr(), r.path.data_ptr(),
-                                  r.counts.data_ptr(), r.next_ids.data_ptr(), r.lens.data_ptr(), r.next_pos.data_ptr(),
-                                  None if dev_err is None else dev_err.data_ptr(), stream_of(dev))
+        _on_device(idx, ("dev_err",), (dev_err,))
+    ints = t.empty((m + 4) * T, dtype=i32, device=kc.device)  # one allocation for the five results
+    path, counts, next_ids, new_lens, new_pos = ints.split_with_sizes([T * m, T, T, T, T])
+    p0 = ints.data_ptr()
+    p1, step = p0 + 4 * T * m, 4 * T
+    rc = _on(t, idx, lambda st: lib().mb_tree_accept(
+        tokens.data_ptr(), parents.data_ptr(), shared, target.data_ptr(), lens.data_ptr(), next_pos.data_ptr(),
+        kc.data_ptr(), vc.data_ptr(), kd.data_ptr(), vd.data_ptr(), _Strides16(*strides), layers, T, m, Hkv, Lmax, d,
+        ps, pd, pp, p0, p1, p1 + step, p1 + 2 * step, p1 + 3 * step, None if dev_err is None else dev_err.data_ptr(),
+        st))
     if rc != 0:
         check(rc, "mb_tree_accept")
-    return r
+    return Accepted(path.view(T, m), counts, next_ids, new_lens, new_pos)
 
 
 __all__ = ["Accepted", "MAX_NODES", "accept_tree", "tree_attention", "tree_depths", "tree_masks"]

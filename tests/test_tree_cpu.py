@@ -60,10 +60,10 @@ def L():
 
 
 def test_workspace_sizes(L):
-    assert L.mb_tree_attn_workspace_size(2, 8, 16, 4, 1024, 128) > 0
+    assert L.mb_tree_attn_workspace_size(2, 8, 16, 4, 1024, 128, 0) > 0
     for bad in [(0, 8, 16, 4, 1024, 128), (2, 65, 16, 4, 1024, 128), (2, 8, 15, 4, 1024, 128),
                 (2, 8, 16, 4, 1024, 257), (2, 8, 16, 4, -1, 128)]:
-        assert L.mb_tree_attn_workspace_size(*bad) == 0
+        assert L.mb_tree_attn_workspace_size(*bad, 1) == 0
     assert L.mb_cache_evict_workspace_size(1, 1, 4, 320, 256) >= 4 * 2 * 64 * 4
     assert L.mb_cache_evict_workspace_size(1, 1, 4, 320, 0) == 0
 
