@@ -52,7 +52,8 @@ struct TreeMmaParams {
   int kept_len;
   int t0, T;    // traces of this launch
   int RB, mb, G, n16, grid, nst, nq;
-  int whole;  // every unit in one CTA: nothing to join
+  bool whole;    // every unit in one CTA: nothing to join
+  bool vec_out;  // 16-byte pieces of output rows
 };
 
 // --- tcgen05 / TMEM -----------------------------------------------------------
@@ -326,7 +327,7 @@ __host__ __device__ inline TreeSmem tree_smem(int panels, int n16, int nst, int 
   s.ring = 0;
   s.q = s.ring + nst * s.stage;
   s.p = s.q + nq * s.qslot;
-  s.misc = s.p + (n16 > 64 ? 2 : 1) * kPanel;
+  s.misc = s.p + (n16 > 64 ? 0 : kPanel);  // many rows: P lies in TMEM
   s.total = s.misc + kMiscBytes;
   return s;
 }
@@ -339,6 +340,93 @@ __device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16,
     *reinterpret_cast<uint4*>(q + (pn * n16 + R) * 128 + (i - pn * per) * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
+}
+
+// Positions of the sequence that are CTA c's.
+__device__ __forceinline__ void cta_share(const TreeMmaParams& p, const TraceTable& tab, int c, int* beg, int* end) {
+  *beg = *end = 0;
+  if (p.whole) {  // one unit per CTA
+    const int units = p.a.Hkv * p.RB, t = c / units;
+    const int span = unit_span(trace_tiles(tab.len[t]));
+    *beg = tab.cum[t] + (c - t * units) * span;
+    *end = *beg + span;
+  } else {
+    const int total = tab.cum[p.T], g = min(p.grid, total);  // CTAs with work
+    if (c < g) {
+      *beg = cut(total, c, g);
+      *end = cut(total, c + 1, g);
+    }
+  }
+}
+
+struct TreeBars {
+  uint64_t *kv_full, *kv_empty, *q_full, *q_empty;
+};
+
+// The TMA warp: K and V tiles of this CTA's segments through the ring, a segment's queries
+// after its first tile (their slot may still be in use).
+template <int PANELS>
+__device__ __forceinline__ void tma_role(const TreeMmaParams& p, const TraceTable& tab, const TreeSmem& lay,
+                                         const TreeBars& bars, int beg, int end, uint32_t ring, uint32_t qbase, int R) {
+  const TreeAttnArgs& a = p.a;
+  bool dead = false;
+  // a cache that is read once streams past what L2 should keep; several row blocks or the
+  // weight pass read it again
+  uint64_t policy;
+  if (p.RB == 1 && (!p.lse || p.kept))
+    policy = policy_evict_first();
+  else
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+  const uint64_t keep = policy_evict_last();
+  int item = 0, seg = 0, st = 0, use = 0;  // K and V tiles of the ring (stage, times used), segments
+  Segment s;
+  for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
+    const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+    for (int j = s.j0; j < s.j0 + s.n; ++j) {
+      const bool draft = j == s.nt - 1;
+      const int rows = tile_rows(s.len, s.nt, a.m, j);
+      for (int kv = 0; kv < 2; ++kv, ++item) {
+        if (use > 0) guarded_wait(bars.kv_empty + st, (use - 1) & 1, dead, a.err);
+        const uint32_t dst = ring + st * lay.stage;
+        if (elect_one()) {
+          if (draft) {
+            mbar_expect_tx(bars.kv_full + st, PANELS * 128 * a.m);
+            for (int pn = 0; pn < PANELS; ++pn)
+              tma_load_4d(dst + pn * kPanel, kv ? &p.mvd : &p.mkd, bars.kv_full + st, pn * 64, s.kvh, 0, s.t, keep);
+          } else if (rows == kTile) {
+            mbar_expect_tx(bars.kv_full + st, PANELS * kPanel);
+            for (int pn = 0; pn < PANELS; ++pn)
+              tma_load_4d(dst + pn * kPanel, kv ? &p.mv : &p.mk, bars.kv_full + st, pn * 64, j * kTile, s.kvh, s.t,
+                          policy);
+          } else {
+            const int boxes = (rows + kBox - 1) / kBox;
+            mbar_expect_tx(bars.kv_full + st, PANELS * 128 * boxes * kBox);
+            for (int pn = 0; pn < PANELS; ++pn)
+              for (int b = 0; b < boxes; ++b)
+                tma_load_4d(dst + pn * kPanel + b * kBox * 128, kv ? &p.mv_end : &p.mk_end, bars.kv_full + st, pn * 64,
+                            j * kTile + b * kBox, s.kvh, s.t, policy);
+          }
+        }
+        __syncwarp();
+        if (++st == p.nst) {
+          st = 0;
+          ++use;
+        }
+      }
+      if (j == s.j0) {
+        if (quse > 0) guarded_wait(bars.q_empty + qs, (quse - 1) & 1, dead, a.err);
+        if (elect_one()) {
+          mbar_expect_tx(bars.q_full + qs, PANELS * R * 128);
+          for (int pn = 0; pn < PANELS; ++pn)
+            tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, bars.q_full + qs, pn * 64, s.kvh * p.G,
+                        s.rb * p.mb, s.t, keep);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  if (dead)  // copies still in flight must land before this CTA's shared memory goes
+    for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(bars.kv_full + i % p.nst, (i / p.nst) & 1);
 }
 
 // PANELS: 64-column panels of the head dim (1: d <= 64, 2: d <= 128). CW: rows per softmax
@@ -357,6 +445,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   uint64_t* q_full = s_empty + 2;                         // [2]
   uint64_t* q_empty = q_full + 2;                         // [2]
   uint64_t* o_empty = q_empty + 2;                        // [2]
+  const TreeBars bars = {kv_full, kv_empty, q_full, q_empty};
   uint64_t* p_full = o_empty + 2;
   uint64_t* pv_done = p_full + 1;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 1);
@@ -405,80 +494,13 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   }
   tc_after_sync();
   const int c = blockIdx.x;
-  int beg = 0, end = 0;
-  if (p.whole) {  // one unit per CTA
-    const int units = a.Hkv * p.RB, t = c / units;
-    const int span = unit_span(trace_tiles(tab.len[t]));
-    beg = tab.cum[t] + (c - t * units) * span;
-    end = beg + span;
-  } else {
-    const int total = tab.cum[p.T], g = min(p.grid, total);  // CTAs with work
-    if (c < g) {
-      beg = cut(total, c, g);
-      end = cut(total, c + 1, g);
-    }
-  }
+  int beg, end;
+  cta_share(p, tab, c, &beg, &end);
   const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q), pbase = smem_u32(smem + lay.p);
 
   if (warp == 4 * WG) {
     // ---------------------------------------------------------------- TMA
-    // a cache that is read once streams past what L2 should keep; several row blocks or the
-    // weight pass read it again
-    uint64_t policy;
-    if (p.RB == 1 && (!p.lse || p.kept))
-      policy = policy_evict_first();
-    else
-      asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
-    const uint64_t keep = policy_evict_last();
-    int item = 0, seg = 0, st = 0, use = 0;  // K and V tiles of the ring (stage, times used), segments
-    Segment s;
-    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
-      const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
-      for (int j = s.j0; j < s.j0 + s.n; ++j) {
-        const bool draft = j == s.nt - 1;
-        const int rows = tile_rows(s.len, s.nt, a.m, j);
-        for (int kv = 0; kv < 2; ++kv, ++item) {
-          if (use > 0) guarded_wait(kv_empty + st, (use - 1) & 1, dead, a.err);
-          const uint32_t dst = ring + st * lay.stage;
-          if (elect_one()) {
-            if (draft) {
-              mbar_expect_tx(kv_full + st, PANELS * 128 * a.m);
-              for (int pn = 0; pn < PANELS; ++pn)
-                tma_load_4d(dst + pn * kPanel, kv ? &p.mvd : &p.mkd, kv_full + st, pn * 64, s.kvh, 0, s.t, keep);
-            } else if (rows == kTile) {
-              mbar_expect_tx(kv_full + st, PANELS * kPanel);
-              for (int pn = 0; pn < PANELS; ++pn)
-                tma_load_4d(dst + pn * kPanel, kv ? &p.mv : &p.mk, kv_full + st, pn * 64, j * kTile, s.kvh, s.t,
-                            policy);
-            } else {
-              const int boxes = (rows + kBox - 1) / kBox;
-              mbar_expect_tx(kv_full + st, PANELS * 128 * boxes * kBox);
-              for (int pn = 0; pn < PANELS; ++pn)
-                for (int b = 0; b < boxes; ++b)
-                  tma_load_4d(dst + pn * kPanel + b * kBox * 128, kv ? &p.mv_end : &p.mk_end, kv_full + st, pn * 64,
-                              j * kTile + b * kBox, s.kvh, s.t, policy);
-            }
-          }
-          __syncwarp();
-          if (++st == p.nst) {
-            st = 0;
-            ++use;
-          }
-        }
-        if (j == s.j0) {  // the queries after the first keys: their slot may still be in use
-          if (quse > 0) guarded_wait(q_empty + qs, (quse - 1) & 1, dead, a.err);
-          if (elect_one()) {
-            mbar_expect_tx(q_full + qs, PANELS * R * 128);
-            for (int pn = 0; pn < PANELS; ++pn)
-              tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, q_full + qs, pn * 64, s.kvh * p.G,
-                          s.rb * p.mb, s.t, keep);
-          }
-          __syncwarp();
-        }
-      }
-    }
-    if (dead)  // copies still in flight must land before this CTA's shared memory goes
-      for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
+    tma_role<PANELS>(p, tab, lay, bars, beg, end, ring, qbase, R);
   } else if (warp == 4 * WG + 1) {
     // ---------------------------------------------------------------- MMA
     const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
@@ -807,6 +829,363 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   if (warp == 4 * WG + 1) tmem_dealloc(*tmem_base, 512);
 }
 
+// ---------------------------------------------------------------------------
+// More than 64 rows: the rows fill the TMEM lanes (S[128 rows, 128 keys], O[128 rows, d]).
+// A thread then holds 64 scores of one row, so the running reference, the sum and the mask are
+// one register each, the vote for a new maximum concerns the two warps that share a row, and P
+// goes back to TMEM as the A operand of the value product (in the place of the scores, once
+// both warps have read them) instead of through shared memory. With keys on the lanes the same
+// work took 3,500 cycles per tile (tables of references and sums per thread, P and both operand
+// streams through shared memory).
+// ---------------------------------------------------------------------------
+constexpr int kRowsThreads = 256 + 64;
+
+// 32 consecutive TMEM columns of packed pairs
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
+      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
+      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+
+// A from TMEM
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "n"(kDescHigh)
+      : "memory");
+}
+
+// Any over the 64 threads of the two warps of a lane quarter (named barrier id).
+__device__ __forceinline__ bool vote_pair(bool v, int id) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(v ? 1u : 0u), "r"(id)
+      : "memory");
+  return r != 0;
+}
+
+template <int PANELS, bool BF16>
+__global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid_constant__ TreeMmaParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int DP = PANELS * 64;
+  constexpr int kSoft = 256;
+  const TreeSmem lay = tree_smem(PANELS, p.n16, p.nst, p.nq);
+  uint8_t* misc = smem + lay.misc;
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(misc);
+  uint64_t* kv_empty = kv_full + kMaxStages;
+  uint64_t* s_full = kv_empty + kMaxStages;  // [2]
+  uint64_t* q_full = s_full + 2;             // [2]
+  uint64_t* q_empty = q_full + 2;            // [2]
+  uint64_t* o_empty = q_empty + 2;           // [2]
+  uint64_t* p_full = o_empty + 2;            // [2]: the next tile's P may be done before this one is used
+  uint64_t* pv_done = p_full + 2;
+  const TreeBars bars = {kv_full, kv_empty, q_full, q_empty};
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 1);
+  float* xchg = reinterpret_cast<float*>(misc + kMiscRef);  // [2][128] between the two warps of a row
+  TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const TreeAttnArgs& a = p.a;
+  const int R = p.mb * p.G;
+  bool dead = false;
+
+  if (warp == 8) {
+    if (lane < 7) prefetch_map(&p.mq + lane);
+    if (lane == 0) {
+      for (int i = 0; i < kMaxStages; ++i) {
+        mbar_init(kv_full + i, 1);
+        mbar_init(kv_empty + i, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full + i, 1);
+        mbar_init(q_full + i, 1);
+        mbar_init(q_empty + i, 1);
+        mbar_init(o_empty + i, kSoft);
+        mbar_init(p_full + i, kSoft);
+      }
+      mbar_init(pv_done, 1);
+      fence_mbar_init();
+    }
+  } else if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_base), 512);
+  } else {
+    zero_query_tail(smem + lay.q, PANELS * p.nq, p.n16, R, tid, kSoft);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  tc_before_sync();
+  if (warp == 8) {
+    prefix_tiles(p, tab, lane, a.Hkv * p.RB);
+    __syncwarp();
+    asm volatile("bar.arrive 9, %0;" ::"n"(kRowsThreads) : "memory");
+  } else {
+    named_bar_sync(9, kRowsThreads);
+  }
+  tc_after_sync();
+  const int c = blockIdx.x;
+  int beg, end;
+  cta_share(p, tab, c, &beg, &end);
+  const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q);
+
+  if (warp == 8) {
+    tma_role<PANELS>(p, tab, lay, bars, beg, end, ring, qbase, R);
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA
+    const uint32_t id_qk = instr_desc(BF16, kTile, false, false);
+    const uint32_t id_pv = instr_desc(BF16, DP, false, true);
+    const uint32_t ring_k = smem_desc(ring, 16), ring_v = smem_desc(ring, kPanel);
+    const uint32_t q_desc = smem_desc(qbase, 16);
+    const uint32_t tmem = *tmem_base;
+    Segment sq = {}, sv = {};
+    int jq = 0, jv = 0, seg_q = -1, seg_v = -1, fq = beg, fv = beg;
+    bool more = true;
+    int st_k = 0, use_k = 0, st_v = 1, use_v = 0;
+    for (int k = 0; more; ++k) {
+      if (jq == sq.n) {
+        more = next_segment(p, tab, fq, end, p.RB, sq);
+        jq = 0;
+        ++seg_q;
+      }
+      if (more) {
+        const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
+        if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
+        guarded_wait(kv_full + st_k, use_k & 1, dead, a.err);
+        // the buffer of tile k - 2 held its P: its value product must have read it
+        if (k >= 2) guarded_wait(pv_done, k & 1, dead, a.err);
+        tc_after_sync();
+        ++jq;
+        if (elect_one()) {
+          const uint32_t ka = ring_k + (st_k * lay.stage >> 4), qa = q_desc + (qs * lay.qslot >> 4);
+#pragma unroll
+          for (int kk = 0; kk < PANELS * 4; ++kk)
+            tc_mma(tmem + (k & 1) * kTile, qa + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2,
+                   ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+          tc_commit(s_full + (k & 1));
+          tc_commit(kv_empty + st_k);
+          if (jq == sq.n) tc_commit(q_empty + qs);
+        }
+        __syncwarp();
+        st_k += 2;
+        if (st_k >= p.nst) {
+          st_k -= p.nst;
+          ++use_k;
+        }
+      }
+      if (k > 0) {
+        const int e = k - 1;
+        if (jv == sv.n) {
+          next_segment(p, tab, fv, end, p.RB, sv);
+          jv = 0;
+          ++seg_v;
+        }
+        guarded_wait(kv_full + st_v, use_v & 1, dead, a.err);
+        if (jv == 0 && seg_v >= 2) guarded_wait(o_empty + (seg_v & 1), ((seg_v >> 1) - 1) & 1, dead, a.err);
+        guarded_wait(p_full + (e & 1), (e >> 1) & 1, dead, a.err);
+        tc_after_sync();
+        const int steps = (tile_rows(sv.len, sv.nt, a.m, sv.j0 + jv) + 15) / 16;
+        if (elect_one()) {
+          const uint32_t va = ring_v + (st_v * lay.stage >> 4);
+          const uint32_t o = tmem + (2 + (seg_v & 1)) * kTile, pa = tmem + (e & 1) * kTile;
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            if (kk < steps) tc_mma_ts(o, pa + kk * 8, va + kk * (2048 >> 4), id_pv, jv > 0 || kk > 0);
+          tc_commit(kv_empty + st_v);
+          tc_commit(pv_done);
+        }
+        __syncwarp();
+        ++jv;
+        st_v += 2;
+        if (st_v >= p.nst) {
+          st_v -= p.nst;
+          ++use_v;
+        }
+      }
+    }
+    if (dead) {  // products still in flight must end before TMEM is freed
+      const long long t0 = clock64();
+      while (clock64() - t0 < 1000000) {
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int grp = warp >> 2, wq = warp & 3;
+    const int row = wq * 32 + lane;  // this thread's row; keys 64 grp .. 64 grp + 63 of a tile
+    const int key0 = 64 * grp;
+    const uint32_t tmem = *tmem_base, lanes = static_cast<uint32_t>(wq * 32) << 16;
+    const float sc = a.scale_log2;
+    const int my_node = row / p.G, my_head = row - my_node * p.G;
+    int seg = 0, k = 0, vst = 1, vuse = 0;
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
+      const uint64_t* mk = a.masks + s.t * a.mask_stride;
+      const int node = s.rb * p.mb + my_node;
+      const bool real_row = row < R && node < a.m;
+      const uint64_t mask = real_row ? mk[node] : 0;
+      const uint64_t mk0 = lane < a.m ? mk[lane] : 0, mk1 = lane + 32 < a.m ? mk[lane + 32] : 0;
+      const uint32_t obuf = tmem + lanes + (2 + (seg & 1)) * kTile;
+      float ref = kNoRef, l = 0.0f;
+      for (int jj = 0; jj < s.n; ++jj, ++k) {
+        const int j = s.j0 + jj;
+        const bool draft = j == s.nt - 1;
+        const int rows = tile_rows(s.len, s.nt, a.m, j);
+        const uint32_t sbuf = tmem + lanes + (k & 1) * kTile;
+        guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
+        tc_after_sync();
+        float x[64];
+#pragma unroll
+        for (int i = 0; i < 64; i += 16) tc_ld16(sbuf + key0 + i, x + i);
+        tc_wait_ld();
+        if (draft || rows < kTile) {
+          // bits of this thread's 64 keys that the row sees
+          uint64_t see = draft ? (grp == 0 ? mask : 0) : ~0ull;
+          const int n = rows - key0;  // valid keys among them
+          see &= n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+          const uint32_t lo = static_cast<uint32_t>(see), hi = static_cast<uint32_t>(see >> 32);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            const bool on = ((i < 32 ? lo : hi) >> (i & 31)) & 1;
+            x[i] = on ? x[i] * sc : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] *= sc;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], x[i]);
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        tc_before_sync();
+        const bool raise = vote_pair(mx > ref + kSlack, 1 + wq);
+        tc_after_sync();  // both warps of the row have read its scores: P may take their place
+        if (raise) {
+          xchg[grp * kTile + row] = mx;
+          if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);  // O as the last product left it
+          named_bar_sync(1 + wq, 64);
+          const float now = fmaxf(fmaxf(xchg[row], xchg[kTile + row]), ref);
+          named_bar_sync(1 + wq, 64);  // read by both before the next exchange
+          const float fade = ex2(ref - now);
+          ref = now;
+          l *= fade;
+          if (jj > 0) {  // each of the two warps rescales half of the row's O
+            tc_after_sync();
+#pragma unroll 1
+            for (int i = 0; i < DP / 2; i += 16) {
+              float o[16];
+              tc_ld16(obuf + grp * (DP / 2) + i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int u = 0; u < 16; ++u) o[u] *= fade;
+              tc_st16(obuf + grp * (DP / 2) + i, o);
+            }
+          }
+        }
+        // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
+        uint32_t pk[32];
+        float sum[4] = {};
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          const float e0 = ex2(x[i] - ref), e1 = ex2(x[i + 1] - ref);
+          sum[i & 2] += e0;
+          sum[(i & 2) + 1] += e1;
+          pk[i / 2] = pack2<BF16>(e0, e1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc_st32(sbuf + 32 * grp, pk);
+        // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
+        // product's last 16-row step reads beyond the valid rows, and unused drafted rows
+        if (grp == 0 && (rows & 15 || draft)) {
+          uint64_t used = mk0 | mk1;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
+          const bool clear = row >= rows ? row < ((rows + 15) & ~15) : draft && !((used >> (row & 63)) & 1);
+          if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
+          if (clear) {
+            for (int pn = 0; pn < PANELS; ++pn)
+              for (int u = 0; u < 8; ++u)
+                *reinterpret_cast<uint4*>(smem + lay.ring + vst * lay.stage + pn * kPanel + row * 128 + u * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        tc_wait_st();
+        tc_before_sync();
+        mbar_arrive(p_full + (k & 1));
+        vst += 2;
+        if (vst >= p.nst) {
+          vst -= p.nst;
+          ++vuse;
+        }
+      }
+      // ------------------------------------------------ end of the segment: sums, output
+      xchg[grp * kTile + row] = l;
+      named_bar_sync(1 + wq, 64);
+      const float sum = xchg[row] + xchg[kTile + row];
+      named_bar_sync(1 + wq, 64);
+      const bool whole = s.n == s.nt, real = mask != 0 && sum != 0.0f;
+      const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
+      if (grp == 0) {
+        if (!whole) {
+          float* ml = p.ml + static_cast<int64_t>(slot) * 2 * kMaxRows;
+          ml[row] = ref;
+          ml[kMaxRows + row] = real ? sum : 0.0f;
+        } else if (p.lse) {
+          const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
+          p.lse[unit * kMaxRows + row] = real ? ref + log2f(sum) : INFINITY;
+        }
+      }
+      const float inv = real ? 1.0f / sum : 0.0f;
+      uint16_t* out = a.out + s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + my_head) * a.os[2];
+      float* part = p.part + (static_cast<int64_t>(slot) * R + row) * DP;
+      guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
+      tc_after_sync();
+#pragma unroll 1
+      for (int i = grp * (DP / 2); i < (grp + 1) * (DP / 2); i += 16) {
+        float o[16];
+        tc_ld16(obuf + i, o);
+        tc_wait_ld();
+        if (!whole) {
+          if (row < R)
+#pragma unroll
+            for (int u = 0; u < 16; u += 4)
+              *reinterpret_cast<float4*>(part + i + u) = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+        } else if (real_row) {
+          uint32_t w[8];
+#pragma unroll
+          for (int u = 0; u < 16; u += 2)
+            w[u / 2] = real ? pack2<BF16>(o[u] * inv, o[u + 1] * inv) : 0u;
+#pragma unroll
+          for (int u = 0; u < 8; u += 4) {  // the head dim is a multiple of 8
+            if (i + 2 * u >= a.d) break;
+            if (p.vec_out) {
+              *reinterpret_cast<uint4*>(out + i + 2 * u) = make_uint4(w[u], w[u + 1], w[u + 2], w[u + 3]);
+            } else {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                out[i + 2 * (u + v)] = static_cast<uint16_t>(w[u + v]);
+                out[i + 2 * (u + v) + 1] = static_cast<uint16_t>(w[u + v] >> 16);
+              }
+            }
+          }
+        }
+      }
+      tc_before_sync();
+      mbar_arrive(o_empty + (seg & 1));
+    }
+  }
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 9) tmem_dealloc(*tmem_base, 512);
+}
+
 // Joins the pieces of the units that were cut between CTAs, in order. One CTA per unit and
 // group of 8 rows; a unit that one CTA held is done already.
 constexpr int kJoinBlock = 256;
@@ -910,9 +1289,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   uint64_t* q_empty = q_full + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(q_empty + 2);
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
-  // the space of P: per warpgroup the rows' lse and draft masks
-  float* lse_s = reinterpret_cast<float*>(smem + lay.p);
-  uint64_t* mask_s = reinterpret_cast<uint64_t*>(smem + lay.p + 2 * kMaxRows * 4);
+  // per warpgroup the rows' lse and draft masks: in the last ring stage, which is left out
+  float* lse_s = reinterpret_cast<float*>(smem + lay.ring + (p.nst - 1) * lay.stage);
+  uint64_t* mask_s = reinterpret_cast<uint64_t*>(lse_s + 2 * kMaxRows);
+  const int nst = p.nst - 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TreeAttnArgs& a = p.a;
@@ -982,7 +1362,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
             }
           }
           __syncwarp();
-          if (++st == p.nst) {
+          if (++st == nst) {
             st = 0;
             ++use;
           }
@@ -1000,7 +1380,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
       }
     }
     if (dead)
-      for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(kv_full + i % p.nst, (i / p.nst) & 1);
+      for (int i = max(0, item - nst); i < item; ++i) mbar_wait(kv_full + i % nst, (i / nst) & 1);
   } else if (warp == 9) {
     const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
     const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
@@ -1028,7 +1408,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
             if (jj + 1 == s.n) tc_commit(q_empty + qs);
           }
           __syncwarp();
-          if (++st == p.nst) {
+          if (++st == nst) {
             st = 0;
             ++use;
           }
@@ -1154,6 +1534,7 @@ static bool tree_plan(int T, int m, int H, int Hkv, int Lmax, int d, TreePlan* p
   pl->mb = (m + pl->RB - 1) / pl->RB;  // even blocks
   pl->RB = (m + pl->mb - 1) / pl->mb;
   pl->n16 = (pl->mb * pl->G + 15) / 16 * 16;
+  if (pl->n16 > 64) pl->n16 = kMaxRows;  // k_tree_attn_rows: rows fill the lanes
   pl->panels = d > 64 ? 2 : 1;
   pl->grid = sm_count();
   // flat tile numbers are 32-bit
@@ -1235,6 +1616,14 @@ static int launch_attn(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
 }
 
 template <int PANELS, bool BF16>
+static int launch_attn_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
+  const int rc = allow_smem<k_tree_attn_rows<PANELS, BF16>>();
+  if (rc != MB_OK) return rc;
+  return launch_with_pdl(k_tree_attn_rows<PANELS, BF16>, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid),
+                         dim3(kRowsThreads), smem, st, p);
+}
+
+template <int PANELS, bool BF16>
 static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
   int rc;
   if (p.n16 <= 16)
@@ -1244,7 +1633,7 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
   else if (p.n16 <= 64)
     rc = launch_attn<PANELS, 16, 4, BF16>(p, smem, st);
   else
-    rc = launch_attn<PANELS, 32, 4, BF16>(p, smem, st);
+    rc = launch_attn_rows<PANELS, BF16>(p, smem, st);
   if (rc != MB_OK || p.whole) return rc;
   const int R = p.mb * p.G;
   return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.T * p.a.Hkv * p.RB, (R + kJoinRows - 1) / kJoinRows),
@@ -1294,6 +1683,7 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   p.grid = pl.grid;
   p.nst = pl.nst;
   p.nq = pl.nq;
+  p.vec_out = aligned(a.out, 16) && a.os[0] % 8 == 0 && a.os[1] % 8 == 0 && a.os[2] % 8 == 0;
   char* w = static_cast<char*>(ws);
   p.part = reinterpret_cast<float*>(w);
   w += static_cast<size_t>(2) * pl.grid * pl.mb * pl.G * pl.panels * 64 * 4;
