@@ -36,6 +36,7 @@ namespace mb {
 constexpr int kTile = 128;      // keys per tile
 constexpr int kBox = 32;        // rows per TMA box of a unit's last cached tile: no more boxes than it needs
 constexpr int kMaxRows = 128;   // rows of a block
+constexpr int kKeysRows = 16;   // up to this many rows the keys fill the TMEM lanes, above it the rows do
 constexpr int kMaxTraces = 127;  // per launch (the table of their lengths lies in shared memory)
 constexpr int kPanel = kTile * 128;  // bytes of a 64-column panel of a tile (128-byte swizzled rows)
 constexpr float kNoRef = -1e30f;     // m_ref before any visible key
@@ -51,7 +52,8 @@ struct TreeMmaParams {
   float* kept_draft;  // [units][R][64] of the drafted rows
   int kept_len;
   int t0, T;    // traces of this launch
-  int RB, mb, G, n16, grid, nst, nq;
+  int RB, mb, G, grid, nst, nq;
+  int n16, used;  // rows of a Q slot; rows of a block in steps of 16
   bool whole;    // every unit in one CTA: nothing to join
   bool vec_out;  // 16-byte pieces of output rows
 };
@@ -194,23 +196,19 @@ __device__ __forceinline__ void guarded_wait(uint64_t* bar, uint32_t parity, boo
   }
 }
 
-// Sums over the 32 lanes of N (16 or 32) columns: v[0..N) of every lane in, the sum of column
-// lane % N out.
-template <int N>
-__device__ __forceinline__ float column_sums(float* v, int lane) {
+// Sums over the 32 lanes of 16 columns: v[0..16) of every lane in, the sum of column lane % 16
+// out.
+__device__ __forceinline__ float column_sums16(float* v, int lane) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    if (2 * o > N) {
+  for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    } else {
-      const bool up = lane & o;
+  for (int o = 8; o; o >>= 1) {
+    const bool up = lane & o;
 #pragma unroll
-      for (int i = 0; i < o; ++i) {
-        const float give = up ? v[i] : v[i + o];
-        const float keep = up ? v[i + o] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-      }
+    for (int i = 0; i < o; ++i) {
+      const float give = up ? v[i] : v[i + o];
+      const float keep = up ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
     }
   }
   return v[0];
@@ -327,7 +325,7 @@ __host__ __device__ inline TreeSmem tree_smem(int panels, int n16, int nst, int 
   s.ring = 0;
   s.q = s.ring + nst * s.stage;
   s.p = s.q + nq * s.qslot;
-  s.misc = s.p + (n16 > 64 ? 0 : kPanel);  // many rows: P lies in TMEM
+  s.misc = s.p + (n16 > kKeysRows ? 0 : kPanel);  // many rows: P lies in TMEM
   s.total = s.misc + kMiscBytes;
   return s;
 }
@@ -429,13 +427,33 @@ __device__ __forceinline__ void tma_role(const TreeMmaParams& p, const TraceTabl
     for (int i = max(0, item - p.nst); i < item; ++i) mbar_wait(bars.kv_full + i % p.nst, (i / p.nst) & 1);
 }
 
-// PANELS: 64-column panels of the head dim (1: d <= 64, 2: d <= 128). CW: rows per softmax
-// warpgroup, WG warpgroups.
-template <int PANELS, int CW, int WG, bool BF16>
-__global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_constant__ TreeMmaParams p) {
+// The next tile's stage: every other item of the ring.
+__device__ __forceinline__ void next_tile(int nst, int& st, int& use) {
+  st += 2;
+  if (st >= nst) {
+    st -= nst;
+    ++use;
+  }
+}
+
+// After a wait gave up: products still in flight must end before TMEM is freed.
+__device__ __forceinline__ void drain_products() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 1000000) {
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 16 rows: the keys fill the TMEM lanes.
+// PANELS: 64-column panels of the head dim (1: d <= 64, 2: d <= 128).
+// ---------------------------------------------------------------------------
+constexpr int kKeysThreads = 128 + 96;  // softmax, TMA, score products, value products
+
+template <int PANELS, bool BF16>
+__global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid_constant__ TreeMmaParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   constexpr int DP = PANELS * 64;
-  constexpr int kSoft = 128 * WG;
+  constexpr int kSoft = 128;
   const TreeSmem lay = tree_smem(PANELS, p.n16, p.nst, p.nq);
   uint8_t* misc = smem + lay.misc;
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(misc);  // [kMaxStages]
@@ -458,7 +476,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   const int R = p.mb * p.G;
   bool dead = false;
 
-  if (warp == 4 * WG) {  // TMA warp
+  if (warp == 4) {  // TMA warp
     if (lane < 7) prefetch_map(&p.mq + lane);
     if (lane == 0) {
       for (int i = 0; i < kMaxStages; ++i) {
@@ -476,21 +494,21 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
       mbar_init(pv_done, 1);
       fence_mbar_init();
     }
-  } else if (warp == 4 * WG + 1) {
-    tmem_alloc(smem_u32(tmem_base), 512);
-  } else if (warp < 4 * WG) {
+  } else if (warp == 5) {
+    tmem_alloc(smem_u32(tmem_base), 128);
+  } else if (warp < 4) {
     zero_query_tail(smem + lay.q, PANELS * p.nq, p.n16, R, tid, kSoft);
-    for (int i = tid; i < kMaxRows; i += kSoft) ref[i] = kNoRef;
+    if (tid < kKeysRows) ref[tid] = kNoRef;
   }
   pdl_wait();  // the lengths, masks, queries and drafts may come from the kernel before
   pdl_launch_dependents();
   tc_before_sync();
-  if (warp == 4 * WG) {  // builds the table and goes straight on to its loads
+  if (warp == 4) {  // builds the table and goes straight on to its loads
     prefix_tiles(p, tab, lane, a.Hkv * p.RB);
     __syncwarp();
-    asm volatile("bar.arrive 2, %0;" ::"n"(128 * WG + 64) : "memory");
+    asm volatile("bar.arrive 2, %0;" ::"n"(kKeysThreads) : "memory");
   } else {
-    named_bar_sync(2, 128 * WG + 64);
+    named_bar_sync(2, kKeysThreads);
   }
   tc_after_sync();
   const int c = blockIdx.x;
@@ -498,99 +516,77 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
   cta_share(p, tab, c, &beg, &end);
   const uint32_t ring = smem_u32(smem + lay.ring), qbase = smem_u32(smem + lay.q), pbase = smem_u32(smem + lay.p);
 
-  if (warp == 4 * WG) {
-    // ---------------------------------------------------------------- TMA
+  if (warp == 4) {
     tma_role<PANELS>(p, tab, lay, bars, beg, end, ring, qbase, R);
-  } else if (warp == 4 * WG + 1) {
-    // ---------------------------------------------------------------- MMA
-    const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
-    const uint32_t id_pv = instr_desc(BF16, p.n16, true, true);
-    const uint32_t ring_k = smem_desc(ring, 16), ring_v = smem_desc(ring, kPanel);
-    const uint32_t q_desc = smem_desc(qbase, 16), p_desc = smem_desc(pbase, kPanel);
+  } else if (warp == 5) {
+    // ---------------------------------------------------------------- scores
+    const uint32_t idesc = instr_desc(BF16, kKeysRows, false, false);
+    const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
     const uint32_t tmem = *tmem_base;
-    // two cursors over the same tiles: scores run one tile ahead of the value product
-    Segment sq = {}, sv = {};
-    int jq = 0, jv = 0, seg_q = -1, seg_v = -1, fq = beg, fv = beg;
-    bool more = true;
-    int st_k = 0, use_k = 0, st_v = 1, use_v = 0;  // their ring stages: tile k's K and V are items 2k, 2k + 1
-    for (int k = 0; more; ++k) {
-      if (jq == sq.n) {
-        more = next_segment(p, tab, fq, end, p.RB, sq);
-        jq = 0;
-        ++seg_q;
-      }
-      if (more) {
-        const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
-        if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
-        guarded_wait(kv_full + st_k, use_k & 1, dead, a.err);
+    int k = 0, seg = 0, st = 0, use = 0;  // tile k's K and V are items 2k and 2k + 1 of the ring
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
+      const int qs = seg & 1;
+      guarded_wait(q_full + qs, (seg >> 1) & 1, dead, a.err);
+      for (int jj = 0; jj < s.n; ++jj, ++k) {
+        guarded_wait(kv_full + st, use & 1, dead, a.err);
         if (k >= 2) guarded_wait(s_empty + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
         tc_after_sync();
-        ++jq;
         if (elect_one()) {
-          const uint32_t ka = ring_k + (st_k * lay.stage >> 4), qb = q_desc + (qs * lay.qslot >> 4);
-          const uint32_t qpanel = p.n16 * 128 >> 4;
+          const uint32_t ka = ring_k + (st * lay.stage >> 4), qb = q_desc + (qs * lay.qslot >> 4);
 #pragma unroll
           for (int kk = 0; kk < PANELS * 4; ++kk)
-            tc_mma(tmem + (k & 1) * kMaxRows, ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2,
-                   qb + (kk >> 2) * qpanel + (kk & 3) * 2, id_qk, kk > 0);
+            tc_mma(tmem + (k & 1) * kKeysRows, ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2,
+                   qb + (kk >> 2) * (kKeysRows * 128 >> 4) + (kk & 3) * 2, idesc, kk > 0);
           tc_commit(s_full + (k & 1));
-          tc_commit(kv_empty + st_k);
-          if (jq == sq.n) tc_commit(q_empty + qs);
+          tc_commit(kv_empty + st);
+          if (jj + 1 == s.n) tc_commit(q_empty + qs);
         }
         __syncwarp();
-        st_k += 2;
-        if (st_k >= p.nst) {
-          st_k -= p.nst;
-          ++use_k;
-        }
+        next_tile(p.nst, st, use);
       }
-      if (k > 0) {
-        const int e = k - 1;
-        if (jv == sv.n) {
-          next_segment(p, tab, fv, end, p.RB, sv);
-          jv = 0;
-          ++seg_v;
-        }
-        guarded_wait(kv_full + st_v, use_v & 1, dead, a.err);
-        if (jv == 0 && seg_v >= 2) guarded_wait(o_empty + (seg_v & 1), ((seg_v >> 1) - 1) & 1, dead, a.err);
-        guarded_wait(p_full, e & 1, dead, a.err);
+    }
+    if (dead) drain_products();
+  } else if (warp == 6) {
+    // ---------------------------------------------------------------- values
+    // (a warp of its own: one that issued both products was busy 1,500 cycles a tile, and a
+    // score product that had to wait for its keys held back a value product that had not)
+    const uint32_t idesc = instr_desc(BF16, kKeysRows, true, true);
+    const uint32_t ring_v = smem_desc(ring, kPanel), p_desc = smem_desc(pbase, kPanel);
+    const uint32_t tmem = *tmem_base;
+    int k = 0, seg = 0, st = 1, use = 0;
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
+      const uint32_t o = tmem + (2 + (seg & 1)) * kKeysRows;
+      for (int jj = 0; jj < s.n; ++jj, ++k) {
+        const int steps = (tile_rows(s.len, s.nt, a.m, s.j0 + jj) + 15) / 16;
+        guarded_wait(kv_full + st, use & 1, dead, a.err);
+        if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
+        guarded_wait(p_full, k & 1, dead, a.err);
         tc_after_sync();
-        const int steps = (tile_rows(sv.len, sv.nt, a.m, sv.j0 + jv) + 15) / 16;
         if (elect_one()) {
-          const uint32_t va = ring_v + (st_v * lay.stage >> 4);
-          const uint32_t o = tmem + (2 + (seg_v & 1)) * kMaxRows;
+          const uint32_t va = ring_v + (st * lay.stage >> 4);
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
-            if (kk < steps) tc_mma(o, va + kk * (2048 >> 4), p_desc + kk * (2048 >> 4), id_pv, jv > 0 || kk > 0);
-          tc_commit(kv_empty + st_v);
+            if (kk < steps) tc_mma(o, va + kk * (2048 >> 4), p_desc + kk * (2048 >> 4), idesc, jj > 0 || kk > 0);
+          tc_commit(kv_empty + st);
           tc_commit(pv_done);
         }
         __syncwarp();
-        ++jv;
-        st_v += 2;
-        if (st_v >= p.nst) {
-          st_v -= p.nst;
-          ++use_v;
-        }
+        next_tile(p.nst, st, use);
       }
     }
-    if (dead) {  // products still in flight must end before TMEM is freed
-      const long long t0 = clock64();
-      while (clock64() - t0 < 1000000) {
-      }
-    }
-  } else if (warp < 4 * WG) {
+    if (dead) drain_products();
+  } else {
     // ---------------------------------------------------------------- softmax
-    const int grp = warp >> 2, wq = warp & 3;
+    const int wq = warp;
     const int key = wq * 32 + lane;  // this thread's key of a tile, and its d of O^T
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    const int col0 = grp * CW;
     const float sc = a.scale_log2;
-    const float* refs = ref + col0;
-    const int my_node = tid / p.G;  // node of row tid within a block
-    float l[CW];
+    const int my_node = tid / p.G;  // node of row tid
+    float l[kKeysRows];
 #pragma unroll
-    for (int i = 0; i < CW; ++i) l[i] = 0.0f;
+    for (int i = 0; i < kKeysRows; ++i) l[i] = 0.0f;
     float* scratch = reinterpret_cast<float*>(smem + lay.p);  // P's space, while no product reads it
     const uint32_t tmem = *tmem_base;
     int seg = 0, k = 0, vst = 1, vuse = 0;
@@ -599,143 +595,108 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
       // this row's mask, and the rows of the draft that any node sees (loads in flight over the
       // first tile)
       const uint64_t* mk = a.masks + s.t * a.mask_stride;
-      const int node = s.rb * p.mb + my_node;
-      const uint64_t my_mask = tid < R && node < a.m ? mk[node] : 0;
+      const uint64_t my_mask = tid < R ? mk[my_node] : 0;  // few rows are one block
       const uint64_t mk0 = lane < a.m ? mk[lane] : 0, mk1 = lane + 32 < a.m ? mk[lane + 32] : 0;
       for (int jj = 0; jj < s.n; ++jj, ++k) {
         const int j = s.j0 + jj;
         const bool draft = j == s.nt - 1;
         const int rows = tile_rows(s.len, s.nt, a.m, j);
-        const uint32_t sbuf = tmem + lanes + (k & 1) * kMaxRows + col0;
+        const uint32_t sbuf = tmem + lanes + (k & 1) * kKeysRows;
         // which of this thread's rows see its key, a bit each
         uint32_t see = key < rows ? ~0u : 0u;
         if (draft) {
-          if (tid < kMaxRows) rowmask[tid] = my_mask;
+          if (tid < kKeysRows) rowmask[tid] = my_mask;
           named_bar_sync(1, kSoft);
           if (key < rows) {
             see = 0;
 #pragma unroll 4
-            for (int i = 0; i < CW; ++i) see |= static_cast<uint32_t>((rowmask[col0 + i] >> key) & 1) << i;
+            for (int i = 0; i < kKeysRows; ++i) see |= static_cast<uint32_t>((rowmask[i] >> key) & 1) << i;
           }
         }
         const bool full = !draft && rows == kTile;
-        // Scores of rows i .. i + 15 less sub (log2 units), -inf for what a row does not see.
-        // Sixteen at a time, read from TMEM again for the exponentials: with all of a thread's
-        // scores in registers it spills, and with L1 given to shared memory a spill goes to L2
-        // (5,600 cycles for a tile's exponentials of 64 rows).
-        float x[16];
-        auto form = [&](int i, bool less_ref) {
-          float r[16];
-          if (less_ref) load16(refs + i, r);
-          tc_ld16(sbuf + i, x);
+        // the rows' scores of this key, less m_ref (log2 units), -inf for what a row does not see
+        float x[kKeysRows], r[kKeysRows];
+        auto form = [&](bool less_ref) {
+          if (less_ref) load16(ref, r);
+          tc_ld16(sbuf, x);
           tc_wait_ld();
 #pragma unroll
-          for (int u = 0; u < 16; ++u) x[u] = less_ref ? fmaf(x[u], sc, -r[u]) : x[u] * sc;
+          for (int u = 0; u < kKeysRows; ++u) x[u] = less_ref ? fmaf(x[u], sc, -r[u]) : x[u] * sc;
           if (!full) {
 #pragma unroll
-            for (int u = 0; u < 16; ++u) x[u] = (see >> (i + u)) & 1 ? x[u] : -INFINITY;
+            for (int u = 0; u < kKeysRows; ++u) x[u] = (see >> u) & 1 ? x[u] : -INFINITY;
           }
         };
         guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
-        float top = -INFINITY;
+        form(true);
+        float top = x[0];
 #pragma unroll
-        for (int i = 0; i < CW; i += 16)
-          if (col0 + i < p.n16) {
-            form(i, true);
-#pragma unroll
-            for (int u = 0; u < 16; ++u) top = fmaxf(top, x[u]);
-          }
+        for (int u = 1; u < kKeysRows; ++u) top = fmaxf(top, x[u]);
         const bool raise = vote_any(top > kSlack, kSoft);
         if (raise) {
           // P's space and O are free once the previous value product has finished
           if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
           tc_after_sync();
-#pragma unroll 1  // rarely run: short code rather than fast code (cold instructions cost most)
-          for (int i = 0; i < CW; i += 16)
-            if (col0 + i < p.n16) {
-              form(i, false);
-              float mine = 0.0f;
+          form(false);
+          float mine = 0.0f;
 #pragma unroll
-              for (int u = 0; u < 16; ++u) {
-                const float mx = warp_max(x[u]);
-                if (u == lane) mine = mx;
-              }
-              if (lane < 16) scratch[wq * kMaxRows + col0 + i + lane] = mine;
-            }
+          for (int u = 0; u < kKeysRows; ++u) {
+            const float mx = warp_max(x[u]);
+            if (u == lane) mine = mx;
+          }
+          if (lane < kKeysRows) scratch[wq * kKeysRows + lane] = mine;
           named_bar_sync(1, kSoft);
-          if (tid < p.n16) {
+          if (tid < kKeysRows) {
             const float old = ref[tid];
             float mx = old;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, scratch[w * kMaxRows + tid]);
+            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, scratch[w * kKeysRows + tid]);
             ref[tid] = mx;
-            scratch[4 * kMaxRows + tid] = ex2(old - mx);
+            scratch[4 * kKeysRows + tid] = ex2(old - mx);
           }
           named_bar_sync(1, kSoft);
-          const float* fade = scratch + 4 * kMaxRows + col0;
           if (jj > 0) {
-            const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
+            const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kKeysRows;
+            load16(scratch + 4 * kKeysRows, r);
 #pragma unroll
-            for (int i = 0; i < CW; ++i) l[i] *= fade[i];
-#pragma unroll 1
-            for (int i = 0; i < CW; i += 16)
-              if (col0 + i < p.n16) {
-                float r[16];
-                load16(fade + i, r);
-                tc_ld16(ob + i, x);
-                tc_wait_ld();
+            for (int u = 0; u < kKeysRows; ++u) l[u] *= r[u];
+            tc_ld16(ob, x);
+            tc_wait_ld();
 #pragma unroll
-                for (int u = 0; u < 16; ++u) x[u] *= r[u];
-                tc_st16(ob + i, x);
-              }
+            for (int u = 0; u < kKeysRows; ++u) x[u] *= r[u];
+            tc_st16(ob, x);
             tc_wait_st();
           }
           named_bar_sync(1, kSoft);  // scratch read: its space becomes P again
+          form(true);
         }
-        float* keep = nullptr;  // where this key's scores go
-        int64_t keep_step = 0;
-        if (CW == 16 && WG == 1 && p.kept && key < rows) {
-          const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
-          keep_step = draft ? 64 : p.kept_len;
-          keep = draft ? p.kept_draft + unit * R * 64 + key : p.kept + unit * R * p.kept_len + j * kTile + key;
-        }
-        // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
-        uint8_t* prow = smem + lay.p + key * 128;
-#pragma unroll
-        for (int i = 0; i < CW; i += 16)
-          if (col0 + i < p.n16) {
-            if (CW == 16 && WG == 1 && p.kept) {
-              form(i, false);
-              float r[16];
-              load16(refs, r);
-#pragma unroll
-              for (int u = 0; u < 16; ++u) {
-                if (keep && u < R) keep[u * keep_step] = x[u];
-                x[u] -= r[u];
-              }
-            } else if (CW > 16 || raise) {
-              form(i, true);
-            }
-            uint32_t pk[8];
-#pragma unroll
-            for (int u = 0; u < 16; u += 2) {
-              const float e0 = ex2(x[u]), e1 = ex2(x[u + 1]);
-              l[i + u] += e0;
-              l[i + u + 1] += e1;
-              pk[u / 2] = pack2<BF16>(e0, e1);
-            }
-            if (i == 0 && k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);  // P's space is free
-            const int n = col0 + i, chunk = (n & 63) >> 3;
-            uint8_t* dst = prow + (n >> 6) * kPanel;
-            *reinterpret_cast<uint4*>(dst + ((chunk ^ (key & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            *reinterpret_cast<uint4*>(dst + (((chunk + 1) ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-          }
         tc_before_sync();
         mbar_arrive(s_empty + (k & 1));
+        if (p.kept && key < rows) {  // the score itself, for the weight pass
+          const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
+          const int64_t step = draft ? 64 : p.kept_len;
+          float* keep = draft ? p.kept_draft + unit * R * 64 + key : p.kept + unit * R * p.kept_len + j * kTile + key;
+#pragma unroll
+          for (int u = 0; u < kKeysRows; ++u)
+            if (u < R) keep[u * step] = x[u] + r[u];
+        }
+        // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
+        uint32_t pk[kKeysRows / 2];
+#pragma unroll
+        for (int u = 0; u < kKeysRows; u += 2) {
+          const float e0 = ex2(x[u]), e1 = ex2(x[u + 1]);
+          l[u] += e0;
+          l[u + 1] += e1;
+          pk[u / 2] = pack2<BF16>(e0, e1);
+        }
+        if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);  // P's space is free
+        uint8_t* prow = smem + lay.p + key * 128;
+        *reinterpret_cast<uint4*>(prow + ((key & 7) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+        *reinterpret_cast<uint4*>(prow + ((1 ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
         // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
         // product's last 16-row step reads beyond the valid rows, and unused drafted rows
-        if (grp == 0 && (rows & 15 || draft)) {
+        if (rows & 15 || draft) {
           uint64_t used = mk0 | mk1;
 #pragma unroll
           for (int o = 16; o; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
@@ -751,51 +712,42 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
         fence_proxy_async_smem();
         tc_before_sync();
         mbar_arrive(p_full);
-        vst += 2;
-        if (vst >= p.nst) {
-          vst -= p.nst;
-          ++vuse;
-        }
+        next_tile(p.nst, vst, vuse);
       }
       // ------------------------------------------------ end of the segment: sums, output
-      constexpr int kSum = CW < 32 ? CW : 32;
-      float sums[CW / kSum];
-#pragma unroll
-      for (int i = 0; i < CW; i += kSum) sums[i / kSum] = column_sums<kSum>(l + i, lane);
+      const float part_sum = column_sums16(l, lane);
       guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
       tc_after_sync();
-#pragma unroll
-      for (int i = 0; i < CW; i += kSum)
-        if (lane < kSum) scratch[wq * kMaxRows + col0 + i + lane] = sums[i / kSum];
+      if (lane < kKeysRows) scratch[wq * kKeysRows + lane] = part_sum;
       named_bar_sync(1, kSoft);
       const bool whole = s.n == s.nt;
       const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
-      if (tid < CW * WG) {
-        const float sum = scratch[tid] + scratch[kMaxRows + tid] + scratch[2 * kMaxRows + tid] +
-                          scratch[3 * kMaxRows + tid];
+      if (tid < kKeysRows) {
+        const float sum = (scratch[tid] + scratch[kKeysRows + tid]) + (scratch[2 * kKeysRows + tid] +
+                                                                       scratch[3 * kKeysRows + tid]);
         const bool real = my_mask != 0 && sum != 0.0f;
         const float top = ref[tid];
-        scratch[4 * kMaxRows + tid] = real ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
+        scratch[4 * kKeysRows + tid] = real ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
         ref[tid] = kNoRef;
         if (!whole) {
           float* ml = p.ml + static_cast<int64_t>(slot) * 2 * kMaxRows;
           ml[tid] = top;
           ml[kMaxRows + tid] = real ? sum : 0.0f;
         } else if (p.lse) {
-          const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
+          const int64_t unit = static_cast<int64_t>(s.t) * a.Hkv + s.kvh;
           p.lse[unit * kMaxRows + tid] = real ? top + log2f(sum) : INFINITY;
         }
       }
       named_bar_sync(1, kSoft);
-      const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kMaxRows + col0;
-      int row = col0, nd = s.rb * p.mb + col0 / p.G, gh = col0 % p.G;  // row, its node, its head of the group
-      uint16_t* out = a.out + s.t * a.os[0] + nd * a.os[1] + (s.kvh * p.G + gh) * a.os[2] + key;
-      float* part = p.part + (static_cast<int64_t>(slot) * R + col0) * DP + key;
+      const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kKeysRows;
+      int row = 0, nd = 0, gh = 0;  // row, its node, its head of the group
+      uint16_t* out = a.out + s.t * a.os[0] + s.kvh * p.G * a.os[2] + key;
+      float* part = p.part + static_cast<int64_t>(slot) * R * DP + key;
 #pragma unroll 1
-      for (int i = 0; i < CW && row < R; i += 4) {
+      for (int i = 0; i < R; i += 4) {
         float o[4];
         tc_ld4(ob + i, o);
-        const float4 inv = *reinterpret_cast<const float4*>(scratch + 4 * kMaxRows + row);
+        const float4 inv = *reinterpret_cast<const float4*>(scratch + 4 * kKeysRows + row);
         tc_wait_ld();
 #pragma unroll
         for (int u = 0; u < 4; ++u, ++row) {
@@ -805,7 +757,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
               if (key < DP) *part = o[u];
               part += DP;
             } else {
-              if (nd < a.m && key < a.d) *out = round16<BF16>(scale == 0.0f ? 0.0f : o[u] * scale);
+              if (key < a.d) *out = round16<BF16>(scale == 0.0f ? 0.0f : o[u] * scale);
               out += a.os[2];
               if (++gh == p.G) {
                 gh = 0;
@@ -819,18 +771,18 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
       tc_before_sync();
       mbar_arrive(o_empty + (seg & 1));
 #pragma unroll
-      for (int i = 0; i < CW; ++i) l[i] = 0.0f;
+      for (int i = 0; i < kKeysRows; ++i) l[i] = 0.0f;
       named_bar_sync(1, kSoft);  // scratch read, m_ref reset
     }
   }
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  if (warp == 4 * WG + 1) tmem_dealloc(*tmem_base, 512);
+  if (warp == 5) tmem_dealloc(*tmem_base, 128);
 }
 
 // ---------------------------------------------------------------------------
-// More than 64 rows: the rows fill the TMEM lanes (S[128 rows, 128 keys], O[128 rows, d]).
+// More than 16 rows: the rows fill the TMEM lanes (S[128 rows, 128 keys], O[128 rows, d]).
 // A thread then holds 64 scores of one row, so the running reference, the sum and the mask are
 // one register each, the vote for a new maximum concerns the two warps that share a row, and P
 // goes back to TMEM as the A operand of the value product (in the place of the scores, once
@@ -838,7 +790,7 @@ __global__ void __launch_bounds__(128 * WG + 64, 1) k_tree_attn(const __grid_con
 // work took 3,500 cycles per tile (tables of references and sums per thread, P and both operand
 // streams through shared memory).
 // ---------------------------------------------------------------------------
-constexpr int kRowsThreads = 256 + 64;
+constexpr int kRowsThreads = 256 + 96;  // softmax, TMA, score products, value products
 
 // 32 consecutive TMEM columns of packed pairs
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* u) {
@@ -885,10 +837,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   uint64_t* q_full = s_full + 2;             // [2]
   uint64_t* q_empty = q_full + 2;            // [2]
   uint64_t* o_empty = q_empty + 2;           // [2]
-  uint64_t* p_full = o_empty + 2;            // [2]: the next tile's P may be done before this one is used
-  uint64_t* pv_done = p_full + 2;
+  uint64_t* p_full = o_empty + 2;            // [2]
+  uint64_t* pv_done = p_full + 2;            // [2]
   const TreeBars bars = {kv_full, kv_empty, q_full, q_empty};
-  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 1);
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 2);
   float* xchg = reinterpret_cast<float*>(misc + kMiscRef);  // [2][128] between the two warps of a row
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
 
@@ -910,8 +862,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         mbar_init(q_empty + i, 1);
         mbar_init(o_empty + i, kSoft);
         mbar_init(p_full + i, kSoft);
+        mbar_init(pv_done + i, 1);
       }
-      mbar_init(pv_done, 1);
       fence_mbar_init();
     }
   } else if (warp == 9) {
@@ -938,82 +890,63 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   if (warp == 8) {
     tma_role<PANELS>(p, tab, lay, bars, beg, end, ring, qbase, R);
   } else if (warp == 9) {
-    // ---------------------------------------------------------------- MMA
-    const uint32_t id_qk = instr_desc(BF16, kTile, false, false);
-    const uint32_t id_pv = instr_desc(BF16, DP, false, true);
-    const uint32_t ring_k = smem_desc(ring, 16), ring_v = smem_desc(ring, kPanel);
-    const uint32_t q_desc = smem_desc(qbase, 16);
+    // ---------------------------------------------------------------- scores
+    const uint32_t idesc = instr_desc(BF16, kTile, false, false);
+    const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
     const uint32_t tmem = *tmem_base;
-    Segment sq = {}, sv = {};
-    int jq = 0, jv = 0, seg_q = -1, seg_v = -1, fq = beg, fv = beg;
-    bool more = true;
-    int st_k = 0, use_k = 0, st_v = 1, use_v = 0;
-    for (int k = 0; more; ++k) {
-      if (jq == sq.n) {
-        more = next_segment(p, tab, fq, end, p.RB, sq);
-        jq = 0;
-        ++seg_q;
-      }
-      if (more) {
-        const int qs = p.nq == 2 ? seg_q & 1 : 0, quse = p.nq == 2 ? seg_q >> 1 : seg_q;
-        if (jq == 0) guarded_wait(q_full + qs, quse & 1, dead, a.err);
-        guarded_wait(kv_full + st_k, use_k & 1, dead, a.err);
-        // the buffer of tile k - 2 held its P: its value product must have read it
-        if (k >= 2) guarded_wait(pv_done, k & 1, dead, a.err);
+    int k = 0, seg = 0, st = 0, use = 0;
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
+      const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+      guarded_wait(q_full + qs, quse & 1, dead, a.err);
+      for (int jj = 0; jj < s.n; ++jj, ++k) {
+        guarded_wait(kv_full + st, use & 1, dead, a.err);
+        // the buffer of tile k - 2 holds its P until its value product has read it
+        if (k >= 2) guarded_wait(pv_done + (k & 1), ((k >> 1) - 1) & 1, dead, a.err);
         tc_after_sync();
-        ++jq;
         if (elect_one()) {
-          const uint32_t ka = ring_k + (st_k * lay.stage >> 4), qa = q_desc + (qs * lay.qslot >> 4);
+          const uint32_t ka = ring_k + (st * lay.stage >> 4), qa = q_desc + (qs * lay.qslot >> 4);
 #pragma unroll
           for (int kk = 0; kk < PANELS * 4; ++kk)
             tc_mma(tmem + (k & 1) * kTile, qa + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2,
-                   ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+                   ka + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, idesc, kk > 0);
           tc_commit(s_full + (k & 1));
-          tc_commit(kv_empty + st_k);
-          if (jq == sq.n) tc_commit(q_empty + qs);
+          tc_commit(kv_empty + st);
+          if (jj + 1 == s.n) tc_commit(q_empty + qs);
         }
         __syncwarp();
-        st_k += 2;
-        if (st_k >= p.nst) {
-          st_k -= p.nst;
-          ++use_k;
-        }
+        next_tile(p.nst, st, use);
       }
-      if (k > 0) {
-        const int e = k - 1;
-        if (jv == sv.n) {
-          next_segment(p, tab, fv, end, p.RB, sv);
-          jv = 0;
-          ++seg_v;
-        }
-        guarded_wait(kv_full + st_v, use_v & 1, dead, a.err);
-        if (jv == 0 && seg_v >= 2) guarded_wait(o_empty + (seg_v & 1), ((seg_v >> 1) - 1) & 1, dead, a.err);
-        guarded_wait(p_full + (e & 1), (e >> 1) & 1, dead, a.err);
+    }
+    if (dead) drain_products();
+  } else if (warp == 10) {
+    // ---------------------------------------------------------------- values
+    const uint32_t idesc = instr_desc(BF16, DP, false, true);
+    const uint32_t ring_v = smem_desc(ring, kPanel);
+    const uint32_t tmem = *tmem_base;
+    int k = 0, seg = 0, st = 1, use = 0;
+    Segment s;
+    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
+      const uint32_t o = tmem + (2 + (seg & 1)) * kTile;
+      for (int jj = 0; jj < s.n; ++jj, ++k) {
+        const int steps = (tile_rows(s.len, s.nt, a.m, s.j0 + jj) + 15) / 16;
+        guarded_wait(kv_full + st, use & 1, dead, a.err);
+        if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
+        guarded_wait(p_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
-        const int steps = (tile_rows(sv.len, sv.nt, a.m, sv.j0 + jv) + 15) / 16;
         if (elect_one()) {
-          const uint32_t va = ring_v + (st_v * lay.stage >> 4);
-          const uint32_t o = tmem + (2 + (seg_v & 1)) * kTile, pa = tmem + (e & 1) * kTile;
+          const uint32_t va = ring_v + (st * lay.stage >> 4), pa = tmem + (k & 1) * kTile;
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
-            if (kk < steps) tc_mma_ts(o, pa + kk * 8, va + kk * (2048 >> 4), id_pv, jv > 0 || kk > 0);
-          tc_commit(kv_empty + st_v);
-          tc_commit(pv_done);
+            if (kk < steps) tc_mma_ts(o, pa + kk * 8, va + kk * (2048 >> 4), idesc, jj > 0 || kk > 0);
+          tc_commit(kv_empty + st);
+          tc_commit(pv_done + (k & 1));
         }
         __syncwarp();
-        ++jv;
-        st_v += 2;
-        if (st_v >= p.nst) {
-          st_v -= p.nst;
-          ++use_v;
-        }
+        next_tile(p.nst, st, use);
       }
     }
-    if (dead) {  // products still in flight must end before TMEM is freed
-      const long long t0 = clock64();
-      while (clock64() - t0 < 1000000) {
-      }
-    }
+    if (dead) drain_products();
   } else {
     // ---------------------------------------------------------------- softmax
     const int grp = warp >> 2, wq = warp & 3;
@@ -1067,7 +1000,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         tc_after_sync();  // both warps of the row have read its scores: P may take their place
         if (raise) {
           xchg[grp * kTile + row] = mx;
-          if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);  // O as the last product left it
+          if (k > 0) guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);  // O as the last product left it
           named_bar_sync(1 + wq, 64);
           const float now = fmaxf(fmaxf(xchg[row], xchg[kTile + row]), ref);
           named_bar_sync(1 + wq, 64);  // read by both before the next exchange
@@ -1118,11 +1051,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         tc_wait_st();
         tc_before_sync();
         mbar_arrive(p_full + (k & 1));
-        vst += 2;
-        if (vst >= p.nst) {
-          vst -= p.nst;
-          ++vuse;
-        }
+        next_tile(p.nst, vst, vuse);
       }
       // ------------------------------------------------ end of the segment: sums, output
       xchg[grp * kTile + row] = l;
@@ -1144,7 +1073,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
       const float inv = real ? 1.0f / sum : 0.0f;
       uint16_t* out = a.out + s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + my_head) * a.os[2];
       float* part = p.part + (static_cast<int64_t>(slot) * R + row) * DP;
-      guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
+      guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);
       tc_after_sync();
 #pragma unroll 1
       for (int i = grp * (DP / 2); i < (grp + 1) * (DP / 2); i += 16) {
@@ -1197,8 +1126,8 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   __shared__ int red[2][kJoinBlock / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const TreeAttnArgs& a = p.a;
-  pdl_wait();
-  pdl_launch_dependents();
+  // Lengths and masks may be read before the attention has finished: it began only after the
+  // kernels that wrote them had.
   const int units = a.Hkv * p.RB;
   const int t = blockIdx.x / units, u = blockIdx.x - t * units;  // trace of this launch
   int before = 0, total = 0;
@@ -1229,40 +1158,40 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   // the CTA that holds position f: the largest c with cut(c) <= f
   const int c0 = static_cast<int>(((static_cast<int64_t>(f0) + 1) * g - 1) / total);
   const int c1 = static_cast<int>(((static_cast<int64_t>(f1) + 1) * g - 1) / total);
-  if (c0 == c1) return;
   const int R = p.mb * p.G;
-  const int kvh = u / p.RB, rb = u - kvh * p.RB;
+  const int kvh = u / p.RB, rb = u - kvh * p.RB, tr = p.t0 + t;
   constexpr int kLanes = DP / 4;  // threads of a row, four values each
-  for (int rr = tid / kLanes; rr < kJoinRows; rr += kJoinBlock / kLanes) {
-    const int n = blockIdx.y * kJoinRows + rr, v = (tid % kLanes) * 4;
-    const int node = rb * p.mb + n / p.G;
-    if (n >= R || node >= a.m) continue;
-    float top = kNoRef;
-    for (int c = c0; c <= c1; ++c)
-      top = fmaxf(top, p.ml[static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * 2 * kMaxRows + n]);
-    float sum = 0.0f, o[4] = {};
+  const int n = blockIdx.y * kJoinRows + tid / kLanes, v = (tid % kLanes) * 4;
+  const int node = rb * p.mb + n / p.G;
+  const bool mine = c0 != c1 && tid / kLanes < kJoinRows && n < R && node < a.m;
+  const bool shown = mine && a.masks[tr * a.mask_stride + node] != 0;
+  uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!mine) return;
+  float top = kNoRef;
 #pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
-      const float w = ex2(p.ml[slot * 2 * kMaxRows + n] - top);
-      const float4 x = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
-      sum = fmaf(w, p.ml[(slot * 2 + 1) * kMaxRows + n], sum);
-      o[0] = fmaf(w, x.x, o[0]);
-      o[1] = fmaf(w, x.y, o[1]);
-      o[2] = fmaf(w, x.z, o[2]);
-      o[3] = fmaf(w, x.w, o[3]);
-    }
-    const int tr = p.t0 + t;
-    const bool real = a.masks[tr * a.mask_stride + node] != 0 && sum != 0.0f;
-    const float inv = real ? 1.0f / sum : 0.0f;
-    uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (v + i < a.d) out[v + i] = round16<BF16>(real ? o[i] * inv : 0.0f);
-    if (p.lse && v == 0)
-      p.lse[((static_cast<int64_t>(tr) * a.Hkv + kvh) * p.RB + rb) * kMaxRows + n] =
-          real ? top + log2f(sum) : INFINITY;
+  for (int c = c0; c <= c1; ++c)
+    top = fmaxf(top, p.ml[static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * 2 * kMaxRows + n]);
+  float sum = 0.0f, o[4] = {};
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
+    const float w = ex2(p.ml[slot * 2 * kMaxRows + n] - top);
+    const float4 x = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
+    sum = fmaf(w, p.ml[(slot * 2 + 1) * kMaxRows + n], sum);
+    o[0] = fmaf(w, x.x, o[0]);
+    o[1] = fmaf(w, x.y, o[1]);
+    o[2] = fmaf(w, x.z, o[2]);
+    o[3] = fmaf(w, x.w, o[3]);
   }
+  const bool real = shown && sum != 0.0f;
+  const float inv = real ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (v + i < a.d) out[v + i] = round16<BF16>(real ? o[i] * inv : 0.0f);
+  if (p.lse && v == 0)
+    p.lse[((static_cast<int64_t>(tr) * a.Hkv + kvh) * p.RB + rb) * kMaxRows + n] = real ? top + log2f(sum) : INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -1382,7 +1311,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     if (dead)
       for (int i = max(0, item - nst); i < item; ++i) mbar_wait(kv_full + i % nst, (i / nst) & 1);
   } else if (warp == 9) {
-    const uint32_t id_qk = instr_desc(BF16, p.n16, false, false);
+    const uint32_t id_qk = instr_desc(BF16, p.used, false, false);
     const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
     const uint32_t qpanel = p.n16 * 128 >> 4;
     int seg = 0, st = 0, use = 0, fills0 = 0, fills1 = 0;
@@ -1415,11 +1344,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
         }
       }
     }
-    if (dead) {
-      const long long t0 = clock64();
-      while (clock64() - t0 < 1000000) {
-      }
-    }
+    if (dead) drain_products();
   } else {
     const int grp = warp >> 2, wq = warp & 3;
     const int key = wq * 32 + lane;
@@ -1446,7 +1371,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
           guarded_wait(s_full + grp, fill & 1, dead, a.err);
           tc_after_sync();
           float w = 0.0f;
-          for (int n = 0; n < p.n16; n += 16) {
+          for (int n = 0; n < p.used; n += 16) {
             float x[16], ls[16];
             load16(lse + n, ls);
             tc_ld16(sbuf + n, x);
@@ -1522,7 +1447,7 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
 constexpr int kWholeRows = 512;
 
 struct TreePlan {
-  int G, RB, mb, n16, panels, nst, nq, grid;
+  int G, RB, mb, n16, used, panels, nst, nq, grid;
   uint32_t smem;
 };
 
@@ -1534,12 +1459,13 @@ static bool tree_plan(int T, int m, int H, int Hkv, int Lmax, int d, TreePlan* p
   pl->mb = (m + pl->RB - 1) / pl->RB;  // even blocks
   pl->RB = (m + pl->mb - 1) / pl->mb;
   pl->n16 = (pl->mb * pl->G + 15) / 16 * 16;
-  if (pl->n16 > 64) pl->n16 = kMaxRows;  // k_tree_attn_rows: rows fill the lanes
+  pl->used = pl->n16;
+  if (pl->n16 > kKeysRows) pl->n16 = kMaxRows;  // k_tree_attn_rows: rows fill the lanes
   pl->panels = d > 64 ? 2 : 1;
   pl->grid = sm_count();
   // flat tile numbers are 32-bit
   if (static_cast<int64_t>(std::min(T, kMaxTraces)) * Hkv * pl->RB * (Lmax / kTile + 2) > 0x7FFFFFFFll) return false;
-  // two Q slots (the next unit's queries load early) where they leave a ring of six stages
+  // two Q slots (the next unit's queries load early) where they leave a ring of five stages
   const uint32_t cap = 227 * 1024;
   for (pl->nq = 2;; --pl->nq) {
     const uint32_t fixed = tree_smem(pl->panels, pl->n16, 0, pl->nq).total;
@@ -1551,7 +1477,7 @@ static bool tree_plan(int T, int m, int H, int Hkv, int Lmax, int d, TreePlan* p
 }
 
 // Rows whose scores are kept for the weight pass rather than formed again from K.
-constexpr int kKeptRows = 16;
+constexpr int kKeptRows = kKeysRows;
 
 size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d, bool with_scores) {
   TreePlan pl;
@@ -1607,12 +1533,12 @@ static int allow_smem() {
   return MB_OK;
 }
 
-template <int PANELS, int CW, int WG, bool BF16>
-static int launch_attn(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  const int rc = allow_smem<k_tree_attn<PANELS, CW, WG, BF16>>();
+template <int PANELS, bool BF16>
+static int launch_attn_keys(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
+  const int rc = allow_smem<k_tree_attn_keys<PANELS, BF16>>();
   if (rc != MB_OK) return rc;
-  return launch_with_pdl(k_tree_attn<PANELS, CW, WG, BF16>, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid),
-                         dim3(128 * WG + 64), smem, st, p);
+  return launch_with_pdl(k_tree_attn_keys<PANELS, BF16>, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid),
+                         dim3(kKeysThreads), smem, st, p);
 }
 
 template <int PANELS, bool BF16>
@@ -1625,15 +1551,8 @@ static int launch_attn_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t 
 
 template <int PANELS, bool BF16>
 static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  int rc;
-  if (p.n16 <= 16)
-    rc = launch_attn<PANELS, 16, 1, BF16>(p, smem, st);
-  else if (p.n16 <= 32)
-    rc = launch_attn<PANELS, 16, 2, BF16>(p, smem, st);
-  else if (p.n16 <= 64)
-    rc = launch_attn<PANELS, 16, 4, BF16>(p, smem, st);
-  else
-    rc = launch_attn_rows<PANELS, BF16>(p, smem, st);
+  const int rc = p.n16 == kKeysRows ? launch_attn_keys<PANELS, BF16>(p, smem, st)
+                                    : launch_attn_rows<PANELS, BF16>(p, smem, st);
   if (rc != MB_OK || p.whole) return rc;
   const int R = p.mb * p.G;
   return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.T * p.a.Hkv * p.RB, (R + kJoinRows - 1) / kJoinRows),
@@ -1680,6 +1599,7 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   p.RB = pl.RB;
   p.mb = pl.mb;
   p.n16 = pl.n16;
+  p.used = pl.used;
   p.grid = pl.grid;
   p.nst = pl.nst;
   p.nq = pl.nq;
