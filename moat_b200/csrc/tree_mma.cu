@@ -54,6 +54,7 @@ struct TreeMmaParams {
   int t0, T;    // traces of this launch
   int RB, mb, G, grid, nst, nq;
   int n16, used;  // rows of a Q slot; rows of a block in steps of 16
+  int tile_cycles, tile_traffic;  // see share_mode
   bool whole;    // every unit in one CTA: nothing to join
   bool vec_out;  // 16-byte pieces of output rows
 };
@@ -229,7 +230,8 @@ struct Segment {  // a run of tiles of one unit
 // Lengths of the launch's traces and where each begins in the sequence, in shared memory.
 struct TraceTable {
   int cum[kMaxTraces + 1];
-  int len[kMaxTraces + 1];
+  int len[kMaxTraces];
+  int max_span;
 };
 
 // Starting and ending a piece costs about as much as a tile; it counts as one in the sequence,
@@ -273,10 +275,11 @@ __device__ __forceinline__ int tile_rows(int len, int nt, int m, int j) {
 
 // Fills the table (warp 0) for `units` units per trace.
 __device__ __forceinline__ void prefix_tiles(const TreeMmaParams& p, TraceTable& tab, int lane, int units) {
-  int base = 0;
+  int base = 0, longest = 0;
   for (int c = 0; c < p.T; c += 32) {
     const int t = c + lane;
     const int len = t < p.T ? trace_len(p.a, p.t0 + t) : 0;
+    longest = max(longest, len);
     int v = t < p.T ? unit_span(trace_tiles(len)) * units : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -289,7 +292,11 @@ __device__ __forceinline__ void prefix_tiles(const TreeMmaParams& p, TraceTable&
     }
     base += __shfl_sync(0xffffffffu, v, 31);
   }
-  if (lane == 0) tab.cum[0] = 0;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0) {
+    tab.cum[0] = 0;
+    tab.max_span = unit_span(trace_tiles(longest));
+  }
 }
 
 template <bool BF16>
@@ -340,19 +347,56 @@ __device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16,
   fence_proxy_async_smem();
 }
 
+// How the sequence is shared out. Cutting units costs their pieces' way through the workspace and
+// the join, 2 to 8 us; it pays where the longest share of whole units would outlast the memory
+// traffic. A tile takes a CTA p.tile_cycles; the memory needs p.tile_traffic cycles for the tiles
+// of one position in every CTA. Whole units are kept as long as the longest share of them, with
+// kShareFixed cycles for starting and ending, ends before the traffic does. Measured, 16 traces of
+// 4,096 rows of 128: 128 units of 128 / 32 rows 52.7 / 46.5 us whole, 59.9 / 49.1 cut; 256 units of 8
+// rows 85.0 dealt out whole, 87.1 cut; but 256 units of 512 to 752 rows 24.9 whole, 22.0 cut.
+enum class Share { kCut, kWholeUnit, kSnapped };
+constexpr int kShareFixed = 12000;
+
+__device__ __forceinline__ Share share_mode(const TreeMmaParams& p, int64_t total, int64_t max_span, int units) {
+  if (p.whole) return Share::kWholeUnit;
+  const int64_t traffic = p.tile_traffic * total - static_cast<int64_t>(kShareFixed) * p.grid;  // x grid CTAs
+  const int64_t longest = max_span * p.tile_cycles * p.grid;
+  if (units <= p.grid) return longest <= traffic ? Share::kWholeUnit : Share::kCut;
+  return longest + p.tile_cycles * total <= traffic ? Share::kSnapped : Share::kCut;
+}
+
+// The unit boundary nearest to position f.
+__device__ __forceinline__ int snap(const TreeMmaParams& p, const TraceTable& tab, int f) {
+  int lo = 0, hi = p.T;  // cum[T] is a boundary too
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.cum[mid] <= f)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  if (lo == p.T) return f;
+  const int span = unit_span(trace_tiles(tab.len[lo]));
+  return tab.cum[lo] + (f - tab.cum[lo] + span / 2) / span * span;
+}
+
 // Positions of the sequence that are CTA c's.
 __device__ __forceinline__ void cta_share(const TreeMmaParams& p, const TraceTable& tab, int c, int* beg, int* end) {
   *beg = *end = 0;
-  if (p.whole) {  // one unit per CTA
-    const int units = p.a.Hkv * p.RB, t = c / units;
+  const int units = p.a.Hkv * p.RB, total = tab.cum[p.T], g = min(p.grid, total);
+  const Share mode = share_mode(p, total, tab.max_span, units * p.T);
+  if (mode == Share::kWholeUnit) {
+    const int t = c / units;
+    if (t >= p.T) return;
     const int span = unit_span(trace_tiles(tab.len[t]));
     *beg = tab.cum[t] + (c - t * units) * span;
     *end = *beg + span;
-  } else {
-    const int total = tab.cum[p.T], g = min(p.grid, total);  // CTAs with work
-    if (c < g) {
-      *beg = cut(total, c, g);
-      *end = cut(total, c + 1, g);
+  } else if (c < g) {  // CTAs with work
+    *beg = cut(total, c, g);
+    *end = cut(total, c + 1, g);
+    if (mode == Share::kSnapped) {
+      *beg = snap(p, tab, *beg);
+      *end = snap(p, tab, *end);
     }
   }
 }
@@ -362,7 +406,7 @@ struct TreeBars {
 };
 
 // The TMA warp: K and V tiles of this CTA's segments through the ring, a segment's queries
-// after its first tile (their slot may still be in use).
+// before them, or after its first tile when their slot may still be in use.
 template <int PANELS>
 __device__ __forceinline__ void tma_role(const TreeMmaParams& p, const TraceTable& tab, const TreeSmem& lay,
                                          const TreeBars& bars, int beg, int end, uint32_t ring, uint32_t qbase, int R) {
@@ -380,6 +424,16 @@ __device__ __forceinline__ void tma_role(const TreeMmaParams& p, const TraceTabl
   Segment s;
   for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
     const int qs = p.nq == 2 ? seg & 1 : 0, quse = p.nq == 2 ? seg >> 1 : seg;
+    auto load_queries = [&] {
+      if (elect_one()) {
+        mbar_expect_tx(bars.q_full + qs, PANELS * R * 128);
+        for (int pn = 0; pn < PANELS; ++pn)
+          tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, bars.q_full + qs, pn * 64, s.kvh * p.G,
+                      s.rb * p.mb, s.t, keep);
+      }
+      __syncwarp();
+    };
+    if (quse == 0) load_queries();
     for (int j = s.j0; j < s.j0 + s.n; ++j) {
       const bool draft = j == s.nt - 1;
       const int rows = tile_rows(s.len, s.nt, a.m, j);
@@ -411,15 +465,9 @@ __device__ __forceinline__ void tma_role(const TreeMmaParams& p, const TraceTabl
           ++use;
         }
       }
-      if (j == s.j0) {
-        if (quse > 0) guarded_wait(bars.q_empty + qs, (quse - 1) & 1, dead, a.err);
-        if (elect_one()) {
-          mbar_expect_tx(bars.q_full + qs, PANELS * R * 128);
-          for (int pn = 0; pn < PANELS; ++pn)
-            tma_load_4d(qbase + qs * lay.qslot + pn * p.n16 * 128, &p.mq, bars.q_full + qs, pn * 64, s.kvh * p.G,
-                        s.rb * p.mb, s.t, keep);
-        }
-        __syncwarp();
+      if (quse > 0 && j == s.j0) {
+        guarded_wait(bars.q_empty + qs, (quse - 1) & 1, dead, a.err);
+        load_queries();
       }
     }
   }
@@ -1123,19 +1171,21 @@ constexpr int kJoinRows = 8;
 template <int PANELS, bool BF16>
 __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant__ TreeMmaParams p) {
   constexpr int DP = PANELS * 64;
-  __shared__ int red[2][kJoinBlock / 32];
+  __shared__ int red[3][kJoinBlock / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const TreeAttnArgs& a = p.a;
   // Lengths and masks may be read before the attention has finished: it began only after the
   // kernels that wrote them had.
   const int units = a.Hkv * p.RB;
   const int t = blockIdx.x / units, u = blockIdx.x - t * units;  // trace of this launch
-  int before = 0, total = 0;
+  int before = 0, total = 0, longest = 0;
   for (int i = tid; i < p.T; i += kJoinBlock) {
-    const int n = unit_span(trace_tiles(trace_len(a, p.t0 + i))) * units;
-    total += n;
-    before += i < t ? n : 0;
+    const int span = unit_span(trace_tiles(trace_len(a, p.t0 + i)));
+    total += span * units;
+    before += i < t ? span * units : 0;
+    longest = max(longest, span);
   }
+  longest = __reduce_max_sync(0xffffffffu, longest);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -1144,6 +1194,7 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   if (lane == 0) {
     red[0][warp] = total;
     red[1][warp] = before;
+    red[2][warp] = longest;
   }
   __syncthreads();
   total = before = 0;
@@ -1151,7 +1202,9 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   for (int w = 0; w < kJoinBlock / 32; ++w) {
     total += red[0][w];
     before += red[1][w];
+    longest = max(longest, red[2][w]);
   }
+  const bool cut_units = share_mode(p, total, longest, units * p.T) == Share::kCut;
   const int nt = trace_tiles(trace_len(a, p.t0 + t));
   const int f0 = before + u * unit_span(nt) + kUnitCost, f1 = f0 + nt - 1;  // its first and last tile
   const int g = min(p.grid, total);
@@ -1163,7 +1216,7 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   constexpr int kLanes = DP / 4;  // threads of a row, four values each
   const int n = blockIdx.y * kJoinRows + tid / kLanes, v = (tid % kLanes) * 4;
   const int node = rb * p.mb + n / p.G;
-  const bool mine = c0 != c1 && tid / kLanes < kJoinRows && n < R && node < a.m;
+  const bool mine = cut_units && c0 != c1 && tid / kLanes < kJoinRows && n < R && node < a.m;
   const bool shown = mine && a.masks[tr * a.mask_stride + node] != 0;
   uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
   pdl_wait();
@@ -1598,6 +1651,11 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   p.G = pl.G;
   p.RB = pl.RB;
   p.mb = pl.mb;
+  // measured: a tile of the keys kernel 1,500 cycles (three quarters at d <= 64), of the rows
+  // kernel 2,000; 128 keys and values of 128 bytes-a-row panels at 6.4 TB/s, 148 SMs
+  p.tile_cycles = pl.n16 > kKeysRows ? 2000 : pl.panels == 2 ? 1500 : 1100;
+  p.tile_traffic = pl.panels == 2 ? 2900 : 1450;
+  if (pl.RB > 1) p.tile_traffic /= pl.RB;  // the row blocks share their keys' traffic
   p.n16 = pl.n16;
   p.used = pl.used;
   p.grid = pl.grid;

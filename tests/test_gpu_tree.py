@@ -140,6 +140,9 @@ SHAPES = [
     (5, 16, 32, 8, 128, [1, 1025, 64, 0, 2000], 2048),
     (16, 1, 16, 16, 128, [1100 - 67 * t for t in range(16)], 1100),  # several odd-length pieces per CTA
     (6, 40, 16, 2, 64, [130, 1300, 700, 0, 901, 2500], 2500),  # row blocks and such pieces
+    (80, 1, 8, 8, 128, [400 - 3 * t for t in range(79)] + [0], 400),  # more units than SMs: dealt out whole
+    (16, 2, 8, 8, 128, [2000 - t for t in range(16)], 2000),  # as many units as SMs, nearly: one each
+    (16, 5, 32, 8, 128, [4100 - t for t in range(16)], 4100),  # the same with more than 16 rows
 ]
 
 

@@ -105,7 +105,7 @@ def test_accept_entry_checks_its_arguments(L):
     assert accept(m=65) == -2 and accept(T=0) == -2 and accept(layers=0) == -2 and accept(Lmax=0) == -2
     assert accept(lens_out=fake) == -2  # in place: another CTA may still read the old length
     assert accept(pos_out=fake) == -2
-    assert accept(T=70000) == -6
+    assert accept(layers=70000) == -6 and accept(Hkv=70000) == -6
 
 
 def test_rope_and_evict_entries_check_their_arguments(L):
