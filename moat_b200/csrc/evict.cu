@@ -6,6 +6,8 @@
 // rows, so nothing is shifted: the j-th row at or beyond the budget that stays (a mover)
 // goes into the j-th row below the budget that leaves (a hole). Holes and movers are
 // disjoint, so the moves have no order among them; only moved rows cost bandwidth.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "common.cuh"
@@ -32,7 +34,7 @@ constexpr int kMaxWarps = 32;
 
 // Order-preserving image of a row's rank: a guarded row above everything, NaN below
 // everything, -0 equal to +0.
-__device__ __forceinline__ uint32_t rank_code(float s, int pos, int64_t recent_from, int sinks) {
+__device__ __forceinline__ uint32_t rank_code(float s, int pos, int recent_from, int sinks) {
   if (pos >= recent_from || pos < sinks) return 0xFFFFFFFFu;
   if (s != s) return 0u;
   const uint32_t b = __float_as_uint(s + 0.0f);
@@ -93,7 +95,7 @@ __device__ __forceinline__ void unit_sync() {
     __syncthreads();
 }
 
-// Sum over the cluster's lower ranks of *word (same place in every CTA), and over all of them.
+// *word (same place in every CTA) summed over the cluster's lower ranks, and over all of them.
 template <int CS>
 __device__ __forceinline__ int ranks_before(uint32_t* word, uint32_t rank, int* all) {
   if (CS == 1) {
@@ -111,29 +113,120 @@ __device__ __forceinline__ int ranks_before(uint32_t* word, uint32_t rank, int* 
   return before;
 }
 
+constexpr int kBins = 2048;  // most bins of a histogram
+
+// The digit at which the unit's counts, from the largest digit of `bins` downwards, reach `need`;
+// how many of that digit are still needed and how many there are. Every CTA of the cluster sums
+// all histograms; result[] is its own. Ends with the cluster in step.
+template <int CS>
+__device__ __forceinline__ void find_digit(const uint32_t* hist, int bins, int need, uint32_t* wsum, int* result) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (bins + blockDim.x - 1) / blockDim.x;  // bins of this thread, from the top: at most 16
+  const int top = bins - 1 - tid * per;
+  unit_sync<CS>();
+  uint32_t bin[16];
+  int sum = 0;
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    bin[u] = 0;
+    if (u < per && top - u >= 0) {
+      if (CS == 1) {
+        bin[u] = hist[top - u];
+      } else {
+#pragma unroll
+        for (uint32_t r = 0; r < CS; ++r) bin[u] += ld_cluster_u32(mapa_shared(smem_u32(hist + top - u), r));
+      }
+      sum += bin[u];
+    }
+  }
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) wsum[warp] = upto;
+  __syncthreads();
+  upto += __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
+  if (upto >= need && upto - sum < need) {  // one thread
+    int left = need - (upto - sum), at = 0, count = 0;
+    bool done = false;
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      if (!done && u < per) {
+        at = u;
+        count = static_cast<int>(bin[u]);
+        done = count >= left;
+        if (!done) left -= count;
+      }
+    result[0] = top - at;
+    result[1] = left;
+    result[2] = count;
+  }
+  unit_sync<CS>();  // and every CTA has read the histograms
+}
+
+// The same for the last `bits` bits of at most 32 kPer ranks that share the bits above, by one warp:
+// the ranks in registers, the answer (the whole rank) bit by bit.
+template <int kPer>
+__device__ __forceinline__ void finish_in_warp(const uint32_t* cand, int n, uint32_t above, int bits, int need, int lane,
+                                               int* result) {
+  uint32_t r[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) r[u] = u * 32 + lane < n ? cand[u * 32 + lane] : 0u;  // absent: 0
+  uint32_t at = above << bits;
+  auto count = [&](auto test) {
+    int c = 0;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) c += test(r[u]);
+    return __reduce_add_sync(0xffffffffu, c);
+  };
+  for (int b = bits - 1; b >= 0; --b) {
+    const uint32_t trial = at | (1u << b);
+    if (count([&](uint32_t x) { return x >= trial; }) >= need) at = trial;
+  }
+  const int larger = count([&](uint32_t x) { return x > at; });
+  const int equal = count([&](uint32_t x) { return x == at; });  // absent ones too if at is 0: more than needed
+  if (lane == 0) {
+    result[0] = static_cast<int>(at);
+    result[1] = need - larger;
+    result[2] = equal;
+  }
+}
+
 // Selection for one (layer, trace, KV head) by a cluster of CS CTAs, each with a slice of the
-// rows. The ranks stay in shared memory: scores and positions are read once. The kept-th
-// largest rank is found eight bits at a time from histograms (joined through distributed
-// shared memory); then every warp sweeps its own run of rows, so that ties, holes and movers
-// are numbered in row order with one exchange of counts each. FUSED (CS = 1): the same CTA
-// moves the rows; otherwise the numbered moves go to the workspace for k_evict_move.
+// rows. Bound by instructions per row where few units share the GPU: scores and positions are
+// read once, their ranks stay in shared memory; the kept-th largest rank is found from three
+// histograms (joined through distributed shared memory), the second and third of only the rows
+// whose first digit is the threshold's (in one warp where they are few); every warp sweeps its own run of rows, so that holes and
+// movers (and ties, where not all of them stay) are numbered in row order with one exchange of
+// counts. FUSED (CS = 1): the same CTA moves the rows; otherwise the numbered moves go to the
+// workspace for k_evict_move.
 template <int CS, bool FUSED>
-__global__ void __launch_bounds__(1024) k_evict(const __grid_constant__ EvictArgs a) {
+__global__ void __launch_bounds__(FUSED ? 512 : 1024) k_evict(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t dyn[];
-  __shared__ uint32_t hist[256];  // this CTA's
-  __shared__ uint32_t digit_s, need_s;
-  __shared__ uint32_t wties[kMaxWarps + 1], wholes[kMaxWarps + 1], wmovers[kMaxWarps + 1];  // [kMaxWarps]: the CTA's
-  uint32_t* code = dyn;               // [slice]
-  uint32_t* stay = code + a.slice;    // [slice / 32]
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t wsum[kMaxWarps];
+  __shared__ int digit[3];
+  __shared__ uint32_t n_cand;
+  __shared__ uint32_t counts[3][kMaxWarps + 1];  // ties, holes, movers: by warp, then the CTA's
+  constexpr int kLow = FUSED ? 22 : 21;  // bits below the first digit
+  constexpr int kFirst = 1 << (32 - kLow);
+  uint32_t* code = dyn;                  // [slice]
+  uint32_t* stay = code + a.slice;       // [slice / 32]
+  uint32_t* cand = stay + a.slice / 32;  // [slice / 4] ranks with the threshold's first digit (FUSED)
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
   const uint32_t rank = CS > 1 ? cluster_ctarank() : 0;
+  for (int i = tid; i < kFirst; i += threads) hist[i] = 0;
+  if (tid == 0) n_cand = 0;
   pdl_wait();
   pdl_launch_dependents();
   const int64_t unit = blockIdx.x / CS;
   const int h = unit % a.Hkv, t = (unit / a.Hkv) % a.T, layer = unit / (static_cast<int64_t>(a.Hkv) * a.T);
   const int len = max(0, min(a.lens[t], a.Lmax));
   const int kept = min(len, a.budget);
-  const int64_t recent_from = static_cast<int64_t>(a.next_pos[t]) - a.recent;
+  const int recent_from =
+      static_cast<int>(max(static_cast<int64_t>(a.next_pos[t]) - a.recent, static_cast<int64_t>(INT_MIN)));
   const float* sc = a.scores + unit * a.Lmax;
   const int32_t* ps = a.positions + unit * a.Lmax;
   float* so = a.scores_out + unit * a.Lmax;
@@ -152,7 +245,6 @@ __global__ void __launch_bounds__(1024) k_evict(const __grid_constant__ EvictArg
     return;  // the whole cluster
   }
   // ranks, and the histogram of their first digit
-  for (int i = tid; i < 256; i += threads) hist[i] = 0;
   __syncthreads();
   if (a.vec_ranks) {  // r0 is a multiple of 128
     const float4* s4 = reinterpret_cast<const float4*>(sc + r0);
@@ -164,125 +256,183 @@ __global__ void __launch_bounds__(1024) k_evict(const __grid_constant__ EvictArg
       const uint4 c = make_uint4(rank_code(s.x, p.x, recent_from, a.sinks), rank_code(s.y, p.y, recent_from, a.sinks),
                                  rank_code(s.z, p.z, recent_from, a.sinks), rank_code(s.w, p.w, recent_from, a.sinks));
       *reinterpret_cast<uint4*>(code + 4 * i) = c;
-      if (4 * i < n) atomicAdd(&hist[c.x >> 24], 1u);
-      if (4 * i + 1 < n) atomicAdd(&hist[c.y >> 24], 1u);
-      if (4 * i + 2 < n) atomicAdd(&hist[c.z >> 24], 1u);
-      if (4 * i + 3 < n) atomicAdd(&hist[c.w >> 24], 1u);
+      if (4 * i < n) atomicAdd(&hist[c.x >> kLow], 1u);
+      if (4 * i + 1 < n) atomicAdd(&hist[c.y >> kLow], 1u);
+      if (4 * i + 2 < n) atomicAdd(&hist[c.z >> kLow], 1u);
+      if (4 * i + 3 < n) atomicAdd(&hist[c.w >> kLow], 1u);
     }
   } else {
 #pragma unroll 4
     for (int i = tid; i < n; i += threads) {
       const uint32_t c = rank_code(sc[r0 + i], ps[r0 + i], recent_from, a.sinks);
       code[i] = c;
-      atomicAdd(&hist[c >> 24], 1u);
+      atomicAdd(&hist[c >> kLow], 1u);
     }
   }
-  uint32_t prefix = 0;
-  int need = kept;
-  for (int shift = 24;; shift -= 8) {
-    unit_sync<CS>();
-    if (warp == 0) {  // lane l has digits 255 - 8 l downwards; find the digit where the count reaches need
-      uint32_t bin[8];
-      int sum = 0;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int b = 255 - 8 * lane - u;
-        if (CS == 1) {
-          bin[u] = hist[b];
-        } else {
-          bin[u] = 0;
-#pragma unroll
-          for (uint32_t r = 0; r < CS; ++r) bin[u] += ld_cluster_u32(mapa_shared(smem_u32(&hist[b]), r));
-        }
-        sum += bin[u];
-      }
-      int upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      const int first = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;  // need <= rows: one lane has it
-      if (lane == first) {
-        int left = need - (upto - sum), u = 0;
-        while (u < 7 && static_cast<int>(bin[u]) < left) left -= bin[u++];
-        digit_s = 255 - 8 * lane - u;
-        need_s = left;
-      }
-    }
-    unit_sync<CS>();  // also: every CTA has read the histograms
-    prefix |= digit_s << shift;
-    need = need_s;
-    if (shift == 0) break;
-    for (int i = tid; i < 256; i += threads) hist[i] = 0;
-    __syncthreads();
+  find_digit<CS>(hist, kFirst, kept, wsum, digit);
+  const uint32_t first = digit[0];
+  int need = digit[1];
+  uint32_t limit = 0;  // the kept-th largest rank
+  bool found = false;
+  if (FUSED) {  // few rows: those of this digit are usually few enough for one warp
+    const uint32_t room = a.slice / 4;
+#pragma unroll 4
     for (int i = tid; i < n; i += threads) {
       const uint32_t c = code[i];
-      if ((c >> shift) == (prefix >> shift)) atomicAdd(&hist[(c >> (shift - 8)) & 255], 1u);
+      if (c >> kLow == first) {
+        const uint32_t at = atomicAdd(&n_cand, 1u);
+        if (at < room) cand[at] = c;
+      }
+    }
+    __syncthreads();
+    found = n_cand <= min(room, 512u);
+    if (found) {
+      if (warp == 0) {
+        if (n_cand <= 64)
+          finish_in_warp<2>(cand, n_cand, first, kLow, need, lane, digit);
+        else
+          finish_in_warp<16>(cand, n_cand, first, kLow, need, lane, digit);
+      }
+      __syncthreads();
+      limit = static_cast<uint32_t>(digit[0]);
     }
   }
-  // every warp's run of rows, whole words of 32
+  if (!found) {
+    auto count_digits = [&](int shift, uint32_t above, int drop, uint32_t mask) {  // of the rows with c >> shift == above
+      for (int i = tid; i < kBins; i += threads) hist[i] = 0;
+      __syncthreads();
+      const uint4* c4 = reinterpret_cast<const uint4*>(code);
+#pragma unroll 2
+      for (int i = tid; i < (n + 3) / 4; i += threads) {
+        const uint4 v = c4[i];
+        const uint32_t c[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (c[u] >> shift == above && 4 * i + u < n) atomicAdd(&hist[(c[u] >> drop) & mask], 1u);
+      }
+    };
+    count_digits(kLow, first, kLow - 11, kBins - 1);
+    find_digit<CS>(hist, kBins, need, wsum, digit);
+    const uint32_t upper = first << 11 | static_cast<uint32_t>(digit[0]);
+    need = digit[1];
+    count_digits(kLow - 11, upper, 0, (1u << (kLow - 11)) - 1);
+    find_digit<CS>(hist, 1 << (kLow - 11), need, wsum, digit);
+    limit = upper << (kLow - 11) | static_cast<uint32_t>(digit[0]);
+  }
+  need = digit[1];
+  const bool all_ties = need == digit[2];
+  // Every warp's run of rows, whole words of 32; a word's bits are gathered by ballots and then
+  // handled by one lane, 32 words at a time.
   const int words = (n + 31) / 32, per = (words + warps - 1) / warps;
   const int w0 = min(words, warp * per), w1 = min(words, w0 + per);
-  int ties = 0;
-  for (int w = w0; w < w1; ++w) {
-    const int i = w * 32 + lane;
-    ties += __popc(__ballot_sync(0xffffffffu, i < n && code[i] == prefix));
-  }
-  auto number = [&](uint32_t* counts, int mine) {  // this warp's first number among the unit's, counts[kMaxWarps] the CTA's
-    if (lane == 0) counts[warp] = mine;
-    __syncthreads();
-    if (warp == 0) {
-      const int v = lane < warps ? static_cast<int>(counts[lane]) : 0;
-      int x = v;
+  auto before_lane = [&](int v) {  // sum over the lower lanes
+    int x = v;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      counts[lane] = x - v;
-      if (lane == 31) counts[kMaxWarps] = x;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
+    return x - v;
   };
-  number(wties, ties);
-  unit_sync<CS>();
-  int all;
-  int tie = ranks_before<CS>(&wties[kMaxWarps], rank, &all) + wties[warp];
+  auto scan = [&](uint32_t* c) {  // counts of the warps before each warp, and of the CTA (one warp)
+    const int v = lane < warps ? static_cast<int>(c[lane]) : 0;
+    const int x = before_lane(v);
+    c[lane] = x;
+    if (lane == 31) c[kMaxWarps] = x + v;
+  };
+  auto gather = [&](int wb, auto test) {  // word wb + lane of this warp's run: bit i is test(row i)
+    uint32_t mine = 0;
+#pragma unroll 4
+    for (int u = 0; u < min(32, w1 - wb); ++u) {
+      const int i = (wb + u) * 32 + lane;
+      const uint32_t bits = __ballot_sync(0xffffffffu, i < n && test(code[i]));
+      mine = u == lane ? bits : mine;
+    }
+    return mine;
+  };
+  int all, tie = 0;
+  if (!all_ties) {  // the first `need` ties of the unit stay
+    int ties = 0;
+    for (int wb = w0; wb < w1; wb += 32) ties += __popc(gather(wb, [&](uint32_t c) { return c == limit; }));
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) counts[0][warp] = ties;
+    __syncthreads();
+    if (warp == 0) scan(counts[0]);
+    unit_sync<CS>();
+    tie = ranks_before<CS>(&counts[0][kMaxWarps], rank, &all) + counts[0][warp];
+  }
+  // of word w: the rows below the budget, the valid rows
+  auto low_rows = [&](int w) {
+    const int below = kept - (r0 + w * 32);
+    return below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1;
+  };
+  auto valid_rows = [&](int w) {
+    const int rows = n - w * 32;
+    return rows >= 32 ? 0xffffffffu : rows <= 0 ? 0u : (1u << rows) - 1;
+  };
   int holes = 0, movers = 0;
-  for (int w = w0; w < w1; ++w) {  // the first `need` ties stay
-    const int i = w * 32 + lane;
-    const uint32_t c = i < n ? code[i] : 0u;
-    const uint32_t tied = __ballot_sync(0xffffffffu, i < n && c == prefix);
-    const bool stays = i < n && (c > prefix || (c == prefix && tie + __popc(tied & ((1u << lane) - 1)) < need));
-    tie += __popc(tied);
-    const uint32_t bits = __ballot_sync(0xffffffffu, stays);
-    if (lane == 0) stay[w] = bits;
-    const uint32_t low = __ballot_sync(0xffffffffu, i < n && r0 + i < kept);
-    holes += __popc(low & ~bits);
+  for (int wb = w0; wb < w1; wb += 32) {
+    const int w = wb + lane;
+    uint32_t bits = gather(wb, [&](uint32_t c) { return c >= limit; });
+    if (!all_ties) {
+      uint32_t tied = gather(wb, [&](uint32_t c) { return c == limit; });
+      const int mine = __popc(tied);
+      int spare = need - tie - before_lane(mine);  // ties of this word that stay
+      tie += __reduce_add_sync(0xffffffffu, mine);
+      for (; tied && spare > 0; --spare) tied &= tied - 1;
+      bits &= ~tied;
+    }
+    if (w < w1) stay[w] = bits;
+    const uint32_t low = w < w1 ? low_rows(w) : 0u;
+    holes += __popc(valid_rows(w) & low & ~bits);
     movers += __popc(bits & ~low);
   }
-  number(wholes, holes);
-  number(wmovers, movers);
+  holes = __reduce_add_sync(0xffffffffu, holes);
+  movers = __reduce_add_sync(0xffffffffu, movers);
+  if (lane == 0) {
+    counts[1][warp] = holes;
+    counts[2][warp] = movers;
+  }
+  __syncthreads();
+  if (warp < 2) scan(counts[1 + warp]);
   unit_sync<CS>();
   int n_moves;
-  int hole = ranks_before<CS>(&wholes[kMaxWarps], rank, &all) + wholes[warp];
-  int mover = ranks_before<CS>(&wmovers[kMaxWarps], rank, &n_moves) + wmovers[warp];
-  // as many rows leave below the budget as stay beyond it
-  int32_t* hole_list = FUSED ? reinterpret_cast<int32_t*>(stay + a.slice / 32) : a.moves + unit * 2 * a.cap;
-  int32_t* mover_list = hole_list + a.cap;
-  for (int w = w0; w < w1; ++w) {
-    const int r = r0 + w * 32 + lane;
-    const uint32_t bits = stay[w], low = __ballot_sync(0xffffffffu, r < kept);
-    const uint32_t valid = __ballot_sync(0xffffffffu, r < r0 + n), below = (1u << lane) - 1;
-    const uint32_t hb = valid & low & ~bits, mb = bits & ~low;
-    if ((hb >> lane) & 1) hole_list[hole + __popc(hb & below)] = r;
-    if ((mb >> lane) & 1) mover_list[mover + __popc(mb & below)] = r;
-    hole += __popc(hb);
-    mover += __popc(mb);
-    if (so != sc && ((bits & low) >> lane) & 1) {
-      so[r] = sc[r];
-      po[r] = ps[r];
-    }
+  const int holes_before = ranks_before<CS>(&counts[1][kMaxWarps], rank, &all);
+  const int movers_before = ranks_before<CS>(&counts[2][kMaxWarps], rank, &n_moves);
+  // As many rows leave below the budget as stay beyond it. The lists are made in shared memory
+  // (FUSED: where they stay; otherwise in the place of the ranks, this CTA's numbers only) and
+  // copied out in order: written from here, a lane's few numbers at a time, they took longer than
+  // all else but the loads.
+  const int cta_holes = static_cast<int>(counts[1][kMaxWarps]), cta_movers = static_cast<int>(counts[2][kMaxWarps]);
+  int32_t* hole_list = reinterpret_cast<int32_t*>(FUSED ? cand + a.slice / 4 : code);
+  int32_t* mover_list = hole_list + (FUSED ? a.cap : cta_holes);
+  int hole = static_cast<int>(counts[1][warp]), mover = static_cast<int>(counts[2][warp]);
+  for (int wb = w0; wb < w1; wb += 32) {
+    const int w = wb + lane;
+    const uint32_t bits = w < w1 ? stay[w] : 0u, low = w < w1 ? low_rows(w) : 0u;
+    uint32_t hb = valid_rows(w) & low & ~bits, mb = bits & ~low;
+    const int nh = __popc(hb), nm = __popc(mb);
+    int at = hole + before_lane(nh);
+    for (; hb; hb &= hb - 1) hole_list[at++] = r0 + w * 32 + __ffs(hb) - 1;
+    at = mover + before_lane(nm);
+    for (; mb; mb &= mb - 1) mover_list[at++] = r0 + w * 32 + __ffs(mb) - 1;
+    hole += __reduce_add_sync(0xffffffffu, nh);
+    mover += __reduce_add_sync(0xffffffffu, nm);
+  }
+  if (!FUSED) {
+    __syncthreads();
+    int32_t* out = a.moves + unit * 2 * a.cap;
+    for (int i = tid; i < cta_holes; i += threads) out[holes_before + i] = hole_list[i];
+    for (int i = tid; i < cta_movers; i += threads) out[a.cap + movers_before + i] = mover_list[i];
+  }
+  if (so != sc) {  // what stays below the budget
+    const int rows = min(n, kept - r0);
+#pragma unroll 4
+    for (int i = tid; i < rows; i += threads)
+      if ((stay[i >> 5] >> (i & 31)) & 1) {
+        so[r0 + i] = sc[r0 + i];
+        po[r0 + i] = ps[r0 + i];
+      }
   }
   if (CS > 1) unit_sync<CS>();  // no CTA leaves while others read its counts
   if (!FUSED) {
@@ -343,16 +493,17 @@ static bool evict_plan(int64_t units, int Lmax, int d, int budget, EvictPlan* pl
       pl->cs *= 2;
   pl->slice = ((Lmax + pl->cs - 1) / pl->cs + 127) & ~127;
   if (pl->slice > kMaxSlice) return false;
-  pl->threads = pl->slice <= 1024 ? 256 : pl->slice <= 4096 ? 512 : 1024;
-  pl->smem = static_cast<size_t>(pl->slice) * 4 + pl->slice / 8 + (pl->fused ? static_cast<size_t>(pl->cap) * 8 : 0);
+  pl->threads = pl->slice <= 1024 ? 128 : pl->slice <= 4096 ? 512 : 1024;
+  pl->smem = static_cast<size_t>(pl->slice) * 4 + pl->slice / 8 +
+             (pl->fused ? pl->slice + static_cast<size_t>(pl->cap) * 8 : 0);
   return true;
 }
 
 template <int CS, bool FUSED>
 static int launch_select(const EvictArgs& a, const EvictPlan& pl, int64_t units, cudaStream_t st) {
   auto kern = k_evict<CS, FUSED>;
-  if (pl.smem > 40 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024) != cudaSuccess) {
+  if (pl.smem > 32 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024) != cudaSuccess) {
     (void)cudaGetLastError();
     return MB_ERR_LAUNCH;
   }
