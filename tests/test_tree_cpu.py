@@ -128,3 +128,12 @@ def test_rope_and_evict_entries_check_their_arguments(L):
     assert evict(so=fake) == -2  # scores in place, positions not
     assert evict(Lmax=0) == -2
     assert evict(ws=None) == -3 and evict(nbytes=16) == -3
+
+
+def test_lookup_draft():
+    from moat_b200.speculative import lookup_draft
+    assert lookup_draft([5, 1, 2, 3, 4, 1, 2], 4) == [3, 4, 1]  # after the earlier "1 2"
+    assert lookup_draft([7, 8, 9, 8], 3) == [9, 8]  # after the earlier "8"
+    assert lookup_draft([1, 2, 3], 5) == [-1] * 4
+    assert lookup_draft([4, 4], 4) == [4, -1, -1]
+    assert lookup_draft([], 1) == []
