@@ -221,7 +221,11 @@ __device__ __forceinline__ int trace_len(const TreeAttnArgs& a, int t) { return 
 __device__ __forceinline__ int trace_tiles(int len) { return (len + kTile - 1) / kTile + 1; }
 
 // First position of CTA c of g when a sequence of w is cut evenly.
-__device__ __forceinline__ int cut(int64_t w, int c, int g) { return static_cast<int>(w * c / g); }
+// (floor(w c / g), without its 64-bit division: that took a CTA's set-up 0.2 us.)
+__device__ __forceinline__ int cut(uint32_t w, uint32_t c, uint32_t g) {
+  const uint32_t q = w / g;
+  return static_cast<int>(q * c + (w - q * g) * c / g);
+}
 
 struct Segment {  // a run of tiles of one unit
   int t, kvh, rb, len, nt, j0, n;
@@ -677,11 +681,14 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         };
         guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
-        form(true);
-        float top = x[0];
+        bool raise = jj == 0;  // a piece's first tile always sets m_ref
+        if (!raise) {
+          form(true);
+          float top = x[0];
 #pragma unroll
-        for (int u = 1; u < kKeysRows; ++u) top = fmaxf(top, x[u]);
-        const bool raise = vote_any(top > kSlack, kSoft);
+          for (int u = 1; u < kKeysRows; ++u) top = fmaxf(top, x[u]);
+          raise = vote_any(top > kSlack, kSoft);
+        }
         if (raise) {
           // P's space and O are free once the previous value product has finished
           if (k > 0) guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
@@ -1222,21 +1229,29 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   pdl_wait();
   pdl_launch_dependents();
   if (!mine) return;
-  float top = kNoRef;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c)
-    top = fmaxf(top, p.ml[static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * 2 * kMaxRows + n]);
-  float sum = 0.0f, o[4] = {};
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t slot = 2 * c + (c == c0 ? 1 : 0);
-    const float w = ex2(p.ml[slot * 2 * kMaxRows + n] - top);
-    const float4 x = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
-    sum = fmaf(w, p.ml[(slot * 2 + 1) * kMaxRows + n], sum);
-    o[0] = fmaf(w, x.x, o[0]);
-    o[1] = fmaf(w, x.y, o[1]);
-    o[2] = fmaf(w, x.z, o[2]);
-    o[3] = fmaf(w, x.w, o[3]);
+  float top = kNoRef, sum = 0.0f, o[4] = {};
+  for (int b = c0; b <= c1; b += 4) {  // four pieces' loads in flight, one round of latency for most units
+    float m[4], l[4];
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (b + i <= c1) {
+        const int64_t slot = 2 * (b + i) + (b + i == c0 ? 1 : 0);
+        m[i] = p.ml[slot * 2 * kMaxRows + n];
+        l[i] = p.ml[(slot * 2 + 1) * kMaxRows + n];
+        x[i] = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (b + i <= c1) {
+        const float now = fmaxf(top, m[i]), fade = ex2(top - now), w = ex2(m[i] - now);
+        top = now;
+        sum = fmaf(w, l[i], sum * fade);
+        o[0] = fmaf(w, x[i].x, o[0] * fade);
+        o[1] = fmaf(w, x[i].y, o[1] * fade);
+        o[2] = fmaf(w, x[i].z, o[2] * fade);
+        o[3] = fmaf(w, x[i].w, o[3] * fade);
+      }
   }
   const bool real = shown && sum != 0.0f;
   const float inv = real ? 1.0f / sum : 0.0f;
