@@ -369,7 +369,8 @@ int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
  * A trace's drafted tokens form a tree of m <= 64 nodes in topological order (node 0 the
  * last chosen token, whose keys are not cached yet). All element types are 16-bit: fp16,
  * or bf16 where is_bf16 = 1. `strides` are HOST arrays of element strides; the head dim is
- * contiguous. Device lengths are clamped to [0, Lmax].
+ * contiguous. Device lengths are clamped to [0, Lmax]. Arguments come as one struct (a call from
+ * Python with 30 arguments cost 5 us of host time to convert them).
  *
  * mb_tree_attn: exact softmax attention of every node over the lens[t] committed rows of
  * its trace and the nodes in its mask (bit j of masks[t][i]: node i sees node j; a mask of
@@ -383,14 +384,24 @@ int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
  * draft_scores [T, Hkv, m] the draft rows' sums. No atomics: results repeat bit for bit.
  * The workspace (with_scores = 1 if scores_out is given) needs no initial contents. dev_err (optional) receives MB_DEVERR_TIMEOUT if a
  * bounded wait inside a kernel gives up (the output is then undefined). */
+typedef struct {
+  const uint16_t *q, *k_cache, *v_cache;
+  const int32_t* lens;
+  const uint16_t *k_draft, *v_draft;
+  const int64_t* masks;
+  uint16_t* out;
+  const float* scores;
+  float *scores_out, *draft_scores;
+  void* workspace;
+  uint32_t* dev_err;
+  size_t workspace_bytes;
+  int64_t strides[18];
+  int32_t shared_masks, is_bf16, T, m, H, Hkv, Lmax, d;
+  float scale;
+} mb_tree_attn_args;
 size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d,
                                    int32_t with_scores);
-int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
-                     const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* masks, int32_t shared_masks,
-                     uint16_t* out, const int64_t* strides, int32_t is_bf16, int32_t T, int32_t m, int32_t H,
-                     int32_t Hkv, int32_t Lmax, int32_t d, float scale, const float* scores, float* scores_out,
-                     float* draft_scores, void* workspace, size_t workspace_bytes, uint32_t* dev_err,
-                     void* stream);
+int32_t mb_tree_attn(const mb_tree_attn_args* args, void* stream);
 
 /* mb_tree_accept: the accepted path of every trace (from the root, the lowest child whose
  * token equals target[parent]; parents [T, m], or [m] if shared_parents; a negative token
@@ -403,12 +414,18 @@ int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t*
  * path [T, m] (-1 after the last), counts, next_ids (target at the last accepted node),
  * lens_out and pos_out [T] (not the inputs' buffers). A trace without room keeps its state
  * (count 0) and sets MB_DEVERR_INDEX in the optional dev_err. */
-int32_t mb_tree_accept(const int32_t* tokens, const int32_t* parents, int32_t shared_parents, const int32_t* target,
-                       const int32_t* lens, const int32_t* next_pos, uint16_t* k_cache, uint16_t* v_cache,
-                       const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* strides, int32_t layers,
-                       int32_t T, int32_t m, int32_t Hkv, int32_t Lmax, int32_t d, float* scores,
-                       const float* draft_scores, int32_t* positions, int32_t* path, int32_t* counts,
-                       int32_t* next_ids, int32_t* lens_out, int32_t* pos_out, uint32_t* dev_err, void* stream);
+typedef struct {
+  const int32_t *tokens, *parents, *target, *lens, *next_pos;
+  uint16_t *k_cache, *v_cache;
+  const uint16_t *k_draft, *v_draft;
+  float* scores;
+  const float* draft_scores;
+  int32_t *positions, *path, *counts, *next_ids, *lens_out, *pos_out;
+  uint32_t* dev_err;
+  int64_t strides[16];
+  int32_t shared_parents, layers, T, m, Hkv, Lmax, d;
+} mb_tree_accept_args;
+int32_t mb_tree_accept(const mb_tree_accept_args* args, void* stream);
 
 /* mb_tree_rope: mb_rope_append's rotation for a tree, into draft buffers: qkv [T, m,
  * (H + 2 Hkv) * dh] (q | k | v), node i at position next_pos[t] + depths[t][i] (depths
@@ -428,11 +445,20 @@ int32_t mb_tree_rope(const uint16_t* qkv, int32_t is_bf16, int32_t T, int32_t m,
  * _out either the same buffers (both) or others, whose rows beyond the kept ones are not
  * written. lens_out [T] (not lens). The workspace needs no initial contents. */
 size_t mb_cache_evict_workspace_size(int32_t layers, int32_t T, int32_t Hkv, int32_t Lmax, int32_t budget);
-int32_t mb_cache_evict(uint16_t* k_cache, uint16_t* v_cache, const int64_t* strides, const float* scores,
-                       const int32_t* positions, float* scores_out, int32_t* positions_out, const int32_t* lens,
-                       const int32_t* next_pos, int32_t* lens_out, int32_t layers, int32_t T, int32_t Hkv,
-                       int32_t Lmax, int32_t d, int32_t budget, int32_t recent, int32_t sinks, void* workspace,
-                       size_t workspace_bytes, void* stream);
+typedef struct {
+  uint16_t *k_cache, *v_cache;
+  const float* scores;
+  const int32_t* positions;
+  float* scores_out;
+  int32_t* positions_out;
+  const int32_t *lens, *next_pos;
+  int32_t* lens_out;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t strides[8];
+  int32_t layers, T, Hkv, Lmax, d, budget, recent, sinks;
+} mb_cache_evict_args;
+int32_t mb_cache_evict(const mb_cache_evict_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -69,11 +69,11 @@ SIGNATURES = {
     "mb_decode_attn_noalloc": (_c_i32, [_vp, _vp, _vp, _vp, _c_i32, _c_i32, _c_i32, _c_i32, _c_f, _vp, _c_i32,
                                         _c_f, _vp]),
     "mb_tree_attn_workspace_size": (_c_sz, [_c_i32] * 7),
-    "mb_tree_attn": (_c_i32, [_vp] * 7 + [_c_i32, _vp, _vp] + [_c_i32] * 7 + [_c_f] + [_vp] * 4 + [_c_sz, _vp, _vp]),
-    "mb_tree_accept": (_c_i32, [_vp, _vp, _c_i32] + [_vp] * 8 + [_c_i32] * 6 + [_vp] * 10),
+    "mb_tree_attn": (_c_i32, [_vp, _vp]),
+    "mb_tree_accept": (_c_i32, [_vp, _vp]),
     "mb_tree_rope": (_c_i32, [_vp] + [_c_i32] * 6 + [_vp, _vp, _c_i32, _vp, _c_i32] + [_vp] * 4),
     "mb_cache_evict_workspace_size": (_c_sz, [_c_i32] * 5),
-    "mb_cache_evict": (_c_i32, [_vp] * 10 + [_c_i32] * 8 + [_vp, _c_sz, _vp]),
+    "mb_cache_evict": (_c_i32, [_vp, _vp]),
 }
 
 _lock = threading.Lock()

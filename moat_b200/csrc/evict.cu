@@ -543,43 +543,41 @@ size_t mb_cache_evict_workspace_size(int32_t layers, int32_t T, int32_t Hkv, int
   return static_cast<size_t>(layers) * T * Hkv * (2 * cap + 1) * 4 + 256;
 }
 
-int32_t mb_cache_evict(uint16_t* k_cache, uint16_t* v_cache, const int64_t* strides, const float* scores,
-                       const int32_t* positions, float* scores_out, int32_t* positions_out, const int32_t* lens,
-                       const int32_t* next_pos, int32_t* lens_out, int32_t layers, int32_t T, int32_t Hkv,
-                       int32_t Lmax, int32_t d, int32_t budget, int32_t recent, int32_t sinks, void* workspace,
-                       size_t workspace_bytes, void* stream) {
-  if (!k_cache || !v_cache || !strides || !scores || !positions || !scores_out || !positions_out || !lens ||
-      !next_pos || !lens_out)
+int32_t mb_cache_evict(const mb_cache_evict_args* g, void* stream) {
+  if (!g || !g->k_cache || !g->v_cache || !g->scores || !g->positions || !g->scores_out || !g->positions_out ||
+      !g->lens || !g->next_pos || !g->lens_out)
     return MB_ERR_NULL;
-  if (layers < 1 || T < 1 || Hkv < 1 || Lmax < 1 || d < 1 || budget < 1 || recent < 0 || sinks < 0) return MB_ERR_ARGS;
-  if (static_cast<int64_t>(recent) + sinks > budget) return MB_ERR_ARGS;
-  if (lens_out == lens) return MB_ERR_ARGS;  // every CTA reads the old lengths
-  if ((scores_out == scores) != (positions_out == positions)) return MB_ERR_ARGS;
+  const int layers = g->layers, T = g->T, Hkv = g->Hkv, Lmax = g->Lmax, d = g->d, budget = g->budget;
+  if (layers < 1 || T < 1 || Hkv < 1 || Lmax < 1 || d < 1 || budget < 1 || g->recent < 0 || g->sinks < 0)
+    return MB_ERR_ARGS;
+  if (static_cast<int64_t>(g->recent) + g->sinks > budget) return MB_ERR_ARGS;
+  if (g->lens_out == g->lens) return MB_ERR_ARGS;  // every CTA reads the old lengths
+  if ((g->scores_out == g->scores) != (g->positions_out == g->positions)) return MB_ERR_ARGS;
   const int64_t units = static_cast<int64_t>(layers) * T * Hkv;
   EvictPlan pl;
   if (units > 0x7FFFFFFll || !evict_plan(units, Lmax, d, budget, &pl)) return MB_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < mb_cache_evict_workspace_size(layers, T, Hkv, Lmax, budget))
+  if (!g->workspace || g->workspace_bytes < mb_cache_evict_workspace_size(layers, T, Hkv, Lmax, budget))
     return MB_ERR_WORKSPACE;
-  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
+  if (!aligned(g->workspace, 16)) return MB_ERR_ALIGN;
   EvictArgs a;
-  a.k = k_cache;
-  a.v = v_cache;
-  bool vec = d % 8 == 0 && d <= 1024 && aligned(k_cache, 16) && aligned(v_cache, 16);
+  a.k = g->k_cache;
+  a.v = g->v_cache;
+  bool vec = d % 8 == 0 && d <= 1024 && aligned(a.k, 16) && aligned(a.v, 16);
   for (int u = 0; u < 4; ++u) {
-    a.ks[u] = strides[u];
-    a.vs[u] = strides[4 + u];
+    a.ks[u] = g->strides[u];
+    a.vs[u] = g->strides[4 + u];
   }
-  for (int u = 0; u < 8; ++u) vec = vec && strides[u] % 8 == 0;
+  for (int u = 0; u < 8; ++u) vec = vec && g->strides[u] % 8 == 0;
   a.vec = vec;
-  a.vec_ranks = Lmax % 4 == 0 && aligned(scores, 16) && aligned(positions, 16);
-  a.scores = scores;
-  a.positions = positions;
-  a.scores_out = scores_out;
-  a.positions_out = positions_out;
-  a.lens = lens;
-  a.next_pos = next_pos;
-  a.lens_out = lens_out;
-  a.counts = static_cast<int32_t*>(workspace);
+  a.vec_ranks = Lmax % 4 == 0 && aligned(g->scores, 16) && aligned(g->positions, 16);
+  a.scores = g->scores;
+  a.positions = g->positions;
+  a.scores_out = g->scores_out;
+  a.positions_out = g->positions_out;
+  a.lens = g->lens;
+  a.next_pos = g->next_pos;
+  a.lens_out = g->lens_out;
+  a.counts = static_cast<int32_t*>(g->workspace);
   a.moves = a.counts + units;
   a.cap = pl.cap;
   a.slice = pl.slice;
@@ -589,8 +587,8 @@ int32_t mb_cache_evict(uint16_t* k_cache, uint16_t* v_cache, const int64_t* stri
   a.Lmax = Lmax;
   a.d = d;
   a.budget = budget;
-  a.recent = recent;
-  a.sinks = sinks;
+  a.recent = g->recent;
+  a.sinks = g->sinks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (pl.fused) return launch_select<1, true>(a, pl, units, st);
   const int rc = pl.cs == 1   ? launch_select<1, false>(a, pl, units, st)

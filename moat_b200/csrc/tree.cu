@@ -313,43 +313,41 @@ size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv,
                   tree_mma_workspace(T, m, H, Hkv, Lmax, d, with_scores != 0));
 }
 
-int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* lens,
-                     const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* masks, int32_t shared_masks,
-                     uint16_t* out, const int64_t* strides, int32_t is_bf16, int32_t T, int32_t m, int32_t H,
-                     int32_t Hkv, int32_t Lmax, int32_t d, float scale, const float* scores, float* scores_out,
-                     float* draft_scores, void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
-  if (!q || !lens || !k_draft || !v_draft || !masks || !out || !strides) return MB_ERR_NULL;
-  if (Lmax > 0 && (!k_cache || !v_cache)) return MB_ERR_NULL;
-  if ((scores_out != nullptr) != (draft_scores != nullptr) || (scores && !scores_out)) return MB_ERR_NULL;
+int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
+  if (!g || !g->q || !g->lens || !g->k_draft || !g->v_draft || !g->masks || !g->out) return MB_ERR_NULL;
+  const int T = g->T, m = g->m, H = g->H, Hkv = g->Hkv, Lmax = g->Lmax, d = g->d;
+  if (Lmax > 0 && (!g->k_cache || !g->v_cache)) return MB_ERR_NULL;
+  if ((g->scores_out != nullptr) != (g->draft_scores != nullptr) || (g->scores && !g->scores_out)) return MB_ERR_NULL;
   if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim)
     return MB_ERR_ARGS;
   if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFFFF00)
     return MB_ERR_UNSUPPORTED;
-  if (!(scale - scale == 0.0f) || is_bf16 < 0 || is_bf16 > 1) return MB_ERR_ARGS;
-  if (!aligned(q, 2) || !aligned(k_cache, 2) || !aligned(v_cache, 2) || !aligned(k_draft, 2) ||
-      !aligned(v_draft, 2) || !aligned(out, 2) || !aligned(lens, 4) || !aligned(masks, 8) || !aligned(scores, 4) ||
-      !aligned(scores_out, 4) || !aligned(draft_scores, 4))
+  if (!(g->scale - g->scale == 0.0f) || g->is_bf16 < 0 || g->is_bf16 > 1) return MB_ERR_ARGS;
+  if (!aligned(g->q, 2) || !aligned(g->k_cache, 2) || !aligned(g->v_cache, 2) || !aligned(g->k_draft, 2) ||
+      !aligned(g->v_draft, 2) || !aligned(g->out, 2) || !aligned(g->lens, 4) || !aligned(g->masks, 8) ||
+      !aligned(g->scores, 4) || !aligned(g->scores_out, 4) || !aligned(g->draft_scores, 4))
     return MB_ERR_ALIGN;
-  if (!workspace || workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, scores_out != nullptr))
+  if (!g->workspace ||
+      g->workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, g->scores_out != nullptr))
     return MB_ERR_WORKSPACE;
-  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
+  if (!aligned(g->workspace, 16)) return MB_ERR_ALIGN;
   TreeAttnArgs a;
-  a.q = q;
-  a.k = k_cache;
-  a.v = v_cache;
-  a.kd = k_draft;
-  a.vd = v_draft;
-  a.out = out;
-  a.lens = lens;
-  a.masks = reinterpret_cast<const uint64_t*>(masks);
-  a.mask_stride = shared_masks ? 0 : m;
+  a.q = g->q;
+  a.k = g->k_cache;
+  a.v = g->v_cache;
+  a.kd = g->k_draft;
+  a.vd = g->v_draft;
+  a.out = g->out;
+  a.lens = g->lens;
+  a.masks = reinterpret_cast<const uint64_t*>(g->masks);
+  a.mask_stride = g->shared_masks ? 0 : m;
   for (int u = 0; u < 3; ++u) {
-    a.qs[u] = strides[u];
-    a.ks[u] = strides[3 + u];
-    a.vs[u] = strides[6 + u];
-    a.kds[u] = strides[9 + u];
-    a.vds[u] = strides[12 + u];
-    a.os[u] = strides[15 + u];
+    a.qs[u] = g->strides[u];
+    a.ks[u] = g->strides[3 + u];
+    a.vs[u] = g->strides[6 + u];
+    a.kds[u] = g->strides[9 + u];
+    a.vds[u] = g->strides[12 + u];
+    a.os[u] = g->strides[15 + u];
   }
   a.T = T;
   a.m = m;
@@ -357,70 +355,67 @@ int32_t mb_tree_attn(const uint16_t* q, const uint16_t* k_cache, const uint16_t*
   a.Hkv = Hkv;
   a.Lmax = Lmax;
   a.d = d;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.scores = scores;
-  a.scores_out = scores_out;
-  a.draft_scores = draft_scores;
-  a.err = dev_err;
+  a.scale_log2 = g->scale * 1.4426950408889634f;
+  a.scores = g->scores;
+  a.scores_out = g->scores_out;
+  a.draft_scores = g->draft_scores;
+  a.err = g->dev_err;
+  const bool bf16 = g->is_bf16 != 0;
   if (tree_mma_workspace(T, m, H, Hkv, Lmax, d, false) && tree_mma_takes(a))
-    return tree_mma_launch(a, is_bf16 != 0, workspace, stream);
+    return tree_mma_launch(a, bf16, g->workspace, stream);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* lse = scores_out ? static_cast<float*>(workspace) : nullptr;
-  int rc = launch_with_pdl(is_bf16 ? k_tree_attn_any<true> : k_tree_attn_any<false>, dim3(T * m * H), dim3(kAnyBlock),
-                           0, st, a, lse);
-  if (rc != MB_OK || !scores_out) return rc;
-  return launch_with_pdl(is_bf16 ? k_tree_weights_any<true> : k_tree_weights_any<false>,
+  float* lse = a.scores_out ? static_cast<float*>(g->workspace) : nullptr;
+  const int rc = launch_with_pdl(bf16 ? k_tree_attn_any<true> : k_tree_attn_any<false>, dim3(T * m * H),
+                                 dim3(kAnyBlock), 0, st, a, lse);
+  if (rc != MB_OK || !a.scores_out) return rc;
+  return launch_with_pdl(bf16 ? k_tree_weights_any<true> : k_tree_weights_any<false>,
                          dim3((Lmax + m + kAnyBlock - 1) / kAnyBlock, T * Hkv), dim3(kAnyBlock), 0, st, a,
                          static_cast<const float*>(lse));
 }
 
-int32_t mb_tree_accept(const int32_t* tokens, const int32_t* parents, int32_t shared_parents, const int32_t* target,
-                       const int32_t* lens, const int32_t* next_pos, uint16_t* k_cache, uint16_t* v_cache,
-                       const uint16_t* k_draft, const uint16_t* v_draft, const int64_t* strides, int32_t layers,
-                       int32_t T, int32_t m, int32_t Hkv, int32_t Lmax, int32_t d, float* scores,
-                       const float* draft_scores, int32_t* positions, int32_t* path, int32_t* counts,
-                       int32_t* next_ids, int32_t* lens_out, int32_t* pos_out, uint32_t* dev_err, void* stream) {
-  if (!tokens || !parents || !target || !lens || !next_pos || !k_cache || !v_cache || !k_draft || !v_draft ||
-      !strides || !path || !counts || !next_ids || !lens_out || !pos_out)
+int32_t mb_tree_accept(const mb_tree_accept_args* g, void* stream) {
+  if (!g || !g->tokens || !g->parents || !g->target || !g->lens || !g->next_pos || !g->k_cache || !g->v_cache ||
+      !g->k_draft || !g->v_draft || !g->path || !g->counts || !g->next_ids || !g->lens_out || !g->pos_out)
     return MB_ERR_NULL;
-  if ((scores != nullptr) != (draft_scores != nullptr)) return MB_ERR_NULL;
-  if (layers < 1 || T < 1 || m < 1 || m > 64 || Hkv < 1 || Lmax < 1 || d < 1) return MB_ERR_ARGS;
-  if (lens_out == lens || pos_out == next_pos) return MB_ERR_ARGS;  // every CTA reads the old lengths
+  if ((g->scores != nullptr) != (g->draft_scores != nullptr)) return MB_ERR_NULL;
+  const int layers = g->layers, T = g->T, m = g->m, Hkv = g->Hkv, d = g->d;
+  if (layers < 1 || T < 1 || m < 1 || m > 64 || Hkv < 1 || g->Lmax < 1 || d < 1) return MB_ERR_ARGS;
+  if (g->lens_out == g->lens || g->pos_out == g->next_pos) return MB_ERR_ARGS;  // every CTA reads the old lengths
   if (static_cast<int64_t>(T) * layers > 0x7FFFFFFFll || layers > 65535 || Hkv > 65535) return MB_ERR_UNSUPPORTED;
   AcceptArgs a;
-  a.tokens = tokens;
-  a.parents = parents;
-  a.parent_stride = shared_parents ? 0 : m;
-  a.target = target;
-  a.lens = lens;
-  a.next_pos = next_pos;
-  a.k = k_cache;
-  a.v = v_cache;
-  a.kd = k_draft;
-  a.vd = v_draft;
-  bool vec = d % 8 == 0 && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_draft, 16) && aligned(v_draft, 16);
+  a.tokens = g->tokens;
+  a.parents = g->parents;
+  a.parent_stride = g->shared_parents ? 0 : m;
+  a.target = g->target;
+  a.lens = g->lens;
+  a.next_pos = g->next_pos;
+  a.k = g->k_cache;
+  a.v = g->v_cache;
+  a.kd = g->k_draft;
+  a.vd = g->v_draft;
+  bool vec = d % 8 == 0 && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.kd, 16) && aligned(a.vd, 16);
   for (int u = 0; u < 4; ++u) {
-    a.ks[u] = strides[u];
-    a.vs[u] = strides[4 + u];
-    a.kds[u] = strides[8 + u];
-    a.vds[u] = strides[12 + u];
+    a.ks[u] = g->strides[u];
+    a.vs[u] = g->strides[4 + u];
+    a.kds[u] = g->strides[8 + u];
+    a.vds[u] = g->strides[12 + u];
   }
-  for (int u = 0; u < 16; ++u) vec = vec && strides[u] % 8 == 0;
+  for (int u = 0; u < 16; ++u) vec = vec && g->strides[u] % 8 == 0;
   a.vec = vec;
-  a.scores = scores;
-  a.draft_scores = draft_scores;
-  a.positions = positions;
-  a.path = path;
-  a.counts = counts;
-  a.next_ids = next_ids;
-  a.lens_out = lens_out;
-  a.pos_out = pos_out;
-  a.err = dev_err;
+  a.scores = g->scores;
+  a.draft_scores = g->draft_scores;
+  a.positions = g->positions;
+  a.path = g->path;
+  a.counts = g->counts;
+  a.next_ids = g->next_ids;
+  a.lens_out = g->lens_out;
+  a.pos_out = g->pos_out;
+  a.err = g->dev_err;
   a.layers = layers;
   a.T = T;
   a.m = m;
   a.Hkv = Hkv;
-  a.Lmax = Lmax;
+  a.Lmax = g->Lmax;
   a.d = d;
   // about two CTAs per SM
   const int groups = std::max(1, std::min<int>(Hkv, 2 * sm_count() / std::max(1, T * layers)));

@@ -17,8 +17,8 @@ it also keeps the accumulated attention weight of every cached row, which
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import NamedTuple
 
 import numpy as np
@@ -59,6 +59,11 @@ def tree_depths(parents) -> np.ndarray:
     return out.reshape(par.shape)
 
 
+# ---------------------------------------------------------------------------
+# Arguments. Each entry point makes one pass of cheap tests over its tensors; only when
+# one of them fails does a second, slower pass find out which and say so. (Checks that
+# named every tensor took 10 us of host time per call, more than many of the kernels.)
+# ---------------------------------------------------------------------------
 def _device_index(x, name: str) -> int:
     """Index of the CUDA device a tensor lies on."""
     try:
@@ -70,9 +75,9 @@ def _device_index(x, name: str) -> int:
     return idx
 
 
-def _on_device(idx: int, names, tensors) -> None:
-    for name, x in zip(names, tensors):
-        if _device_index(x, name) != idx:
+def _on_device(idx: int, **tensors) -> None:
+    for name, x in tensors.items():
+        if x is not None and _device_index(x, name) != idx:
             raise ValueError(f"{name} must be on cuda:{idx}")
 
 
@@ -82,15 +87,11 @@ def _plain(x, shape, dtype, name) -> None:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)}")
 
 
-def _strides(tensors, axes: int, dtype, what: str):
-    """The leading strides of tensors of one dtype that are contiguous along their last axis."""
-    out = ()
+def _rows(dtype, what: str, *tensors) -> None:
+    """Tensors of one dtype, contiguous along their last axis."""
     for x in tensors:
-        st = x.stride()
-        if x.dtype is not dtype or (st[axes] != 1 and x.shape[axes] > 1):
+        if x.dtype is not dtype or (x.stride(-1) != 1 and x.shape[-1] > 1):
             raise ValueError(what)
-        out += st[:axes]
-    return out
 
 
 class _Workspaces:
@@ -101,30 +102,77 @@ class _Workspaces:
     def __init__(self):
         self._bufs, self._outgrown = {}, []
 
-    def get(self, t, idx: int, stream: int, nbytes: int):
-        buf = self._bufs.get((idx, stream))
-        if buf is None or buf.numel() < nbytes:
-            if buf is not None:
-                self._outgrown.append(buf)
-                nbytes = max(nbytes, 2 * buf.numel())
+    def get(self, idx: int, stream: int, nbytes: int):
+        """(address, bytes)"""
+        have = self._bufs.get((idx, stream))
+        if have is None or have[1] < nbytes:
+            t = _lib.torch()
+            if have is not None:
+                self._outgrown.append(have)
+                nbytes = max(nbytes, 2 * have[1])
             buf = t.empty(max(nbytes, 1 << 20), dtype=t.uint8, device=t.device("cuda", idx))
-            self._bufs[(idx, stream)] = buf
-        return buf
+            have = self._bufs[(idx, stream)] = (buf.data_ptr(), buf.numel(), buf)
+        return have
 
 
-def _on(t, idx: int, call):
+def _on(idx: int, call):
     """``call(stream)`` with device ``idx`` current."""
-    if idx == t.cuda.current_device():
+    t = _torch()
+    if idx == t._C._cuda_getDevice():
         return call(stream_of(idx))
     with t.cuda.device(idx):
         return call(stream_of(idx))
 
 
-_Strides18 = ctypes.c_int64 * 18
-_Strides16 = ctypes.c_int64 * 16
+_modules = []
+
+
+def _torch():
+    if not _modules:
+        _modules.append(_lib.torch())
+    return _modules[0]
+
+
 _ws = _Workspaces()
 _sizes = {}  # workspace bytes by geometry
-_ATTN_NAMES = ("q", "k_cache", "v_cache", "lens", "k_draft", "v_draft", "masks")
+# the C structs mb_tree_attn_args and mb_tree_accept_args
+_AttnArgs = struct.Struct("@13PN18q8if")
+_AcceptArgs = struct.Struct("@18P16q7i")
+
+
+def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, scores, scores_out, draft_scores, dev_err):
+    t = _torch()
+    idx = _device_index(q, "q")
+    _on_device(idx, k_cache=k_cache, v_cache=v_cache, lens=lens, k_draft=k_draft, v_draft=v_draft, masks=masks, out=out,
+               scores=scores, scores_out=scores_out, draft_scores=draft_scores, dev_err=dev_err)
+    if q.dim() != 4 or k_cache.dim() != 4:
+        raise ValueError("q must be [T, m, H, d] and the caches [T, Hkv, Lmax, d]")
+    T, m, H, d = q.shape
+    Hkv, Lmax = k_cache.shape[1:3]
+    if not 1 <= m <= MAX_NODES:
+        raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {m}")
+    if T < 1 or Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads do not divide among {Hkv} KV heads")
+    if not 1 <= d <= 256:
+        raise ValueError(f"head dim must be 1 to 256, got {d}")
+    if k_cache.shape != (T, Hkv, Lmax, d) or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache / v_cache must be [{T}, {Hkv}, Lmax, {d}]")
+    if k_draft.shape != (T, m, Hkv, d) or v_draft.shape != k_draft.shape:
+        raise ValueError(f"k_draft / v_draft must be [{T}, {m}, {Hkv}, {d}]")
+    if q.dtype not in (t.float16, t.bfloat16):
+        raise ValueError("q must be fp16 or bf16")
+    _plain(lens, (T,), t.int32, "lens")
+    _plain(masks, (m,) if masks.dim() == 1 else (T, m), t.int64, "masks")
+    if out.shape != q.shape:
+        raise ValueError(f"out must be [{T}, {m}, {H}, {d}]")
+    _rows(q.dtype, "q, out, caches and drafts must share one dtype and be contiguous along the head dim", q, k_cache,
+          v_cache, k_draft, v_draft, out)
+    if scores is not None:
+        _plain(scores, (T, Hkv, Lmax), t.float32, "scores")
+        _plain(scores_out, (T, Hkv, Lmax), t.float32, "scores_out")
+        _plain(draft_scores, (T, Hkv, m), t.float32, "draft_scores")
+    elif scores_out is not None or draft_scores is not None:
+        raise ValueError("scores_out and draft_scores need scores")
 
 
 def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=None, out=None, scores=None,
@@ -153,72 +201,67 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     probability to the inputs' type before its product with V). Repeated calls give the same
     bits. Returns ``out``, or ``(out, scores_out, draft_scores)`` with ``scores``.
     """
-    t = _lib.torch()
-    idx = _device_index(q, "q")
-    _on_device(idx, _ATTN_NAMES, (q, k_cache, v_cache, lens, k_draft, v_draft, masks))
-    if q.dim() != 4 or k_cache.dim() != 4:
-        raise ValueError("q must be [T, m, H, d] and the caches [T, Hkv, Lmax, d]")
-    T, m, H, d = q.shape
-    cache = k_cache.shape
-    Hkv, Lmax = cache[1], cache[2]
-    if not 1 <= m <= MAX_NODES:
-        raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {m}")
-    if T < 1 or Hkv < 1 or H < 1 or H % Hkv:
-        raise ValueError(f"{H} query heads do not divide among {Hkv} KV heads")
-    if not 1 <= d <= 256:
-        raise ValueError(f"head dim must be 1 to 256, got {d}")
-    if cache != (T, Hkv, Lmax, d) or v_cache.shape != cache:
-        raise ValueError(f"k_cache / v_cache must be [{T}, {Hkv}, Lmax, {d}]")
-    drafts = (T, m, Hkv, d)
-    if k_draft.shape != drafts or v_draft.shape != drafts:
-        raise ValueError(f"k_draft / v_draft must be {list(drafts)}")
-    dt = q.dtype
-    if dt is not t.float16 and dt is not t.bfloat16:
-        raise ValueError("q must be fp16 or bf16")
-    _plain(lens, (T,), t.int32, "lens")
-    shared = masks.dim() == 1
-    _plain(masks, (m,) if shared else (T, m), t.int64, "masks")
-    if out is None:
-        out = t.empty((T, m, H, d), dtype=dt, device=q.device)
-    elif _device_index(out, "out") != idx or out.shape != q.shape:
-        raise ValueError(f"out must be [{T}, {m}, {H}, {d}] on cuda:{idx}")
-    strides = _strides((q, k_cache, v_cache, k_draft, v_draft, out), 3, dt,
-                       "q, out, caches and drafts must share one dtype and be contiguous along the head dim")
+    t = _torch()
+    try:
+        idx = q.get_device()
+        T, m, H, d = rows = q.shape
+        cache, drafts, dt = k_cache.shape, k_draft.shape, q.dtype
+        Hkv, Lmax = cache[1], cache[2]
+        if out is None:
+            out = t.empty_like(q, memory_format=t.contiguous_format)
+        if scores is not None:
+            scores_out = scores if scores_out is None else scores_out
+            if draft_scores is None:
+                draft_scores = t.empty((T, Hkv, m), dtype=t.float32, device=q.device)
+        sq, sk, sv = q.stride(), k_cache.stride(), v_cache.stride()
+        skd, svd, so = k_draft.stride(), v_draft.stride(), out.stride()
+        fine = (idx >= 0 and idx == k_cache.get_device() == v_cache.get_device() == lens.get_device()
+                == k_draft.get_device() == v_draft.get_device() == masks.get_device() == out.get_device()
+                and 1 <= m <= MAX_NODES and T >= 1 and Hkv >= 1 and H >= 1 and H % Hkv == 0 and 1 <= d <= 256
+                and len(cache) == 4 and cache[0] == T and cache[3] == d and v_cache.shape == cache
+                and drafts == (T, m, Hkv, d) and v_draft.shape == drafts and out.shape == rows
+                and (dt is t.float16 or dt is t.bfloat16)
+                and dt is k_cache.dtype is v_cache.dtype is k_draft.dtype is v_draft.dtype is out.dtype
+                and (sq[3] == sk[3] == sv[3] == skd[3] == svd[3] == so[3] == 1 or d == 1)
+                and lens.dtype is t.int32 and lens.shape == (T,) and lens.is_contiguous()
+                and masks.dtype is t.int64 and (masks.shape == (T, m) or masks.shape == (m,))
+                and masks.is_contiguous()
+                and (dev_err is None or dev_err.get_device() == idx))
+        if fine and scores is not None:
+            f32, rows = t.float32, (T, Hkv, Lmax)
+            fine = (idx == scores.get_device() == scores_out.get_device() == draft_scores.get_device()
+                    and f32 is scores.dtype is scores_out.dtype is draft_scores.dtype
+                    and scores.shape == rows and scores_out.shape == rows and draft_scores.shape == (T, Hkv, m)
+                    and scores.is_contiguous() and scores_out.is_contiguous() and draft_scores.is_contiguous())
+        elif fine:
+            fine = scores_out is None and draft_scores is None
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, q if out is None else out, scores,
+                         scores_out, draft_scores, dev_err)
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not math.isfinite(sc):
         raise ValueError("scale must be finite")
-    ps = pso = pds = None
-    if scores is not None:
-        scores_out = scores if scores_out is None else scores_out
-        if draft_scores is None:
-            draft_scores = t.empty((T, Hkv, m), dtype=t.float32, device=q.device)
-        _on_device(idx, ("scores", "scores_out", "draft_scores"), (scores, scores_out, draft_scores))
-        f32, rows = t.float32, (T, Hkv, Lmax)
-        _plain(scores, rows, f32, "scores")
-        _plain(scores_out, rows, f32, "scores_out")
-        _plain(draft_scores, (T, Hkv, m), f32, "draft_scores")
-        ps, pso, pds = scores.data_ptr(), scores_out.data_ptr(), draft_scores.data_ptr()
-    elif scores_out is not None or draft_scores is not None:
-        raise ValueError("scores_out and draft_scores need scores")
-    if dev_err is not None:
-        _on_device(idx, ("dev_err",), (dev_err,))
     L = lib()
-    geometry = (T, m, H, Hkv, Lmax, d, ps is not None)
+    geometry = (T, m, H, Hkv, Lmax, d, scores is not None)
     nbytes = _sizes.get(geometry)
     if nbytes is None:
         nbytes = _sizes[geometry] = int(L.mb_tree_attn_workspace_size(*geometry))
 
     def call(st):
-        ws = _ws.get(t, idx, st, nbytes)
-        return L.mb_tree_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(),
-                              k_draft.data_ptr(), v_draft.data_ptr(), masks.data_ptr(), shared, out.data_ptr(),
-                              _Strides18(*strides), dt is t.bfloat16, T, m, H, Hkv, Lmax, d, sc, ps, pso, pds,
-                              ws.data_ptr(), ws.numel(), None if dev_err is None else dev_err.data_ptr(), st)
+        ws = _ws.get(idx, st, nbytes)
+        return L.mb_tree_attn(_AttnArgs.pack(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(), k_draft.data_ptr(),
+            v_draft.data_ptr(), masks.data_ptr(), out.data_ptr(), 0 if scores is None else scores.data_ptr(),
+            0 if scores is None else scores_out.data_ptr(), 0 if scores is None else draft_scores.data_ptr(), ws[0],
+            0 if dev_err is None else dev_err.data_ptr(), ws[1], *sq[:3], *sk[:3], *sv[:3], *skd[:3], *svd[:3],
+            *so[:3], masks.dim() == 1, dt is t.bfloat16, T, m, H, Hkv, Lmax, d, sc), st)
 
-    rc = _on(t, idx, call)
+    rc = _on(idx, call)
     if rc != 0:
         check(rc, "mb_tree_attn")
-    return out if ps is None else (out, scores_out, draft_scores)
+    return out if scores is None else (out, scores_out, draft_scores)
 
 
 class Accepted(NamedTuple):
@@ -240,7 +283,41 @@ def _five(x, name):
     return x
 
 
-_ACCEPT_NAMES = ("tokens", "parents", "target", "lens", "next_pos", "v_cache", "k_draft", "v_draft")
+def _check_accept(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, scores, draft_scores,
+                  positions, dev_err):
+    t = _torch()
+    idx = _device_index(k_cache, "k_cache")
+    _on_device(idx, tokens=tokens, parents=parents, target=target, lens=lens, next_pos=next_pos, v_cache=v_cache,
+               k_draft=k_draft, v_draft=v_draft, scores=scores, draft_scores=draft_scores, positions=positions,
+               dev_err=dev_err)
+    kc, vc, kd, vd = (_five(x, n) for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (k_draft, "k_draft"),
+                                               (v_draft, "v_draft")))
+    layers, T, Hkv, Lmax, d = kc.shape
+    m = kd.shape[2]
+    if not 1 <= m <= MAX_NODES:
+        raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {m}")
+    if min(layers, T, Hkv, Lmax, d) < 1:
+        raise ValueError("the caches must not be empty")
+    if vc.shape != kc.shape:
+        raise ValueError("k_cache and v_cache must have one shape")
+    if kd.shape != (layers, T, m, Hkv, d) or vd.shape != kd.shape:
+        raise ValueError(f"drafts must be [{layers}, {T}, m, {Hkv}, {d}]")
+    what = "caches and drafts must share one 16-bit dtype and be contiguous along the head dim"
+    if kc.element_size() != 2:
+        raise ValueError(what)
+    _rows(kc.dtype, what, kc, vc, kd, vd)
+    i32 = t.int32
+    for x, shape, name in ((tokens, (T, m), "tokens"), (target, (T, m), "target"), (lens, (T,), "lens"),
+                           (next_pos, (T,), "next_pos"), (parents, (m,) if parents.dim() == 1 else (T, m), "parents")):
+        _plain(x, shape, i32, name)
+    if (scores is None) != (draft_scores is None):
+        raise ValueError("scores and draft_scores go together")
+    lead = k_cache.shape[:-2]
+    if scores is not None:
+        _plain(scores, (*lead, Lmax), t.float32, "scores")
+        _plain(draft_scores, (*lead, m), t.float32, "draft_scores")
+    if positions is not None:
+        _plain(positions, (*lead, Lmax), i32, "positions")
 
 
 def accept_tree(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, *, scores=None,
@@ -260,59 +337,56 @@ def accept_tree(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_dra
     ``next_pos[t] + j``. A trace without room for its accepted rows keeps its state (count
     0) and sets bit 2 of ``dev_err`` (int32 CUDA tensor, optional). 16-bit element types.
     """
-    t = _lib.torch()
-    idx = _device_index(k_cache, "k_cache")
-    _on_device(idx, _ACCEPT_NAMES, (tokens, parents, target, lens, next_pos, v_cache, k_draft, v_draft))
-    kc, vc, kd, vd = (_five(x, n) for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (k_draft, "k_draft"),
-                                               (v_draft, "v_draft")))
-    layers, T, Hkv, Lmax, d = kc.shape
-    drafts = kd.shape
-    m = drafts[2]
-    if not 1 <= m <= MAX_NODES:
-        raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {m}")
-    if min(layers, T, Hkv, Lmax, d) < 1:
-        raise ValueError("the caches must not be empty")
-    if vc.shape != kc.shape:
-        raise ValueError("k_cache and v_cache must have one shape")
-    if drafts != (layers, T, m, Hkv, d) or vd.shape != drafts:
-        raise ValueError(f"drafts must be [{layers}, {T}, m, {Hkv}, {d}]")
-    what = "caches and drafts must share one 16-bit dtype and be contiguous along the head dim"
-    if kc.element_size() != 2:
-        raise ValueError(what)
-    strides = _strides((kc, vc, kd, vd), 4, kc.dtype, what)
-    i32 = t.int32
-    _plain(tokens, (T, m), i32, "tokens")
-    _plain(target, (T, m), i32, "target")
-    _plain(lens, (T,), i32, "lens")
-    _plain(next_pos, (T,), i32, "next_pos")
-    shared = parents.dim() == 1
-    _plain(parents, (m,) if shared else (T, m), i32, "parents")
-    if (scores is None) != (draft_scores is None):
-        raise ValueError("scores and draft_scores go together")
-    lead = (layers, T, Hkv) if k_cache.dim() == 5 else (T, Hkv)
-    ps = pd = pp = None
-    if scores is not None:
-        _on_device(idx, ("scores", "draft_scores"), (scores, draft_scores))
-        _plain(scores, lead + (Lmax,), t.float32, "scores")
-        _plain(draft_scores, lead + (m,), t.float32, "draft_scores")
-        ps, pd = scores.data_ptr(), draft_scores.data_ptr()
-    if positions is not None:
-        _on_device(idx, ("positions",), (positions,))
-        _plain(positions, lead + (Lmax,), i32, "positions")
-        pp = positions.data_ptr()
-    if dev_err is not None:
-        _on_device(idx, ("dev_err",), (dev_err,))
-    ints = t.empty((m + 4) * T, dtype=i32, device=kc.device)  # one allocation for the five results
-    path, counts, next_ids, new_lens, new_pos = ints.split_with_sizes([T * m, T, T, T, T])
-    p0 = ints.data_ptr()
-    p1, step = p0 + 4 * T * m, 4 * T
-    rc = _on(t, idx, lambda st: lib().mb_tree_accept(
-        tokens.data_ptr(), parents.data_ptr(), shared, target.data_ptr(), lens.data_ptr(), next_pos.data_ptr(),
-        kc.data_ptr(), vc.data_ptr(), kd.data_ptr(), vd.data_ptr(), _Strides16(*strides), layers, T, m, Hkv, Lmax, d,
-        ps, pd, pp, p0, p1, p1 + step, p1 + 2 * step, p1 + 3 * step, None if dev_err is None else dev_err.data_ptr(),
-        st))
+    t = _torch()
+    try:
+        idx = k_cache.get_device()
+        full, drafts, dt, i32 = tuple(k_cache.shape), tuple(k_draft.shape), k_cache.dtype, t.int32
+        layers = full[0] if len(full) == 5 else 1
+        T, Hkv, Lmax, d = full[-4:]
+        m = drafts[-3]
+        pair, one = (T, m), (T,)
+        sk, sv, skd, svd = k_cache.stride(), v_cache.stride(), k_draft.stride(), v_draft.stride()
+        fine = (idx >= 0 and idx == v_cache.get_device() == k_draft.get_device() == v_draft.get_device()
+                == tokens.get_device() == parents.get_device() == target.get_device() == lens.get_device()
+                == next_pos.get_device()
+                and 1 <= m <= MAX_NODES and 4 <= len(full) <= 5 and min(full) >= 1 and v_cache.shape == full
+                and drafts == (*full[:-3], m, Hkv, d) and v_draft.shape == drafts
+                and dt is v_cache.dtype is k_draft.dtype is v_draft.dtype and dt.itemsize == 2
+                and (sk[-1] == sv[-1] == skd[-1] == svd[-1] == 1 or d == 1)
+                and i32 is tokens.dtype is parents.dtype is target.dtype is lens.dtype is next_pos.dtype
+                and tokens.shape == pair and target.shape == pair and lens.shape == one and next_pos.shape == one
+                and (parents.shape == pair or parents.shape == (m,))
+                and tokens.is_contiguous() and parents.is_contiguous() and target.is_contiguous()
+                and lens.is_contiguous() and next_pos.is_contiguous()
+                and (scores is None) == (draft_scores is None)
+                and (dev_err is None or dev_err.get_device() == idx))
+        if fine and scores is not None:
+            fine = (idx == scores.get_device() == draft_scores.get_device()
+                    and scores.dtype is draft_scores.dtype is t.float32 and scores.shape == full[:-1]
+                    and draft_scores.shape == (*full[:-2], m) and scores.is_contiguous()
+                    and draft_scores.is_contiguous())
+        if fine and positions is not None:
+            fine = (positions.get_device() == idx and positions.dtype is i32 and positions.shape == full[:-1]
+                    and positions.is_contiguous())
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _check_accept(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, scores, draft_scores,
+                      positions, dev_err)
+    # strides by (layer, trace, head or node, row or head); without a layer axis its stride is not used
+    lead = () if len(full) == 5 else (0,)
+    ints = t.empty(T * (m + 4), dtype=i32, device=k_cache.device)  # one allocation for the five results
+    p0, step = ints.data_ptr(), 4 * T
+    rc = _on(idx, lambda st: lib().mb_tree_accept(_AcceptArgs.pack(
+        tokens.data_ptr(), parents.data_ptr(), target.data_ptr(), lens.data_ptr(), next_pos.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr(),
+        0 if scores is None else scores.data_ptr(), 0 if scores is None else draft_scores.data_ptr(),
+        0 if positions is None else positions.data_ptr(), p0 + 4 * step, p0, p0 + step, p0 + 2 * step, p0 + 3 * step,
+        0 if dev_err is None else dev_err.data_ptr(), *lead, *sk[:-1], *lead, *sv[:-1], *lead, *skd[:-1], *lead,
+        *svd[:-1], parents.dim() == 1, layers, T, m, Hkv, Lmax, d), st))
     if rc != 0:
         check(rc, "mb_tree_accept")
+    counts, next_ids, new_lens, new_pos, path = ints.split_with_sizes([T, T, T, T, T * m])
     return Accepted(path.view(T, m), counts, next_ids, new_lens, new_pos)
 
 

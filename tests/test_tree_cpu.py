@@ -68,66 +68,89 @@ def test_workspace_sizes(L):
     assert L.mb_cache_evict_workspace_size(1, 1, 4, 320, 0) == 0
 
 
-def test_attention_entry_checks_its_arguments(L):
-    fake = ctypes.c_void_p(0x10000)  # never dereferenced: validation fails first
-    st = (ctypes.c_int64 * 18)(*([128] * 18))
+FAKE, OTHER = 0x10000, 0x20000  # never dereferenced: validation fails first
 
-    def attn(q=fake, k=fake, masks=fake, strides=st, bf16=0, T=1, m=4, H=8, Hkv=2, Lmax=64, d=128, scale=0.1,
-             scores=None, scores_out=None, draft=None, ws=fake, nbytes=1 << 30):
-        return L.mb_tree_attn(q, k, fake, fake, fake, fake, masks, 0, fake, strides, bf16, T, m, H, Hkv, Lmax, d,
-                              scale, scores, scores_out, draft, ws, nbytes, None, None)
-    assert attn(q=None) == -1
-    assert attn(k=None) == -1
-    assert attn(masks=None) == -1
-    assert attn(strides=None) == -1
-    assert attn(scores_out=fake) == -1  # draft_scores missing
-    assert attn(scores=fake) == -1  # nowhere to put the sums
+
+def test_attention_entry_checks_its_arguments(L):
+    from moat_b200.tree import _AttnArgs
+
+    def attn(q=FAKE, k=FAKE, masks=FAKE, bf16=0, T=1, m=4, H=8, Hkv=2, Lmax=64, d=128, scale=0.1, scores=0,
+             scores_out=0, draft=0, ws=FAKE, nbytes=1 << 30):
+        return L.mb_tree_attn(_AttnArgs.pack(q, k, FAKE, FAKE, FAKE, FAKE, masks, FAKE, scores, scores_out, draft, ws, 0,
+                                             nbytes, *[128] * 18, 0, bf16, T, m, H, Hkv, Lmax, d, scale), None)
+    assert L.mb_tree_attn(None, None) == -1
+    assert attn(q=0) == -1
+    assert attn(k=0) == -1
+    assert attn(masks=0) == -1
+    assert attn(scores_out=FAKE) == -1  # draft_scores missing
+    assert attn(scores=FAKE) == -1  # nowhere to put the sums
     assert attn(m=0) == -2 and attn(m=65) == -2
     assert attn(H=7) == -2 and attn(Hkv=0) == -2
     assert attn(d=257) == -2 and attn(T=0) == -2 and attn(Lmax=-1) == -2
     assert attn(scale=float("inf")) == -2 and attn(scale=float("nan")) == -2
     assert attn(bf16=2) == -2
-    assert attn(ws=None) == -3 and attn(nbytes=16) == -3
-    assert attn(q=ctypes.c_void_p(0x10001)) == -5
-    assert attn(masks=ctypes.c_void_p(0x10004)) == -5
+    assert attn(ws=0) == -3 and attn(nbytes=16) == -3
+    assert attn(q=0x10001) == -5
+    assert attn(masks=0x10004) == -5
 
 
 def test_accept_entry_checks_its_arguments(L):
-    fake, other = ctypes.c_void_p(0x10000), ctypes.c_void_p(0x20000)
-    st = (ctypes.c_int64 * 16)(*([128] * 16))
+    from moat_b200.tree import _AcceptArgs
 
-    def accept(tokens=fake, lens=fake, layers=1, T=1, m=4, Hkv=2, Lmax=64, d=128, scores=None, draft=None,
-               lens_out=other, pos_out=other):
-        return L.mb_tree_accept(tokens, fake, 0, fake, lens, fake, fake, fake, fake, fake, st, layers, T, m, Hkv, Lmax,
-                                d, scores, draft, None, fake, fake, fake, lens_out, pos_out, None, None)
-    assert accept(tokens=None) == -1
-    assert accept(scores=fake) == -1  # draft_scores missing
+    def accept(tokens=FAKE, lens=FAKE, layers=1, T=1, m=4, Hkv=2, Lmax=64, d=128, scores=0, draft=0, lens_out=OTHER,
+               pos_out=OTHER):
+        return L.mb_tree_accept(_AcceptArgs.pack(tokens, FAKE, FAKE, lens, FAKE, FAKE, FAKE, FAKE, FAKE, scores, draft, 0,
+                                                 FAKE, FAKE, FAKE, lens_out, pos_out, 0, *[128] * 16, 0, layers, T, m,
+                                                 Hkv, Lmax, d), None)
+    assert L.mb_tree_accept(None, None) == -1
+    assert accept(tokens=0) == -1
+    assert accept(scores=FAKE) == -1  # draft_scores missing
     assert accept(m=65) == -2 and accept(T=0) == -2 and accept(layers=0) == -2 and accept(Lmax=0) == -2
-    assert accept(lens_out=fake) == -2  # in place: another CTA may still read the old length
-    assert accept(pos_out=fake) == -2
+    assert accept(lens_out=FAKE) == -2  # in place: another CTA may still read the old length
+    assert accept(pos_out=FAKE) == -2
     assert accept(layers=70000) == -6 and accept(Hkv=70000) == -6
 
 
 def test_rope_and_evict_entries_check_their_arguments(L):
-    fake, other = ctypes.c_void_p(0x10000), ctypes.c_void_p(0x20000)
+    from moat_b200.evict import _Args
+    fake = ctypes.c_void_p(FAKE)
     assert L.mb_tree_rope(None, 0, 1, 4, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, None, None) == -1
     assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 127, fake, fake, 0, fake, 64, fake, fake, None, None) == -2
     assert L.mb_tree_rope(fake, 0, 1, 65, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, None, None) == -2
     assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 128, fake, fake, 0, ctypes.c_void_p(0x10004), 64, fake, fake, None,
                           None) == -5
-    st = (ctypes.c_int64 * 8)(*([128] * 8))
 
-    def evict(k=fake, so=other, po=other, lens_out=other, budget=32, recent=8, sinks=4, ws=fake, nbytes=1 << 30,
-              Lmax=64):
-        return L.mb_cache_evict(k, fake, st, fake, fake, so, po, fake, fake, lens_out, 1, 1, 2, Lmax, 128, budget,
-                                recent, sinks, ws, nbytes, None)
-    assert evict(k=None) == -1
+    def evict(k=FAKE, so=OTHER, po=OTHER, lens_out=OTHER, budget=32, recent=8, sinks=4, ws=FAKE, nbytes=1 << 30, Lmax=64):
+        return L.mb_cache_evict(_Args.pack(k, FAKE, FAKE, FAKE, so, po, FAKE, FAKE, lens_out, ws, nbytes, *[128] * 8, 1, 1,
+                                           2, Lmax, 128, budget, recent, sinks), None)
+    assert L.mb_cache_evict(None, None) == -1
+    assert evict(k=0) == -1
     assert evict(budget=0) == -2 and evict(recent=-1) == -2 and evict(sinks=-1) == -2
     assert evict(budget=11) == -2  # cannot hold the recent rows and the sinks
-    assert evict(lens_out=fake) == -2
-    assert evict(so=fake) == -2  # scores in place, positions not
+    assert evict(lens_out=FAKE) == -2
+    assert evict(so=FAKE) == -2  # scores in place, positions not
     assert evict(Lmax=0) == -2
-    assert evict(ws=None) == -3 and evict(nbytes=16) == -3
+    assert evict(Lmax=1 << 20) == -6  # more rows than a cluster's shared memory ranks
+    assert evict(ws=0) == -3 and evict(nbytes=16) == -3
+
+
+def test_argument_structs_match_the_header():
+    """The packed formats have the size that the compiler gives the structs of the header."""
+    import subprocess
+    import tempfile
+    from moat_b200 import evict, tree
+    src = ('#include <stdio.h>\n#include "moat_b200.h"\nint main(void) { printf("%zu %zu %zu %zu", '
+           'sizeof(mb_tree_attn_args), sizeof(mb_tree_accept_args), sizeof(mb_cache_evict_args), '
+           'offsetof(mb_tree_attn_args, scale)); return 0; }\n')
+    with tempfile.TemporaryDirectory() as tmp:
+        c, exe = f"{tmp}/s.c", f"{tmp}/s"
+        with open(c, "w") as f:
+            f.write(src)
+        root = __file__.rsplit("/", 2)[0]
+        subprocess.run(["gcc", "-I", f"{root}/include", c, "-o", exe], check=True)
+        sizes = [int(x) for x in subprocess.run([exe], capture_output=True, check=True, text=True).stdout.split()]
+    pad = [-(-s.size // 8) * 8 for s in (tree._AttnArgs, tree._AcceptArgs, evict._Args)]
+    assert sizes[:3] == pad and sizes[3] == tree._AttnArgs.size - 4
 
 
 def test_lookup_draft():
