@@ -868,6 +868,29 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
       : "memory");
 }
 
+// Two fp32 operations in one instruction, and the largest of three.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Any over the 64 threads of the two warps of a lane quarter (named barrier id).
 __device__ __forceinline__ bool vote_pair(bool v, int id) {
   uint32_t r;
@@ -1031,6 +1054,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
 #pragma unroll
         for (int i = 0; i < 64; i += 16) tc_ld16(sbuf + key0 + i, x + i);
         tc_wait_ld();
+        // scores are x * f: f is the scale, or 1 where the scale is applied with the mask. For a
+        // negative scale the products change sign first, so that the largest x is the largest score.
+        float f = fabsf(sc);
+        if (sc < 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] = -x[i];
+        }
         if (draft || rows < kTile) {
           // bits of this thread's 64 keys that the row sees
           uint64_t see = draft ? (grp == 0 ? mask : 0) : ~0ull;
@@ -1040,16 +1070,17 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
             const bool on = ((i < 32 ? lo : hi) >> (i & 31)) & 1;
-            x[i] = on ? x[i] * sc : -INFINITY;
+            x[i] = on ? x[i] * f : -INFINITY;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] *= sc;
+          f = 1.0f;
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], x[i]);
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int i = 0; i < 64; i += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) top[u] = max3(top[u], x[i + u], x[i + u + 4]);
+        }
+        const float mx = max3(top[0], top[1], fmaxf(top[2], top[3])) * f;
         tc_before_sync();
         const bool raise = vote_pair(mx > ref + kSlack, 1 + wq);
         tc_after_sync();  // both warps of the row have read its scores: P may take their place
@@ -1077,15 +1108,17 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         }
         // p = 2^(x - m_ref), one rounding to the inputs' type for the product with V
         uint32_t pk[32];
-        float sum[4] = {};
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float2 f2 = make_float2(f, f), ref2 = make_float2(-ref, -ref);
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
-          const float e0 = ex2(x[i] - ref), e1 = ex2(x[i + 1] - ref);
-          sum[i & 2] += e0;
-          sum[(i & 2) + 1] += e1;
-          pk[i / 2] = pack2<BF16>(e0, e1);
+          float2 e = fma2(make_float2(x[i], x[i + 1]), f2, ref2);
+          e.x = ex2(e.x);
+          e.y = ex2(e.y);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+          pk[i / 2] = pack2<BF16>(e.x, e.y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_st32(sbuf + 32 * grp, pk);
         // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
         // product's last 16-row step reads beyond the valid rows, and unused drafted rows
@@ -1182,7 +1215,8 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const TreeAttnArgs& a = p.a;
   // Lengths and masks may be read before the attention has finished: it began only after the
-  // kernels that wrote them had.
+  // kernels that wrote them had. For the same reason the weight pass may start now.
+  pdl_launch_dependents();
   const int units = a.Hkv * p.RB;
   const int t = blockIdx.x / units, u = blockIdx.x - t * units;  // trace of this launch
   int before = 0, total = 0, longest = 0;
@@ -1227,7 +1261,6 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   const bool shown = mine && a.masks[tr * a.mask_stride + node] != 0;
   uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
   pdl_wait();
-  pdl_launch_dependents();
   if (!mine) return;
   float top = kNoRef, sum = 0.0f, o[4] = {};
   for (int b = c0; b <= c1; b += 4) {  // four pieces' loads in flight, one round of latency for most units
@@ -1314,14 +1347,17 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   } else {
     zero_query_tail(smem + lay.q, PANELS * p.nq, p.n16, R, tid, kSoft);
   }
-  pdl_wait();
-  pdl_launch_dependents();
-  // units are (trace, KV head) here: the sequence has no row blocks
-  if (warp == 0) prefix_tiles(p, tab, lane, a.Hkv);
+  // Lengths, queries, keys and masks were written before the attention began, so the TMA and MMA
+  // warps do not wait for the join: the first score products are ready when its results are.
   tc_before_sync();
-  __syncthreads();
+  if (warp == 8) {
+    prefix_tiles(p, tab, lane, a.Hkv);  // units are (trace, KV head) here: the sequence has no row blocks
+    __syncwarp();
+    asm volatile("bar.arrive 3, %0;" ::"n"(kWeightThreads) : "memory");
+  } else {
+    named_bar_sync(3, kWeightThreads);
+  }
   tc_after_sync();
-  const uint32_t tmem = *tmem_base;
   const int total = tab.cum[p.T];
   const int g = min(p.grid, total);
   const int c = blockIdx.x;
@@ -1382,6 +1418,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     const uint32_t id_qk = instr_desc(BF16, p.used, false, false);
     const uint32_t ring_k = smem_desc(ring, 16), q_desc = smem_desc(qbase, 16);
     const uint32_t qpanel = p.n16 * 128 >> 4;
+    const uint32_t tmem = *tmem_base;
     int seg = 0, st = 0, use = 0, fills0 = 0, fills1 = 0;
     Segment s;
     for (int f = beg; next_segment(p, tab, f, end, 1, s);) {
@@ -1420,7 +1457,9 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     const float sc = a.scale_log2;
     float* lse = lse_s + grp * kMaxRows;
     uint64_t* rowmask = mask_s + grp * kMaxRows;
-    const uint32_t sbuf = tmem + lanes + grp * kMaxRows;
+    const uint32_t sbuf = *tmem_base + lanes + grp * kMaxRows;
+    pdl_wait();  // the join's denominators
+    pdl_launch_dependents();
     int fill = 0;
     Segment s;
     for (int f = beg; next_segment(p, tab, f, end, 1, s);) {
@@ -1469,7 +1508,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  if (warp == 9) tmem_dealloc(tmem, 256);
+  if (warp == 9) tmem_dealloc(*tmem_base, 256);
 }
 
 // The same sums where the attention kept its scores (few rows): a thread per four cached rows.
