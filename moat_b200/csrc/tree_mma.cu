@@ -495,6 +495,36 @@ __device__ __forceinline__ void drain_products() {
   }
 }
 
+// A softmax thread's masks for a segment: its row's, and two of the trace's (node lane and lane +
+// 32). Loaded while the segment before it ends; volatile, because the compiler moved the loads
+// down to the drafted tile that uses them, which then took 2,700 cycles instead of 300.
+struct SegmentMasks {
+  uint64_t row, lo, hi;
+};
+
+__device__ __forceinline__ uint64_t ld_mask(const uint64_t* p) {
+  uint64_t v;
+  asm volatile("ld.global.u64 %0, [%1];" : "=l"(v) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ SegmentMasks load_masks(const TreeAttnArgs& a, int t, int node, bool has_row, int lane) {
+  const uint64_t* mk = a.masks + t * a.mask_stride;
+  SegmentMasks m;
+  m.row = has_row ? ld_mask(mk + node) : 0;
+  m.lo = lane < a.m ? ld_mask(mk + lane) : 0;
+  m.hi = lane + 32 < a.m ? ld_mask(mk + lane + 32) : 0;
+  return m;
+}
+
+// Drafted rows that any node sees, one bit each (a warp's masks together are the trace's).
+__device__ __forceinline__ uint64_t rows_in_use(const SegmentMasks& m) {
+  const uint64_t u = m.lo | m.hi;
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(u));
+  const uint32_t hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(u >> 32));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
 // ---------------------------------------------------------------------------
 // Up to 16 rows: the keys fill the TMEM lanes.
 // PANELS: 64-column panels of the head dim (1: d <= 64, 2: d <= 128).
@@ -642,13 +672,12 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
     float* scratch = reinterpret_cast<float*>(smem + lay.p);  // P's space, while no product reads it
     const uint32_t tmem = *tmem_base;
     int seg = 0, k = 0, vst = 1, vuse = 0;
-    Segment s;
-    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
-      // this row's mask, and the rows of the draft that any node sees (loads in flight over the
-      // first tile)
-      const uint64_t* mk = a.masks + s.t * a.mask_stride;
-      const uint64_t my_mask = tid < R ? mk[my_node] : 0;  // few rows are one block
-      const uint64_t mk0 = lane < a.m ? mk[lane] : 0, mk1 = lane + 32 < a.m ? mk[lane + 32] : 0;
+    Segment s, next;
+    SegmentMasks masks = {}, next_masks = {};
+    int f = beg;
+    bool more = next_segment(p, tab, f, end, p.RB, s);
+    if (more) masks = load_masks(a, s.t, my_node, tid < R, lane);  // few rows are one block
+    for (; more; ++seg, s = next, masks = next_masks) {
       for (int jj = 0; jj < s.n; ++jj, ++k) {
         const int j = s.j0 + jj;
         const bool draft = j == s.nt - 1;
@@ -657,7 +686,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         // which of this thread's rows see its key, a bit each
         uint32_t see = key < rows ? ~0u : 0u;
         if (draft) {
-          if (tid < kKeysRows) rowmask[tid] = my_mask;
+          if (tid < kKeysRows) rowmask[tid] = masks.row;
           named_bar_sync(1, kSoft);
           if (key < rows) {
             see = 0;
@@ -752,9 +781,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
         // product's last 16-row step reads beyond the valid rows, and unused drafted rows
         if (rows & 15 || draft) {
-          uint64_t used = mk0 | mk1;
-#pragma unroll
-          for (int o = 16; o; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
+          const uint64_t used = draft ? rows_in_use(masks) : 0;
           const bool clear = key >= rows ? key < ((rows + 15) & ~15) : draft && !((used >> (key & 63)) & 1);
           if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
           if (clear) {
@@ -770,6 +797,8 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         next_tile(p.nst, vst, vuse);
       }
       // ------------------------------------------------ end of the segment: sums, output
+      more = next_segment(p, tab, f, end, p.RB, next);  // under the last value product
+      if (more) next_masks = load_masks(a, next.t, my_node, tid < R, lane);
       const float part_sum = column_sums16(l, lane);
       guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
       tc_after_sync();
@@ -780,7 +809,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
       if (tid < kKeysRows) {
         const float sum = (scratch[tid] + scratch[kKeysRows + tid]) + (scratch[2 * kKeysRows + tid] +
                                                                        scratch[3 * kKeysRows + tid]);
-        const bool real = my_mask != 0 && sum != 0.0f;
+        const bool real = masks.row != 0 && sum != 0.0f;
         const float top = ref[tid];
         scratch[4 * kKeysRows + tid] = real ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
         ref[tid] = kNoRef;
@@ -1034,13 +1063,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     const float sc = a.scale_log2;
     const int my_node = row / p.G, my_head = row - my_node * p.G;
     int seg = 0, k = 0, vst = 1, vuse = 0;
-    Segment s;
-    for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
-      const uint64_t* mk = a.masks + s.t * a.mask_stride;
+    Segment s, next;
+    SegmentMasks masks = {}, next_masks = {};
+    int f = beg;
+    bool more = next_segment(p, tab, f, end, p.RB, s);
+    auto masks_of = [&](const Segment& g) {
+      const int node = g.rb * p.mb + my_node;
+      return load_masks(a, g.t, node, row < R && node < a.m, lane);
+    };
+    if (more) masks = masks_of(s);
+    for (; more; ++seg, s = next, masks = next_masks) {
       const int node = s.rb * p.mb + my_node;
       const bool real_row = row < R && node < a.m;
-      const uint64_t mask = real_row ? mk[node] : 0;
-      const uint64_t mk0 = lane < a.m ? mk[lane] : 0, mk1 = lane + 32 < a.m ? mk[lane + 32] : 0;
       const uint32_t obuf = tmem + lanes + (2 + (seg & 1)) * kTile;
       float ref = kNoRef, l = 0.0f;
       for (int jj = 0; jj < s.n; ++jj, ++k) {
@@ -1063,7 +1097,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         }
         if (draft || rows < kTile) {
           // bits of this thread's 64 keys that the row sees
-          uint64_t see = draft ? (grp == 0 ? mask : 0) : ~0ull;
+          uint64_t see = draft ? (grp == 0 ? masks.row : 0) : ~0ull;
           const int n = rows - key0;  // valid keys among them
           see &= n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
           const uint32_t lo = static_cast<uint32_t>(see), hi = static_cast<uint32_t>(see >> 32);
@@ -1123,9 +1157,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
         // product's last 16-row step reads beyond the valid rows, and unused drafted rows
         if (grp == 0 && (rows & 15 || draft)) {
-          uint64_t used = mk0 | mk1;
-#pragma unroll
-          for (int o = 16; o; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
+          const uint64_t used = draft ? rows_in_use(masks) : 0;
           const bool clear = row >= rows ? row < ((rows + 15) & ~15) : draft && !((used >> (row & 63)) & 1);
           if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
           if (clear) {
@@ -1142,11 +1174,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         next_tile(p.nst, vst, vuse);
       }
       // ------------------------------------------------ end of the segment: sums, output
+      more = next_segment(p, tab, f, end, p.RB, next);  // under the last value product
+      if (more) next_masks = masks_of(next);
       xchg[grp * kTile + row] = l;
       named_bar_sync(1 + wq, 64);
       const float sum = xchg[row] + xchg[kTile + row];
       named_bar_sync(1 + wq, 64);
-      const bool whole = s.n == s.nt, real = mask != 0 && sum != 0.0f;
+      const bool whole = s.n == s.nt, real = masks.row != 0 && sum != 0.0f;
       const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
       if (grp == 0) {
         if (!whole) {
