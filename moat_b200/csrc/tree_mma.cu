@@ -47,6 +47,7 @@ struct TreeMmaParams {
   CUtensorMap mq, mk, mv, mk_end, mv_end, mkd, mvd;  // (seven in a row: prefetched by index)
   float* part;  // [2 * grid][rows][DP] unnormalised O of a unit's pieces
   float* ml;    // [2 * grid][2][kMaxRows] their m_ref and sum
+  int join_passes;  // rows of a join CTA, in passes of its threads
   float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
   float* kept;  // [units][R][kept_len] scores of the cached rows, kept for the weight pass, or null
   float* kept_draft;  // [units][R][64] of the drafted rows
@@ -1237,96 +1238,85 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   if (warp == 9) tmem_dealloc(*tmem_base, 512);
 }
 
-// Joins the pieces of the units that were cut between CTAs, in order. One CTA per unit and
-// group of 8 rows; a unit that one CTA held is done already.
+// Joins the pieces of the units that were cut between CTAs, in order. CTA (x, y) looks at the
+// boundary between attention CTAs x and x + 1: if a unit's first cut lies there, it joins a group
+// of the unit's rows. Where the cuts lie it works out from the lengths, which it may read before
+// the attention has finished (that began only after the kernels that wrote them had), so that one
+// round of loads is left after the wait. One CTA per unit and 8 rows, most with nothing to join,
+// took 6 us after a 17 us attention; notes left by the attention, read after the wait, 1 to 2.5 us
+// more than this where the units are few.
 constexpr int kJoinBlock = 256;
-constexpr int kJoinRows = 8;
 
 template <int PANELS, bool BF16>
 __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant__ TreeMmaParams p) {
   constexpr int DP = PANELS * 64;
-  __shared__ int red[3][kJoinBlock / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const TreeAttnArgs& a = p.a;
-  // Lengths and masks may be read before the attention has finished: it began only after the
-  // kernels that wrote them had. For the same reason the weight pass may start now.
-  pdl_launch_dependents();
-  const int units = a.Hkv * p.RB;
-  const int t = blockIdx.x / units, u = blockIdx.x - t * units;  // trace of this launch
-  int before = 0, total = 0, longest = 0;
-  for (int i = tid; i < p.T; i += kJoinBlock) {
-    const int span = unit_span(trace_tiles(trace_len(a, p.t0 + i)));
-    total += span * units;
-    before += i < t ? span * units : 0;
-    longest = max(longest, span);
-  }
-  longest = __reduce_max_sync(0xffffffffu, longest);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  if (lane == 0) {
-    red[0][warp] = total;
-    red[1][warp] = before;
-    red[2][warp] = longest;
-  }
-  __syncthreads();
-  total = before = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinBlock / 32; ++w) {
-    total += red[0][w];
-    before += red[1][w];
-    longest = max(longest, red[2][w]);
-  }
-  const bool cut_units = share_mode(p, total, longest, units * p.T) == Share::kCut;
-  const int nt = trace_tiles(trace_len(a, p.t0 + t));
-  const int f0 = before + u * unit_span(nt) + kUnitCost, f1 = f0 + nt - 1;  // its first and last tile
-  const int g = min(p.grid, total);
-  // the CTA that holds position f: the largest c with cut(c) <= f
-  const int c0 = static_cast<int>(((static_cast<int64_t>(f0) + 1) * g - 1) / total);
-  const int c1 = static_cast<int>(((static_cast<int64_t>(f1) + 1) * g - 1) / total);
-  const int R = p.mb * p.G;
-  const int kvh = u / p.RB, rb = u - kvh * p.RB, tr = p.t0 + t;
   constexpr int kLanes = DP / 4;  // threads of a row, four values each
-  const int n = blockIdx.y * kJoinRows + tid / kLanes, v = (tid % kLanes) * 4;
-  const int node = rb * p.mb + n / p.G;
-  const bool mine = cut_units && c0 != c1 && tid / kLanes < kJoinRows && n < R && node < a.m;
-  const bool shown = mine && a.masks[tr * a.mask_stride + node] != 0;
-  uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
-  pdl_wait();
-  if (!mine) return;
-  float top = kNoRef, sum = 0.0f, o[4] = {};
-  for (int b = c0; b <= c1; b += 4) {  // four pieces' loads in flight, one round of latency for most units
-    float m[4], l[4];
-    float4 x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (b + i <= c1) {
-        const int64_t slot = 2 * (b + i) + (b + i == c0 ? 1 : 0);
-        m[i] = p.ml[slot * 2 * kMaxRows + n];
-        l[i] = p.ml[(slot * 2 + 1) * kMaxRows + n];
-        x[i] = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
-      }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (b + i <= c1) {
-        const float now = fmaxf(top, m[i]), fade = ex2(top - now), w = ex2(m[i] - now);
-        top = now;
-        sum = fmaf(w, l[i], sum * fade);
-        o[0] = fmaf(w, x[i].x, o[0] * fade);
-        o[1] = fmaf(w, x[i].y, o[1] * fade);
-        o[2] = fmaf(w, x[i].z, o[2] * fade);
-        o[3] = fmaf(w, x[i].w, o[3] * fade);
-      }
+  __shared__ TraceTable tab;
+  const int tid = threadIdx.x;
+  const TreeAttnArgs& a = p.a;
+  pdl_launch_dependents();  // the weight pass loads its keys meanwhile
+  const int units = a.Hkv * p.RB;
+  if (tid < 32) prefix_tiles(p, tab, tid, units);
+  __syncthreads();
+  const int total = tab.cum[p.T], g = min(p.grid, total), c0 = blockIdx.x;
+  if (c0 + 1 >= g || share_mode(p, total, tab.max_span, units * p.T) != Share::kCut) return;
+  const int here = cut(total, c0 + 1, g);
+  int lo = 0, hi = p.T - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.cum[mid] <= here)
+      lo = mid;
+    else
+      hi = mid - 1;
   }
-  const bool real = shown && sum != 0.0f;
-  const float inv = real ? 1.0f / sum : 0.0f;
+  const int nt = trace_tiles(tab.len[lo]), span = unit_span(nt), u = (here - tab.cum[lo]) / span;
+  const int tile0 = tab.cum[lo] + u * span + kUnitCost;
+  // the unit at the boundary began at or after it, or was cut before
+  if (here <= tile0 || tile0 < cut(total, c0, g)) return;
+  // its last piece: the largest c with cut(c) <= the position of its last tile
+  const int c1 = static_cast<int>((static_cast<int64_t>(tile0 + nt) * g - 1) / total);
+  const int tr = p.t0 + lo, kvh = u / p.RB, rb = u - kvh * p.RB;
+  const int R = p.mb * p.G, v = (tid % kLanes) * 4;
+  int n = blockIdx.y * p.join_passes * (kJoinBlock / kLanes) + tid / kLanes;
+  pdl_wait();
+  for (int pass = 0; pass < p.join_passes; ++pass, n += kJoinBlock / kLanes) {
+    const int node = rb * p.mb + n / p.G;
+    if (n >= R || node >= a.m) break;
+    const bool shown = a.masks[tr * a.mask_stride + node] != 0;
+    float top = kNoRef, sum = 0.0f, o[4] = {};
+    for (int b = c0; b <= c1; b += 4) {  // four pieces' loads in flight, one round of latency for most units
+      float m[4], l[4];
+      float4 x[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (v + i < a.d) out[v + i] = round16<BF16>(real ? o[i] * inv : 0.0f);
-  if (p.lse && v == 0)
-    p.lse[((static_cast<int64_t>(tr) * a.Hkv + kvh) * p.RB + rb) * kMaxRows + n] = real ? top + log2f(sum) : INFINITY;
+      for (int i = 0; i < 4; ++i)
+        if (b + i <= c1) {
+          const int64_t slot = 2 * (b + i) + (b + i == c0 ? 1 : 0);
+          m[i] = p.ml[slot * 2 * kMaxRows + n];
+          l[i] = p.ml[(slot * 2 + 1) * kMaxRows + n];
+          x[i] = *reinterpret_cast<const float4*>(p.part + (slot * R + n) * DP + v);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (b + i <= c1) {
+          const float now = fmaxf(top, m[i]), fade = ex2(top - now), w = ex2(m[i] - now);
+          top = now;
+          sum = fmaf(w, l[i], sum * fade);
+          o[0] = fmaf(w, x[i].x, o[0] * fade);
+          o[1] = fmaf(w, x[i].y, o[1] * fade);
+          o[2] = fmaf(w, x[i].z, o[2] * fade);
+          o[3] = fmaf(w, x[i].w, o[3] * fade);
+        }
+    }
+    const bool real = shown && sum != 0.0f;
+    const float inv = real ? 1.0f / sum : 0.0f;
+    uint16_t* out = a.out + tr * a.os[0] + node * a.os[1] + (kvh * p.G + n % p.G) * a.os[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (v + i < a.d) out[v + i] = round16<BF16>(real ? o[i] * inv : 0.0f);
+    if (p.lse && v == 0)
+      p.lse[((static_cast<int64_t>(tr) * a.Hkv + kvh) * p.RB + rb) * kMaxRows + n] =
+          real ? top + log2f(sum) : INFINITY;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1695,9 +1685,9 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
   const int rc = p.n16 == kKeysRows ? launch_attn_keys<PANELS, BF16>(p, smem, st)
                                     : launch_attn_rows<PANELS, BF16>(p, smem, st);
   if (rc != MB_OK || p.whole) return rc;
-  const int R = p.mb * p.G;
-  return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.T * p.a.Hkv * p.RB, (R + kJoinRows - 1) / kJoinRows),
-                         dim3(kJoinBlock), 0, st, p);
+  const int rows = p.join_passes * kJoinBlock / (PANELS * 16);
+  return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.grid - 1, (p.mb * p.G + rows - 1) / rows), dim3(kJoinBlock),
+                         0, st, p);
 }
 
 template <int PANELS, bool BF16>
@@ -1755,6 +1745,10 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   w += static_cast<size_t>(2) * pl.grid * pl.mb * pl.G * pl.panels * 64 * 4;
   p.ml = reinterpret_cast<float*>(w);
   w += static_cast<size_t>(2) * pl.grid * 2 * kMaxRows * 4;
+  // join CTAs that find a unit to join: about as many as the GPU holds at once
+  const int per_pass = kJoinBlock / (pl.panels * 16), groups = (pl.mb * pl.G + per_pass - 1) / per_pass;
+  const int64_t cuts = std::min<int64_t>(static_cast<int64_t>(a.T) * a.Hkv * pl.RB, pl.grid - 1);
+  p.join_passes = static_cast<int>(std::max<int64_t>(1, cuts * groups / (4 * pl.grid)));
   p.lse = p.kept = p.kept_draft = nullptr;
   p.kept_len = (a.Lmax + 3) / 4 * 4;
   if (a.scores_out) {
