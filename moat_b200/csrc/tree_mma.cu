@@ -178,13 +178,13 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
-// CTA-wide "any" over the softmax warps.
-__device__ __forceinline__ bool vote_any(bool v, int threads) {
+// "Any" over the threads of a named barrier.
+__device__ __forceinline__ bool vote_any(bool v, int id, int threads) {
   uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(v ? 1u : 0u), "r"(threads)
+      : "r"(v ? 1u : 0u), "r"(id), "r"(threads)
       : "memory");
   return r != 0;
 }
@@ -324,7 +324,8 @@ struct TreeSmem {
   uint32_t misc, total;
 };
 constexpr int kMaxStages = 8;
-constexpr uint32_t kMiscBars = 256;                          // barriers, TMEM base
+constexpr uint32_t kMiscBars = 256;                          // barriers, TMEM base, noted rows
+constexpr uint32_t kMiscNoted = 240;
 constexpr uint32_t kMiscRef = kMiscBars;                     // m_ref [128]
 constexpr uint32_t kMiscMask = kMiscRef + kMaxRows * 4;      // draft masks by row [128]
 constexpr uint32_t kMiscTab = kMiscMask + kMaxRows * 8;      // TraceTable
@@ -496,11 +497,11 @@ __device__ __forceinline__ void drain_products() {
   }
 }
 
-// A softmax thread's masks for a segment: its row's, and two of the trace's (node lane and lane +
-// 32). Loaded while the segment before it ends; volatile, because the compiler moved the loads
-// down to the drafted tile that uses them, which then took 2,700 cycles instead of 300.
+// Masks of a trace for a segment, two per lane of a warp (node lane and lane + 32). Loads are
+// volatile: the compiler moved them down to the drafted tile that uses them, which then took 2,700
+// cycles instead of 300.
 struct SegmentMasks {
-  uint64_t row, lo, hi;
+  uint64_t lo, hi;
 };
 
 __device__ __forceinline__ uint64_t ld_mask(const uint64_t* p) {
@@ -509,10 +510,9 @@ __device__ __forceinline__ uint64_t ld_mask(const uint64_t* p) {
   return v;
 }
 
-__device__ __forceinline__ SegmentMasks load_masks(const TreeAttnArgs& a, int t, int node, bool has_row, int lane) {
+__device__ __forceinline__ SegmentMasks load_masks(const TreeAttnArgs& a, int t, int lane) {
   const uint64_t* mk = a.masks + t * a.mask_stride;
   SegmentMasks m;
-  m.row = has_row ? ld_mask(mk + node) : 0;
   m.lo = lane < a.m ? ld_mask(mk + lane) : 0;
   m.hi = lane + 32 < a.m ? ld_mask(mk + lane + 32) : 0;
   return m;
@@ -524,6 +524,90 @@ __device__ __forceinline__ uint64_t rows_in_use(const SegmentMasks& m) {
   const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(u));
   const uint32_t hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(u >> 32));
   return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// A value that is not finite must not reach a node that does not see its row, but in the product
+// with V it would (0 x inf is NaN). So the drafted rows, the only ones that some nodes see and
+// others do not, are looked through: what is not finite becomes 0 in shared memory, the row is
+// noted, and the output's end adds it for the nodes that see it.
+template <bool BF16>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {  // bits 15 and 31: the low, the high half
+  constexpr uint32_t e = BF16 ? 0x7F807F80u : 0x7C007C00u, one = BF16 ? 0x00800080u : 0x04000400u;
+  return ((x & e) + one) & 0x80008000u;
+}
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint16_t x) {
+  return (not_finite2<BF16>(x) & 0x8000u) != 0;
+}
+
+// Makes a V tile fit for its product, by the warp that issues it (idle until P is there; done by
+// the softmax warps it cost them 300 to 1,000 cycles per unit): lines beyond the valid rows in the
+// last 16-row step, and drafted rows that no node sees, may hold anything and become 0; of the other
+// drafted rows what is not finite does, and noted[0..1] gets their bits.
+template <int PANELS, bool BF16>
+__device__ __forceinline__ void prepare_values(uint8_t* tile, int rows, bool draft, const SegmentMasks& masks, int lane,
+                                               volatile uint32_t* noted) {
+  auto piece = [&](int line, int i) {  // 16 bytes: piece i of a line's PANELS * 8
+    return reinterpret_cast<uint4*>(tile + (i >> 3) * kPanel + line * 128 + (i & 7) * 16);
+  };
+  const int end = (rows + 15) & ~15;
+  for (int i = lane; i < (end - rows) * PANELS * 8; i += 32)
+    *piece(rows + i / (PANELS * 8), i % (PANELS * 8)) = make_uint4(0, 0, 0, 0);
+  if (draft) {
+    uint64_t unused = ~rows_in_use(masks) & (rows == 64 ? ~0ull : (1ull << rows) - 1);
+    for (; unused; unused &= unused - 1)
+      if (lane < PANELS * 8) *piece(__ffsll(unused) - 1, lane) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+    uint32_t bad = 0;
+#pragma unroll 4
+    for (int i = lane; i < rows * PANELS * 8; i += 32) {
+      const uint4 x = *piece(i / (PANELS * 8), i % (PANELS * 8));
+      bad |= not_finite2<BF16>(x.x) | not_finite2<BF16>(x.y) | not_finite2<BF16>(x.z) | not_finite2<BF16>(x.w);
+    }
+    uint32_t lo = 0, hi = 0;
+    if (__any_sync(0xffffffffu, bad != 0)) {  // rare: line by line
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+        bool found = false;
+        if (lane < PANELS * 8) {
+          uint4 x = *piece(r, lane);
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t b = not_finite2<BF16>(w[u]);
+            found |= b != 0;
+            w[u] &= ~((b >> 15) * 0xFFFFu);
+          }
+          *piece(r, lane) = x;
+        }
+        const uint32_t bit = __any_sync(0xffffffffu, found) ? 1u << (r & 31) : 0u;
+        if (r < 32)
+          lo |= bit;
+        else
+          hi |= bit;
+      }
+    }
+    if (lane == 0) {
+      noted[0] = lo;
+      noted[1] = hi;
+    }
+    __threadfence_block();
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// The sum over the noted rows in `rows` that are not finite at head-dim position c of trace t's
+// drafted values (0 if all are).
+template <bool BF16>
+__device__ __noinline__ float noted_values(const TreeAttnArgs& a, int t, int kvh, uint64_t rows, int c) {
+  float sum = 0.0f;
+  for (; rows; rows &= rows - 1) {
+    const uint16_t v = a.vd[t * a.vds[0] + (__ffsll(rows) - 1) * a.vds[1] + kvh * a.vds[2] + c];
+    if (not_finite<BF16>(v))
+      sum += BF16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
+  }
+  return sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -553,6 +637,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
   float* ref = reinterpret_cast<float*>(misc + kMiscRef);
   uint64_t* rowmask = reinterpret_cast<uint64_t*>(misc + kMiscMask);
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
+  volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);  // drafted rows, see prepare_values
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TreeAttnArgs& a = p.a;
@@ -641,9 +726,13 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
     Segment s;
     for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
       const uint32_t o = tmem + (2 + (seg & 1)) * kKeysRows;
+      const SegmentMasks masks = load_masks(a, s.t, lane);
       for (int jj = 0; jj < s.n; ++jj, ++k) {
-        const int steps = (tile_rows(s.len, s.nt, a.m, s.j0 + jj) + 15) / 16;
+        const bool draft = s.j0 + jj == s.nt - 1;
+        const int rows = tile_rows(s.len, s.nt, a.m, s.j0 + jj), steps = (rows + 15) / 16;
         guarded_wait(kv_full + st, use & 1, dead, a.err);
+        if (rows & 15 || draft)
+          prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted);
         if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
         guarded_wait(p_full, k & 1, dead, a.err);
         tc_after_sync();
@@ -672,13 +761,16 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
     for (int i = 0; i < kKeysRows; ++i) l[i] = 0.0f;
     float* scratch = reinterpret_cast<float*>(smem + lay.p);  // P's space, while no product reads it
     const uint32_t tmem = *tmem_base;
-    int seg = 0, k = 0, vst = 1, vuse = 0;
+    int seg = 0, k = 0;
     Segment s, next;
-    SegmentMasks masks = {}, next_masks = {};
+    uint64_t mask = 0, next_mask = 0;  // of row tid
     int f = beg;
     bool more = next_segment(p, tab, f, end, p.RB, s);
-    if (more) masks = load_masks(a, s.t, my_node, tid < R, lane);  // few rows are one block
-    for (; more; ++seg, s = next, masks = next_masks) {
+    auto mask_of = [&](const Segment& g) {  // few rows are one block
+      return tid < R ? ld_mask(a.masks + g.t * a.mask_stride + my_node) : 0;
+    };
+    if (more) mask = mask_of(s);
+    for (; more; ++seg, s = next, mask = next_mask) {
       for (int jj = 0; jj < s.n; ++jj, ++k) {
         const int j = s.j0 + jj;
         const bool draft = j == s.nt - 1;
@@ -687,7 +779,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         // which of this thread's rows see its key, a bit each
         uint32_t see = key < rows ? ~0u : 0u;
         if (draft) {
-          if (tid < kKeysRows) rowmask[tid] = masks.row;
+          if (tid < kKeysRows) rowmask[tid] = mask;
           named_bar_sync(1, kSoft);
           if (key < rows) {
             see = 0;
@@ -717,7 +809,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
           float top = x[0];
 #pragma unroll
           for (int u = 1; u < kKeysRows; ++u) top = fmaxf(top, x[u]);
-          raise = vote_any(top > kSlack, kSoft);
+          raise = vote_any(top > kSlack, 1, kSoft);
         }
         if (raise) {
           // P's space and O are free once the previous value product has finished
@@ -779,27 +871,13 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         uint8_t* prow = smem + lay.p + key * 128;
         *reinterpret_cast<uint4*>(prow + ((key & 7) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         *reinterpret_cast<uint4*>(prow + ((1 ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-        // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
-        // product's last 16-row step reads beyond the valid rows, and unused drafted rows
-        if (rows & 15 || draft) {
-          const uint64_t used = draft ? rows_in_use(masks) : 0;
-          const bool clear = key >= rows ? key < ((rows + 15) & ~15) : draft && !((used >> (key & 63)) & 1);
-          if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
-          if (clear) {
-            for (int pn = 0; pn < PANELS; ++pn)
-              for (int u = 0; u < 8; ++u)
-                *reinterpret_cast<uint4*>(smem + lay.ring + vst * lay.stage + pn * kPanel + key * 128 + u * 16) =
-                    make_uint4(0, 0, 0, 0);
-          }
-        }
         fence_proxy_async_smem();
         tc_before_sync();
         mbar_arrive(p_full);
-        next_tile(p.nst, vst, vuse);
       }
       // ------------------------------------------------ end of the segment: sums, output
       more = next_segment(p, tab, f, end, p.RB, next);  // under the last value product
-      if (more) next_masks = load_masks(a, next.t, my_node, tid < R, lane);
+      if (more) next_mask = mask_of(next);
       const float part_sum = column_sums16(l, lane);
       guarded_wait(pv_done, (k - 1) & 1, dead, a.err);
       tc_after_sync();
@@ -810,7 +888,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
       if (tid < kKeysRows) {
         const float sum = (scratch[tid] + scratch[kKeysRows + tid]) + (scratch[2 * kKeysRows + tid] +
                                                                        scratch[3 * kKeysRows + tid]);
-        const bool real = masks.row != 0 && sum != 0.0f;
+        const bool real = mask != 0 && sum != 0.0f;
         const float top = ref[tid];
         scratch[4 * kKeysRows + tid] = real ? 1.0f / sum : 0.0f;  // 0 marks a row without keys
         ref[tid] = kNoRef;
@@ -825,6 +903,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
       }
       named_bar_sync(1, kSoft);
       const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kKeysRows;
+      const uint64_t bad = s.j0 + s.n == s.nt ? static_cast<uint64_t>(noted[1]) << 32 | noted[0] : 0;
       int row = 0, nd = 0, gh = 0;  // row, its node, its head of the group
       uint16_t* out = a.out + s.t * a.os[0] + s.kvh * p.G * a.os[2] + key;
       float* part = p.part + static_cast<int64_t>(slot) * R * DP + key;
@@ -838,6 +917,8 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         for (int u = 0; u < 4; ++u, ++row) {
           const float scale = u == 0 ? inv.x : u == 1 ? inv.y : u == 2 ? inv.z : inv.w;
           if (row < R) {
+            if (bad && (bad & rowmask[row]) && key < a.d)
+              o[u] += noted_values<BF16>(a, s.t, s.kvh, bad & rowmask[row], key);
             if (!whole) {
               if (key < DP) *part = o[u];
               part += DP;
@@ -921,17 +1002,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// Any over the 64 threads of the two warps of a lane quarter (named barrier id).
-__device__ __forceinline__ bool vote_pair(bool v, int id) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(v ? 1u : 0u), "r"(id)
-      : "memory");
-  return r != 0;
-}
-
 template <int PANELS, bool BF16>
 __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid_constant__ TreeMmaParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -951,6 +1021,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 2);
   float* xchg = reinterpret_cast<float*>(misc + kMiscRef);  // [2][128] between the two warps of a row
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
+  volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);  // drafted rows, see scrub_line
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TreeAttnArgs& a = p.a;
@@ -1036,9 +1107,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     Segment s;
     for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
       const uint32_t o = tmem + (2 + (seg & 1)) * kTile;
+      const SegmentMasks masks = load_masks(a, s.t, lane);
       for (int jj = 0; jj < s.n; ++jj, ++k) {
-        const int steps = (tile_rows(s.len, s.nt, a.m, s.j0 + jj) + 15) / 16;
+        const bool draft = s.j0 + jj == s.nt - 1;
+        const int rows = tile_rows(s.len, s.nt, a.m, s.j0 + jj), steps = (rows + 15) / 16;
         guarded_wait(kv_full + st, use & 1, dead, a.err);
+        if (rows & 15 || draft)
+          prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted);
         if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
         guarded_wait(p_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
@@ -1063,17 +1138,17 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     const uint32_t tmem = *tmem_base, lanes = static_cast<uint32_t>(wq * 32) << 16;
     const float sc = a.scale_log2;
     const int my_node = row / p.G, my_head = row - my_node * p.G;
-    int seg = 0, k = 0, vst = 1, vuse = 0;
+    int seg = 0, k = 0;
     Segment s, next;
-    SegmentMasks masks = {}, next_masks = {};
+    uint64_t mask = 0, next_mask = 0;  // of this row
     int f = beg;
     bool more = next_segment(p, tab, f, end, p.RB, s);
-    auto masks_of = [&](const Segment& g) {
+    auto mask_of = [&](const Segment& g) {
       const int node = g.rb * p.mb + my_node;
-      return load_masks(a, g.t, node, row < R && node < a.m, lane);
+      return row < R && node < a.m ? ld_mask(a.masks + g.t * a.mask_stride + node) : 0;
     };
-    if (more) masks = masks_of(s);
-    for (; more; ++seg, s = next, masks = next_masks) {
+    if (more) mask = mask_of(s);
+    for (; more; ++seg, s = next, mask = next_mask) {
       const int node = s.rb * p.mb + my_node;
       const bool real_row = row < R && node < a.m;
       const uint32_t obuf = tmem + lanes + (2 + (seg & 1)) * kTile;
@@ -1098,7 +1173,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         }
         if (draft || rows < kTile) {
           // bits of this thread's 64 keys that the row sees
-          uint64_t see = draft ? (grp == 0 ? masks.row : 0) : ~0ull;
+          uint64_t see = draft ? (grp == 0 ? mask : 0) : ~0ull;
           const int n = rows - key0;  // valid keys among them
           see &= n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
           const uint32_t lo = static_cast<uint32_t>(see), hi = static_cast<uint32_t>(see >> 32);
@@ -1117,7 +1192,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         }
         const float mx = max3(top[0], top[1], fmaxf(top[2], top[3])) * f;
         tc_before_sync();
-        const bool raise = vote_pair(mx > ref + kSlack, 1 + wq);
+        const bool raise = vote_any(mx > ref + kSlack, 1 + wq, 64);
         tc_after_sync();  // both warps of the row have read its scores: P may take their place
         if (raise) {
           xchg[grp * kTile + row] = mx;
@@ -1155,33 +1230,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_st32(sbuf + 32 * grp, pk);
-        // rows of V that no node sees may hold anything, and 0 x NaN is NaN: zero what the
-        // product's last 16-row step reads beyond the valid rows, and unused drafted rows
-        if (grp == 0 && (rows & 15 || draft)) {
-          const uint64_t used = draft ? rows_in_use(masks) : 0;
-          const bool clear = row >= rows ? row < ((rows + 15) & ~15) : draft && !((used >> (row & 63)) & 1);
-          if (__any_sync(0xffffffffu, clear)) guarded_wait(kv_full + vst, vuse & 1, dead, a.err);
-          if (clear) {
-            for (int pn = 0; pn < PANELS; ++pn)
-              for (int u = 0; u < 8; ++u)
-                *reinterpret_cast<uint4*>(smem + lay.ring + vst * lay.stage + pn * kPanel + row * 128 + u * 16) =
-                    make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
         tc_wait_st();
         tc_before_sync();
         mbar_arrive(p_full + (k & 1));
-        next_tile(p.nst, vst, vuse);
       }
       // ------------------------------------------------ end of the segment: sums, output
       more = next_segment(p, tab, f, end, p.RB, next);  // under the last value product
-      if (more) next_masks = masks_of(next);
+      if (more) next_mask = mask_of(next);
       xchg[grp * kTile + row] = l;
       named_bar_sync(1 + wq, 64);
       const float sum = xchg[row] + xchg[kTile + row];
       named_bar_sync(1 + wq, 64);
-      const bool whole = s.n == s.nt, real = masks.row != 0 && sum != 0.0f;
+      const bool whole = s.n == s.nt, real = mask != 0 && sum != 0.0f;
       const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
       if (grp == 0) {
         if (!whole) {
@@ -1198,11 +1258,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
       float* part = p.part + (static_cast<int64_t>(slot) * R + row) * DP;
       guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);
       tc_after_sync();
+      const uint64_t bad =
+          s.j0 + s.n == s.nt ? mask & (static_cast<uint64_t>(noted[1]) << 32 | noted[0]) : 0;
 #pragma unroll 1
       for (int i = grp * (DP / 2); i < (grp + 1) * (DP / 2); i += 16) {
         float o[16];
         tc_ld16(obuf + i, o);
         tc_wait_ld();
+        if (bad) {
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+            if (i + u < a.d) o[u] += noted_values<BF16>(a, s.t, s.kvh, bad, i + u);
+        }
         if (!whole) {
           if (row < R)
 #pragma unroll

@@ -198,8 +198,8 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     on, so its replays and other calls of that stream must not overlap.
 
     fp32 scores, softmax and sums; one rounding at the output (and one of each unnormalised
-    probability to the inputs' type before its product with V). Repeated calls give the same
-    bits. Returns ``out``, or ``(out, scores_out, draft_scores)`` with ``scores``.
+    probability to the inputs' type before its product with V). Values that are not finite
+    reach only the nodes that see their row. Repeated calls give the same bits. Returns ``out``, or ``(out, scores_out, draft_scores)`` with ``scores``.
     """
     t = _torch()
     try:

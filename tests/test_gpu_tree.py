@@ -163,6 +163,38 @@ def test_rows_that_no_node_sees_do_not_matter(cuda, shape, stale):
     check(inputs(cuda, *shape, seed=3, padded=True, stale=stale), weights=True)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("T,m,H,Hkv,d,lens,Lmax", [(2, 7, 4, 2, 128, [40, 300], 300), (2, 40, 8, 2, 64, [0, 1500], 1500),
+                                                   (2, 5, 4, 2, 33, [40, 200], 200), (2, 9, 2, 2, 96, [9, 2600], 2600)])
+def test_values_that_are_not_finite_reach_only_who_sees_them(cuda, T, m, H, Hkv, d, lens, Lmax, bad, dtype):
+    """One value of one drafted row (and, in another run, one of its key's): the nodes that
+    see the row get NaN or the infinity there, every other output is what it was."""
+    import torch
+    from moat_b200.tree import tree_attention
+    x = inputs(cuda, T, m, H, Hkv, d, lens, Lmax, dtype=dtype, seed=m)
+    node, c = m // 3, d - 3
+    sees = ((x["masks"] >> node) & 1).bool()  # [T, m]
+    assert bool(sees.any()) and not bool(sees.all())
+    clean = tree_attention(**x)
+    v = x["v_draft"].clone()
+    v[:, node, :, c] = bad
+    got = tree_attention(**{**x, "v_draft": v})
+    assert not bool(torch.isfinite(got[sees][..., c]).any())
+    if not math.isnan(bad):
+        assert bool((got[sees][..., c] == bad).all())
+    rest = torch.ones(got.shape, dtype=torch.bool, device=cuda)
+    rest[..., c] = ~sees.unsqueeze(-1)
+    assert torch.equal(got[rest], clean[rest])
+    k = x["k_draft"].clone()
+    k[:, node, :, c] = float("nan")
+    scores = torch.zeros((T, Hkv, Lmax), device=cuda)
+    got, so, ds = tree_attention(**{**x, "k_draft": k}, scores=scores)
+    assert bool(torch.isnan(got[sees]).all())
+    ref, tol = reference(x)[:2]  # a row's rounding may depend on the others' maxima
+    assert bool(((got.double() - ref).abs()[~sees] <= tol[~sees]).all())
+
+
 def test_lengths_out_of_range_are_clamped(cuda):
     x = inputs(cuda, 3, 2, 4, 2, 64, [-5, 70, 64], 64, seed=4)
     check(x, weights=True)
