@@ -86,6 +86,9 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 
 template <int CS>
 __device__ __forceinline__ void unit_sync() {
@@ -114,30 +117,38 @@ __device__ __forceinline__ int ranks_before(uint32_t* word, uint32_t rank, int* 
 }
 
 constexpr int kBins = 2048;  // most bins of a histogram
+constexpr uint32_t kFewRanks = 128;  // compared with one another, one per thread (no CTA is smaller)
 
 // The digit at which the unit's counts, from the largest digit of `bins` downwards, reach `need`;
-// how many of that digit are still needed and how many there are. Every CTA of the cluster sums
-// all histograms; result[] is its own. Ends with the cluster in step.
+// how many of that digit are still needed and how many there are. Of a cluster every CTA sums its
+// share of the bins over all histograms and leaves the sums with every CTA, in `total` (each CTA
+// reading all histograms, 16 units of 8,277 rows took 65 us in place of 26: remote words are the
+// bound). The histogram may be written again on return.
 template <int CS>
-__device__ __forceinline__ void find_digit(const uint32_t* hist, int bins, int need, uint32_t* wsum, int* result) {
+__device__ __forceinline__ void find_digit(const uint32_t* hist, uint32_t* total, int bins, int need, uint32_t* wsum,
+                                           int* result) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unit_sync<CS>();
+  if (CS > 1) {
+    const int share = bins / CS, from = static_cast<int>(cluster_ctarank()) * share;
+    for (int i = from + tid; i < from + share; i += blockDim.x) {
+      uint32_t x = 0;
+#pragma unroll
+      for (uint32_t r = 0; r < CS; ++r) x += ld_cluster_u32(mapa_shared(smem_u32(hist + i), r));
+#pragma unroll
+      for (uint32_t r = 0; r < CS; ++r) st_cluster_u32(mapa_shared(smem_u32(total + i), r), x);
+    }
+    unit_sync<CS>();
+  }
+  const uint32_t* sums = CS > 1 ? total : hist;
   const int per = (bins + blockDim.x - 1) / blockDim.x;  // bins of this thread, from the top: at most 16
   const int top = bins - 1 - tid * per;
-  unit_sync<CS>();
   uint32_t bin[16];
   int sum = 0;
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
-    bin[u] = 0;
-    if (u < per && top - u >= 0) {
-      if (CS == 1) {
-        bin[u] = hist[top - u];
-      } else {
-#pragma unroll
-        for (uint32_t r = 0; r < CS; ++r) bin[u] += ld_cluster_u32(mapa_shared(smem_u32(hist + top - u), r));
-      }
-      sum += bin[u];
-    }
+    bin[u] = u < per && top - u >= 0 ? sums[top - u] : 0u;
+    sum += bin[u];
   }
   int upto = sum;
 #pragma unroll
@@ -163,10 +174,33 @@ __device__ __forceinline__ void find_digit(const uint32_t* hist, int bins, int n
     result[1] = left;
     result[2] = count;
   }
-  unit_sync<CS>();  // and every CTA has read the histograms
+  __syncthreads();
 }
 
-// The same for the last `bits` bits of at most 32 kPer ranks that share the bits above, by one warp:
+// The same for n <= blockDim.x ranks: every thread counts those above its own.
+__device__ __forceinline__ void count_above(const uint32_t* cand, int n, int need, int* result) {
+  if (static_cast<int>(threadIdx.x) >= n) return;
+  const uint32_t mine = cand[threadIdx.x];
+  int larger = 0, equal = 0;
+  const uint4* c4 = reinterpret_cast<const uint4*>(cand);
+#pragma unroll 4
+  for (int i = 0; i < n / 4; ++i) {
+    const uint4 c = c4[i];
+    larger += (c.x > mine) + (c.y > mine) + (c.z > mine) + (c.w > mine);
+    equal += (c.x == mine) + (c.y == mine) + (c.z == mine) + (c.w == mine);
+  }
+  for (int i = n & ~3; i < n; ++i) {
+    larger += cand[i] > mine;
+    equal += cand[i] == mine;
+  }
+  if (larger < need && need <= larger + equal) {  // threads of one rank
+    result[0] = static_cast<int>(mine);
+    result[1] = need - larger;
+    result[2] = equal;
+  }
+}
+
+// And for the last `bits` bits of at most 32 kPer ranks that share the bits above, by one warp:
 // the ranks in registers, the answer (the whole rank) bit by bit.
 template <int kPer>
 __device__ __forceinline__ void finish_in_warp(const uint32_t* cand, int n, uint32_t above, int bits, int need, int lane,
@@ -198,14 +232,17 @@ __device__ __forceinline__ void finish_in_warp(const uint32_t* cand, int n, uint
 // rows. Bound by instructions per row where few units share the GPU: scores and positions are
 // read once, their ranks stay in shared memory; the kept-th largest rank is found from three
 // histograms (joined through distributed shared memory), the second and third of only the rows
-// whose first digit is the threshold's (in one warp where they are few); every warp sweeps its own run of rows, so that holes and
-// movers (and ties, where not all of them stay) are numbered in row order with one exchange of
-// counts. FUSED (CS = 1): the same CTA moves the rows; otherwise the numbered moves go to the
-// workspace for k_evict_move.
+// whose first digit is the threshold's (FUSED: those are compared directly where they are few);
+// every warp sweeps its own run of rows, so that holes and movers (and ties, where not all of them
+// stay) are numbered in row order with one exchange of counts. FUSED (CS = 1): the same CTA moves
+// the rows; otherwise the numbered moves go to the workspace for k_evict_move.
+// Measured: 4 units of 300 rows 8.3 us, all latency; 6,144 units of 600 to 760 rows of 128, of which 512
+// stay, 158 us (90 % of the bytes' time at 6.44 TB/s); 64 units of 60,001 to 65,536 rows, of which 32,768
+// stay, 217 us (78 %), 35 of them this kernel.
 template <int CS, bool FUSED>
 __global__ void __launch_bounds__(FUSED ? 512 : 1024) k_evict(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t dyn[];
-  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t hist[kBins], total[CS > 1 ? kBins : 1];
   __shared__ uint32_t wsum[kMaxWarps];
   __shared__ int digit[3];
   __shared__ uint32_t n_cand;
@@ -269,12 +306,20 @@ __global__ void __launch_bounds__(FUSED ? 512 : 1024) k_evict(const __grid_const
       atomicAdd(&hist[c >> kLow], 1u);
     }
   }
-  find_digit<CS>(hist, kFirst, kept, wsum, digit);
-  const uint32_t first = digit[0];
-  int need = digit[1];
-  uint32_t limit = 0;  // the kept-th largest rank
-  bool found = false;
-  if (FUSED) {  // few rows: those of this digit are usually few enough for one warp
+  uint32_t first = 0, limit = 0;  // the threshold's first digit; the kept-th largest rank
+  int need = kept;
+  bool found = FUSED && n <= static_cast<int>(kFewRanks);
+  if (found) {
+    __syncthreads();
+    count_above(code, n, need, digit);
+    __syncthreads();
+    limit = static_cast<uint32_t>(digit[0]);
+  } else {
+    find_digit<CS>(hist, total, kFirst, kept, wsum, digit);
+    first = digit[0];
+    need = digit[1];
+  }
+  if (FUSED && !found) {  // few rows: those of this digit are usually few enough to be compared
     const uint32_t room = a.slice / 4;
 #pragma unroll 4
     for (int i = tid; i < n; i += threads) {
@@ -287,12 +332,10 @@ __global__ void __launch_bounds__(FUSED ? 512 : 1024) k_evict(const __grid_const
     __syncthreads();
     found = n_cand <= min(room, 512u);
     if (found) {
-      if (warp == 0) {
-        if (n_cand <= 64)
-          finish_in_warp<2>(cand, n_cand, first, kLow, need, lane, digit);
-        else
-          finish_in_warp<16>(cand, n_cand, first, kLow, need, lane, digit);
-      }
+      if (n_cand <= kFewRanks)
+        count_above(cand, static_cast<int>(n_cand), need, digit);
+      else if (warp == 0)
+        finish_in_warp<16>(cand, n_cand, first, kLow, need, lane, digit);
       __syncthreads();
       limit = static_cast<uint32_t>(digit[0]);
     }
@@ -312,11 +355,11 @@ __global__ void __launch_bounds__(FUSED ? 512 : 1024) k_evict(const __grid_const
       }
     };
     count_digits(kLow, first, kLow - 11, kBins - 1);
-    find_digit<CS>(hist, kBins, need, wsum, digit);
+    find_digit<CS>(hist, total, kBins, need, wsum, digit);
     const uint32_t upper = first << 11 | static_cast<uint32_t>(digit[0]);
     need = digit[1];
     count_digits(kLow - 11, upper, 0, (1u << (kLow - 11)) - 1);
-    find_digit<CS>(hist, 1 << (kLow - 11), need, wsum, digit);
+    find_digit<CS>(hist, total, 1 << (kLow - 11), need, wsum, digit);
     limit = upper << (kLow - 11) | static_cast<uint32_t>(digit[0]);
   }
   need = digit[1];
@@ -484,12 +527,17 @@ constexpr int kMaxSlice = 48 * 1024;  // ranks of a CTA: 192 KB
 static bool evict_plan(int64_t units, int Lmax, int d, int budget, EvictPlan* pl) {
   pl->cap = budget < Lmax ? std::min(budget, Lmax - budget) : 0;
   // One CTA that also moves its rows, where the units alone fill the GPU or the moves are few
-  // (a second kernel costs more than the moves); its lists lie in shared memory.
+  // (a second kernel costs more than the moves); its lists lie in shared memory. Measured, one /
+  // two kernels: 6,144 units of 760 rows 158 / 246 us, 384 of 4,000 91 / 95, 4 of 300 9.9 / 11.8; but 32 of
+  // 2,000 rows, 976 of 128 moved, 16.0 / 12.5.
   pl->fused = Lmax <= 4096 && (units >= 2 * sm_count() || static_cast<int64_t>(pl->cap) * d <= 32 * 1024);
   pl->cs = 1;
-  if (!pl->fused)  // enough CTAs per unit to use the SMs, slices that fit
+  // Enough CTAs per unit to use the SMs, slices that fit; a cluster's exchanges cost more than they
+  // save for a few thousand rows. Measured, one CTA / a cluster: 16 units of 8,277 rows 20 / 24 us, 17 of
+  // 18,767 32 / 26, 8 of 64,000 49 / 31.
+  if (!pl->fused)
     while (pl->cs < 16 && ((Lmax + pl->cs - 1) / pl->cs > kMaxSlice ||
-                          (pl->cs < 8 && units * pl->cs * 2 <= sm_count() && Lmax / pl->cs > 2048)))
+                          (pl->cs < 8 && units * pl->cs * 2 <= sm_count() && Lmax / pl->cs > 8192)))
       pl->cs *= 2;
   pl->slice = ((Lmax + pl->cs - 1) / pl->cs + 127) & ~127;
   if (pl->slice > kMaxSlice) return false;
@@ -503,7 +551,7 @@ template <int CS, bool FUSED>
 static int launch_select(const EvictArgs& a, const EvictPlan& pl, int64_t units, cudaStream_t st) {
   auto kern = k_evict<CS, FUSED>;
   if (pl.smem > 32 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024) != cudaSuccess) {
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
     (void)cudaGetLastError();
     return MB_ERR_LAUNCH;
   }

@@ -1,29 +1,36 @@
 // Tree attention on the fifth-generation tensor cores (sm_100a).
 //
-// Rows and keys. The queries that read one KV head, nodes x heads of its group, form R <= 128
-// rows (more are cut into row blocks). Keys come in tiles of 128 rows. The score product is
-// taken transposed,
-//   S^T[128 keys, R] = K_tile[128, d] Q^T[d, R],     O^T[d, R] += V_tile^T[d, 128] P^T[128, R],
-// so the 128 TMEM lanes are keys and d, never the few queries: a tile costs tensor time in
-// proportion to R (N of the instruction, in steps of 16), each thread holds one key, and the
-// exponentials of a tile are spread over all threads whatever R is. V needs no transposition:
-// its rows, as TMA brings them, are the M-major operand; P^T is written as the N-major one.
+// The queries that read one KV head, nodes x heads of its group, form R <= 128 rows (more are cut
+// into row blocks); keys come in tiles of 128. Bound by memory where R is small (4 d bytes per key
+// for 4 d R operations); the tensor cores and the exponentials (one per row and key, 16 per cycle
+// and SM) reach the memory's pace near R = 128. Two kernels share one frame:
+//   k_tree_attn_keys (R <= 16) puts the keys on the 128 TMEM lanes,
+//     S^T[keys, R] = K Q^T,  O^T[d, R] += V^T P^T,
+//   so a tile's exponentials are spread over all threads however few rows there are;
+//   k_tree_attn_rows puts the rows there, S[rows, keys] = Q K^T, O[rows, d] += P V, and a thread
+//   has one row. V as TMA brings it is the M-major, or N-major, operand: nothing is transposed.
 //
-// Softmax. A running maximum per row would need a reduction across the key lanes for every
-// tile. Instead a row keeps a reference m_ref and p = 2^(x - m_ref) may grow to 2^8 (harmless
-// for the rounding of p: the precision is relative); only when some x exceeds m_ref + 8 (one
-// vote per tile) are the maxima taken, m_ref raised and O^T and the sums rescaled. Sums are
-// fp32 per thread (key lane), joined once per segment.
+// Softmax. A running maximum would have to be exchanged between threads for every tile. Instead a
+// row keeps a reference m_ref and p = 2^(x - m_ref) may grow to 2^8 (harmless for the rounding of
+// p, whose precision is relative); only when some x exceeds m_ref + 8 (one vote per tile) are the
+// maxima taken, m_ref raised and O and the sums rescaled. Sums and O are fp32; p is rounded once, to
+// the inputs' type, for its product with V.
 //
 // Work. The tiles of all (trace, KV head, row block) units, from the device lengths, form one
-// sequence that is cut evenly among the CTAs (one per SM): unequal lengths, one long trace and
-// many short ones all fill the GPU. A unit inside one CTA is written directly; the pieces of a
-// unit cut between CTAs leave (m_ref, sum, O) in the workspace and k_tree_join adds them in
-// order. No atomics: results repeat bit for bit.
+// sequence that is shared out among one CTA per SM (share_mode): unequal lengths, one long trace and
+// many short ones all fill the GPU. A unit inside one CTA is written directly; the pieces of a cut
+// unit leave (m_ref, sum, O) in the workspace and k_tree_join adds them in order. No atomics:
+// results repeat bit for bit.
 //
-// Each CTA: 4 or 8 softmax warps, a TMA warp that streams K and V tiles through a ring, an MMA
-// warp one score product ahead of the softmax. Every wait is bounded; a wait that gives up
-// sets MB_DEVERR_TIMEOUT and the CTA runs through without waiting.
+// Each CTA: softmax warps, a TMA warp that streams K and V tiles through a ring of up to 8 stages, a
+// warp that issues score products, one tile ahead of the softmax, and one that issues value
+// products. Every wait is bounded; one that gives up sets MB_DEVERR_TIMEOUT and its thread runs
+// through without waiting.
+//
+// Measured on a B200 (calls replayed from a graph; of the 6.44 TB/s of a copy): 16 traces x 16 heads x
+// 4,096 rows of 128: R = 1 82.4 us (6.5 TB/s, all of it), R = 16 84.4 us; 8 KV heads, R = 32 45.0, R = 128
+// 45.8 us (6.0 TB/s); one trace of 130,001 rows, 8 KV heads, R = 4 87 us (6.1 TB/s); 16 traces of 512 to
+// 752 rows, R = 8 22 us (3.9 TB/s: the time to start, end and join, about 8 us, counts).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -33,10 +40,13 @@
 
 namespace mb {
 
-constexpr int kTile = 128;      // keys per tile
-constexpr int kBox = 32;        // rows per TMA box of a unit's last cached tile: no more boxes than it needs
-constexpr int kMaxRows = 128;   // rows of a block
-constexpr int kKeysRows = 16;   // up to this many rows the keys fill the TMEM lanes, above it the rows do
+constexpr int kTile = 128;  // keys per tile
+constexpr int kBox = 32;    // rows per TMA box of a unit's last cached tile: no more boxes than it needs
+constexpr int kMaxRows = 128;  // rows of a block
+// Up to this many rows the keys fill the TMEM lanes, above it the rows do. Measured, keys / rows: 256
+// units of 512 to 752 rows, R = 8 22.2 / 24.0 us; 64 units of 500, R = 8 8.9 / 10.7; R = 16 of 4,096
+// rows 84.4 / 83.0, of head dim 64 20.6 / 22.4.
+constexpr int kKeysRows = 16;
 constexpr int kMaxTraces = 127;  // per launch (the table of their lengths lies in shared memory)
 constexpr int kPanel = kTile * 128;  // bytes of a 64-column panel of a tile (128-byte swizzled rows)
 constexpr float kNoRef = -1e30f;     // m_ref before any visible key
@@ -353,13 +363,13 @@ __device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16,
   fence_proxy_async_smem();
 }
 
-// How the sequence is shared out. Cutting units costs their pieces' way through the workspace and
-// the join, 2 to 8 us; it pays where the longest share of whole units would outlast the memory
-// traffic. A tile takes a CTA p.tile_cycles; the memory needs p.tile_traffic cycles for the tiles
-// of one position in every CTA. Whole units are kept as long as the longest share of them, with
-// kShareFixed cycles for starting and ending, ends before the traffic does. Measured, 16 traces of
-// 4,096 rows of 128: 128 units of 128 / 32 rows 52.7 / 46.5 us whole, 59.9 / 49.1 cut; 256 units of 8
-// rows 85.0 dealt out whole, 87.1 cut; but 256 units of 512 to 752 rows 24.9 whole, 22.0 cut.
+// How the sequence is shared out. Cutting units evenly costs their pieces' way through the workspace
+// and the join, 2 to 12 us; whole units cost idle CTAs at the end, which does not matter while the
+// memory is the bound. A tile takes a CTA p.tile_cycles; the memory needs p.tile_traffic cycles for
+// the tiles of one position in every CTA. Whole units are kept as long as the longest share of them,
+// with kShareFixed cycles for starting and ending, ends before the traffic does. Measured, 16 traces
+// of 4,096 rows of 128: 128 units of 128 / 32 rows 45.8 / 45.0 us whole, 57.4 / 46.9 cut; 256 units of 8
+// rows 83.2 dealt out whole, 87.6 cut; but 256 units of 512 to 752 rows 24.9 whole, 22.0 cut.
 enum class Share { kCut, kWholeUnit, kSnapped };
 constexpr int kShareFixed = 12000;
 
@@ -1641,7 +1651,8 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Caches this short are not cut: a CTA does its whole unit and no join follows.
+// Caches this short are not cut: a CTA does its whole unit and no join follows. Measured: 16 units of
+// 203 rows 6.8 us (8.2 cut), 144 units of 100 to 500 rows 8.8 us (13.7 cut).
 constexpr int kWholeRows = 512;
 
 struct TreePlan {
@@ -1674,7 +1685,9 @@ static bool tree_plan(int T, int m, int H, int Hkv, int Lmax, int d, TreePlan* p
   return pl->nst >= 4;
 }
 
-// Rows whose scores are kept for the weight pass rather than formed again from K.
+// Rows whose scores are kept for the weight pass rather than formed again from K: 8 R bytes of
+// workspace traffic per key instead of 2 d. Measured, 256 units of 4,096 rows of 128: R = 1 90.7 us
+// (123.7 formed again), R = 8 97.8 (125.7), R = 16 114.0 (127.3); head dim 64, R = 16 alike.
 constexpr int kKeptRows = kKeysRows;
 
 size_t tree_mma_workspace(int T, int m, int H, int Hkv, int Lmax, int d, bool with_scores) {
