@@ -647,7 +647,8 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
   float* ref = reinterpret_cast<float*>(misc + kMiscRef);
   uint64_t* rowmask = reinterpret_cast<uint64_t*>(misc + kMiscMask);
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
-  volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);  // drafted rows, see prepare_values
+  // drafted rows, see prepare_values: two segments' (the next one's value warp may be ahead)
+  volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TreeAttnArgs& a = p.a;
@@ -742,7 +743,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
         const int rows = tile_rows(s.len, s.nt, a.m, s.j0 + jj), steps = (rows + 15) / 16;
         guarded_wait(kv_full + st, use & 1, dead, a.err);
         if (rows & 15 || draft)
-          prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted);
+          prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted + 2 * (seg & 1));
         if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
         guarded_wait(p_full, k & 1, dead, a.err);
         tc_after_sync();
@@ -913,7 +914,8 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
       }
       named_bar_sync(1, kSoft);
       const uint32_t ob = tmem + lanes + (2 + (seg & 1)) * kKeysRows;
-      const uint64_t bad = s.j0 + s.n == s.nt ? static_cast<uint64_t>(noted[1]) << 32 | noted[0] : 0;
+      const volatile uint32_t* nt = noted + 2 * (seg & 1);
+      const uint64_t bad = s.j0 + s.n == s.nt ? static_cast<uint64_t>(nt[1]) << 32 | nt[0] : 0;
       int row = 0, nd = 0, gh = 0;  // row, its node, its head of the group
       uint16_t* out = a.out + s.t * a.os[0] + s.kvh * p.G * a.os[2] + key;
       float* part = p.part + static_cast<int64_t>(slot) * R * DP + key;
@@ -1031,7 +1033,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 2);
   float* xchg = reinterpret_cast<float*>(misc + kMiscRef);  // [2][128] between the two warps of a row
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
-  volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);  // drafted rows, see scrub_line
+  volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);  // drafted rows of two segments
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TreeAttnArgs& a = p.a;
@@ -1123,7 +1125,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         const int rows = tile_rows(s.len, s.nt, a.m, s.j0 + jj), steps = (rows + 15) / 16;
         guarded_wait(kv_full + st, use & 1, dead, a.err);
         if (rows & 15 || draft)
-          prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted);
+          prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted + 2 * (seg & 1));
         if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
         guarded_wait(p_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
@@ -1268,8 +1270,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
       float* part = p.part + (static_cast<int64_t>(slot) * R + row) * DP;
       guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);
       tc_after_sync();
-      const uint64_t bad =
-          s.j0 + s.n == s.nt ? mask & (static_cast<uint64_t>(noted[1]) << 32 | noted[0]) : 0;
+      const volatile uint32_t* nt = noted + 2 * (seg & 1);
+      const uint64_t bad = s.j0 + s.n == s.nt ? mask & (static_cast<uint64_t>(nt[1]) << 32 | nt[0]) : 0;
 #pragma unroll 1
       for (int i = grp * (DP / 2); i < (grp + 1) * (DP / 2); i += 16) {
         float o[16];

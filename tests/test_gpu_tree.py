@@ -195,6 +195,25 @@ def test_values_that_are_not_finite_reach_only_who_sees_them(cuda, T, m, H, Hkv,
     assert bool(((got.double() - ref).abs()[~sees] <= tol[~sees]).all())
 
 
+@pytest.mark.parametrize("m,H,Hkv", [(7, 8, 8), (12, 16, 8)])
+def test_values_that_are_not_finite_stay_in_their_trace(cuda, m, H, Hkv):
+    """Many traces without cached rows (one tile each, several per CTA); every other one has a
+    NaN in one drafted row, another row in each."""
+    import torch
+    from moat_b200.tree import tree_attention
+    T, d = 101, 128
+    x = inputs(cuda, T, m, H, Hkv, d, [0] * T, 8, seed=m)
+    clean = tree_attention(**x)
+    v, rest = x["v_draft"].clone(), torch.ones(clean.shape, dtype=torch.bool, device=cuda)
+    for t in range(0, T, 2):
+        v[t, t % m, :, t % d] = float("nan")
+        rest[t, :, :, t % d] = ~((x["masks"][t] >> (t % m)) & 1).bool().unsqueeze(-1)
+    for _ in range(20):
+        got = tree_attention(**{**x, "v_draft": v})
+        assert bool(torch.isnan(got[~rest]).all())
+        assert torch.equal(got[rest], clean[rest])
+
+
 def test_lengths_out_of_range_are_clamped(cuda):
     x = inputs(cuda, 3, 2, 4, 2, 64, [-5, 70, 64], 64, seed=4)
     check(x, weights=True)
