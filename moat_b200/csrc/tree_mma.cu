@@ -328,7 +328,7 @@ __device__ __forceinline__ uint16_t round16(float x) {
   return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
 }
 
-// Shared memory: ring | Q slots | P | barriers and small tables.
+// Shared memory: ring | Q slots | P (rows kernel: outputs on their way) | barriers and small tables.
 struct TreeSmem {
   uint32_t ring, q, p, stage, qslot;  // byte offsets, bytes per stage / slot
   uint32_t misc, total;
@@ -348,7 +348,7 @@ __host__ __device__ inline TreeSmem tree_smem(int panels, int n16, int nst, int 
   s.ring = 0;
   s.q = s.ring + nst * s.stage;
   s.p = s.q + nq * s.qslot;
-  s.misc = s.p + (n16 > kKeysRows ? 0 : kPanel);  // many rows: P lies in TMEM
+  s.misc = s.p + kPanel;
   s.total = s.misc + kMiscBytes;
   return s;
 }
@@ -618,6 +618,21 @@ __device__ __noinline__ float noted_values(const TreeAttnArgs& a, int t, int kvh
       sum += BF16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
   }
   return sum;
+}
+
+// Adds them to columns c0 .. c1 - 1 of an output row, of either form.
+template <bool BF16>
+__device__ __noinline__ void add_noted(const TreeAttnArgs& a, int t, int kvh, uint64_t rows, uint16_t* out, float* part,
+                                       int c0, int c1) {
+  for (int c = c0; c < c1; ++c) {
+    const float v = noted_values<BF16>(a, t, kvh, rows, c);
+    if (v == 0.0f) continue;
+    if (part)
+      part[c] += v;
+    else
+      out[c] = round16<BF16>((BF16 ? __uint_as_float(static_cast<uint32_t>(out[c]) << 16)
+                                   : __half2float(__ushort_as_half(out[c]))) + v);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1150,6 +1165,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     const uint32_t tmem = *tmem_base, lanes = static_cast<uint32_t>(wq * 32) << 16;
     const float sc = a.scale_log2;
     const int my_node = row / p.G, my_head = row - my_node * p.G;
+    auto stage_piece = [&](int r, int q) {  // 16 bytes of row r's line in the warp's 2 KB
+      return reinterpret_cast<uint4*>(smem + lay.p + warp * 2048 + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
+    };
     int seg = 0, k = 0;
     Segment s, next;
     uint64_t mask = 0, next_mask = 0;  // of this row
@@ -1266,8 +1284,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         }
       }
       const float inv = real ? 1.0f / sum : 0.0f;
-      uint16_t* out = a.out + s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + my_head) * a.os[2];
-      float* part = p.part + (static_cast<int64_t>(slot) * R + row) * DP;
+      uint16_t* out =
+          real_row ? a.out + s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + my_head) * a.os[2] : nullptr;
+      float* part = p.part + (static_cast<int64_t>(slot) * R + wq * 32) * DP;  // of the warp's rows
       guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);
       tc_after_sync();
       const volatile uint32_t* nt = noted + 2 * (seg & 1);
@@ -1277,35 +1296,67 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         float o[16];
         tc_ld16(obuf + i, o);
         tc_wait_ld();
-        if (bad) {
-#pragma unroll
-          for (int u = 0; u < 16; ++u)
-            if (i + u < a.d) o[u] += noted_values<BF16>(a, s.t, s.kvh, bad, i + u);
-        }
+        // Through shared memory, so that a store writes 64 bytes of a row, not 16: a line of 64
+        // bytes per row, its pieces swizzled.
         if (!whole) {
-          if (row < R)
 #pragma unroll
-            for (int u = 0; u < 16; u += 4)
-              *reinterpret_cast<float4*>(part + i + u) = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
-        } else if (real_row) {
+          for (int q = 0; q < 4; ++q)
+            *stage_piece(lane, q) = make_uint4(__float_as_uint(o[4 * q]), __float_as_uint(o[4 * q + 1]),
+                                               __float_as_uint(o[4 * q + 2]), __float_as_uint(o[4 * q + 3]));
+          __syncwarp();
+          uint4 y[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) y[u] = *stage_piece(8 * u + (lane >> 2), lane & 3);
+          float* to = part + (lane >> 2) * DP + i + (lane & 3) * 4;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (8 * u + (lane >> 2) < R - wq * 32) *reinterpret_cast<uint4*>(to + 8 * u * DP) = y[u];
+          __syncwarp();
+        } else {
+          const int half = (i >> 4) & 1;  // 32 columns at a time
           uint32_t w[8];
 #pragma unroll
-          for (int u = 0; u < 16; u += 2)
-            w[u / 2] = real ? pack2<BF16>(o[u] * inv, o[u + 1] * inv) : 0u;
+          for (int u = 0; u < 16; u += 2) w[u / 2] = real ? pack2<BF16>(o[u] * inv, o[u + 1] * inv) : 0u;
+          *stage_piece(lane, 2 * half) = make_uint4(w[0], w[1], w[2], w[3]);
+          *stage_piece(lane, 2 * half + 1) = make_uint4(w[4], w[5], w[6], w[7]);
+          if (half) {
+            __syncwarp();
+            const int col = i - 16 + (lane & 3) * 8;  // the head dim is a multiple of 8
+            uint4 y[4];
+            unsigned long long to[4];  // of the four rows, 0 if there is none
 #pragma unroll
-          for (int u = 0; u < 8; u += 4) {  // the head dim is a multiple of 8
-            if (i + 2 * u >= a.d) break;
-            if (p.vec_out) {
-              *reinterpret_cast<uint4*>(out + i + 2 * u) = make_uint4(w[u], w[u + 1], w[u + 2], w[u + 3]);
-            } else {
+            for (int u = 0; u < 4; ++u) {
+              y[u] = *stage_piece(8 * u + (lane >> 2), lane & 3);
+              to[u] = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), 8 * u + (lane >> 2));
+            }
+            if (col < a.d && p.vec_out) {
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                out[i + 2 * (u + v)] = static_cast<uint16_t>(w[u + v]);
-                out[i + 2 * (u + v) + 1] = static_cast<uint16_t>(w[u + v] >> 16);
+              for (int u = 0; u < 4; ++u)
+                if (to[u]) *reinterpret_cast<uint4*>(to[u] + 2 * col) = y[u];
+            } else if (col < a.d) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (!to[u]) continue;
+                uint16_t* o16 = reinterpret_cast<uint16_t*>(to[u]) + col;
+                const uint32_t z[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                  o16[2 * v] = static_cast<uint16_t>(z[v]);
+                  o16[2 * v + 1] = static_cast<uint16_t>(z[v] >> 16);
+                }
               }
             }
+            __syncwarp();
           }
         }
+      }
+      if (__any_sync(0xffffffffu, bad != 0)) {  // rare; after the warp's stores
+        __syncwarp();
+        const int c0 = grp * (DP / 2), c1 = min(a.d, c0 + DP / 2);
+        if (bad && !whole)
+          add_noted<BF16>(a, s.t, s.kvh, bad, nullptr, part + lane * DP, c0, c1);
+        else if (bad && real)
+          add_noted<BF16>(a, s.t, s.kvh, bad, out, nullptr, c0, c1);
       }
       tc_before_sync();
       mbar_arrive(o_empty + (seg & 1));
