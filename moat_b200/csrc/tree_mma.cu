@@ -979,9 +979,15 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
 // A thread then holds 64 scores of one row, so the running reference, the sum and the mask are
 // one register each, the vote for a new maximum concerns the two warps that share a row, and P
 // goes back to TMEM as the A operand of the value product (in the place of the scores, once
-// both warps have read them) instead of through shared memory. With keys on the lanes the same
-// work took 3,500 cycles per tile (tables of references and sums per thread, P and both operand
-// streams through shared memory).
+// both warps have read them) instead of through shared memory. A tile takes 2,000 cycles, so that
+// head dims of 128 run at the memory's pace where a unit is one row block, and head dim 64, or
+// several row blocks per KV head, at the softmax's: 16 traces x 4,096 rows, 8 KV heads, R = 128, head
+// dim 128 / 64 45 / 42 us; 4 traces x 4,096 rows, 4 KV heads, R = 512 34 us. With keys on the lanes the
+// same tile took 3,500 cycles (tables of references and sums per thread, P and both operand streams
+// through shared memory). Two groups of four warps on alternate tiles, 128 scores a thread, came to
+// the same times for long runs of tiles and 10 % longer ones for short units; an eighth or a quarter of
+// the exponentials as polynomials changed nothing or cost 4 %: the exponential unit is not the bound
+// but the chain of a tile's steps (scores from TMEM, maxima, vote, exponentials, P to TMEM).
 // ---------------------------------------------------------------------------
 constexpr int kRowsThreads = 256 + 96;  // softmax, TMA, score products, value products
 
@@ -1296,6 +1302,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         float o[16];
         tc_ld16(obuf + i, o);
         tc_wait_ld();
+        // Through shared memory, so that a store writes 64 bytes of a row, not 16: a line of 64
         // Through shared memory, so that a store writes 64 bytes of a row, not 16: a line of 64
         // bytes per row, its pieces swizzled.
         if (!whole) {
