@@ -443,7 +443,8 @@ int32_t mb_tree_rope(const uint16_t* qkv, int32_t is_bf16, int32_t T, int32_t m,
  * that leaves (K, V, score and position). caches [layers, T, Hkv, Lmax, d], strides[8]:
  * (layer, t, h, l) of k_cache and v_cache; scores / positions [layers, T, Hkv, Lmax], their
  * _out either the same buffers (both) or others, whose rows beyond the kept ones are not
- * written. lens_out [T] (not lens). The workspace needs no initial contents. */
+ * written. lens_out [T] (not lens). Up to 786,432 rows per head (a cluster's shared memory), else
+ * MB_ERR_UNSUPPORTED. The workspace needs no initial contents. */
 size_t mb_cache_evict_workspace_size(int32_t layers, int32_t T, int32_t Hkv, int32_t Lmax, int32_t budget);
 typedef struct {
   uint16_t *k_cache, *v_cache;

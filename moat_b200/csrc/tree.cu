@@ -20,8 +20,13 @@ namespace mb {
 
 // ---------------------------------------------------------------------------
 // What the tensor-core path (tree_mma.cu) does not take: head dims above 128 or no multiple of
-// 8, strides or addresses off 16 bytes, broadcast axes, groups of more than 128 heads. One CTA
-// per (trace, node, head), fp32 online softmax.
+// 8, strides or addresses off 16 bytes, broadcast axes, groups of more than 128 heads. A CTA has
+// eight rows (nodes x heads of a group) of a KV head and a span of its keys, with fp32 online
+// softmax over chunks of 128; spans are joined by k_tree_any_join. A warp's lanes lie along the
+// head dim, four keys at a time, so that any alignment is read in whole lines, and share out the
+// sums of 8 x 4 products by halving. Bound by instructions (two bytes per load, fp32 FMAs). Measured:
+// 16 traces x 16 heads x 2,048 rows of 256, one node / eight nodes over 4 KV heads 744 / 679 us (a key per
+// thread, one row per CTA: 2,630 / 4,850); one trace of 16,000 rows 402 us.
 // ---------------------------------------------------------------------------
 constexpr int kAnyBlock = 128;
 constexpr int kMaxHeadDim = 256;
@@ -45,101 +50,277 @@ __device__ __forceinline__ const uint16_t* tree_row(const uint16_t* cache, const
   return draft + t * ds[0] + (l - len) * ds[1] + kvh * ds[2];
 }
 
-// lse[t, h, i] (log2 units, +inf for a node that sees nothing) is written for the weight pass.
+constexpr int kLaneDims = kMaxHeadDim / 32;
+
+// A row's elements lane, lane + 32, ..., 0 beyond the head dim. Loads without a condition: one
+// in a branch is waited for before the next starts.
 template <bool BF16>
-__global__ void __launch_bounds__(kAnyBlock) k_tree_attn_any(TreeAttnArgs a, float* __restrict__ lse) {
-  __shared__ float qs[kMaxHeadDim];
-  __shared__ float p[kAnyBlock];
-  __shared__ float red[kAnyBlock / 32];
+__device__ __forceinline__ void load_lane_row(float* r, const uint16_t* row, int d, int lane) {
+  uint16_t x[kLaneDims];
+#pragma unroll
+  for (int u = 0; u < kLaneDims; ++u) x[u] = row[min(lane + 32 * u, d - 1)];
+#pragma unroll
+  for (int u = 0; u < kLaneDims; ++u) r[u] = lane + 32 * u < d ? to_f32<BF16>(x[u]) : 0.0f;
+}
+
+__device__ __forceinline__ float lane_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The warp's sum of v[lane]: each step hands over half of the values that are left.
+__device__ __forceinline__ float lane_sums32(float* v, int lane) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float give = lane & o ? v[i] : v[i + o], keep = lane & o ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  return v[0];
+}
+
+constexpr int kAnyRows = 8;
+struct AnySpans {
+  float* part;  // [splits][rows of all units][d] unnormalised outputs, where splits > 1
+  float* ml;    // [splits][rows of all units][2] their maxima (log2 units) and sums
+  float* lse;   // [t, h, i] log2 units, +inf for a node that sees nothing; or null
+  int splits, span, groups;
+};
+
+// Output and lse of row r (node x group + head of the group) of a unit.
+template <bool BF16>
+__device__ __forceinline__ void any_output(const TreeAttnArgs& a, float* lse, int unit, int r, int c, float acc,
+                                           float top, float sum) {
+  const int G = a.H / a.Hkv, t = unit / a.Hkv, i = r / G, h = (unit % a.Hkv) * G + r % G;
+  if (c < a.d)
+    a.out[t * a.os[0] + i * a.os[1] + h * a.os[2] + c] = from_f32<BF16>(sum == 0.0f ? 0.0f : acc / sum);
+  if (lse && c == 0)
+    lse[(static_cast<int64_t>(t) * a.H + h) * a.m + i] = sum == 0.0f ? INFINITY : top + log2f(sum);
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kAnyBlock) k_tree_attn_any(const __grid_constant__ TreeAttnArgs a,
+                                                             const __grid_constant__ AnySpans s) {
+  __shared__ __align__(16) float p[kAnyBlock * kAnyRows];  // [key][row]
+  __shared__ float fade_s[kAnyRows], top_s[kAnyRows], sum_s[kAnyRows];
   pdl_wait();
   pdl_launch_dependents();
-  const int tid = threadIdx.x;
-  const int h = blockIdx.x % a.H, i = (blockIdx.x / a.H) % a.m, t = blockIdx.x / (a.H * a.m);
-  const int kvh = h / (a.H / a.Hkv);
-  const uint64_t mask = a.masks[t * a.mask_stride + i];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = blockIdx.x % s.splits, grp = blockIdx.x / s.splits % s.groups;
+  const int unit = blockIdx.x / (s.splits * s.groups), t = unit / a.Hkv, kvh = unit % a.Hkv;
+  const int G = a.H / a.Hkv, R = a.m * G, r0 = grp * kAnyRows;
   const int len = max(0, min(a.lens[t], a.Lmax));
-  const uint16_t* q = a.q + t * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-  for (int c = tid; c < a.d; c += kAnyBlock) qs[c] = to_f32<BF16>(q[c]) * a.scale_log2;
-  float acc[kMaxHeadDim / kAnyBlock] = {};
-  float top = -INFINITY, sum = 0.0f;
-  const int total = mask ? len + a.m : 0;
-  for (int l0 = 0; l0 < total; l0 += kAnyBlock) {
-    const int l = l0 + tid;
-    float x = -INFINITY;
-    __syncthreads();  // qs written; the previous chunk's p read
-    if (l < total && (l < len || (mask >> (l - len)) & 1)) {
-      const uint16_t* k = tree_row(a.k, a.ks, a.kd, a.kds, t, kvh, len, l);
-      x = 0.0f;
-      for (int c = 0; c < a.d; ++c) x = fmaf(qs[c], to_f32<BF16>(k[c]), x);
+  const int begin = split * s.span, end = min(len + a.m, begin + s.span);
+  float q[kAnyRows][kLaneDims];
+#pragma unroll
+  for (int r = 0; r < kAnyRows; ++r) {
+    const int row = min(r0 + r, R - 1);
+    load_lane_row<BF16>(q[r], a.q + t * a.qs[0] + (row / G) * a.qs[1] + (kvh * G + row % G) * a.qs[2], a.d, lane);
+  }
+  // after the halving a lane has the score of row lane / 4 for one of the four keys
+  const int my_row = r0 + (lane >> 2);
+  const uint64_t mask = my_row < R ? a.masks[t * a.mask_stride + my_row / G] : 0;
+  float acc[kAnyRows][kMaxHeadDim / kAnyBlock] = {};
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {};  // of rows warp and warp + 4
+  for (int l0 = begin; l0 < end; l0 += kAnyBlock) {
+#pragma unroll 1
+    for (int e = 0; e < 32; e += 4) {
+      float k[4][kLaneDims], dot[32];
+      const int key = warp * 32 + e;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        load_lane_row<BF16>(k[u], tree_row(a.k, a.ks, a.kd, a.kds, t, kvh, len, min(l0 + key + u, end - 1)), a.d, lane);
+#pragma unroll
+      for (int r = 0; r < kAnyRows; ++r) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float x = 0.0f;
+#pragma unroll
+          for (int v = 0; v < kLaneDims; ++v) x = fmaf(q[r][v], k[u][v], x);
+          dot[r * 4 + u] = x;
+        }
+      }
+      const float x = lane_sums32(dot, lane) * a.scale_log2;
+      const int at = key + (lane & 3), l = l0 + at;
+      const bool seen = mask != 0 && l < end && (l < len || (mask >> (l - len)) & 1);
+      p[at * kAnyRows + (lane >> 2)] = seen ? x : -INFINITY;
     }
-    float mx = x;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
     __syncthreads();
-    mx = top;
 #pragma unroll
-    for (int w = 0; w < kAnyBlock / 32; ++w) mx = fmaxf(mx, red[w]);
-    const float base = mx == -INFINITY ? 0.0f : mx;  // nothing seen yet: every weight is 0
-    p[tid] = exp2f(x - base);
-    const float fade = exp2f(top - base);
-    top = mx;
+    for (int y = 0; y < 2; ++y) {
+      const int r = warp + 4 * y;
+      float x[4], mx = top[y], all = 0.0f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        x[u] = p[(lane + 32 * u) * kAnyRows + r];
+        mx = fmaxf(mx, x[u]);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float base = mx == -INFINITY ? 0.0f : mx;  // nothing seen yet: every weight is 0
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = exp2f(x[u] - base);
+        p[(lane + 32 * u) * kAnyRows + r] = w;
+        all += w;
+      }
+      const float fade = exp2f(top[y] - base);
+      sum[y] = sum[y] * fade + lane_sum(all);
+      top[y] = mx;
+      if (lane == 0) fade_s[r] = fade;
+    }
     __syncthreads();
-    sum *= fade;
-    const int n = min(kAnyBlock, total - l0);
-    for (int j = 0; j < n; ++j) sum += p[j];
+#pragma unroll
+    for (int r = 0; r < kAnyRows; ++r) {
+#pragma unroll
+      for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) acc[r][u] *= fade_s[r];
+    }
+    const int n = min(kAnyBlock, end - l0);
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      uint16_t v[8][kMaxHeadDim / kAnyBlock];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t* row = tree_row(a.v, a.vs, a.vd, a.vds, t, kvh, len, l0 + min(j0 + e, n - 1));
+#pragma unroll
+        for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) v[e][u] = row[min(tid + u * kAnyBlock, a.d - 1)];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float4 w0 = *reinterpret_cast<const float4*>(p + (j0 + e) * kAnyRows);
+        const float4 w1 = *reinterpret_cast<const float4*>(p + (j0 + e) * kAnyRows + 4);
+        const float w[kAnyRows] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) {
+          const float x = to_f32<BF16>(v[e][u]);
+#pragma unroll
+          for (int r = 0; r < kAnyRows; ++r)  // what a row without weight holds is not used
+            acc[r][u] = fmaf(w[r], w[r] != 0.0f ? x : 0.0f, acc[r][u]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      top_s[warp + 4 * y] = top[y];
+      sum_s[warp + 4 * y] = sum[y];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kAnyRows; ++r) {
+    if (r0 + r >= R) break;
+    const int64_t at = (static_cast<int64_t>(split) * a.T * a.Hkv + unit) * R + r0 + r;
 #pragma unroll
     for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) {
       const int c = tid + u * kAnyBlock;
-      if (c < a.d) {
-        float s = acc[u] * fade;
-        for (int j = 0; j < n; ++j) {
-          const float w = p[j];
-          if (w != 0.0f) s = fmaf(w, to_f32<BF16>(tree_row(a.v, a.vs, a.vd, a.vds, t, kvh, len, l0 + j)[c]), s);
-        }
-        acc[u] = s;
-      }
+      if (s.splits == 1)
+        any_output<BF16>(a, s.lse, unit, r0 + r, c, acc[r][u], top_s[r], sum_s[r]);
+      else if (c < a.d)
+        s.part[at * a.d + c] = acc[r][u];
     }
+    if (s.splits > 1 && tid < 2) s.ml[at * 2 + tid] = tid ? sum_s[r] : top_s[r];
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* o = a.out + t * a.os[0] + i * a.os[1] + h * a.os[2];
-#pragma unroll
-  for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) {
-    const int c = tid + u * kAnyBlock;
-    if (c < a.d) o[c] = from_f32<BF16>(acc[u] * inv);
-  }
-  if (lse && tid == 0) lse[(static_cast<int64_t>(t) * a.H + h) * a.m + i] = sum == 0.0f ? INFINITY : top + log2f(sum);
 }
 
-// Weight of one row: a thread recomputes its row's score against every query of the KV
-// head, in a fixed order (no atomics: the sums repeat bit for bit).
+// One CTA per row of a unit: its spans, in order.
+template <bool BF16>
+__global__ void __launch_bounds__(kAnyBlock) k_tree_any_join(const __grid_constant__ TreeAttnArgs a,
+                                                             const __grid_constant__ AnySpans s) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int R = a.m * (a.H / a.Hkv);
+  const int64_t rows = static_cast<int64_t>(a.T) * a.Hkv * R, at = blockIdx.x;
+  float top = -INFINITY, sum = 0.0f, acc[kMaxHeadDim / kAnyBlock] = {};
+  for (int k = 0; k < s.splits; ++k) top = fmaxf(top, s.ml[(k * rows + at) * 2]);
+  for (int k = 0; k < s.splits; ++k) {
+    const int64_t piece = k * rows + at;
+    const float part = s.ml[piece * 2 + 1];
+    if (part == 0.0f) continue;
+    const float f = exp2f(s.ml[piece * 2] - top);
+    sum += part * f;
+#pragma unroll
+    for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u) {
+      const int c = threadIdx.x + u * kAnyBlock;
+      if (c < a.d) acc[u] += s.part[piece * a.d + c] * f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kMaxHeadDim / kAnyBlock; ++u)
+    any_output<BF16>(a, s.lse, static_cast<int>(at / R), static_cast<int>(at % R), threadIdx.x + u * kAnyBlock, acc[u],
+                     top, sum);
+}
+
+// Weights of the rows, four per warp at a time: their scores against every query of the KV head
+// once more, summed in a fixed order (no atomics: the sums repeat bit for bit).
 template <bool BF16>
 __global__ void __launch_bounds__(kAnyBlock) k_tree_weights_any(TreeAttnArgs a, const float* __restrict__ lse) {
   pdl_wait();
   pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kvh = blockIdx.y % a.Hkv, t = blockIdx.y / a.Hkv;
-  const int len = max(0, min(a.lens[t], a.Lmax));
-  const int l = blockIdx.x * kAnyBlock + threadIdx.x;
-  if (l >= len + a.m) return;
+  const int len = max(0, min(a.lens[t], a.Lmax)), total = len + a.m;
   const int G = a.H / a.Hkv;
-  const uint16_t* k = tree_row(a.k, a.ks, a.kd, a.kds, t, kvh, len, l);
-  float w = 0.0f;
-  for (int i = 0; i < a.m; ++i) {
-    const uint64_t mask = a.masks[t * a.mask_stride + i];
-    if (mask == 0 || (l >= len && !((mask >> (l - len)) & 1))) continue;
-    for (int g = 0; g < G; ++g) {
-      const int h = kvh * G + g;
-      const uint16_t* q = a.q + t * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-      float x = 0.0f;
-      for (int c = 0; c < a.d; ++c) x = fmaf(to_f32<BF16>(q[c]) * a.scale_log2, to_f32<BF16>(k[c]), x);
-      w += exp2f(x - lse[(static_cast<int64_t>(t) * a.H + h) * a.m + i]);
+  const int64_t unit = static_cast<int64_t>(t) * a.Hkv + kvh;
+  const int begin = blockIdx.x * kAnyBlock + warp * 32, end = min(total, begin + 32);
+  for (int l0 = begin; l0 < end; l0 += 4) {
+    float k[4][kLaneDims], w[4] = {};
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      load_lane_row<BF16>(k[u], tree_row(a.k, a.ks, a.kd, a.kds, t, kvh, len, min(l0 + u, end - 1)), a.d, lane);
+    for (int i = 0; i < a.m; ++i) {
+      const uint64_t mask = a.masks[t * a.mask_stride + i];
+      if (mask == 0) continue;
+      for (int g = 0; g < G; ++g) {
+        const int h = kvh * G + g;
+        float q[kLaneDims];
+        load_lane_row<BF16>(q, a.q + t * a.qs[0] + i * a.qs[1] + h * a.qs[2], a.d, lane);
+        const float norm = lse[(static_cast<int64_t>(t) * a.H + h) * a.m + i];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int l = l0 + u;
+          float x = 0.0f;
+#pragma unroll
+          for (int v = 0; v < kLaneDims; ++v) x = fmaf(q[v] * a.scale_log2, k[u][v], x);
+          x = lane_sum(x);
+          if (l < len || (l < total && (mask >> (l - len)) & 1)) w[u] += exp2f(x - norm);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int l = l0 + u;
+      if (l >= end || lane != u) continue;
+      if (l < len)
+        a.scores_out[unit * a.Lmax + l] = (a.scores ? a.scores[unit * a.Lmax + l] : 0.0f) + w[u];
+      else
+        a.draft_scores[unit * a.m + (l - len)] = w[u];
     }
   }
-  const int64_t unit = static_cast<int64_t>(t) * a.Hkv + kvh;
-  if (l < len)
-    a.scores_out[unit * a.Lmax + l] = (a.scores ? a.scores[unit * a.Lmax + l] : 0.0f) + w;
-  else
-    a.draft_scores[unit * a.m + (l - len)] = w;
+}
+
+// Shares the keys of the general path out: about four CTAs per SM, spans of 256 keys or more.
+// Returns the bytes of workspace and, with `spans`, lays them out in `ws`.
+static size_t any_plan(int T, int m, int H, int Hkv, int Lmax, int d, void* ws, AnySpans* spans) {
+  const int R = m * (H / Hkv), groups = (R + kAnyRows - 1) / kAnyRows;
+  const int64_t ctas = static_cast<int64_t>(T) * Hkv * groups, keys = static_cast<int64_t>(Lmax) + m;
+  int64_t splits = std::min<int64_t>(4 * sm_count() / ctas, (keys + 255) / 256);
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+  const int64_t span = ((keys + splits - 1) / splits + kAnyBlock - 1) / kAnyBlock * kAnyBlock;
+  splits = (keys + span - 1) / span;
+  auto bytes = [](size_t n) { return (n * 4 + 255) / 256 * 256; };
+  const size_t rows = static_cast<size_t>(T) * H * m, pieces = splits > 1 ? splits * rows : 0;
+  if (spans) {
+    char* w = static_cast<char*>(ws);
+    *spans = {reinterpret_cast<float*>(w + bytes(rows)), reinterpret_cast<float*>(w + bytes(rows) + bytes(pieces * d)),
+              reinterpret_cast<float*>(w), static_cast<int>(splits), static_cast<int>(span), groups};
+  }
+  return bytes(rows) + bytes(pieces * d) + bytes(pieces * 2);
 }
 
 // ---------------------------------------------------------------------------
@@ -309,8 +490,7 @@ extern "C" {
 size_t mb_tree_attn_workspace_size(int32_t T, int32_t m, int32_t H, int32_t Hkv, int32_t Lmax, int32_t d,
                                    int32_t with_scores) {
   if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim) return 0;
-  return std::max((static_cast<size_t>(T) * H * m * 4 + 255) / 256 * 256,  // lse of the general path
-                  tree_mma_workspace(T, m, H, Hkv, Lmax, d, with_scores != 0));
+  return std::max(any_plan(T, m, H, Hkv, Lmax, d, nullptr, nullptr), tree_mma_workspace(T, m, H, Hkv, Lmax, d, with_scores != 0));
 }
 
 int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
@@ -320,7 +500,7 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
   if ((g->scores_out != nullptr) != (g->draft_scores != nullptr) || (g->scores && !g->scores_out)) return MB_ERR_NULL;
   if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim)
     return MB_ERR_ARGS;
-  if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFFFF00)
+  if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFF0000)
     return MB_ERR_UNSUPPORTED;
   if (!(g->scale - g->scale == 0.0f) || g->is_bf16 < 0 || g->is_bf16 > 1) return MB_ERR_ARGS;
   if (!aligned(g->q, 2) || !aligned(g->k_cache, 2) || !aligned(g->v_cache, 2) || !aligned(g->k_draft, 2) ||
@@ -364,13 +544,21 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
   if (tree_mma_workspace(T, m, H, Hkv, Lmax, d, false) && tree_mma_takes(a))
     return tree_mma_launch(a, bf16, g->workspace, stream);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* lse = a.scores_out ? static_cast<float*>(g->workspace) : nullptr;
-  const int rc = launch_with_pdl(bf16 ? k_tree_attn_any<true> : k_tree_attn_any<false>, dim3(T * m * H),
-                                 dim3(kAnyBlock), 0, st, a, lse);
+  AnySpans sp;
+  any_plan(T, m, H, Hkv, Lmax, d, g->workspace, &sp);
+  const int64_t rows = static_cast<int64_t>(T) * H * m;
+  const float* lse = sp.lse;
+  if (!a.scores_out) sp.lse = nullptr;
+  const int64_t ctas = static_cast<int64_t>(T) * Hkv * sp.groups * sp.splits;
+  if (ctas > 0x7FFFFFFFll) return MB_ERR_UNSUPPORTED;
+  int rc = launch_with_pdl(bf16 ? k_tree_attn_any<true> : k_tree_attn_any<false>, dim3(static_cast<unsigned>(ctas)),
+                           dim3(kAnyBlock), 0, st, a, sp);
+  if (rc == MB_OK && sp.splits > 1)
+    rc = launch_with_pdl(bf16 ? k_tree_any_join<true> : k_tree_any_join<false>, dim3(static_cast<unsigned>(rows)),
+                         dim3(kAnyBlock), 0, st, a, sp);
   if (rc != MB_OK || !a.scores_out) return rc;
   return launch_with_pdl(bf16 ? k_tree_weights_any<true> : k_tree_weights_any<false>,
-                         dim3((Lmax + m + kAnyBlock - 1) / kAnyBlock, T * Hkv), dim3(kAnyBlock), 0, st, a,
-                         static_cast<const float*>(lse));
+                         dim3((Lmax + m + kAnyBlock - 1) / kAnyBlock, T * Hkv), dim3(kAnyBlock), 0, st, a, lse);
 }
 
 int32_t mb_tree_accept(const mb_tree_accept_args* g, void* stream) {

@@ -279,6 +279,21 @@ def test_strides_and_alignment(cuda, d):
     assert got.data_ptr() == out.data_ptr() and bool((out[..., d:] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("T,m,H,Hkv,d,lens,Lmax", [(1, 1, 2, 2, 256, [5000], 5000), (3, 5, 6, 2, 200, [3000, 0, 257], 3001),
+                                                   (2, 3, 2, 1, 1, [600, 511], 600), (2, 2, 150, 1, 64, [300, 128], 300),
+                                                   (1, 64, 4, 1, 77, [1025], 1100)])
+def test_general_path_with_spans_of_the_keys(cuda, T, m, H, Hkv, d, lens, Lmax, dtype):
+    """Head dims and groups that the tensor cores do not take; long caches cut into spans, some
+    of which a short trace leaves empty."""
+    import torch
+    x = inputs(cuda, T, m, H, Hkv, d, lens, Lmax, dtype=dtype, seed=m + d)
+    x["masks"][-1, m // 2] = 0  # a node that sees nothing
+    first = check(x, weights=True)
+    assert torch.equal(first, check(x))
+    assert bool((first[-1, m // 2] == 0).all())
+
+
 def test_one_tree_for_all_traces(cuda):
     import torch
     x = inputs(cuda, 3, 6, 4, 4, 64, [5, 200, 131], 200, seed=9)
