@@ -58,6 +58,7 @@ struct TreeMmaParams {
   float* part;  // [2 * grid][rows][DP] unnormalised O of a unit's pieces
   float* ml;    // [2 * grid][2][kMaxRows] their m_ref and sum
   int join_passes;  // rows of a join CTA, in passes of its threads
+  bool join_by_unit;
   float* lse;   // [units][kMaxRows] log2 of the softmax denominators (weight pass), or null
   float* kept;  // [units][R][kept_len] scores of the cached rows, kept for the weight pass, or null
   float* kept_draft;  // [units][R][64] of the drafted rows
@@ -1375,9 +1376,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   if (warp == 9) tmem_dealloc(*tmem_base, 512);
 }
 
-// Joins the pieces of the units that were cut between CTAs, in order. CTA (x, y) looks at the
-// boundary between attention CTAs x and x + 1: if a unit's first cut lies there, it joins a group
-// of the unit's rows. Where the cuts lie it works out from the lengths, which it may read before
+// Joins the pieces of the units that were cut between CTAs, in order: CTA (x, y) a group of the rows
+// of unit x (join_by_unit) or of the unit whose first cut lies at boundary x between attention CTAs.
+// Where the cuts lie it works out from the lengths, which it may read before
 // the attention has finished (that began only after the kernels that wrote them had), so that one
 // round of loads is left after the wait. One CTA per unit and 8 rows, most with nothing to join,
 // took 6 us after a 17 us attention; notes left by the attention, read after the wait, 1 to 2.5 us
@@ -1395,23 +1396,33 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   const int units = a.Hkv * p.RB;
   if (tid < 32) prefix_tiles(p, tab, tid, units);
   __syncthreads();
-  const int total = tab.cum[p.T], g = min(p.grid, total), c0 = blockIdx.x;
-  if (c0 + 1 >= g || share_mode(p, total, tab.max_span, units * p.T) != Share::kCut) return;
-  const int here = cut(total, c0 + 1, g);
-  int lo = 0, hi = p.T - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (tab.cum[mid] <= here)
-      lo = mid;
-    else
-      hi = mid - 1;
+  const int total = tab.cum[p.T], g = min(p.grid, total);
+  if (share_mode(p, total, tab.max_span, units * p.T) != Share::kCut) return;
+  int lo, u, c0;
+  if (p.join_by_unit) {
+    lo = blockIdx.x / units;
+    u = blockIdx.x - lo * units;
+  } else {
+    c0 = blockIdx.x;
+    if (c0 + 1 >= g) return;
+    const int here = cut(total, c0 + 1, g);
+    lo = 0;
+    int hi = p.T - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tab.cum[mid] <= here)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    u = (here - tab.cum[lo]) / unit_span(trace_tiles(tab.len[lo]));
   }
-  const int nt = trace_tiles(tab.len[lo]), span = unit_span(nt), u = (here - tab.cum[lo]) / span;
-  const int tile0 = tab.cum[lo] + u * span + kUnitCost;
-  // the unit at the boundary began at or after it, or was cut before
-  if (here <= tile0 || tile0 < cut(total, c0, g)) return;
-  // its last piece: the largest c with cut(c) <= the position of its last tile
+  const int nt = trace_tiles(tab.len[lo]), tile0 = tab.cum[lo] + u * unit_span(nt) + kUnitCost;
+  // its first and its last piece: the largest c with cut(c) <= the position of a tile
+  const int first = static_cast<int>((static_cast<int64_t>(tile0 + 1) * g - 1) / total);
   const int c1 = static_cast<int>((static_cast<int64_t>(tile0 + nt) * g - 1) / total);
+  if (first == c1 || (!p.join_by_unit && first != c0)) return;  // whole, or first cut elsewhere
+  c0 = first;
   const int tr = p.t0 + lo, kvh = u / p.RB, rb = u - kvh * p.RB;
   const int R = p.mb * p.G, v = (tid % kLanes) * 4;
   int n = blockIdx.y * p.join_passes * (kJoinBlock / kLanes) + tid / kLanes;
@@ -1826,7 +1837,7 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
                                     : launch_attn_rows<PANELS, BF16>(p, smem, st);
   if (rc != MB_OK || p.whole) return rc;
   const int rows = p.join_passes * kJoinBlock / (PANELS * 16);
-  return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.grid - 1, (p.mb * p.G + rows - 1) / rows), dim3(kJoinBlock),
+  return launch_with_pdl(k_tree_join<PANELS, BF16>, dim3(p.join_by_unit ? p.T * p.a.Hkv * p.RB : p.grid - 1, (p.mb * p.G + rows - 1) / rows), dim3(kJoinBlock),
                          0, st, p);
 }
 
@@ -1904,6 +1915,12 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
     p.t0 = t0;
     p.T = std::min(kMaxTraces, a.T - t0);
     p.whole = a.Lmax <= kWholeRows && p.T * a.Hkv * pl.RB <= pl.grid;
+    // Few units have a join CTA each; more units than boundaries, or so few that their CTAs would all
+    // lie on the first SMs that come free, one per boundary, most with nothing to join. Measured, by
+    // unit / by boundary: 32 units of 128 rows, 16 row groups 35.3 / 38.8 us, 64 units 32.3 / 35.1; but 8
+    // units of 32 rows, 4 row groups 88.8 / 87.1.
+    const int units = p.T * a.Hkv * pl.RB;
+    p.join_by_unit = units < pl.grid && units * groups >= pl.grid / 2;
     int rc;
     if (pl.panels == 2)
       rc = bf16 ? launch_all<2, true>(p, pl.smem, st) : launch_all<2, false>(p, pl.smem, st);
