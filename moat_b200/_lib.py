@@ -1,19 +1,22 @@
 """ctypes binding of the in-tree CUDA library (C ABI in ``include/moat_b200.h``).
 
-There is no CPU fallback: if ``moat_b200/_lib/libmoat_b200.so`` is missing or does
-not load, every accelerated entry point raises. Build it with
+There is no CPU fallback: if ``moat_b200/_lib/libmoat_b200.so`` (or, for the entry points
+that take torch tensors through it, ``moat_bind.so``) is missing or does not load, every accelerated entry point raises. Build it with
 ``python -m moat_b200.build``.
 """
 
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
 import numpy as np
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libmoat_b200.so")
+BIND_PATH = os.path.join(os.path.dirname(LIB_PATH), "moat_bind.so")
 
 _c_i32, _c_i64, _c_sz, _c_f, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float, ctypes.c_void_p
 
@@ -78,6 +81,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_bind = None
 
 
 class MoatError(RuntimeError):
@@ -99,6 +103,28 @@ def lib() -> ctypes.CDLL:
                     fn.restype, fn.argtypes = res, args
                 _lib = handle
     return _lib
+
+
+def bind():
+    """The extension module that takes torch tensors to the drafted-decoding entry points
+    (``csrc/bind.cpp``), loaded once; raises if it has not been built."""
+    global _bind
+    if _bind is None:
+        handle = lib()
+        torch()  # its libraries first
+        with _lock:
+            if _bind is None:
+                if not os.path.exists(BIND_PATH):
+                    raise ImportError(f"moat_b200 binding not built: {BIND_PATH} is missing "
+                                      f"(run `python -m moat_b200.build`)")
+                loader = importlib.machinery.ExtensionFileLoader("moat_bind", BIND_PATH)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader("moat_bind", loader))
+                loader.exec_module(module)
+                module.set_entry_points(*(ctypes.cast(getattr(handle, name), _vp).value for name in (
+                    "mb_tree_attn", "mb_tree_attn_workspace_size", "mb_tree_accept", "mb_cache_evict",
+                    "mb_cache_evict_workspace_size")))
+                _bind = module
+    return _bind
 
 
 def check(rc: int, what: str) -> None:

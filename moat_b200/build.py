@@ -1,4 +1,5 @@
-"""Build recipe for the in-tree CUDA library ``moat_b200/_lib/libmoat_b200.so``.
+"""Build recipe for the in-tree CUDA library ``moat_b200/_lib/libmoat_b200.so`` and the
+extension module ``moat_bind.so`` beside it (``csrc/bind.cpp``, against the installed torch).
 
 Compiles every ``moat_b200/csrc/*.cu`` for sm_100a only (B200), in parallel, and links
 one shared library with the C ABI declared in ``include/moat_b200.h``. nvcc
@@ -20,6 +21,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIBDIR, "libmoat_b200.so")
+BIND = os.path.join(LIBDIR, "moat_bind.so")
 OBJDIR = os.path.join(ROOT, "_build", "obj")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -52,7 +54,8 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
-    """Compile the CUDA sources into the in-tree shared library; returns its path."""
+    """Compile the CUDA sources into the in-tree shared library, and the binding; returns its path."""
+    build_bind(force)
     srcs = sources()
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")]
     deps.append(os.path.join(ROOT, "include", "moat_b200.h"))
@@ -71,6 +74,31 @@ def build(verbose: bool = False, force: bool = False) -> str:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
     return LIB
+
+
+def build_bind(force: bool = False) -> str:
+    """Compile the extension module; returns its path."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "bind.cpp")
+    deps = [src, os.path.join(ROOT, "include", "moat_b200.h"), torch.__file__]
+    if not force and os.path.exists(BIND) and all(os.path.getmtime(d) <= os.path.getmtime(BIND) for d in deps):
+        return BIND
+    os.makedirs(LIBDIR, exist_ok=True)
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    tmp = BIND + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(home, "include"), "-I", sysconfig.get_paths()["include"],
+           "-I", os.path.join(cuda, "include"), src, "-o", tmp, "-L", os.path.join(home, "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {src}:\n{r.stderr}")
+    os.replace(tmp, BIND)
+    return BIND
 
 
 if __name__ == "__main__":

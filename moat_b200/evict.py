@@ -11,14 +11,8 @@ The reference keeps every row until its cache overflows (``batch_generator.py:79
 
 from __future__ import annotations
 
-import struct
-
-from ._lib import check, lib
-from .tree import _device_index, _five, _on, _on_device, _plain, _rows, _torch, _Workspaces
-
-_ws = _Workspaces()
-_sizes = {}  # workspace bytes by geometry
-_Args = struct.Struct("@10PN8q8i")  # the C struct mb_cache_evict_args
+from . import _lib
+from .tree import _device_index, _done, _five, _on_device, _plain, _rows, _torch
 
 
 def _check_evict(k_cache, v_cache, scores, positions, lens, next_pos, scores_out, positions_out):
@@ -63,55 +57,14 @@ def evict_cache(k_cache, v_cache, scores, positions, lens, next_pos, budget: int
 
     Returns ``(scores_out, positions_out, new_lens)``.
     """
-    t = _torch()
     scores_out = scores if scores_out is None else scores_out
     positions_out = positions if positions_out is None else positions_out
-    try:
-        idx = k_cache.get_device()
-        full, dt, i32, f32 = tuple(k_cache.shape), k_cache.dtype, t.int32, t.float32
-        layers = full[0] if len(full) == 5 else 1
-        T, Hkv, Lmax, d = full[-4:]
-        rows, one = full[:-1], (T,)
-        sk, sv = k_cache.stride(), v_cache.stride()
-        fine = (idx >= 0 and idx == v_cache.get_device() == scores.get_device() == positions.get_device()
-                == lens.get_device() == next_pos.get_device() == scores_out.get_device() == positions_out.get_device()
-                and 4 <= len(full) <= 5 and min(full) >= 1 and v_cache.shape == full and dt is v_cache.dtype
-                and dt.itemsize == 2 and (sk[-1] == sv[-1] == 1 or d == 1)
-                and f32 is scores.dtype is scores_out.dtype
-                and i32 is positions.dtype is positions_out.dtype is lens.dtype is next_pos.dtype
-                and scores.shape == rows and scores_out.shape == rows and positions.shape == rows
-                and positions_out.shape == rows and lens.shape == one and next_pos.shape == one
-                and scores.is_contiguous() and scores_out.is_contiguous() and positions.is_contiguous()
-                and positions_out.is_contiguous() and lens.is_contiguous() and next_pos.is_contiguous())
-    except (AttributeError, ValueError, IndexError):
-        fine = False
-    if not fine:
-        _check_evict(k_cache, v_cache, scores, positions, lens, next_pos, scores_out, positions_out)
-    budget, recent, sinks = int(budget), int(recent), int(sinks)
-    if not (budget >= 1 and recent >= 0 and sinks >= 0 and recent + sinks <= budget):
-        raise ValueError("budget must be positive and hold the recent rows and the sinks")
-    ps, pp, pso, ppo = scores.data_ptr(), positions.data_ptr(), scores_out.data_ptr(), positions_out.data_ptr()
-    if (pso == ps) != (ppo == pp):
-        raise ValueError("scores and positions are both updated in place, or neither")
-    new_lens = t.empty_like(lens)
-    L = lib()
-    geometry = (layers, T, Hkv, Lmax, budget)
-    nbytes = _sizes.get(geometry)
-    if nbytes is None:
-        nbytes = _sizes[geometry] = int(L.mb_cache_evict_workspace_size(*geometry))
-    lead = () if len(full) == 5 else (0,)
-
-    def call(st):
-        ws = _ws.get(idx, st, nbytes)
-        return L.mb_cache_evict(_Args.pack(
-            k_cache.data_ptr(), v_cache.data_ptr(), ps, pp, pso, ppo, lens.data_ptr(), next_pos.data_ptr(),
-            new_lens.data_ptr(), ws[0], ws[1], *lead, *sk[:-1], *lead, *sv[:-1], layers, T, Hkv, Lmax, d, budget, recent,
-            sinks), st)
-
-    rc = _on(idx, call)
-    if rc != 0:
-        check(rc, "mb_cache_evict")
-    return scores_out, positions_out, new_lens
+    r = _lib.bind().evict(k_cache, v_cache, scores, positions, lens, next_pos, scores_out, positions_out, int(budget),
+                          int(recent), int(sinks))
+    if r is None or type(r) is int:
+        _done(r, "mb_cache_evict", _check_evict, k_cache, v_cache, scores, positions, lens, next_pos, scores_out,
+              positions_out)
+    return r
 
 
 __all__ = ["evict_cache"]

@@ -17,14 +17,12 @@ it also keeps the accumulated attention weight of every cached row, which
 
 from __future__ import annotations
 
-import math
-import struct
 from typing import NamedTuple
 
 import numpy as np
 
 from . import _lib
-from ._lib import check, lib, stream_of
+from ._lib import check
 
 MAX_NODES = 64  # one bit per node in a mask
 
@@ -60,9 +58,8 @@ def tree_depths(parents) -> np.ndarray:
 
 
 # ---------------------------------------------------------------------------
-# Arguments. Each entry point makes one pass of cheap tests over its tensors; only when
-# one of them fails does a second, slower pass find out which and say so. (Checks that
-# named every tensor took 10 us of host time per call, more than many of the kernels.)
+# Arguments. The binding (csrc/bind.cpp) tests all of a call's tensors; only where one does
+# not fit does a second, slower pass here find out which and say so.
 # ---------------------------------------------------------------------------
 def _device_index(x, name: str) -> int:
     """Index of the CUDA device a tensor lies on."""
@@ -94,36 +91,6 @@ def _rows(dtype, what: str, *tensors) -> None:
             raise ValueError(what)
 
 
-class _Workspaces:
-    """Scratch per (device, stream), grown as needed; the kernels expect no initial contents,
-    and calls that share a buffer are ordered by their stream. A buffer that was outgrown is
-    kept: a captured graph may still use it."""
-
-    def __init__(self):
-        self._bufs, self._outgrown = {}, []
-
-    def get(self, idx: int, stream: int, nbytes: int):
-        """(address, bytes)"""
-        have = self._bufs.get((idx, stream))
-        if have is None or have[1] < nbytes:
-            t = _lib.torch()
-            if have is not None:
-                self._outgrown.append(have)
-                nbytes = max(nbytes, 2 * have[1])
-            buf = t.empty(max(nbytes, 1 << 20), dtype=t.uint8, device=t.device("cuda", idx))
-            have = self._bufs[(idx, stream)] = (buf.data_ptr(), buf.numel(), buf)
-        return have
-
-
-def _on(idx: int, call):
-    """``call(stream)`` with device ``idx`` current."""
-    t = _torch()
-    if idx == t._C._cuda_getDevice():
-        return call(stream_of(idx))
-    with t.cuda.device(idx):
-        return call(stream_of(idx))
-
-
 _modules = []
 
 
@@ -133,15 +100,22 @@ def _torch():
     return _modules[0]
 
 
-_ws = _Workspaces()
-_sizes = {}  # workspace bytes by geometry
-# the C structs mb_tree_attn_args and mb_tree_accept_args
-_AttnArgs = struct.Struct("@13PN18q8if")
-_AcceptArgs = struct.Struct("@18P16q7i")
+def _done(result, entry: str, explain, *args):
+    """The result of a call through the binding: a status is an error, None means that an
+    argument does not fit, which ``explain(*args)`` says."""
+    if result is None:
+        explain(*args)
+        raise ValueError(f"arguments of {entry} do not fit")
+    if type(result) is int:
+        check(result, entry)
+    return result
 
 
 def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, scores, scores_out, draft_scores, dev_err):
     t = _torch()
+    out = q if out is None else out
+    if scores is not None:
+        scores_out = scores if scores_out is None else scores_out
     idx = _device_index(q, "q")
     _on_device(idx, k_cache=k_cache, v_cache=v_cache, lens=lens, k_draft=k_draft, v_draft=v_draft, masks=masks, out=out,
                scores=scores, scores_out=scores_out, draft_scores=draft_scores, dev_err=dev_err)
@@ -170,7 +144,8 @@ def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, sc
     if scores is not None:
         _plain(scores, (T, Hkv, Lmax), t.float32, "scores")
         _plain(scores_out, (T, Hkv, Lmax), t.float32, "scores_out")
-        _plain(draft_scores, (T, Hkv, m), t.float32, "draft_scores")
+        if draft_scores is not None:
+            _plain(draft_scores, (T, Hkv, m), t.float32, "draft_scores")
     elif scores_out is not None or draft_scores is not None:
         raise ValueError("scores_out and draft_scores need scores")
 
@@ -201,67 +176,12 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     probability to the inputs' type before its product with V). Values that are not finite
     reach only the nodes that see their row. Repeated calls give the same bits. Returns ``out``, or ``(out, scores_out, draft_scores)`` with ``scores``.
     """
-    t = _torch()
-    try:
-        idx = q.get_device()
-        T, m, H, d = rows = q.shape
-        cache, drafts, dt = k_cache.shape, k_draft.shape, q.dtype
-        Hkv, Lmax = cache[1], cache[2]
-        if out is None:
-            out = t.empty_like(q, memory_format=t.contiguous_format)
-        if scores is not None:
-            scores_out = scores if scores_out is None else scores_out
-            if draft_scores is None:
-                draft_scores = t.empty((T, Hkv, m), dtype=t.float32, device=q.device)
-        sq, sk, sv = q.stride(), k_cache.stride(), v_cache.stride()
-        skd, svd, so = k_draft.stride(), v_draft.stride(), out.stride()
-        fine = (idx >= 0 and idx == k_cache.get_device() == v_cache.get_device() == lens.get_device()
-                == k_draft.get_device() == v_draft.get_device() == masks.get_device() == out.get_device()
-                and 1 <= m <= MAX_NODES and T >= 1 and Hkv >= 1 and H >= 1 and H % Hkv == 0 and 1 <= d <= 256
-                and len(cache) == 4 and cache[0] == T and cache[3] == d and v_cache.shape == cache
-                and drafts == (T, m, Hkv, d) and v_draft.shape == drafts and out.shape == rows
-                and (dt is t.float16 or dt is t.bfloat16)
-                and dt is k_cache.dtype is v_cache.dtype is k_draft.dtype is v_draft.dtype is out.dtype
-                and (sq[3] == sk[3] == sv[3] == skd[3] == svd[3] == so[3] == 1 or d == 1)
-                and lens.dtype is t.int32 and lens.shape == (T,) and lens.is_contiguous()
-                and masks.dtype is t.int64 and (masks.shape == (T, m) or masks.shape == (m,))
-                and masks.is_contiguous()
-                and (dev_err is None or dev_err.get_device() == idx))
-        if fine and scores is not None:
-            f32, rows = t.float32, (T, Hkv, Lmax)
-            fine = (idx == scores.get_device() == scores_out.get_device() == draft_scores.get_device()
-                    and f32 is scores.dtype is scores_out.dtype is draft_scores.dtype
-                    and scores.shape == rows and scores_out.shape == rows and draft_scores.shape == (T, Hkv, m)
-                    and scores.is_contiguous() and scores_out.is_contiguous() and draft_scores.is_contiguous())
-        elif fine:
-            fine = scores_out is None and draft_scores is None
-    except (AttributeError, ValueError, IndexError):
-        fine = False
-    if not fine:
-        _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, q if out is None else out, scores,
-                         scores_out, draft_scores, dev_err)
-    sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(sc):
-        raise ValueError("scale must be finite")
-    L = lib()
-    geometry = (T, m, H, Hkv, Lmax, d, scores is not None)
-    nbytes = _sizes.get(geometry)
-    if nbytes is None:
-        nbytes = _sizes[geometry] = int(L.mb_tree_attn_workspace_size(*geometry))
-
-    def call(st):
-        ws = _ws.get(idx, st, nbytes)
-        return L.mb_tree_attn(_AttnArgs.pack(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(), k_draft.data_ptr(),
-            v_draft.data_ptr(), masks.data_ptr(), out.data_ptr(), 0 if scores is None else scores.data_ptr(),
-            0 if scores is None else scores_out.data_ptr(), 0 if scores is None else draft_scores.data_ptr(), ws[0],
-            0 if dev_err is None else dev_err.data_ptr(), ws[1], *sq[:3], *sk[:3], *sv[:3], *skd[:3], *svd[:3],
-            *so[:3], masks.dim() == 1, dt is t.bfloat16, T, m, H, Hkv, Lmax, d, sc), st)
-
-    rc = _on(idx, call)
-    if rc != 0:
-        check(rc, "mb_tree_attn")
-    return out if scores is None else (out, scores_out, draft_scores)
+    r = _lib.bind().attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, scale, out, scores, scores_out,
+                              draft_scores, dev_err)
+    if r is None or type(r) is int:
+        _done(r, "mb_tree_attn", _check_attention, q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, scores,
+              scores_out, draft_scores, dev_err)
+    return r
 
 
 class Accepted(NamedTuple):
@@ -337,57 +257,12 @@ def accept_tree(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_dra
     ``next_pos[t] + j``. A trace without room for its accepted rows keeps its state (count
     0) and sets bit 2 of ``dev_err`` (int32 CUDA tensor, optional). 16-bit element types.
     """
-    t = _torch()
-    try:
-        idx = k_cache.get_device()
-        full, drafts, dt, i32 = tuple(k_cache.shape), tuple(k_draft.shape), k_cache.dtype, t.int32
-        layers = full[0] if len(full) == 5 else 1
-        T, Hkv, Lmax, d = full[-4:]
-        m = drafts[-3]
-        pair, one = (T, m), (T,)
-        sk, sv, skd, svd = k_cache.stride(), v_cache.stride(), k_draft.stride(), v_draft.stride()
-        fine = (idx >= 0 and idx == v_cache.get_device() == k_draft.get_device() == v_draft.get_device()
-                == tokens.get_device() == parents.get_device() == target.get_device() == lens.get_device()
-                == next_pos.get_device()
-                and 1 <= m <= MAX_NODES and 4 <= len(full) <= 5 and min(full) >= 1 and v_cache.shape == full
-                and drafts == (*full[:-3], m, Hkv, d) and v_draft.shape == drafts
-                and dt is v_cache.dtype is k_draft.dtype is v_draft.dtype and dt.itemsize == 2
-                and (sk[-1] == sv[-1] == skd[-1] == svd[-1] == 1 or d == 1)
-                and i32 is tokens.dtype is parents.dtype is target.dtype is lens.dtype is next_pos.dtype
-                and tokens.shape == pair and target.shape == pair and lens.shape == one and next_pos.shape == one
-                and (parents.shape == pair or parents.shape == (m,))
-                and tokens.is_contiguous() and parents.is_contiguous() and target.is_contiguous()
-                and lens.is_contiguous() and next_pos.is_contiguous()
-                and (scores is None) == (draft_scores is None)
-                and (dev_err is None or dev_err.get_device() == idx))
-        if fine and scores is not None:
-            fine = (idx == scores.get_device() == draft_scores.get_device()
-                    and scores.dtype is draft_scores.dtype is t.float32 and scores.shape == full[:-1]
-                    and draft_scores.shape == (*full[:-2], m) and scores.is_contiguous()
-                    and draft_scores.is_contiguous())
-        if fine and positions is not None:
-            fine = (positions.get_device() == idx and positions.dtype is i32 and positions.shape == full[:-1]
-                    and positions.is_contiguous())
-    except (AttributeError, ValueError, IndexError):
-        fine = False
-    if not fine:
-        _check_accept(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, scores, draft_scores,
-                      positions, dev_err)
-    # strides by (layer, trace, head or node, row or head); without a layer axis its stride is not used
-    lead = () if len(full) == 5 else (0,)
-    ints = t.empty(T * (m + 4), dtype=i32, device=k_cache.device)  # one allocation for the five results
-    p0, step = ints.data_ptr(), 4 * T
-    rc = _on(idx, lambda st: lib().mb_tree_accept(_AcceptArgs.pack(
-        tokens.data_ptr(), parents.data_ptr(), target.data_ptr(), lens.data_ptr(), next_pos.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr(),
-        0 if scores is None else scores.data_ptr(), 0 if scores is None else draft_scores.data_ptr(),
-        0 if positions is None else positions.data_ptr(), p0 + 4 * step, p0, p0 + step, p0 + 2 * step, p0 + 3 * step,
-        0 if dev_err is None else dev_err.data_ptr(), *lead, *sk[:-1], *lead, *sv[:-1], *lead, *skd[:-1], *lead,
-        *svd[:-1], parents.dim() == 1, layers, T, m, Hkv, Lmax, d), st))
-    if rc != 0:
-        check(rc, "mb_tree_accept")
-    counts, next_ids, new_lens, new_pos, path = ints.split_with_sizes([T, T, T, T, T * m])
-    return Accepted(path.view(T, m), counts, next_ids, new_lens, new_pos)
+    r = _lib.bind().accept(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, scores,
+                           draft_scores, positions, dev_err)
+    if r is None or type(r) is int:
+        _done(r, "mb_tree_accept", _check_accept, tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft,
+              v_draft, scores, draft_scores, positions, dev_err)
+    return Accepted._make(r)
 
 
 __all__ = ["Accepted", "MAX_NODES", "accept_tree", "tree_attention", "tree_depths", "tree_masks"]

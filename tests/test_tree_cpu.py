@@ -2,6 +2,7 @@
 argument checks of the C entry points (they fail before any CUDA call)."""
 
 import ctypes
+import struct
 
 import numpy as np
 import pytest
@@ -69,11 +70,13 @@ def test_workspace_sizes(L):
 
 
 FAKE, OTHER = 0x10000, 0x20000  # never dereferenced: validation fails first
+# the C structs mb_tree_attn_args, mb_tree_accept_args and mb_cache_evict_args
+_AttnArgs = struct.Struct("@13PN18q8if")
+_AcceptArgs = struct.Struct("@18P16q7i")
+_Args = struct.Struct("@10PN8q8i")
 
 
 def test_attention_entry_checks_its_arguments(L):
-    from moat_b200.tree import _AttnArgs
-
     def attn(q=FAKE, k=FAKE, masks=FAKE, bf16=0, T=1, m=4, H=8, Hkv=2, Lmax=64, d=128, scale=0.1, scores=0,
              scores_out=0, draft=0, ws=FAKE, nbytes=1 << 30):
         return L.mb_tree_attn(_AttnArgs.pack(q, k, FAKE, FAKE, FAKE, FAKE, masks, FAKE, scores, scores_out, draft, ws, 0,
@@ -95,8 +98,6 @@ def test_attention_entry_checks_its_arguments(L):
 
 
 def test_accept_entry_checks_its_arguments(L):
-    from moat_b200.tree import _AcceptArgs
-
     def accept(tokens=FAKE, lens=FAKE, layers=1, T=1, m=4, Hkv=2, Lmax=64, d=128, scores=0, draft=0, lens_out=OTHER,
                pos_out=OTHER):
         return L.mb_tree_accept(_AcceptArgs.pack(tokens, FAKE, FAKE, lens, FAKE, FAKE, FAKE, FAKE, FAKE, scores, draft, 0,
@@ -112,7 +113,6 @@ def test_accept_entry_checks_its_arguments(L):
 
 
 def test_rope_and_evict_entries_check_their_arguments(L):
-    from moat_b200.evict import _Args
     fake = ctypes.c_void_p(FAKE)
     assert L.mb_tree_rope(None, 0, 1, 4, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, None, None) == -1
     assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 127, fake, fake, 0, fake, 64, fake, fake, None, None) == -2
@@ -138,7 +138,6 @@ def test_argument_structs_match_the_header():
     """The packed formats have the size that the compiler gives the structs of the header."""
     import subprocess
     import tempfile
-    from moat_b200 import evict, tree
     src = ('#include <stdio.h>\n#include "moat_b200.h"\nint main(void) { printf("%zu %zu %zu %zu", '
            'sizeof(mb_tree_attn_args), sizeof(mb_tree_accept_args), sizeof(mb_cache_evict_args), '
            'offsetof(mb_tree_attn_args, scale)); return 0; }\n')
@@ -149,8 +148,8 @@ def test_argument_structs_match_the_header():
         root = __file__.rsplit("/", 2)[0]
         subprocess.run(["gcc", "-I", f"{root}/include", c, "-o", exe], check=True)
         sizes = [int(x) for x in subprocess.run([exe], capture_output=True, check=True, text=True).stdout.split()]
-    pad = [-(-s.size // 8) * 8 for s in (tree._AttnArgs, tree._AcceptArgs, evict._Args)]
-    assert sizes[:3] == pad and sizes[3] == tree._AttnArgs.size - 4
+    pad = [-(-s.size // 8) * 8 for s in (_AttnArgs, _AcceptArgs, _Args)]
+    assert sizes[:3] == pad and sizes[3] == _AttnArgs.size - 4
 
 
 def test_lookup_draft():
