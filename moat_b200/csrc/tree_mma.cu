@@ -1041,6 +1041,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   extern __shared__ __align__(1024) uint8_t smem[];
   constexpr int DP = PANELS * 64;
   constexpr int kSoft = 256;
+  constexpr uint32_t kO = 2 * kTile;  // TMEM columns: scores of two tiles, then an O of either half of the keys
   const TreeSmem lay = tree_smem(PANELS, p.n16, p.nst, p.nq);
   uint8_t* misc = smem + lay.misc;
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(misc);
@@ -1048,12 +1049,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
   uint64_t* s_full = kv_empty + kMaxStages;  // [2]
   uint64_t* q_full = s_full + 2;             // [2]
   uint64_t* q_empty = q_full + 2;            // [2]
-  uint64_t* o_empty = q_empty + 2;           // [2]
-  uint64_t* p_full = o_empty + 2;            // [2]
-  uint64_t* pv_done = p_full + 2;            // [2]
+  uint64_t* p_full = q_empty + 2;            // [2 halves][2]
+  uint64_t* pv_done = p_full + 4;            // [2]
+  uint64_t* o_empty = pv_done + 2;
   const TreeBars bars = {kv_full, kv_empty, q_full, q_empty};
-  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(pv_done + 2);
-  float* xchg = reinterpret_cast<float*>(misc + kMiscRef);  // [2][128] between the two warps of a row
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(o_empty + 1);
+  float2* xchg = reinterpret_cast<float2*>(misc + kMiscRef);  // [128] between the two threads of a row
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
   volatile uint32_t* noted = reinterpret_cast<uint32_t*>(misc + kMiscNoted);  // drafted rows of two segments
 
@@ -1073,10 +1074,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         mbar_init(s_full + i, 1);
         mbar_init(q_full + i, 1);
         mbar_init(q_empty + i, 1);
-        mbar_init(o_empty + i, kSoft);
-        mbar_init(p_full + i, kSoft);
+        mbar_init(p_full + i, kSoft / 2);
+        mbar_init(p_full + 2 + i, kSoft / 2);
         mbar_init(pv_done + i, 1);
       }
+      mbar_init(o_empty, kSoft);
       fence_mbar_init();
     }
   } else if (warp == 9) {
@@ -1140,7 +1142,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     int k = 0, seg = 0, st = 1, use = 0;
     Segment s;
     for (int f = beg; next_segment(p, tab, f, end, p.RB, s); ++seg) {
-      const uint32_t o = tmem + (2 + (seg & 1)) * kTile;
       const SegmentMasks masks = load_masks(a, s.t, lane);
       for (int jj = 0; jj < s.n; ++jj, ++k) {
         const bool draft = s.j0 + jj == s.nt - 1;
@@ -1148,16 +1149,23 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         guarded_wait(kv_full + st, use & 1, dead, a.err);
         if (rows & 15 || draft)
           prepare_values<PANELS, BF16>(smem + lay.ring + st * lay.stage, rows, draft, masks, lane, noted + 2 * (seg & 1));
-        if (jj == 0 && seg >= 2) guarded_wait(o_empty + (seg & 1), ((seg >> 1) - 1) & 1, dead, a.err);
-        guarded_wait(p_full + (k & 1), (k >> 1) & 1, dead, a.err);
-        tc_after_sync();
-        if (elect_one()) {
-          const uint32_t va = ring_v + (st * lay.stage >> 4), pa = tmem + (k & 1) * kTile;
+        if (jj == 0 && seg >= 1) guarded_wait(o_empty, (seg - 1) & 1, dead, a.err);
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
-            if (kk < steps) tc_mma_ts(o, pa + kk * 8, va + kk * (2048 >> 4), idesc, jj > 0 || kk > 0);
-          tc_commit(kv_empty + st);
-          tc_commit(pv_done + (k & 1));
+        for (int half = 0; half < 2; ++half) {
+          guarded_wait(p_full + 2 * half + (k & 1), (k >> 1) & 1, dead, a.err);
+          tc_after_sync();
+          if (elect_one()) {
+            const uint32_t va = ring_v + (st * lay.stage >> 4) + half * (8192 >> 4);
+            const uint32_t pa = tmem + (k & 1) * kTile + half * 64, o = tmem + kO + half * DP;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              if (half * 4 + kk < steps) tc_mma_ts(o, pa + kk * 8, va + kk * (2048 >> 4), idesc, jj > 0 || kk > 0);
+            if (half == 1) {
+              tc_commit(kv_empty + st);
+              tc_commit(pv_done + (k & 1));
+            }
+          }
+          __syncwarp();
         }
         __syncwarp();
         next_tile(p.nst, st, use);
@@ -1169,6 +1177,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     const int grp = warp >> 2, wq = warp & 3;
     const int row = wq * 32 + lane;  // this thread's row; keys 64 grp .. 64 grp + 63 of a tile
     const int key0 = 64 * grp;
+    const bool idle = wq * 32 >= R;  // no row of the warp is real
     const uint32_t tmem = *tmem_base, lanes = static_cast<uint32_t>(wq * 32) << 16;
     const float sc = a.scale_log2;
     const int my_node = row / p.G, my_head = row - my_node * p.G;
@@ -1188,7 +1197,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
     for (; more; ++seg, s = next, mask = next_mask) {
       const int node = s.rb * p.mb + my_node;
       const bool real_row = row < R && node < a.m;
-      const uint32_t obuf = tmem + lanes + (2 + (seg & 1)) * kTile;
+      const uint32_t obuf = tmem + lanes + kO;
       float ref = kNoRef, l = 0.0f;
       for (int jj = 0; jj < s.n; ++jj, ++k) {
         const int j = s.j0 + jj;
@@ -1197,6 +1206,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
         const uint32_t sbuf = tmem + lanes + (k & 1) * kTile;
         guarded_wait(s_full + (k & 1), (k >> 1) & 1, dead, a.err);
         tc_after_sync();
+        if (idle || rows <= key0) {  // nothing of this half is used
+          mbar_arrive(p_full + 2 * grp + (k & 1));
+          continue;
+        }
         float x[64];
 #pragma unroll
         for (int i = 0; i < 64; i += 16) tc_ld16(sbuf + key0 + i, x + i);
@@ -1228,28 +1241,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
           for (int u = 0; u < 4; ++u) top[u] = max3(top[u], x[i + u], x[i + u + 4]);
         }
         const float mx = max3(top[0], top[1], fmaxf(top[2], top[3])) * f;
-        tc_before_sync();
-        const bool raise = vote_any(mx > ref + kSlack, 1 + wq, 64);
-        tc_after_sync();  // both warps of the row have read its scores: P may take their place
-        if (raise) {
-          xchg[grp * kTile + row] = mx;
-          if (k > 0) guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);  // O as the last product left it
-          named_bar_sync(1 + wq, 64);
-          const float now = fmaxf(fmaxf(xchg[row], xchg[kTile + row]), ref);
-          named_bar_sync(1 + wq, 64);  // read by both before the next exchange
-          const float fade = ex2(ref - now);
+        if (__any_sync(0xffffffffu, mx > ref + kSlack)) {
+          const float now = fmaxf(mx, ref), fade = ex2(ref - now);
           ref = now;
           l *= fade;
-          if (jj > 0) {  // each of the two warps rescales half of the row's O
+          if (jj > 0) {  // O as the last product left it
+            guarded_wait(pv_done + ((k - 1) & 1), ((k - 1) >> 1) & 1, dead, a.err);
             tc_after_sync();
 #pragma unroll 1
-            for (int i = 0; i < DP / 2; i += 16) {
+            for (int i = 0; i < DP; i += 16) {
               float o[16];
-              tc_ld16(obuf + grp * (DP / 2) + i, o);
+              tc_ld16(obuf + grp * DP + i, o);
               tc_wait_ld();
 #pragma unroll
               for (int u = 0; u < 16; ++u) o[u] *= fade;
-              tc_st16(obuf + grp * (DP / 2) + i, o);
+              tc_st16(obuf + grp * DP + i, o);
             }
           }
         }
@@ -1266,31 +1272,45 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
           pk[i / 2] = pack2<BF16>(e.x, e.y);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        tc_st32(sbuf + 32 * grp, pk);
+        tc_st32(sbuf + key0, pk);  // in the place of this half's scores
         tc_wait_st();
         tc_before_sync();
-        mbar_arrive(p_full + (k & 1));
+        mbar_arrive(p_full + 2 * grp + (k & 1));
       }
       // ------------------------------------------------ end of the segment: sums, output
       more = next_segment(p, tab, f, end, p.RB, next);  // under the last value product
       if (more) next_mask = mask_of(next);
-      xchg[grp * kTile + row] = l;
-      named_bar_sync(1 + wq, 64);
-      const float sum = xchg[row] + xchg[kTile + row];
-      named_bar_sync(1 + wq, 64);
-      const bool whole = s.n == s.nt, real = mask != 0 && sum != 0.0f;
+      // The two halves' parts of a row: the second hands over its reference and sum and gets the
+      // factors for the two O. Without a tile of more than 64 keys nothing valid is in the second's
+      // (such a tile is the segment's first or there is none).
+      const bool has1 = tile_rows(s.len, s.nt, a.m, s.j0) > 64, whole = s.n == s.nt;
       const int slot = 2 * c + (s.j0 > 0 ? 0 : 1);
+      float2 fac;
+      if (grp == 1) xchg[row] = make_float2(ref, l);
+      named_bar_sync(1 + wq, 64);
       if (grp == 0) {
+        const float2 other = xchg[row];
+        const float both = fmaxf(ref, other.x);
+        fac = make_float2(ex2(ref - both), ex2(other.x - both));
+        const float sum = l * fac.x + other.y * fac.y;
+        const bool some = mask != 0 && sum != 0.0f;
         if (!whole) {
           float* ml = p.ml + static_cast<int64_t>(slot) * 2 * kMaxRows;
-          ml[row] = ref;
-          ml[kMaxRows + row] = real ? sum : 0.0f;
-        } else if (p.lse) {
-          const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
-          p.lse[unit * kMaxRows + row] = real ? ref + log2f(sum) : INFINITY;
+          ml[row] = both;
+          ml[kMaxRows + row] = some ? sum : 0.0f;
+        } else {
+          if (p.lse) {
+            const int64_t unit = (static_cast<int64_t>(s.t) * a.Hkv + s.kvh) * p.RB + s.rb;
+            p.lse[unit * kMaxRows + row] = some ? both + log2f(sum) : INFINITY;
+          }
+          const float inv = some ? 1.0f / sum : 0.0f;
+          fac = make_float2(some ? fac.x * inv : -1.0f, fac.y * inv);  // -1: a row without keys
         }
+        xchg[row] = fac;
       }
-      const float inv = real ? 1.0f / sum : 0.0f;
+      named_bar_sync(1 + wq, 64);
+      if (grp == 1) fac = xchg[row];
+      const bool real = !(fac.x < 0.0f);
       uint16_t* out =
           real_row ? a.out + s.t * a.os[0] + node * a.os[1] + (s.kvh * p.G + my_head) * a.os[2] : nullptr;
       float* part = p.part + (static_cast<int64_t>(slot) * R + wq * 32) * DP;  // of the warp's rows
@@ -1300,10 +1320,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
       const uint64_t bad = s.j0 + s.n == s.nt ? mask & (static_cast<uint64_t>(nt[1]) << 32 | nt[0]) : 0;
 #pragma unroll 1
       for (int i = grp * (DP / 2); i < (grp + 1) * (DP / 2); i += 16) {
-        float o[16];
+        float o[16], o1[16];
         tc_ld16(obuf + i, o);
+        tc_ld16(obuf + DP + i, o1);
         tc_wait_ld();
-        // Through shared memory, so that a store writes 64 bytes of a row, not 16: a line of 64
+#pragma unroll
+        for (int u = 0; u < 16; ++u) o[u] = o[u] * fac.x + (has1 ? o1[u] * fac.y : 0.0f);
         // Through shared memory, so that a store writes 64 bytes of a row, not 16: a line of 64
         // bytes per row, its pieces swizzled.
         if (!whole) {
@@ -1324,7 +1346,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
           const int half = (i >> 4) & 1;  // 32 columns at a time
           uint32_t w[8];
 #pragma unroll
-          for (int u = 0; u < 16; u += 2) w[u / 2] = real ? pack2<BF16>(o[u] * inv, o[u + 1] * inv) : 0u;
+          for (int u = 0; u < 16; u += 2) w[u / 2] = real ? pack2<BF16>(o[u], o[u + 1]) : 0u;
           *stage_piece(lane, 2 * half) = make_uint4(w[0], w[1], w[2], w[3]);
           *stage_piece(lane, 2 * half + 1) = make_uint4(w[4], w[5], w[6], w[7]);
           if (half) {
@@ -1367,7 +1389,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) k_tree_attn_rows(const __grid
           add_noted<BF16>(a, s.t, s.kvh, bad, out, nullptr, c0, c1);
       }
       tc_before_sync();
-      mbar_arrive(o_empty + (seg & 1));
+      mbar_arrive(o_empty);
     }
   }
   tc_before_sync();
