@@ -977,18 +977,19 @@ __global__ void __launch_bounds__(kKeysThreads, 1) k_tree_attn_keys(const __grid
 
 // ---------------------------------------------------------------------------
 // More than 16 rows: the rows fill the TMEM lanes (S[128 rows, 128 keys], O[128 rows, d]).
-// A thread then holds 64 scores of one row, so the running reference, the sum and the mask are
-// one register each, the vote for a new maximum concerns the two warps that share a row, and P
-// goes back to TMEM as the A operand of the value product (in the place of the scores, once
-// both warps have read them) instead of through shared memory. A tile takes 2,000 cycles, so that
-// head dims of 128 run at the memory's pace where a unit is one row block, and head dim 64, or
-// several row blocks per KV head, at the softmax's: 16 traces x 4,096 rows, 8 KV heads, R = 128, head
-// dim 128 / 64 45 / 42 us; 4 traces x 4,096 rows, 4 KV heads, R = 512 34 us. With keys on the lanes the
-// same tile took 3,500 cycles (tables of references and sums per thread, P and both operand streams
-// through shared memory). Two groups of four warps on alternate tiles, 128 scores a thread, came to
-// the same times for long runs of tiles and 10 % longer ones for short units; an eighth or a quarter of
-// the exponentials as polynomials changed nothing or cost 4 %: the exponential unit is not the bound
-// but the chain of a tile's steps (scores from TMEM, maxima, vote, exponentials, P to TMEM).
+// A thread holds 64 scores of one row, so the running reference, the sum and the mask are one
+// register each. Either half of a tile's keys belongs to four warps of its own with their own
+// reference, sums and O (added with their factors when the segment ends), so that no warp waits
+// for another within a tile. P goes back to TMEM as the A operand of the value product, in the place
+// of its half's scores, instead of through shared memory. A tile takes 1,800 cycles, so that head
+// dims of 128 run at the memory's pace where a unit is one row block, and head dim 64, or several row
+// blocks per KV head, at the softmax's: 16 traces x 4,096 rows, 8 KV heads, R = 128, head dim 128 / 64
+// 45 / 42 us; 4 traces x 4,096 rows, 4 KV heads, R = 512 31 us. With keys on the lanes the same tile took
+// 3,500 cycles (tables of references and sums per thread, P and both operand streams through shared
+// memory). What did not help: two groups of four warps on alternate tiles, 128 scores a thread (the
+// same times for long runs of tiles, 10 % longer ones for short units); an eighth or a quarter of
+// the exponentials as polynomials (nothing, 4 % longer); turns at the exponentials for the two warps
+// of a row (tiles of 1,480 cycles, the same times).
 // ---------------------------------------------------------------------------
 constexpr int kRowsThreads = 256 + 96;  // softmax, TMA, score products, value products
 
