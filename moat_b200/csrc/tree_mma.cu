@@ -371,15 +371,21 @@ __device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16,
 // with kShareFixed cycles for starting and ending, ends before the traffic does. Measured, 16 traces
 // of 4,096 rows of 128: 128 units of 128 / 32 rows 45.8 / 45.0 us whole, 57.4 / 46.9 cut; 256 units of 8
 // rows 83.2 dealt out whole, 87.6 cut; but 256 units of 512 to 752 rows 24.9 whole, 22.0 cut.
+// Units so short that the longest share of whole ones outlasts the even one by less than a join
+// takes, kJoinCycles, are not cut either. Measured, whole / cut: 128 units of 200 to 300 rows 9.7 / 13.6 us,
+// 256 of them 15.7 / 19.0, 100 units of 300 to 620 rows and 64 query rows 12.9 / 17.8.
 enum class Share { kCut, kWholeUnit, kSnapped };
-constexpr int kShareFixed = 12000;
+constexpr int kShareFixed = 12000, kJoinCycles = 8000;
 
 __device__ __forceinline__ Share share_mode(const TreeMmaParams& p, int64_t total, int64_t max_span, int units) {
   if (p.whole) return Share::kWholeUnit;
   const int64_t traffic = p.tile_traffic * total - static_cast<int64_t>(kShareFixed) * p.grid;  // x grid CTAs
   const int64_t longest = max_span * p.tile_cycles * p.grid;
-  if (units <= p.grid) return longest <= traffic ? Share::kWholeUnit : Share::kCut;
-  return longest + p.tile_cycles * total <= traffic ? Share::kSnapped : Share::kCut;
+  if (units <= p.grid)
+    return longest <= traffic || (max_span - total / p.grid) * p.tile_cycles <= kJoinCycles ? Share::kWholeUnit
+                                                                                            : Share::kCut;
+  return longest + p.tile_cycles * total <= traffic || max_span * p.tile_cycles <= kJoinCycles ? Share::kSnapped
+                                                                                                 : Share::kCut;
 }
 
 // The unit boundary nearest to position f.
