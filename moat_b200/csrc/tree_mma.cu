@@ -373,9 +373,10 @@ __device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16,
 // rows 83.2 dealt out whole, 87.6 cut; but 256 units of 512 to 752 rows 24.9 whole, 22.0 cut.
 // Units so short that the longest share of whole ones outlasts the even one by less than a join
 // takes, kJoinCycles, are not cut either. Measured, whole / cut: 128 units of 200 to 300 rows 9.7 / 13.6 us,
-// 256 of them 15.7 / 19.0, 100 units of 300 to 620 rows and 64 query rows 12.9 / 17.8.
+// 256 of them 15.7 / 19.0, 100 units of 300 to 620 rows and 64 query rows 12.9 / 17.8, 32 units of 500 to 700
+// rows 10.3 / 11.2.
 enum class Share { kCut, kWholeUnit, kSnapped };
-constexpr int kShareFixed = 12000, kJoinCycles = 8000;
+constexpr int kShareFixed = 12000, kJoinCycles = 12000;
 
 __device__ __forceinline__ Share share_mode(const TreeMmaParams& p, int64_t total, int64_t max_span, int units) {
   if (p.whole) return Share::kWholeUnit;
