@@ -369,8 +369,9 @@ __device__ __forceinline__ void zero_query_tail(uint8_t* q, int panels, int n16,
 // memory is the bound. A tile takes a CTA p.tile_cycles; the memory needs p.tile_traffic cycles for
 // the tiles of one position in every CTA. Whole units are kept as long as the longest share of them,
 // with kShareFixed cycles for starting and ending, ends before the traffic does. Measured, 16 traces
-// of 4,096 rows of 128: 128 units of 128 / 32 rows 45.8 / 45.0 us whole, 57.4 / 46.9 cut; 256 units of 8
-// rows 83.2 dealt out whole, 87.6 cut; but 256 units of 512 to 752 rows 24.9 whole, 22.0 cut.
+// of 4,096 rows of 128: 128 units of 128 / 32 rows 47.5 / 45.7 us whole, 55.7 / 47.6 cut; 256 units of 8
+// rows 84.4 dealt out whole, 88.2 cut; 256 units of 512 to 752 rows 22.7 and 22.4; of a few long units
+// only pieces fill the GPU.
 // Units so short that the longest share of whole ones outlasts the even one by less than a join
 // takes, kJoinCycles, are not cut either. Measured, whole / cut: 128 units of 200 to 300 rows 9.7 / 13.6 us,
 // 256 of them 15.7 / 19.0, 100 units of 300 to 620 rows and 64 query rows 12.9 / 17.8, 32 units of 500 to 700
@@ -1752,8 +1753,9 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Caches this short are not cut: a CTA does its whole unit and no join follows. Measured: 16 units of
-// 203 rows 6.8 us (8.2 cut), 144 units of 100 to 500 rows 8.8 us (13.7 cut).
+// Caches this short are not cut, whatever their lengths: a CTA does its whole unit and no join is
+// launched. Measured: 16 units of 203 rows 6.8 us (7.1 with a join that finds nothing to do), 144 units
+// of 100 to 500 rows 9.0 us (9.7).
 constexpr int kWholeRows = 512;
 
 struct TreePlan {
