@@ -1424,18 +1424,23 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   const int tid = threadIdx.x;
   const TreeAttnArgs& a = p.a;
   pdl_launch_dependents();  // the weight pass loads its keys meanwhile
+  // Without a unit to join. What comes after this grid waits for it alone, so it must not complete
+  // before the attention has: its first CTA stays until then (all of them: trees of 63 25.1 us, 24.7 so).
+  auto leave = [] {
+    if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+  };
   const int units = a.Hkv * p.RB;
   if (tid < 32) prefix_tiles(p, tab, tid, units);
   __syncthreads();
   const int total = tab.cum[p.T], g = min(p.grid, total);
-  if (share_mode(p, total, tab.max_span, units * p.T) != Share::kCut) return;
+  if (share_mode(p, total, tab.max_span, units * p.T) != Share::kCut) return leave();
   int lo, u, c0;
   if (p.join_by_unit) {
     lo = blockIdx.x / units;
     u = blockIdx.x - lo * units;
   } else {
     c0 = blockIdx.x;
-    if (c0 + 1 >= g) return;
+    if (c0 + 1 >= g) return leave();
     const int here = cut(total, c0 + 1, g);
     lo = 0;
     int hi = p.T - 1;
@@ -1452,7 +1457,7 @@ __global__ void __launch_bounds__(kJoinBlock) k_tree_join(const __grid_constant_
   // its first and its last piece: the largest c with cut(c) <= the position of a tile
   const int first = static_cast<int>((static_cast<int64_t>(tile0 + 1) * g - 1) / total);
   const int c1 = static_cast<int>((static_cast<int64_t>(tile0 + nt) * g - 1) / total);
-  if (first == c1 || (!p.join_by_unit && first != c0)) return;  // whole, or first cut elsewhere
+  if (first == c1 || (!p.join_by_unit && first != c0)) return leave();  // whole, or first cut elsewhere
   c0 = first;
   const int tr = p.t0 + lo, kvh = u / p.RB, rb = u - kvh * p.RB;
   const int R = p.mb * p.G, v = (tid % kLanes) * 4;
