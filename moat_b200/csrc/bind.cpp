@@ -55,6 +55,9 @@ bool plain(const Tensor* x, ScalarType type, IntArrayRef shape) {
   return x->scalar_type() == type && x->sizes() == shape && x->is_contiguous();
 }
 
+// The device error word: the kernels do 32-bit atomics on its first element.
+bool error_word(const Tensor* x) { return x->scalar_type() == at::kInt && x->numel() > 0; }
+
 bool unit_stride(const Tensor* x) { return x->stride(-1) == 1 || x->size(-1) == 1; }
 
 bool small(IntArrayRef sizes) {
@@ -152,7 +155,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     } else if (args[10] != Py_None || args[11] != Py_None) {
       return none();
     }
-    if (args[12] != Py_None && !dev.add(err = tensor(args[12]))) return none();
+    if (args[12] != Py_None && (!dev.add(err = tensor(args[12])) || !error_word(err))) return none();
     double scale = 1.0 / std::sqrt(static_cast<double>(d));
     if (args[7] != Py_None) {
       scale = PyFloat_AsDouble(args[7]);
@@ -262,7 +265,7 @@ PyObject* accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     if (args[11] != Py_None && (!dev.add(positions = tensor(args[11])) || !plain(positions, at::kInt, rows)))
       return none();
-    if (args[12] != Py_None && !dev.add(err = tensor(args[12]))) return none();
+    if (args[12] != Py_None && (!dev.add(err = tensor(args[12])) || !error_word(err))) return none();
     c10::cuda::OptionalCUDAGuard guard;
     if (c10::cuda::current_device() != dev.index) guard.set_index(dev.index);
     const Tensor all = make({c.T * (m + 4)}, at::kInt, dev.index);  // one allocation for the five results

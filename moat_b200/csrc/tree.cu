@@ -505,7 +505,7 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
   if (!(g->scale - g->scale == 0.0f) || g->is_bf16 < 0 || g->is_bf16 > 1) return MB_ERR_ARGS;
   if (!aligned(g->q, 2) || !aligned(g->k_cache, 2) || !aligned(g->v_cache, 2) || !aligned(g->k_draft, 2) ||
       !aligned(g->v_draft, 2) || !aligned(g->out, 2) || !aligned(g->lens, 4) || !aligned(g->masks, 8) ||
-      !aligned(g->scores, 4) || !aligned(g->scores_out, 4) || !aligned(g->draft_scores, 4))
+      !aligned(g->scores, 4) || !aligned(g->scores_out, 4) || !aligned(g->draft_scores, 4) || !aligned(g->dev_err, 4))
     return MB_ERR_ALIGN;
   if (!g->workspace ||
       g->workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, g->scores_out != nullptr))
@@ -570,6 +570,7 @@ int32_t mb_tree_accept(const mb_tree_accept_args* g, void* stream) {
   if (layers < 1 || T < 1 || m < 1 || m > 64 || Hkv < 1 || g->Lmax < 1 || d < 1) return MB_ERR_ARGS;
   if (g->lens_out == g->lens || g->pos_out == g->next_pos) return MB_ERR_ARGS;  // every CTA reads the old lengths
   if (static_cast<int64_t>(T) * layers > 0x7FFFFFFFll || layers > 65535 || Hkv > 65535) return MB_ERR_UNSUPPORTED;
+  if (!aligned(g->dev_err, 4)) return MB_ERR_ALIGN;
   AcceptArgs a;
   a.tokens = g->tokens;
   a.parents = g->parents;
@@ -619,7 +620,7 @@ int32_t mb_tree_rope(const uint16_t* qkv, int32_t is_bf16, int32_t T, int32_t m,
   if (T < 1 || m < 1 || m > 64 || H < 1 || Hkv < 1 || dh < 2 || dh % 2 != 0 || positions < 1) return MB_ERR_ARGS;
   if (is_bf16 < 0 || is_bf16 > 1) return MB_ERR_ARGS;
   if (T > 65535) return MB_ERR_UNSUPPORTED;
-  if (!aligned(cs, 8)) return MB_ERR_ALIGN;
+  if (!aligned(cs, 8) || !aligned(dev_err, 4)) return MB_ERR_ALIGN;
   return launch_with_pdl(is_bf16 ? k_tree_rope<true> : k_tree_rope<false>, dim3(H + Hkv, m, T), dim3(64), 0,
                          static_cast<cudaStream_t>(stream), qkv, m, H, Hkv, dh, next_pos, depths,
                          static_cast<int64_t>(shared_depths ? 0 : m), reinterpret_cast<const float2*>(cs), positions,

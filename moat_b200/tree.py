@@ -84,6 +84,12 @@ def _plain(x, shape, dtype, name) -> None:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)}")
 
 
+def _error_word(t, x) -> None:
+    """The device error word, if there is one."""
+    if x is not None and (x.dtype is not t.int32 or x.numel() < 1):
+        raise ValueError("dev_err must be an int32 tensor of one word or more")
+
+
 def _rows(dtype, what: str, *tensors) -> None:
     """Tensors of one dtype, contiguous along their last axis."""
     for x in tensors:
@@ -148,6 +154,7 @@ def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, sc
             _plain(draft_scores, (T, Hkv, m), t.float32, "draft_scores")
     elif scores_out is not None or draft_scores is not None:
         raise ValueError("scores_out and draft_scores need scores")
+    _error_word(t, dev_err)
 
 
 def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=None, out=None, scores=None,
@@ -238,6 +245,7 @@ def _check_accept(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_d
         _plain(draft_scores, (*lead, m), t.float32, "draft_scores")
     if positions is not None:
         _plain(positions, (*lead, Lmax), i32, "positions")
+    _error_word(t, dev_err)
 
 
 def accept_tree(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_draft, v_draft, *, scores=None,

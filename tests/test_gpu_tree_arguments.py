@@ -1,0 +1,35 @@
+"""Refusals of drafted decoding's entry points: what a kernel would read or write out of place
+is an error before anything is launched."""
+
+import pytest
+
+from test_gpu_tree import inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def accept_args(cuda, T=2, m=4, Hkv=2, Lmax=16, d=64, layers=3):
+    import torch
+    i = torch.zeros((T, m), dtype=torch.int32, device=cuda)
+    n = torch.zeros(T, dtype=torch.int32, device=cuda)
+    k = torch.zeros((layers, T, Hkv, Lmax, d), dtype=torch.float16, device=cuda)
+    kd = torch.ones((layers, T, m, Hkv, d), dtype=torch.float16, device=cuda)
+    return dict(tokens=i, parents=i, target=i, lens=n, next_pos=n, k_cache=k, v_cache=k.clone(), k_draft=kd,
+                v_draft=kd.clone())
+
+
+def test_an_error_word_is_a_32_bit_word(cuda):
+    """The kernels set its bits with a 32-bit atomic."""
+    import torch
+    from moat_b200.tree import accept_tree, tree_attention
+    x = inputs(cuda, 2, 4, 8, 2, 64, [5, 9], 16, seed=1)
+    a = accept_args(cuda)
+    i32 = torch.zeros(4, dtype=torch.int32, device=cuda)
+    for err in (i32[:0], i32.view(torch.uint8)[1:2], i32.short(), i32.long(), i32.float(), i32.cpu()):
+        with pytest.raises(ValueError, match="dev_err"):
+            tree_attention(**x, dev_err=err)
+        with pytest.raises(ValueError, match="dev_err"):
+            accept_tree(**a, dev_err=err)
+    tree_attention(**x, dev_err=i32[1:])
+    accept_tree(**a, dev_err=i32[1:])
+    assert not bool(i32.any())

@@ -1,0 +1,34 @@
+"""More argument checks of drafted decoding's C entry points: they fail before any CUDA call, so
+the addresses are never looked at."""
+
+import ctypes
+import struct
+
+import pytest
+
+from moat_b200 import _lib
+
+FAKE, OTHER, ODD = 0x10000, 0x20000, 0x30002
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+def attention(L, err=0, strides=(128,) * 18, T=1, m=4, H=8, Hkv=2, Lmax=64, nbytes=1 << 30):
+    """mb_tree_attn_args; without a workspace, a call that passes the checks before it ends with -3."""
+    return L.mb_tree_attn(struct.pack("@13PN18q8if", *[FAKE] * 8, 0, 0, 0, FAKE, err, nbytes, *strides, 0, 0, T, m, H,
+                                      Hkv, Lmax, 128, 0.1), None)
+
+
+def accept(L, err=0, strides=(128,) * 16, layers=1, T=1, Hkv=2, Lmax=64):
+    return L.mb_tree_accept(struct.pack("@18P16q7i", *[FAKE] * 9, 0, 0, 0, FAKE, FAKE, FAKE, OTHER, OTHER, err, *strides,
+                                        0, layers, T, 4, Hkv, Lmax, 128), None)
+
+
+def test_the_error_word_is_aligned(L):
+    assert attention(L, err=ODD) == -5
+    assert accept(L, err=ODD) == -5
+    fake = ctypes.c_void_p(FAKE)
+    assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, ctypes.c_void_p(ODD), None) == -5
