@@ -369,8 +369,9 @@ int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
  * A trace's drafted tokens form a tree of m <= 64 nodes in topological order (node 0 the
  * last chosen token, whose keys are not cached yet). All element types are 16-bit: fp16,
  * or bf16 where is_bf16 = 1. `strides` are HOST arrays of element strides; the head dim is
- * contiguous. Device lengths are clamped to [0, Lmax]. Arguments come as one struct (a call from
- * Python with 30 arguments cost 5 us of host time to convert them).
+ * contiguous; what is read may be broadcast (stride 0), what is written not. Device lengths are
+ * clamped to [0, Lmax]. Arguments come as one struct (a call from Python with 30 arguments cost
+ * 5 us of host time to convert them).
  *
  * mb_tree_attn: exact softmax attention of every node over the lens[t] committed rows of
  * its trace and the nodes in its mask (bit j of masks[t][i]: node i sees node j; a mask of

@@ -60,6 +60,14 @@ bool error_word(const Tensor* x) { return x->scalar_type() == at::kInt && x->num
 
 bool unit_stride(const Tensor* x) { return x->stride(-1) == 1 || x->size(-1) == 1; }
 
+// Every element has a place of its own as far as broadcast axes go: what is written by several CTAs
+// must not share addresses.
+bool no_broadcast(const Tensor* x) {
+  for (int64_t u = 0; u < x->dim(); ++u)
+    if (x->stride(u) == 0 && x->size(u) > 1) return false;
+  return true;
+}
+
 bool small(IntArrayRef sizes) {
   for (int64_t n : sizes)
     if (n > INT_MAX) return false;
@@ -143,7 +151,9 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       return none();
     Tensor made[2];
     const Tensor* out = args[8] == Py_None ? &(made[0] = make(q->sizes(), type, dev.index)) : tensor(args[8]);
-    if (!dev.add(out) || out->sizes() != q->sizes() || out->scalar_type() != type || !unit_stride(out)) return none();
+    if (!dev.add(out) || out->sizes() != q->sizes() || out->scalar_type() != type || !unit_stride(out) ||
+        !no_broadcast(out))
+      return none();
     const Tensor *scores = nullptr, *scores_out = nullptr, *draft_scores = nullptr, *err = nullptr;
     if (args[9] != Py_None) {
       scores = tensor(args[9]);
@@ -213,7 +223,8 @@ struct Cache {
   bool read(const Tensor* k, const Tensor* v) {
     lead = static_cast<int>(k->dim()) - 4;
     if (lead < 0 || lead > 1 || k->numel() == 0 || !small(k->sizes()) || v->sizes() != k->sizes() ||
-        v->scalar_type() != k->scalar_type() || k->element_size() != 2 || !unit_stride(k) || !unit_stride(v))
+        v->scalar_type() != k->scalar_type() || k->element_size() != 2 || !unit_stride(k) || !unit_stride(v) ||
+        !no_broadcast(k) || !no_broadcast(v))  // its rows are written
       return false;
     layers = lead ? k->size(0) : 1;
     T = k->size(lead);

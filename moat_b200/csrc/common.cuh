@@ -31,6 +31,13 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 bool encode_tmap_3d_u8(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides[2],
                        const uint32_t box[3]);
 
+// Whether an axis of a tensor that is written has a stride of 0: several CTAs would write one place.
+inline bool broadcast(const int64_t* strides, const int (&lengths)[3]) {
+  for (int u = 0; u < 3; ++u)
+    if (lengths[u] > 1 && strides[u] == 0) return true;
+  return false;
+}
+
 // Encode a 4-D tiled tensor map of 16-bit elements with 128-byte swizzle (dims inner ->
 // outer, strides of dims 1 to 3 in bytes, box[0] = 64); what lies outside reads as zero.
 // Returns false if the driver rejects the parameters.

@@ -601,6 +601,8 @@ int32_t mb_cache_evict(const mb_cache_evict_args* g, void* stream) {
   if (static_cast<int64_t>(g->recent) + g->sinks > budget) return MB_ERR_ARGS;
   if (g->lens_out == g->lens) return MB_ERR_ARGS;  // every CTA reads the old lengths
   if ((g->scores_out == g->scores) != (g->positions_out == g->positions)) return MB_ERR_ARGS;
+  for (const int64_t* s : {g->strides, g->strides + 4})
+    if ((layers > 1 && s[0] == 0) || broadcast(s + 1, {T, Hkv, Lmax})) return MB_ERR_ARGS;
   const int64_t units = static_cast<int64_t>(layers) * T * Hkv;
   EvictPlan pl;
   if (units > 0x7FFFFFFll || !evict_plan(units, Lmax, d, budget, &pl)) return MB_ERR_UNSUPPORTED;

@@ -502,6 +502,7 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
     return MB_ERR_ARGS;
   if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFF0000)
     return MB_ERR_UNSUPPORTED;
+  if (broadcast(g->strides + 15, {T, m, H})) return MB_ERR_ARGS;
   if (!(g->scale - g->scale == 0.0f) || g->is_bf16 < 0 || g->is_bf16 > 1) return MB_ERR_ARGS;
   if (!aligned(g->q, 2) || !aligned(g->k_cache, 2) || !aligned(g->v_cache, 2) || !aligned(g->k_draft, 2) ||
       !aligned(g->v_draft, 2) || !aligned(g->out, 2) || !aligned(g->lens, 4) || !aligned(g->masks, 8) ||
@@ -569,6 +570,8 @@ int32_t mb_tree_accept(const mb_tree_accept_args* g, void* stream) {
   const int layers = g->layers, T = g->T, m = g->m, Hkv = g->Hkv, d = g->d;
   if (layers < 1 || T < 1 || m < 1 || m > 64 || Hkv < 1 || g->Lmax < 1 || d < 1) return MB_ERR_ARGS;
   if (g->lens_out == g->lens || g->pos_out == g->next_pos) return MB_ERR_ARGS;  // every CTA reads the old lengths
+  for (const int64_t* s : {g->strides, g->strides + 4})
+    if ((layers > 1 && s[0] == 0) || broadcast(s + 1, {T, Hkv, g->Lmax})) return MB_ERR_ARGS;
   if (static_cast<int64_t>(T) * layers > 0x7FFFFFFFll || layers > 65535 || Hkv > 65535) return MB_ERR_UNSUPPORTED;
   if (!aligned(g->dev_err, 4)) return MB_ERR_ALIGN;
   AcceptArgs a;

@@ -12,7 +12,7 @@ The reference keeps every row until its cache overflows (``batch_generator.py:79
 from __future__ import annotations
 
 from . import _lib
-from .tree import _device_index, _done, _five, _on_device, _plain, _rows, _torch
+from .tree import _device_index, _done, _five, _on_device, _own_places, _plain, _rows, _torch
 
 
 def _check_evict(k_cache, v_cache, scores, positions, lens, next_pos, scores_out, positions_out):
@@ -29,6 +29,7 @@ def _check_evict(k_cache, v_cache, scores, positions, lens, next_pos, scores_out
     if kc.element_size() != 2:
         raise ValueError(what)
     _rows(kc.dtype, what, kc, vc)
+    _own_places(k_cache=kc, v_cache=vc)
     full = k_cache.shape[:-1]
     _plain(scores, full, t.float32, "scores")
     _plain(scores_out, full, t.float32, "scores_out")

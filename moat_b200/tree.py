@@ -97,6 +97,13 @@ def _rows(dtype, what: str, *tensors) -> None:
             raise ValueError(what)
 
 
+def _own_places(**tensors) -> None:
+    """Tensors that are written: no broadcast axes."""
+    for name, x in tensors.items():
+        if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+            raise ValueError(f"{name} is written and must not be broadcast along an axis")
+
+
 _modules = []
 
 
@@ -147,6 +154,7 @@ def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, sc
         raise ValueError(f"out must be [{T}, {m}, {H}, {d}]")
     _rows(q.dtype, "q, out, caches and drafts must share one dtype and be contiguous along the head dim", q, k_cache,
           v_cache, k_draft, v_draft, out)
+    _own_places(out=out)
     if scores is not None:
         _plain(scores, (T, Hkv, Lmax), t.float32, "scores")
         _plain(scores_out, (T, Hkv, Lmax), t.float32, "scores_out")
@@ -233,6 +241,7 @@ def _check_accept(tokens, parents, target, lens, next_pos, k_cache, v_cache, k_d
     if kc.element_size() != 2:
         raise ValueError(what)
     _rows(kc.dtype, what, kc, vc, kd, vd)
+    _own_places(k_cache=kc, v_cache=vc)
     i32 = t.int32
     for x, shape, name in ((tokens, (T, m), "tokens"), (target, (T, m), "target"), (lens, (T,), "lens"),
                            (next_pos, (T,), "next_pos"), (parents, (m,) if parents.dim() == 1 else (T, m), "parents")):

@@ -33,3 +33,35 @@ def test_an_error_word_is_a_32_bit_word(cuda):
     tree_attention(**x, dev_err=i32[1:])
     accept_tree(**a, dev_err=i32[1:])
     assert not bool(i32.any())
+
+
+def test_what_is_written_is_not_broadcast(cuda):
+    """Several CTAs would write one place; what is only read may be broadcast."""
+    import torch
+    from moat_b200.evict import evict_cache
+    from moat_b200.tree import accept_tree, tree_attention
+    x = inputs(cuda, 2, 4, 8, 2, 64, [5, 9], 16, seed=1)
+    for axis in range(3):
+        shape = list(x["q"].shape)
+        shape[axis] = 1
+        with pytest.raises(ValueError, match="broadcast"):
+            tree_attention(**x, out=torch.zeros(shape, dtype=torch.float16, device=cuda).expand(x["q"].shape))
+    one = torch.zeros((1, 1, 8, 64), dtype=torch.float16, device=cuda)  # an axis of length 1 may have any stride
+    y = inputs(cuda, 1, 1, 8, 2, 64, [5], 16, seed=1)
+    tree_attention(**y, out=one.as_strided(one.shape, (0, 0, 64, 1)))
+    a = accept_args(cuda)
+    s = torch.zeros((3, 2, 2, 16), device=cuda)
+    p = torch.zeros((3, 2, 2, 16), dtype=torch.int32, device=cuda)
+    for axis in range(4):
+        for name in ("k_cache", "v_cache"):
+            shape = list(a["k_cache"].shape)
+            shape[axis] = 1
+            wide = {name: torch.zeros(shape, dtype=torch.float16, device=cuda).expand(a["k_cache"].shape)}
+            with pytest.raises(ValueError, match="broadcast"):
+                accept_tree(**{**a, **wide})
+            caches = {**{n: a[n] for n in ("k_cache", "v_cache")}, **wide}
+            with pytest.raises(ValueError, match="broadcast"):
+                evict_cache(**caches, scores=s, positions=p, lens=a["lens"], next_pos=a["lens"], budget=8, recent=2)
+    draft = a["k_draft"][:1].expand(a["k_draft"].shape)
+    accept_tree(**{**a, "k_draft": draft, "tokens": a["tokens"] + 1})
+    assert bool((a["k_cache"][:, :, :, 0] == 1).all())

@@ -32,3 +32,23 @@ def test_the_error_word_is_aligned(L):
     assert accept(L, err=ODD) == -5
     fake = ctypes.c_void_p(FAKE)
     assert L.mb_tree_rope(fake, 0, 1, 4, 8, 2, 128, fake, fake, 0, fake, 64, fake, fake, ctypes.c_void_p(ODD), None) == -5
+
+
+def evict(L, strides):
+    return L.mb_cache_evict(struct.pack("@10PN8q8i", *[FAKE] * 4, OTHER, OTHER, FAKE, FAKE, OTHER, 0, 0, *strides, 2, 2,
+                                        2, 64, 128, 32, 8, 4), None)
+
+
+def test_broadcast_strides_of_what_is_written(L):
+    """0 along an axis of more than one element."""
+    def zero(at, n):
+        return [0 if u == at else 128 for u in range(n)]
+    for u in range(15, 18):
+        assert attention(L, strides=zero(u, 18), T=2, nbytes=0) == -2
+    assert attention(L, strides=zero(15, 18), nbytes=0) == -3  # T = 1: the stride is never used
+    for u in range(15):
+        assert attention(L, strides=zero(u, 18), T=2, nbytes=0) == -3  # inputs may be broadcast
+    for u in range(8):
+        assert accept(L, strides=zero(u, 16), layers=2, T=2) == -2
+        assert evict(L, zero(u, 8)) == -2
+    assert evict(L, [128] * 8) == -3
