@@ -378,13 +378,15 @@ int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
  * 0 is padding and gives a zero output):
  *   x_l = scale q_i . k_l, p = softmax(x) (fp32), out_i = sum_l p_l v_l.
  * q / out [T, m, H, d], caches [T, Hkv, Lmax, d], drafts [T, m, Hkv, d]; query head h reads
- * KV head h / (H / Hkv); d <= 256. strides[18]: (t, i, h) of q, (t, h, l) of k_cache and of
- * v_cache, (t, i, h) of k_draft, v_draft and out. masks [T, m], or [m] if shared_masks.
+ * KV head h / (H / Hkv); d <= 256; out overlaps no input (without scores_out it may be q).
+ * strides[18]: (t, i, h) of q, (t, h, l) of k_cache and of v_cache, (t, i, h) of k_draft,
+ * v_draft and out. masks [T, m], or [m] if shared_masks.
  * scores_out (optional, [T, Hkv, Lmax] fp32): row l < lens[t] gets scores[l] (0 if scores
  * is NULL; scores may be scores_out) plus its weight summed over the nodes and heads;
  * draft_scores [T, Hkv, m] the draft rows' sums. No atomics: results repeat bit for bit.
- * The workspace (with_scores = 1 if scores_out is given) needs no initial contents. dev_err (optional) receives MB_DEVERR_TIMEOUT if a
- * bounded wait inside a kernel gives up (the output is then undefined). */
+ * The workspace (with_scores = 1 if scores_out is given) needs no initial contents. dev_err
+ * (optional) receives MB_DEVERR_TIMEOUT if a bounded wait inside a kernel gives up (the output
+ * is then undefined). */
 typedef struct {
   const uint16_t *q, *k_cache, *v_cache;
   const int32_t* lens;

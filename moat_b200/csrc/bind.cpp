@@ -162,6 +162,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (!dev.add(scores, scores_out, draft_scores) || !plain(scores, at::kFloat, {T, Hkv, Lmax}) ||
           !plain(scores_out, at::kFloat, {T, Hkv, Lmax}) || !plain(draft_scores, at::kFloat, {T, Hkv, m}))
         return none();
+      if (out->data_ptr() == q->data_ptr()) return none();  // the weights read q after the outputs are there
     } else if (args[10] != Py_None || args[11] != Py_None) {
       return none();
     }

@@ -503,6 +503,7 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
   if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFF0000)
     return MB_ERR_UNSUPPORTED;
   if (broadcast(g->strides + 15, {T, m, H})) return MB_ERR_ARGS;
+  if (g->draft_scores && g->out == g->q) return MB_ERR_ARGS;  // the weights read q after the outputs are there
   if (!(g->scale - g->scale == 0.0f) || g->is_bf16 < 0 || g->is_bf16 > 1) return MB_ERR_ARGS;
   if (!aligned(g->q, 2) || !aligned(g->k_cache, 2) || !aligned(g->v_cache, 2) || !aligned(g->k_draft, 2) ||
       !aligned(g->v_draft, 2) || !aligned(g->out, 2) || !aligned(g->lens, 4) || !aligned(g->masks, 8) ||

@@ -126,7 +126,7 @@ def _done(result, entry: str, explain, *args):
 
 def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, scores, scores_out, draft_scores, dev_err):
     t = _torch()
-    out = q if out is None else out
+    given, out = out, q if out is None else out
     if scores is not None:
         scores_out = scores if scores_out is None else scores_out
     idx = _device_index(q, "q")
@@ -156,6 +156,8 @@ def _check_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, out, sc
           v_cache, k_draft, v_draft, out)
     _own_places(out=out)
     if scores is not None:
+        if given is not None and out.data_ptr() == q.data_ptr():
+            raise ValueError("with scores, out must not be q")
         _plain(scores, (T, Hkv, Lmax), t.float32, "scores")
         _plain(scores_out, (T, Hkv, Lmax), t.float32, "scores_out")
         if draft_scores is not None:
@@ -175,7 +177,8 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     * ``lens`` int32 ``[T]``, ``masks`` int64 ``[T, m]`` or ``[m]`` (one tree for every
       trace): node ``i`` sees all committed rows and the nodes whose bit is set. A mask of 0
       marks padding: the node sees nothing and its output is 0.
-    * ``out``: optional result ``[T, m, H, d]``; ``scale`` defaults to ``1/sqrt(d)``.
+    * ``out``: optional result ``[T, m, H, d]`` that overlaps no input (without ``scores`` it
+      may be ``q`` itself); ``scale`` defaults to ``1/sqrt(d)``.
     * ``scores`` float32 ``[T, Hkv, Lmax]``: also compute, for every row, its attention
       weight summed over the nodes and the heads of its group. ``scores_out`` (default: in
       place) gets ``scores`` plus that sum in the first ``lens[t]`` rows and keeps the

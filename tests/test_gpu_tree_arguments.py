@@ -65,3 +65,17 @@ def test_what_is_written_is_not_broadcast(cuda):
     draft = a["k_draft"][:1].expand(a["k_draft"].shape)
     accept_tree(**{**a, "k_draft": draft, "tokens": a["tokens"] + 1})
     assert bool((a["k_cache"][:, :, :, 0] == 1).all())
+
+
+@pytest.mark.parametrize("T,m,H,Hkv,d,lens,Lmax", [(2, 1, 4, 2, 128, [300, 40], 300), (2, 40, 8, 2, 64, [2000, 9], 2000),
+                                                   (1, 20, 4, 2, 256, [900], 900), (9, 8, 8, 8, 128, [700] * 9, 700)])
+def test_the_output_in_the_queries_place(cuda, T, m, H, Hkv, d, lens, Lmax):
+    """Without scores it is the same; with them the weights would read queries that are no longer there."""
+    import torch
+    from moat_b200.tree import tree_attention
+    x = inputs(cuda, T, m, H, Hkv, d, lens, Lmax, seed=2)
+    want = tree_attention(**x)
+    q = x["q"].clone()
+    assert tree_attention(**{**x, "q": q}, out=q) is q and torch.equal(q, want)
+    with pytest.raises(ValueError, match="q"):
+        tree_attention(**x, out=x["q"], scores=torch.zeros((T, Hkv, Lmax), device=cuda))

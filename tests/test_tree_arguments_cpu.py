@@ -52,3 +52,11 @@ def test_broadcast_strides_of_what_is_written(L):
         assert accept(L, strides=zero(u, 16), layers=2, T=2) == -2
         assert evict(L, zero(u, 8)) == -2
     assert evict(L, [128] * 8) == -3
+
+
+def test_the_output_in_the_queries_place_with_scores(L):
+    def call(q, scores):
+        return L.mb_tree_attn(struct.pack("@13PN18q8if", q, *[OTHER] * 6, FAKE, 0, scores, scores, 0, 0, 0, *[128] * 18,
+                                          0, 0, 1, 4, 8, 2, 64, 128, 0.1), None)
+    assert call(FAKE, OTHER) == -2
+    assert call(FAKE, 0) == -3 and call(OTHER, OTHER) == -3
