@@ -8,14 +8,13 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
 #include <cmath>
-#include <map>
-#include <utility>
 #include <vector>
 
 #include "moat_b200.h"
@@ -91,20 +90,11 @@ Tensor part_of(const Tensor& x, int64_t offset, IntArrayRef shape) {
   return part;
 }
 
-// Scratch per (device, stream), grown as needed; the kernels expect no initial contents, and calls
-// that share a buffer are ordered by their stream. A buffer that was outgrown is kept: a captured
-// graph may still use it. Never freed: at exit the allocator may be gone first.
-struct Workspaces {
-  std::map<std::pair<int, cudaStream_t>, std::vector<Tensor>>& all =
-      *new std::map<std::pair<int, cudaStream_t>, std::vector<Tensor>>;
-  const Tensor& get(int device, cudaStream_t stream, int64_t bytes) {
-    std::vector<Tensor>& bufs = all[{device, stream}];
-    const int64_t have = bufs.empty() ? 0 : bufs.back().numel();
-    if (have < bytes) bufs.push_back(make({std::max<int64_t>({bytes, 2 * have, 1 << 20})}, at::kByte, device));
-    return bufs.back();
-  }
-};
-Workspaces attention_space, eviction_space;
+// Scratch of one call, from torch's allocator on the current device and stream: it goes back when
+// the call has been enqueued, and whatever gets it next on that stream comes after. The kernels
+// expect no initial contents. A call that is captured takes it from its graph's pool, so that
+// graphs share none.
+c10::DataPtr scratch(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 // Runs `body`; a C++ exception becomes a Python error.
 template <class Body>
@@ -179,8 +169,8 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     c10::cuda::OptionalCUDAGuard guard;
     if (c10::cuda::current_device() != dev.index) guard.set_index(dev.index);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index).stream();
-    const Tensor& space = attention_space.get(
-        dev.index, stream, static_cast<int64_t>(tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, scores != nullptr)));
+    const size_t bytes = tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, scores != nullptr);
+    const c10::DataPtr space = scratch(bytes);
     mb_tree_attn_args a;
     a.q = address<uint16_t>(q);
     a.k_cache = address<uint16_t>(k);
@@ -193,8 +183,8 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.scores = address<float>(scores);
     a.scores_out = address<float>(scores_out);
     a.draft_scores = address<float>(draft_scores);
-    a.workspace = space.data_ptr();
-    a.workspace_bytes = space.numel();
+    a.workspace = space.get();
+    a.workspace_bytes = bytes;
     a.dev_err = address<uint32_t>(err);
     const Tensor* strided[6] = {q, k, v, kd, vd, out};
     for (int i = 0; i < 6; ++i)
@@ -354,9 +344,9 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (c10::cuda::current_device() != dev.index) guard.set_index(dev.index);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index).stream();
     const Tensor new_lens = make({c.T}, at::kInt, dev.index);
-    const Tensor& space = eviction_space.get(
-        dev.index, stream,
-        static_cast<int64_t>(cache_evict_workspace_size(c.layers, c.T, c.Hkv, c.Lmax, static_cast<int>(number[0]))));
+    const size_t bytes =
+        cache_evict_workspace_size(c.layers, c.T, c.Hkv, c.Lmax, static_cast<int>(number[0]));
+    const c10::DataPtr space = scratch(bytes);
     mb_cache_evict_args a;
     a.k_cache = address<uint16_t>(k);
     a.v_cache = address<uint16_t>(v);
@@ -367,8 +357,8 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.lens = address<int32_t>(lens);
     a.next_pos = address<int32_t>(next_pos);
     a.lens_out = address<int32_t>(&new_lens);
-    a.workspace = space.data_ptr();
-    a.workspace_bytes = space.numel();
+    a.workspace = space.get();
+    a.workspace_bytes = bytes;
     c.strides(k, a.strides);
     c.strides(v, a.strides + 4);
     a.layers = c.layers;

@@ -187,8 +187,9 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
     * ``dev_err``: optional int32 CUDA tensor whose first word receives device error bits
       (bounded waits).
 
-    Scratch belongs to the stream; a captured graph keeps that of the stream it was captured
-    on, so its replays and other calls of that stream must not overlap.
+    Scratch comes from torch's allocator for the length of the call (a captured call's from
+    its graph's pool); with scores and up to 16 rows (nodes x heads of a group) it holds a
+    float per row and cached row.
 
     fp32 scores, softmax and sums; one rounding at the output (and one of each unnormalised
     probability to the inputs' type before its product with V). Values that are not finite
