@@ -153,6 +153,24 @@ inline int launch_with_pdl(Kern kern, dim3 grid, dim3 block, size_t smem, cudaSt
   return MB_OK;
 }
 
+// Host: once per device, lets a kernel take `bytes` of dynamic shared memory (more than 48 KB with the
+// static part need it), and be launched in clusters of more than 8 CTAs.
+template <auto KERN>
+inline int opt_in(int bytes, bool large_clusters = false) {
+  static bool done[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_ERR_LAUNCH;
+  if (done[dev]) return MB_OK;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      (large_clusters &&
+       cudaFuncSetAttribute(KERN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+    (void)cudaGetLastError();
+    return MB_ERR_LAUNCH;
+  }
+  done[dev] = true;
+  return MB_OK;
+}
+
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

@@ -549,16 +549,9 @@ static bool evict_plan(int64_t units, int Lmax, int d, int budget, EvictPlan* pl
 
 template <int CS, bool FUSED>
 static int launch_select(const EvictArgs& a, const EvictPlan& pl, int64_t units, cudaStream_t st) {
-  auto kern = k_evict<CS, FUSED>;
-  if (pl.smem > 32 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return MB_ERR_LAUNCH;
-  }
-  if (CS > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return MB_ERR_LAUNCH;
-  }
+  // whatever the size: of a cluster 17 KB are static
+  const int rc = opt_in<k_evict<CS, FUSED>>(200 * 1024, CS > 8);
+  if (rc != MB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * CS));
   cfg.blockDim = dim3(pl.threads);
@@ -572,7 +565,7 @@ static int launch_select(const EvictArgs& a, const EvictPlan& pl, int64_t units,
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CS > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, k_evict<CS, FUSED>, a) != cudaSuccess) {
     (void)cudaGetLastError();
     return MB_ERR_LAUNCH;
   }

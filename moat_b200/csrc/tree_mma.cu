@@ -1837,24 +1837,9 @@ static bool tree_map(CUtensorMap* map, const void* base, int d, int n0, int64_t 
   return encode_tmap_4d_u16(map, base, dims, strides, box);
 }
 
-// Lets a kernel take all of an SM's shared memory, once per device.
-template <void (*KERN)(TreeMmaParams)>
-static int allow_smem() {
-  static bool done[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_ERR_LAUNCH;
-  if (done[dev]) return MB_OK;
-  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return MB_ERR_LAUNCH;
-  }
-  done[dev] = true;
-  return MB_OK;
-}
-
 template <int PANELS, bool BF16>
 static int launch_attn_keys(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  const int rc = allow_smem<k_tree_attn_keys<PANELS, BF16>>();
+  const int rc = opt_in<k_tree_attn_keys<PANELS, BF16>>(227 * 1024);
   if (rc != MB_OK) return rc;
   return launch_with_pdl(k_tree_attn_keys<PANELS, BF16>, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid),
                          dim3(kKeysThreads), smem, st, p);
@@ -1862,7 +1847,7 @@ static int launch_attn_keys(const TreeMmaParams& p, uint32_t smem, cudaStream_t 
 
 template <int PANELS, bool BF16>
 static int launch_attn_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  const int rc = allow_smem<k_tree_attn_rows<PANELS, BF16>>();
+  const int rc = opt_in<k_tree_attn_rows<PANELS, BF16>>(227 * 1024);
   if (rc != MB_OK) return rc;
   return launch_with_pdl(k_tree_attn_rows<PANELS, BF16>, dim3(p.whole ? p.T * p.a.Hkv * p.RB : p.grid),
                          dim3(kRowsThreads), smem, st, p);
@@ -1880,7 +1865,7 @@ static int launch_rows(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
 
 template <int PANELS, bool BF16>
 static int launch_weights(const TreeMmaParams& p, uint32_t smem, cudaStream_t st) {
-  const int rc = allow_smem<k_tree_weights<PANELS, BF16>>();
+  const int rc = opt_in<k_tree_weights<PANELS, BF16>>(227 * 1024);
   if (rc != MB_OK) return rc;
   return launch_with_pdl(k_tree_weights<PANELS, BF16>, dim3(p.grid), dim3(kWeightThreads), smem, st, p);
 }
