@@ -1527,9 +1527,11 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
   uint64_t* q_empty = q_full + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(q_empty + 2);
   TraceTable& tab = *reinterpret_cast<TraceTable*>(misc + kMiscTab);
-  // per warpgroup the rows' lse and draft masks: in the last ring stage, which is left out
+  // per warpgroup the rows' lse and draft masks, and a bit per row that sees anything: in the last
+  // ring stage, which is left out
   float* lse_s = reinterpret_cast<float*>(smem + lay.ring + (p.nst - 1) * lay.stage);
   uint64_t* mask_s = reinterpret_cast<uint64_t*>(lse_s + 2 * kMaxRows);
+  uint32_t* live_s = reinterpret_cast<uint32_t*>(mask_s + 2 * kMaxRows);
   const int nst = p.nst - 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1665,6 +1667,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
     const float sc = a.scale_log2;
     float* lse = lse_s + grp * kMaxRows;
     uint64_t* rowmask = mask_s + grp * kMaxRows;
+    uint32_t* live = live_s + grp * (kMaxRows / 32);
     const uint32_t sbuf = *tmem_base + lanes + grp * kMaxRows;
     pdl_wait();  // the join's denominators
     pdl_launch_dependents();
@@ -1676,31 +1679,45 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
         named_bar_sync(1 + grp, 128);  // the last block's tables read
         const int i = rb * p.mb + key / p.G;
         const bool node = key < R && i < a.m;  // the last block may hold fewer nodes
-        lse[key] = node ? p.lse[(unit * p.RB + rb) * kMaxRows + key] : INFINITY;
+        const float norm = node ? p.lse[(unit * p.RB + rb) * kMaxRows + key] : INFINITY;
+        lse[key] = norm;
         rowmask[key] = node ? a.masks[s.t * a.mask_stride + i] : 0;
+        const uint32_t seeing = __ballot_sync(0xffffffffu, norm != INFINITY);
+        if (lane == 0) live[wq] = seeing;
         named_bar_sync(1 + grp, 128);
+        bool all_live = true;
+        for (int n = 0; n < p.used; n += 16) all_live &= (live[n >> 5] >> (n & 16) & 0xFFFFu) == 0xFFFFu;
         for (int jj = grp; jj < s.n; jj += 2, ++fill) {
           const int j = s.j0 + jj;
           const bool draft = j == s.nt - 1;
           const int rows = tile_rows(s.len, s.nt, a.m, j);
           guarded_wait(s_full + grp, fill & 1, dead, a.err);
           tc_after_sync();
-          float w = 0.0f;
-          for (int n = 0; n < p.used; n += 16) {
-            float x[16], ls[16];
+          // Rows that see nothing (padding nodes, the block's tail) are left out by their bits: their
+          // scores may be anything, and 2^(x - inf) is 0 only for an x that is a number below inf.
+          // Measured, 4 traces of 16 nodes, one padded: 36.7 us (without the test 36.2, with a condition
+          // per row, which becomes a branch, in place of the & 37.2).
+          float w = 0.0f, x[16], ls[16];
+          auto add = [&](int n, auto weigh) {
             load16(lse + n, ls);
             tc_ld16(sbuf + n, x);
             tc_wait_ld();
             float part = 0.0f;
-            if (draft) {
 #pragma unroll
-              for (int u = 0; u < 16; ++u)
-                part += (rowmask[n + u] >> (key & 63)) & 1 ? ex2(fmaf(x[u], sc, -ls[u])) : 0.0f;
-            } else {
-#pragma unroll
-              for (int u = 0; u < 16; ++u) part += ex2(fmaf(x[u], sc, -ls[u]));
-            }
+            for (int u = 0; u < 16; ++u) part += weigh(u, ex2(fmaf(x[u], sc, -ls[u])));
             w += part;
+          };
+          if (draft) {
+            for (int n = 0; n < p.used; n += 16)
+              add(n, [&](int u, float e) { return (rowmask[n + u] >> (key & 63)) & 1 ? e : 0.0f; });
+          } else if (all_live) {
+            for (int n = 0; n < p.used; n += 16) add(n, [](int, float e) { return e; });
+          } else {
+            for (int n = 0; n < p.used; n += 16) {
+              const uint32_t on = live[n >> 5] >> (n & 16) & 0xFFFFu;
+              if (on != 0)
+                add(n, [&](int u, float e) { return __uint_as_float(__float_as_uint(e) & (0u - ((on >> u) & 1u))); });
+            }
           }
           tc_before_sync();
           mbar_arrive(s_empty + grp);
@@ -1739,6 +1756,7 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
     float w[4] = {};
     const float* x = p.kept + unit * R * p.kept_len + l0;
     for (int r = 0; r < R; ++r) {
+      if (lse[r] == INFINITY) continue;  // a row that sees nothing: its scores may be anything
       const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(r) * p.kept_len);
       w[0] += ex2(v.x - lse[r]);
       w[1] += ex2(v.y - lse[r]);
@@ -1750,7 +1768,8 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
   }
   if (blockIdx.x == 0 && tid < a.m) {
     float w = 0.0f;
-    for (int r = 0; r < R; ++r) w += ex2(p.kept_draft[(unit * R + r) * 64 + tid] - lse[r]);
+    for (int r = 0; r < R; ++r)
+      if (lse[r] != INFINITY) w += ex2(p.kept_draft[(unit * R + r) * 64 + tid] - lse[r]);
     a.draft_scores[unit * a.m + tid] = w;
   }
 }

@@ -1,0 +1,49 @@
+"""Row weights beside what no node sees: padding nodes' queries, infinite scores. References and
+tolerances as in test_gpu_tree.py."""
+
+import pytest
+
+from test_gpu_tree import check, inputs, reference
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [
+    # T, m, H, Hkv, d, lens, Lmax; every third trace has fewer nodes than m, and a node has several heads
+    (3, 3, 4, 2, 128, [700, 0, 300], 700),  # kept scores
+    (3, 8, 4, 2, 64, [130, 1300, 256], 1300),
+    (3, 17, 6, 2, 128, [500, 3, 129], 512),  # formed again
+    (3, 63, 16, 2, 64, [33, 0, 900], 901),  # several row blocks
+    (3, 5, 4, 2, 200, [40, 600, 300], 600),  # general path
+]
+ids = dict(ids=lambda s: "x".join(map(str, s[:5])))
+
+
+@pytest.mark.parametrize("stale", [float("nan"), float("inf"), -float("inf"), 65504.0])
+@pytest.mark.parametrize("shape", SHAPES, **ids)
+def test_queries_of_padding_nodes_do_not_matter(cuda, shape, stale):
+    x = inputs(cuda, *shape, seed=3, padded=True, stale=stale)
+    padding = x["masks"] == 0
+    assert bool(padding.any())
+    x["q"][padding] = stale
+    check(x, weights=True)
+
+
+@pytest.mark.parametrize("shape", SHAPES, **ids)
+def test_a_key_that_weighs_nothing(cuda, shape):
+    """A cached key with an infinite element whose score is -inf for every node: its weight is 0."""
+    import torch
+    from moat_b200.tree import tree_attention
+    x = inputs(cuda, *shape, seed=4, padded=True)
+    T, m, H, Hkv, d, lens, Lmax = shape
+    rel = reference(x)[4]
+    x["q"][..., 5] = x["q"][..., 5].abs() + 0.5
+    for t, n in enumerate(lens):
+        if n > 0:
+            x["k_cache"][t, :, n // 2, 5] = -float("inf")
+    ref, tol, wc, wd, _ = reference(x)
+    out, so, ds = tree_attention(**x, scores=torch.zeros((T, Hkv, Lmax), device=cuda))
+    assert bool(((out.double() - ref).abs() <= tol).all())
+    assert bool(((so.double() - wc).abs() <= 2 * rel * wc + 1e-30).all())  # the queries grew by less than that
+    assert bool(((ds.double() - wd).abs() <= 2 * rel * wd + 1e-30).all())
+    for t, n in enumerate(lens):
+        assert n == 0 or bool((so[t, :, n // 2] == 0).all())
