@@ -1741,7 +1741,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) k_tree_weights(const __grid
 constexpr int kKeptBlock = 128;
 
 __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_constant__ TreeMmaParams p) {
-  __shared__ float lse[16];
+  __shared__ float lse[kKeysRows];
+  __shared__ uint64_t see[kKeysRows];  // drafted rows
   pdl_wait();
   pdl_launch_dependents();
   const TreeAttnArgs& a = p.a;
@@ -1750,7 +1751,10 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
   const int64_t unit = static_cast<int64_t>(p.t0) * a.Hkv + blockIdx.y;
   const int len = trace_len(a, t), l0 = (blockIdx.x * kKeptBlock + tid) * 4;
   if (blockIdx.x * kKeptBlock * 4 >= len && blockIdx.x > 0) return;
-  if (tid < R) lse[tid] = p.lse[unit * kMaxRows + tid];
+  if (tid < R) {
+    lse[tid] = p.lse[unit * kMaxRows + tid];
+    see[tid] = a.masks[t * a.mask_stride + tid / p.G];
+  }
   __syncthreads();
   if (l0 < len) {
     float w[4] = {};
@@ -1768,8 +1772,8 @@ __global__ void __launch_bounds__(kKeptBlock) k_tree_weights_kept(const __grid_c
   }
   if (blockIdx.x == 0 && tid < a.m) {
     float w = 0.0f;
-    for (int r = 0; r < R; ++r)
-      if (lse[r] != INFINITY) w += ex2(p.kept_draft[(unit * R + r) * 64 + tid] - lse[r]);
+    for (int r = 0; r < R; ++r)  // by the masks: the kept -inf of a row that is not seen, less an lse of NaN, is NaN
+      if ((see[r] >> tid) & 1) w += ex2(p.kept_draft[(unit * R + r) * 64 + tid] - lse[r]);
     a.draft_scores[unit * a.m + tid] = w;
   }
 }

@@ -47,3 +47,23 @@ def test_a_key_that_weighs_nothing(cuda, shape):
     assert bool(((ds.double() - wd).abs() <= 2 * rel * wd + 1e-30).all())
     for t, n in enumerate(lens):
         assert n == 0 or bool((so[t, :, n // 2] == 0).all())
+
+
+@pytest.mark.parametrize("m,H,Hkv,d,n", [(3, 4, 2, 128, 300), (7, 4, 2, 64, 40), (9, 16, 2, 128, 700), (5, 4, 2, 200, 90)])
+def test_an_infinite_score_reaches_only_the_rows_that_its_node_sees(cuda, m, H, Hkv, d, n):
+    """Node 1's own key gives it a score of +inf, so what it weighs is not a number; node 2, its
+    sibling, is not seen by it: that row's weight is its own nodes'."""
+    import torch
+    from moat_b200.tree import tree_attention, tree_masks
+    x = inputs(cuda, 2, m, H, Hkv, d, [n, 0], n, seed=m)
+    x["masks"] = torch.from_numpy(tree_masks([-1, 0, 0] + [2] * (m - 3))).to(cuda)
+    rel = reference(x)[4]
+    x["q"][..., 5] = x["q"][..., 5].abs() + 0.5
+    clean = {**x, "masks": x["masks"].clone()}
+    clean["masks"][1] = 0
+    wd = reference(clean)[3]
+    x["k_draft"][:, 1, :, 5] = float("inf")
+    out, so, ds = tree_attention(**x, scores=torch.zeros((2, Hkv, n), device=cuda))
+    assert not bool(torch.isfinite(out[:, 1]).any()) and bool(torch.isfinite(out[:, 2:]).all())
+    assert bool(torch.isnan(so[0]).all()) and bool(torch.isnan(ds[..., :2]).all())
+    assert bool(((ds.double() - wd).abs() <= 2 * rel * wd + 1e-30)[..., 2:].all())
