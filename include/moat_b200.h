@@ -383,8 +383,9 @@ int32_t mb_advance_positions(int32_t* pos, int32_t N, void* stream);
  * v_draft and out. masks [T, m], or [m] if shared_masks.
  * scores_out (optional, [T, Hkv, Lmax] fp32): row l < lens[t] gets scores[l] (0 if scores
  * is NULL; scores may be scores_out) plus its weight summed over the nodes and heads;
- * draft_scores [T, Hkv, m] the draft rows' sums. No atomics: results repeat bit for bit.
- * The workspace (with_scores = 1 if scores_out is given) needs no initial contents. dev_err
+ * draft_scores [T, Hkv, m] the draft rows' sums (where Lmax = 0 it alone asks for them). No
+ * atomics: results repeat bit for bit.
+ * The workspace (with_scores = 1 if draft_scores is given) needs no initial contents. dev_err
  * (optional) receives MB_DEVERR_TIMEOUT if a bounded wait inside a kernel gives up (the output
  * is then undefined). */
 typedef struct {

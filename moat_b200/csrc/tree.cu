@@ -497,20 +497,22 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
   if (!g || !g->q || !g->lens || !g->k_draft || !g->v_draft || !g->masks || !g->out) return MB_ERR_NULL;
   const int T = g->T, m = g->m, H = g->H, Hkv = g->Hkv, Lmax = g->Lmax, d = g->d;
   if (Lmax > 0 && (!g->k_cache || !g->v_cache)) return MB_ERR_NULL;
-  if ((g->scores_out != nullptr) != (g->draft_scores != nullptr) || (g->scores && !g->scores_out)) return MB_ERR_NULL;
+  const bool weights = g->draft_scores != nullptr;  // without a cache there are no other scores
+  if ((g->scores_out != nullptr) != weights && !(weights && Lmax == 0)) return MB_ERR_NULL;
+  if (g->scores && !g->scores_out) return MB_ERR_NULL;
   if (T < 1 || m < 1 || m > 64 || Hkv < 1 || H < Hkv || H % Hkv != 0 || Lmax < 0 || d < 1 || d > kMaxHeadDim)
     return MB_ERR_ARGS;
   if (static_cast<int64_t>(T) * m * H > 0x7FFFFFFFll || static_cast<int64_t>(T) * Hkv > 65535 || Lmax > 0x7FFF0000)
     return MB_ERR_UNSUPPORTED;
   if (broadcast(g->strides + 15, {T, m, H})) return MB_ERR_ARGS;
-  if (g->draft_scores && g->out == g->q) return MB_ERR_ARGS;  // the weights read q after the outputs are there
+  if (weights && g->out == g->q) return MB_ERR_ARGS;  // the weights read q after the outputs are there
   if (!(g->scale - g->scale == 0.0f) || g->is_bf16 < 0 || g->is_bf16 > 1) return MB_ERR_ARGS;
   if (!aligned(g->q, 2) || !aligned(g->k_cache, 2) || !aligned(g->v_cache, 2) || !aligned(g->k_draft, 2) ||
       !aligned(g->v_draft, 2) || !aligned(g->out, 2) || !aligned(g->lens, 4) || !aligned(g->masks, 8) ||
       !aligned(g->scores, 4) || !aligned(g->scores_out, 4) || !aligned(g->draft_scores, 4) || !aligned(g->dev_err, 4))
     return MB_ERR_ALIGN;
   if (!g->workspace ||
-      g->workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, g->scores_out != nullptr))
+      g->workspace_bytes < mb_tree_attn_workspace_size(T, m, H, Hkv, Lmax, d, weights))
     return MB_ERR_WORKSPACE;
   if (!aligned(g->workspace, 16)) return MB_ERR_ALIGN;
   TreeAttnArgs a;
@@ -539,7 +541,7 @@ int32_t mb_tree_attn(const mb_tree_attn_args* g, void* stream) {
   a.d = d;
   a.scale_log2 = g->scale * 1.4426950408889634f;
   a.scores = g->scores;
-  a.scores_out = g->scores_out;
+  a.scores_out = weights && !g->scores_out ? g->draft_scores : g->scores_out;  // Lmax = 0: no row is written
   a.draft_scores = g->draft_scores;
   a.err = g->dev_err;
   const bool bf16 = g->is_bf16 != 0;

@@ -67,3 +67,9 @@ def test_an_infinite_score_reaches_only_the_rows_that_its_node_sees(cuda, m, H, 
     assert not bool(torch.isfinite(out[:, 1]).any()) and bool(torch.isfinite(out[:, 2:]).all())
     assert bool(torch.isnan(so[0]).all()) and bool(torch.isnan(ds[..., :2]).all())
     assert bool(((ds.double() - wd).abs() <= 2 * rel * wd + 1e-30)[..., 2:].all())
+
+
+@pytest.mark.parametrize("T,m,H,Hkv,d", [(1, 1, 1, 1, 64), (2, 5, 4, 2, 128), (2, 33, 8, 2, 64), (1, 3, 2, 1, 33)])
+def test_weights_without_a_cache(cuda, T, m, H, Hkv, d):
+    """Lmax = 0: there is nothing but the draft."""
+    check(inputs(cuda, T, m, H, Hkv, d, [0] * T, 0, seed=m), weights=True)

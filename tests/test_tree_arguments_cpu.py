@@ -60,3 +60,12 @@ def test_the_output_in_the_queries_place_with_scores(L):
                                           0, 0, 1, 4, 8, 2, 64, 128, 0.1), None)
     assert call(FAKE, OTHER) == -2
     assert call(FAKE, 0) == -3 and call(OTHER, OTHER) == -3
+
+
+def test_weights_without_a_cache_need_only_the_drafts(L):
+    def call(Lmax, scores_out, draft, cache=0, m=4):
+        return L.mb_tree_attn(struct.pack("@13PN18q8if", FAKE, cache, cache, FAKE, FAKE, FAKE, FAKE, OTHER, 0, scores_out,
+                                          draft, 0, 0, 0, *[128] * 18, 0, 0, 1, m, 8, 2, Lmax, 128, 0.1), None)
+    assert call(0, 0, FAKE) == -3 and call(0, FAKE, FAKE) == -3 and call(0, 0, 0) == -3
+    assert call(0, FAKE, 0) == -1  # nowhere to put the drafts' sums
+    assert call(1, 0, FAKE, cache=FAKE) == -1  # nor the rows'
