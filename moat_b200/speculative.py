@@ -11,7 +11,9 @@ table's softmax, whose attention differs by about 3e-4, so near-ties may fall th
 
 With a ``budget`` the caches hold at most that many rows (plus those since the last
 eviction): ``tree_attention`` sums up the attention weight of every cached row and
-``evict_cache`` keeps the recent rows, the first ones and the heaviest.
+``evict_cache`` keeps the recent rows, the first ones and the heaviest. What was drafted has a
+say in which: every drafted node counts, also one that is rejected afterwards; a missing one
+(-1), and what hangs on it, does not.
 
     dec = Int4Decoder(cfg, n_traces=16)
     spec = TreeDecoder(dec, parents=[-1, 0, 1, 2, 0], budget=512, capacity=640)
@@ -53,6 +55,7 @@ class _Shape:
         self.parents = t.from_numpy(par).to(device)
         self.masks = t.from_numpy(tree_masks(par)).to(device)
         self.depths = t.from_numpy(tree_depths(par)).to(device)
+        self.nodes = t.arange(m, dtype=t.int64, device=device)
         cfg, N = dec.cfg, dec.N
         D, H, dh, F = cfg.hidden, cfg.heads, cfg.head_dim, cfg.ffn
         rows = N * m
@@ -125,6 +128,13 @@ class TreeDecoder:
         self.longest = 0  # or a later position
 
     # -------------------------------------------------------------------------
+    def _drafted_masks(self, s: _Shape):
+        """Masks ``[N, m]`` of the tree in ``s.tokens``: a missing node, and what hangs on it,
+        is padding."""
+        t = _lib.torch()
+        missing = ((s.tokens < 0).long() << s.nodes).sum(dim=1, keepdim=True)  # a bit per node
+        return t.where((s.masks & missing) == 0, s.masks, 0)
+
     def _layers(self, s: _Shape):
         """The tree in ``s.tokens`` through all layers: leaves the draft's keys, values and
         scores in ``s``, the residual in ``s.x`` and the last layer's output in ``s.o``."""
@@ -134,8 +144,8 @@ class TreeDecoder:
         st = stream_of(self.dev)
         err = self.dev_err.data_ptr()
         p = lambda x: x.data_ptr()  # noqa: E731
-        # a missing draft (-1) is embedded as token 0: no other node's path leads through it
-        ids = s.tokens.clamp(min=0)
+        # a missing draft (-1) is embedded as token 0: no node sees it
+        ids, masks = s.tokens.clamp(min=0), self._drafted_masks(s)
         check(L.mb_embed(p(ids), rows, p(dec.embed), cfg.vocab, D, p(s.x), err, st), "mb_embed")
         y = None
         for li, lw in enumerate(dec.layers):
@@ -146,7 +156,7 @@ class TreeDecoder:
             scores = {}
             if self.scores is not None:
                 scores = dict(scores=self.scores[li], draft_scores=s.draft_scores[li])
-            tree_attention(s.q, self.k_cache[li], self.v_cache[li], self.lens, s.k_draft[li], s.v_draft[li], s.masks,
+            tree_attention(s.q, self.k_cache[li], self.v_cache[li], self.lens, s.k_draft[li], s.v_draft[li], masks,
                            scale=dec.scale, out=s.att, dev_err=self.dev_err, **scores)
             check(L.mb_int4_gemm(p(s.att), p(lw["wo"]), p(s.o), rows, D, D, err, st), "o_proj")
             check(L.mb_add_rmsnorm(p(s.x), p(s.o), p(lw["ffn_norm"]), rows, D, cfg.eps, p(s.h), st), "mb_add_rmsnorm")

@@ -69,3 +69,24 @@ def test_weights_without_a_cache_need_only_the_drafts(L):
     assert call(0, 0, FAKE) == -3 and call(0, FAKE, FAKE) == -3 and call(0, 0, 0) == -3
     assert call(0, FAKE, 0) == -1  # nowhere to put the drafts' sums
     assert call(1, 0, FAKE, cache=FAKE) == -1  # nor the rows'
+
+
+def test_masks_of_missing_drafts():
+    """A node without a token, and what hangs on it, is padding; the others keep their ancestors."""
+    import types
+
+    import torch
+    from moat_b200.speculative import TreeDecoder
+    from moat_b200.tree import tree_masks
+    parents = [-1, 0, 0, 1, 2, 3] + list(range(5, 63))
+    masks = torch.from_numpy(tree_masks(parents))
+    tokens = torch.zeros((4, 64), dtype=torch.int32)
+    tokens[1, 1] = -1
+    tokens[2, 63] = -7
+    tokens[3, 0] = -1
+    s = types.SimpleNamespace(tokens=tokens, masks=masks, nodes=torch.arange(64))
+    got = TreeDecoder._drafted_masks(None, s)
+    assert got.is_contiguous() and got.dtype == torch.int64
+    assert torch.equal(got[0], masks) and torch.equal(got[2, :63], masks[:63]) and int(got[2, 63]) == 0
+    assert [i for i in range(64) if got[1, i] != 0] == [0, 2, 4]
+    assert int(got[1, 4]) == 0b10101 and not bool(got[3].any())
