@@ -188,9 +188,15 @@ class TreeDecoder:
         self.ids.copy_(r.next_ids)
         return r
 
+    def _read_lengths(self):
+        """The true lengths in place of the bounds; waits for the device."""
+        self.rows, self.longest = int(self.lens.max()), int(self.next_pos.max())
+
     def _make_room(self, m: int):
-        """Room for m more rows in every trace: evicts when the bound on the lengths says so
-        (the lengths themselves stay on the device)."""
+        """Room for m more rows in every trace; evicts where there is none. The lengths stay on
+        the device: they are read only where the bounds kept here leave no room."""
+        if self.rows + m > self.capacity or self.longest + m > self.max_positions:
+            self._read_lengths()
         if self.longest + m > self.max_positions:
             raise ValueError("the sequence is longer than max_positions")
         if self.rows + m > self.capacity:
@@ -256,8 +262,7 @@ class TreeDecoder:
                 hist.extend(d[i - 1] for i in nodes[1:] if i > 0)
                 if token >= 0:
                     hist.append(token)
-            # the true lengths replace the bounds
-            self.rows, self.longest = int(self.lens.max()), int(self.next_pos.max())
+            self._read_lengths()
         return [hist[n:] for hist, n in zip(self.history, first)]
 
 

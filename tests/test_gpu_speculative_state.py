@@ -139,3 +139,31 @@ def test_a_long_run_without_drafts(cuda, monkeypatch, parents):
     spec.generate(30, lambda hist, m: [-1] * (m - 1))
     assert spec.next_pos.tolist() == [89] * 3
     assert check_events(dec, spec, events) >= 3 * 4 * 3  # traces, heads of all layers, times
+
+
+@pytest.mark.parametrize("kw", [dict(capacity=24), dict(capacity=40, max_positions=24)])
+def test_steps_fill_the_cache(cuda, kw):
+    """Rejected drafts take no room, in calls of step() as in generate()."""
+    dec, spec = make(cuda, parents=[-1, 0, 1, 2, 3], **kw)
+    spec.prefill(prompt(cuda, 3, 5, 1000))
+    none = np.full((3, 4), -1, np.int32)
+    for i in range(16):
+        assert spec.lens.tolist() == [4 + i] * 3
+        spec.step(none)
+    with pytest.raises(ValueError):
+        spec.step(none)
+    assert spec.lens.tolist() == [20] * 3
+
+
+def test_step_and_generate_keep_the_same_rows(cuda):
+    runs = []
+    for stepwise in (True, False):
+        dec, spec = make(cuda, parents=[-1, 0, 1, 0], capacity=56, budget=40, recent=12, sinks=2, max_positions=400)
+        spec.prefill(prompt(cuda, 3, 30, 1000), chunk=8)
+        if stepwise:
+            for _ in range(60):
+                spec.step(np.full((3, 3), -1, np.int32))
+        else:
+            spec.generate(60, lambda hist, m: [-1] * 3)
+        runs.append((spec.ids.tolist(), spec.lens.tolist(), spec.positions.tolist(), spec.scores.tolist()))
+    assert runs[0] == runs[1]
