@@ -213,7 +213,8 @@ class TreeDecoder:
     def prefill(self, prompt_ids, chunk: int = 32):
         """Run a prompt ``[N, P]`` through the model, ``chunk`` positions at a time as a chain
         whose every node is accepted. All but the last token end up in the caches; the last
-        one is the next step's root."""
+        one is the next step's root. Beside a budget that leaves less room than a chunk, chunks
+        are smaller. A prompt that does not fit is refused before anything changes."""
         t = _lib.torch()
         if prompt_ids.dim() != 2 or prompt_ids.shape[0] != self.N or prompt_ids.shape[1] < 1:
             raise ValueError(f"prompt ids must be [{self.N}, P]")
@@ -221,8 +222,15 @@ class TreeDecoder:
             raise ValueError(f"chunk must be 1 to {MAX_NODES}")
         ids = prompt_ids.to(device=self.dev, dtype=t.int32)
         P, at, s = int(ids.shape[1]), 0, None
+        self._read_lengths()
+        if self.longest + P - 1 > self.max_positions:
+            raise ValueError("the sequence is longer than max_positions")
+        if self.budget is None and self.rows + P - 1 > self.capacity:
+            raise ValueError("KV cache is full")
         while at < P - 1:
             n = min(chunk, P - 1 - at)
+            if self.budget is not None:
+                n = min(n, self.capacity - min(self.rows, self.budget))
             if s is None or s.m != n:
                 s = _Shape(self.dec, range(-1, n - 1), self.dev)
             self._make_room(n)

@@ -167,3 +167,26 @@ def test_step_and_generate_keep_the_same_rows(cuda):
             spec.generate(60, lambda hist, m: [-1] * 3)
         runs.append((spec.ids.tolist(), spec.lens.tolist(), spec.positions.tolist(), spec.scores.tolist()))
     assert runs[0] == runs[1]
+
+
+@pytest.mark.parametrize("parents,capacity", [([-1, 0, 1, 2], 46), ([-1], 41)])
+def test_a_prompt_in_little_room(cuda, monkeypatch, parents, capacity):
+    """Room for fewer rows than a chunk beside the budget: the chunks become smaller."""
+    dec, spec = make(cuda, parents=parents, capacity=capacity, budget=40, recent=12, sinks=2, max_positions=400)
+    events = watch(spec, monkeypatch)
+    spec.prefill(prompt(cuda, 3, 60, 1000))
+    assert spec.next_pos.tolist() == [59] * 3
+    spec.generate(5, lambda hist, m: [-1] * (m - 1))
+    assert spec.next_pos.tolist() == [64] * 3 and max(spec.lens.tolist()) <= capacity
+    assert check_events(dec, spec, events) > 0
+
+
+def test_a_prompt_without_room_changes_nothing(cuda):
+    for kw, P in ((dict(capacity=20), 22), (dict(capacity=60, max_positions=20), 22),
+                  (dict(capacity=56, budget=40, recent=12, max_positions=50), 52)):
+        dec, spec = make(cuda, parents=[-1, 0], **kw)
+        with pytest.raises(ValueError):
+            spec.prefill(prompt(cuda, 3, P, 1000), chunk=4)
+        assert spec.lens.tolist() == [0] * 3 and spec.history == [[]] * 3
+        spec.prefill(prompt(cuda, 3, 9, 1000), chunk=4)
+        run_checked(dec, spec, 2, lambda hist, m: [-1] * (m - 1))
