@@ -118,6 +118,7 @@ class TreeDecoder:
         self.lens = t.zeros(self.N, dtype=t.int32, device=self.dev)
         self.next_pos = t.zeros_like(self.lens)
         self.ids = t.zeros_like(self.lens)  # each trace's last chosen token, not yet in the cache
+        self.pending = False  # no token has been chosen yet
         self.dev_err = t.zeros(1, dtype=t.int32, device=self.dev)
         self.logits = t.empty((self.N * self.m, cfg.vocab), dtype=t.float16, device=self.dev)
         self._logits_lm = (self.logits if dec.lm_cols == cfg.vocab
@@ -213,20 +214,27 @@ class TreeDecoder:
     def prefill(self, prompt_ids, chunk: int = 32):
         """Run a prompt ``[N, P]`` through the model, ``chunk`` positions at a time as a chain
         whose every node is accepted. All but the last token end up in the caches; the last
-        one is the next step's root. Beside a budget that leaves less room than a chunk, chunks
-        are smaller. A prompt that does not fit is refused before anything changes."""
+        one is the next step's root. After tokens or another prompt, the token chosen last, which
+        is not in the caches yet, comes before this one. Beside a budget that leaves less room
+        than a chunk, chunks are smaller. A prompt that does not fit is refused before anything
+        changes."""
         t = _lib.torch()
         if prompt_ids.dim() != 2 or prompt_ids.shape[0] != self.N or prompt_ids.shape[1] < 1:
             raise ValueError(f"prompt ids must be [{self.N}, P]")
         if not 1 <= chunk <= MAX_NODES:
             raise ValueError(f"chunk must be 1 to {MAX_NODES}")
         ids = prompt_ids.to(device=self.dev, dtype=t.int32)
+        row_tokens = ids.tolist()
+        if self.pending:
+            ids = t.cat([self.ids.unsqueeze(1), ids], 1)
         P, at, s = int(ids.shape[1]), 0, None
         self._read_lengths()
         if self.longest + P - 1 > self.max_positions:
             raise ValueError("the sequence is longer than max_positions")
         if self.budget is None and self.rows + P - 1 > self.capacity:
             raise ValueError("KV cache is full")
+        self.ids.copy_(ids[:, 0])
+        self.pending = True
         while at < P - 1:
             n = min(chunk, P - 1 - at)
             if self.budget is not None:
@@ -235,11 +243,11 @@ class TreeDecoder:
                 s = _Shape(self.dec, range(-1, n - 1), self.dev)
             self._make_room(n)
             s.tokens.copy_(ids[:, at:at + n])
+            s.tokens[:, 0].copy_(self.ids)  # an idle trace stays idle
             self._layers(s)
             self._accept(s, ids[:, at + 1:at + n + 1].contiguous())
             at += n
-        self.ids.copy_(ids[:, -1])
-        for hist, row in zip(self.history, ids.tolist()):
+        for hist, row in zip(self.history, row_tokens):
             hist.extend(row)
 
     def step(self, drafts):
@@ -252,6 +260,7 @@ class TreeDecoder:
         if tuple(drafts.shape) != (self.N, self.m - 1):
             raise ValueError(f"drafts must be [{self.N}, {self.m - 1}]")
         self._make_room(self.m)
+        self.pending = True
         s.tokens[:, 0].copy_(self.ids)
         s.tokens[:, 1:].copy_(drafts)
         self._layers(s)

@@ -190,3 +190,26 @@ def test_a_prompt_without_room_changes_nothing(cuda):
         assert spec.lens.tolist() == [0] * 3 and spec.history == [[]] * 3
         spec.prefill(prompt(cuda, 3, 9, 1000), chunk=4)
         run_checked(dec, spec, 2, lambda hist, m: [-1] * (m - 1))
+
+
+def test_a_prompt_after_tokens(cuda):
+    """The next turn of a conversation: the last chosen token comes before it."""
+    rng = np.random.default_rng(2)
+    dec, spec = make(cuda, parents=[-1, 0, 0, 1])
+    spec.prefill(prompt(cuda, 3, 7, 1000), chunk=4)
+    for P in (1, 6, 9):
+        run_checked(dec, spec, 3, lambda hist, m: rng.integers(-1, 1000, m - 1).tolist())
+        spec.prefill(prompt(cuda, 3, P, 1000, seed=P), chunk=4)
+    run_checked(dec, spec, 3, lambda hist, m: rng.integers(-1, 1000, m - 1).tolist())
+    for n, hist in enumerate(spec.history):
+        assert int(spec.next_pos[n]) == len(hist) - 1 and int(spec.ids[n]) == hist[-1]
+
+
+def test_a_prompt_after_a_prompt(cuda):
+    dec, spec = make(cuda, parents=[-1, 0])
+    ids = prompt(cuda, 3, 12, 1000)
+    spec.prefill(ids[:, :1])
+    spec.prefill(ids[:, 1:5])
+    spec.prefill(ids[:, 5:], chunk=3)
+    assert spec.lens.tolist() == [11] * 3 and spec.history == ids.tolist()
+    run_checked(dec, spec, 3, lambda hist, m: [-1])
