@@ -133,6 +133,18 @@ def check(rc: int, what: str) -> None:
         raise MoatError(f"{what} failed: {msg} (status {rc})")
 
 
+# bits of a device error word (MB_DEVERR_* of the header)
+_DEVICE_ERRORS = {1: "a bounded wait gave up", 2: "an index (token id, position or cache row) was out of range",
+                  4: "a row's maximum was not finite"}
+
+
+def check_device(word: int, what: str) -> None:
+    """Raise for the bits of a device error word that has been read."""
+    if word:
+        known = [text for bit, text in _DEVICE_ERRORS.items() if word & bit] or ["unknown"]
+        raise MoatError(f"{what} failed on the device: {'; '.join(known)} (error word {word})")
+
+
 # ---------------------------------------------------------------------------
 # tensor plumbing (torch is the device-memory / stream provider)
 # ---------------------------------------------------------------------------

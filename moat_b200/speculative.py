@@ -26,7 +26,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import _lib
-from ._lib import check, lib, stream_of
+from ._lib import check, check_device, lib, stream_of
 from .decode import rope_table
 from .evict import evict_cache
 from .tree import MAX_NODES, accept_tree, tree_attention, tree_depths, tree_masks
@@ -85,7 +85,7 @@ class TreeDecoder:
       evicted, and no scores are kept.
 
     The caches are this object's own; traces may differ in length (``lens``, on the device).
-    ``dev_err`` collects the device error bits.
+    ``dev_err`` collects the device error bits; ``generate`` raises for them.
     """
 
     def __init__(self, dec, parents, capacity=None, budget=None, recent: int = 64, sinks: int = 4,
@@ -275,6 +275,7 @@ class TreeDecoder:
             drafts = [draft(hist, self.m) for hist in self.history]
             r = self.step(drafts)
             path, nxt = r.path.tolist(), r.next_ids.tolist()  # also waits for the step
+            check_device(int(self.dev_err), "drafted decoding")
             for hist, d, nodes, token in zip(self.history, drafts, path, nxt):
                 hist.extend(d[i - 1] for i in nodes[1:] if i > 0)
                 if token >= 0:

@@ -213,3 +213,23 @@ def test_a_prompt_after_a_prompt(cuda):
     spec.prefill(ids[:, 5:], chunk=3)
     assert spec.lens.tolist() == [11] * 3 and spec.history == ids.tolist()
     run_checked(dec, spec, 3, lambda hist, m: [-1])
+
+
+def test_device_errors_are_raised(cuda):
+    """A drafted token outside the vocabulary sets the index bit."""
+    from moat_b200._lib import MoatError
+    dec, spec = make(cuda, parents=[-1, 0])
+    spec.prefill(prompt(cuda, 3, 7, 1000))
+    spec.generate(2, lambda hist, m: [-1])
+    with pytest.raises(MoatError, match="index"):
+        spec.generate(2, lambda hist, m: [1000])
+
+
+def test_device_errors_of_a_prompt_are_raised(cuda):
+    from moat_b200._lib import MoatError
+    dec, spec = make(cuda, parents=[-1, 0])
+    ids = prompt(cuda, 3, 7, 1000)
+    ids[1, 3] = 5000
+    spec.prefill(ids)
+    with pytest.raises(MoatError, match="index"):
+        spec.generate(1, lambda hist, m: [-1])

@@ -90,3 +90,10 @@ def test_masks_of_missing_drafts():
     assert torch.equal(got[0], masks) and torch.equal(got[2, :63], masks[:63]) and int(got[2, 63]) == 0
     assert [i for i in range(64) if got[1, i] != 0] == [0, 2, 4]
     assert int(got[1, 4]) == 0b10101 and not bool(got[3].any())
+
+
+def test_device_error_words_are_spelled_out():
+    _lib.check_device(0, "a step")
+    for word, text in ((1, "wait"), (2, "index"), (3, "wait.*index"), (4, "finite"), (1 << 20, "unknown")):
+        with pytest.raises(_lib.MoatError, match=text):
+            _lib.check_device(word, "a step")
