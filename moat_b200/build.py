@@ -1,5 +1,6 @@
 """Build recipe for the in-tree CUDA library ``moat_b200/_lib/libmoat_b200.so`` and the
-extension module ``moat_bind.so`` beside it (``csrc/bind.cpp``, against the installed torch).
+extension module ``moat_bind.so`` beside it (``csrc/bind.cpp``, against the installed torch;
+left out where there is none).
 
 Compiles every ``moat_b200/csrc/*.cu`` for sm_100a only (B200), in parallel, and links
 one shared library with the C ABI declared in ``include/moat_b200.h``. nvcc
@@ -54,8 +55,15 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
-    """Compile the CUDA sources into the in-tree shared library, and the binding; returns its path."""
+    """Compile the CUDA sources into the in-tree shared library, then the binding where torch is
+    installed; returns the library's path."""
+    build_library(verbose, force)
     build_bind(force)
+    return LIB
+
+
+def build_library(verbose: bool = False, force: bool = False) -> str:
+    """Compile the CUDA sources, which need no torch; returns the library's path."""
     srcs = sources()
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")]
     deps.append(os.path.join(ROOT, "include", "moat_b200.h"))
@@ -76,11 +84,13 @@ def build(verbose: bool = False, force: bool = False) -> str:
     return LIB
 
 
-def build_bind(force: bool = False) -> str:
-    """Compile the extension module; returns its path."""
+def build_bind(force: bool = False) -> str | None:
+    """Compile the extension module; returns its path, or None where there is no torch."""
     import sysconfig
-
-    import torch
+    try:
+        import torch
+    except ModuleNotFoundError:
+        return None
     src = os.path.join(CSRC, "bind.cpp")
     deps = [src, os.path.join(ROOT, "include", "moat_b200.h"), torch.__file__]
     if not force and os.path.exists(BIND) and all(os.path.getmtime(d) <= os.path.getmtime(BIND) for d in deps):
