@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
@@ -96,13 +97,13 @@ Tensor part_of(const Tensor& x, int64_t offset, IntArrayRef shape) {
 // graphs share none.
 c10::DataPtr scratch(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
-// Runs `body`; a C++ exception becomes a Python error.
+// Runs `body`; a C++ exception becomes torch's Python error for it (out of memory is its own).
 template <class Body>
 PyObject* guarded(Body body) {
   try {
     return body();
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }

@@ -70,3 +70,23 @@ def test_graphs_captured_on_one_stream_replay_side_by_side(cuda):
     torch.cuda.synchronize()
     for a, b in zip(eager, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_scratch_beyond_the_memory_is_torchs_error(cuda):
+    """400 MB of kept scores where the process may have 100 MB more than it has."""
+    import torch
+    from moat_b200.tree import tree_attention
+    torch.cuda.empty_cache()
+    x = inputs(cuda, 4, 2, 64, 8, 64, [3] * 4, 8, seed=1)
+    for name in ("k_cache", "v_cache"):  # without temporaries, whose place could hold the scratch
+        x[name] = torch.zeros((4, 8, 200000, 64), dtype=torch.float16, device=cuda)
+    s = torch.zeros((4, 8, 200000), device=cuda)
+    torch.cuda.synchronize()
+    total = torch.cuda.get_device_properties(cuda).total_memory
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (100 << 20)) / total, cuda)
+        with pytest.raises(torch.OutOfMemoryError):
+            tree_attention(**x, scores=s)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0, cuda)
+    assert tree_attention(**x, scores=s)[1] is s
