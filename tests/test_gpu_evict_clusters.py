@@ -40,3 +40,12 @@ run(torch.device("cuda:0"), None, 1, 2, {Lmax}, 16, [{Lmax - 3}], 5000, 64, 4, s
 ])
 def test_clusters(cuda, T, Hkv, Lmax, d, lens, budget, recent, sinks, in_place):
     run(cuda, None, T, Hkv, Lmax, d, lens, budget, recent, sinks, in_place=in_place, seed=Lmax)
+
+
+def test_the_most_rows(cuda):
+    """786,432 rows are what a cluster of 16 ranks; one more is refused."""
+    from moat_b200._lib import MoatError
+    n = 786432
+    run(cuda, None, 1, 1, n, 8, [n], 300000, 1000, 4)
+    with pytest.raises(MoatError):
+        run(cuda, None, 1, 1, n + 1, 8, [n], 300000, 1000, 4)

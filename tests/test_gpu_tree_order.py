@@ -19,6 +19,9 @@ pytestmark = pytest.mark.gpu
     (40, 3, 24, 8, [600 - 13 * t for t in range(40)], 640),
     (12, 24, 8, 8, [700 - 31 * t for t in range(12)], 1024),  # fewer, scores formed again
     (130, 2, 2, 2, [560 - 4 * t for t in range(130)], 576),  # two launches
+    (130, 20, 2, 2, [560 - 4 * t for t in range(130)], 576),  # and scores formed again
+    (130, 2, 2, 2, [6000 if t in (3, 128) else 17 for t in range(130)], 6000),  # units cut in either
+    (130, 9, 4, 2, [6000 if t in (3, 128) else 17 for t in range(130)], 6000),
 ])
 def test_eviction_right_after_attention(cuda, T, m, H, Hkv, lens, Lmax):
     import torch
