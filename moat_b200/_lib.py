@@ -1,8 +1,8 @@
 """ctypes binding of the in-tree CUDA library (C ABI in ``include/moat_b200.h``).
 
 There is no CPU fallback: if ``moat_b200/_lib/libmoat_b200.so`` (or, for the entry points
-that take torch tensors through it, ``moat_bind.so``) is missing or does not load, every accelerated entry point raises. Build it with
-``python -m moat_b200.build``.
+that take torch tensors through it, ``moat_bind.so``) is missing or does not load, every
+accelerated entry point raises. Build it with ``python -m moat_b200.build``.
 """
 
 from __future__ import annotations

@@ -30,7 +30,8 @@
 // Measured on a B200 (calls replayed from a graph; of the 6.44 TB/s of a copy): 16 traces x 16 heads x
 // 4,096 rows of 128: R = 1 82.4 us (6.5 TB/s, all of it), R = 16 84.4 us; 8 KV heads, R = 32 45.0, R = 128
 // 45.8 us (6.0 TB/s); one trace of 130,001 rows, 8 KV heads, R = 4 87 us (6.1 TB/s); 16 traces of 512 to
-// 752 rows, R = 8 22 us (3.9 TB/s: the time to start, end and join, about 8 us, counts).
+// 752 rows, R = 8 22 us (3.9 TB/s: 256 whole units for 148 CTAs, 7 to 18 tiles and starts each where 12.8
+// would be even; a CTA with 16 takes about 13 us, starting and ending the rest).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -1926,7 +1927,9 @@ int tree_mma_launch(const TreeAttnArgs& a, bool bf16, void* ws, void* stream) {
   p.RB = pl.RB;
   p.mb = pl.mb;
   // measured: a tile of the keys kernel 1,500 cycles (three quarters at d <= 64), of the rows
-  // kernel 2,000; 128 keys and values of 128 bytes-a-row panels at 6.4 TB/s, 148 SMs
+  // kernel 2,000 when the constants of share_mode were measured (1,800 since either half of a tile keeps
+  // its own reference; the constants stand as they were measured together); 128 keys and values of
+  // 128 bytes-a-row panels at 6.4 TB/s, 148 SMs
   p.tile_cycles = pl.n16 > kKeysRows ? 2000 : pl.panels == 2 ? 1500 : 1100;
   p.tile_traffic = pl.panels == 2 ? 2900 : 1450;
   if (pl.RB > 1) p.tile_traffic /= pl.RB;  // the row blocks share their keys' traffic

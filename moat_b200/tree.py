@@ -183,7 +183,6 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
       weight summed over the nodes and the heads of its group. ``scores_out`` (default: in
       place) gets ``scores`` plus that sum in the first ``lens[t]`` rows and keeps the
       others; ``draft_scores`` float32 ``[T, Hkv, m]`` gets the sums of the draft's rows.
-
     * ``dev_err``: optional int32 CUDA tensor whose first word receives device error bits
       (bounded waits).
 
@@ -193,7 +192,8 @@ def tree_attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, *, scale=
 
     fp32 scores, softmax and sums; one rounding at the output (and one of each unnormalised
     probability to the inputs' type before its product with V). Values that are not finite
-    reach only the nodes that see their row. Repeated calls give the same bits. Returns ``out``, or ``(out, scores_out, draft_scores)`` with ``scores``.
+    reach only the nodes that see their row. Repeated calls give the same bits. Returns ``out``,
+    or ``(out, scores_out, draft_scores)`` with ``scores``.
     """
     r = _lib.bind().attention(q, k_cache, v_cache, lens, k_draft, v_draft, masks, scale, out, scores, scores_out,
                               draft_scores, dev_err)
